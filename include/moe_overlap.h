@@ -532,6 +532,41 @@ MOE_API int32_t moe_router_topk_backward(const float* probs, const int64_t* topk
                                          float* grad_logits, void* stream);
 
 /*
+ * The whole routed-experts layer for a few tokens (num_tokens <= 128): the gate,
+ * top-k, up-projection with exact GELU, down-projection and weighted sum of
+ * src/train_moe_baseline.py:315-441 without the exchange.
+ *   x             [num_tokens, hidden], row stride ldx
+ *   router_w      [num_experts, hidden], row stride ldr: the gate's weights; the
+ *                 logits are summed in 64 bits, router_bias (float[num_experts] or
+ *                 NULL) is added, the top-k go by the logits (ties to the lower id),
+ *                 their softmax probabilities are divided by their sum when
+ *                 renormalize != 0, and topk_idx / topk_weights are outputs.
+ *                 NULL: topk_idx / topk_weights are inputs; a slot with expert -1
+ *                 adds nothing, a token whose slots are all -1 gets zeros.  An id
+ *                 outside [-1, num_experts) counts as -1 and records
+ *                 MOE_ERR_INVALID_ARG in `status`.
+ *   w1, w2        [num_experts, ffn, hidden] and [num_experts, hidden, ffn] (nn.Linear
+ *                 layout), expert and row strides in elements
+ *   topk_idx      [num_tokens, topk] int64;  topk_weights [num_tokens, topk] float
+ *   out           [num_tokens, hidden], row stride ldo; must not overlap x
+ *   workspace     moe_few_tokens_workspace(...) bytes of device memory, 16-byte
+ *                 aligned, used by this call only; its contents need no set-up
+ * dtype (MOE_DTYPE_BF16 or MOE_DTYPE_F16) is that of x, router_w, w1, w2 and out.
+ * Rows start on 16 bytes; hidden and ffn are multiples of 8; num_experts <= 256;
+ * topk <= 16.
+ */
+MOE_API int64_t moe_few_tokens_workspace(int32_t num_tokens, int32_t hidden, int32_t ffn,
+                                         int32_t num_experts, int32_t topk);
+MOE_API int32_t moe_few_tokens(const void* x, int64_t ldx, const void* router_w, int64_t ldr,
+                               const float* router_bias, const void* w1, int64_t w1_stride_e,
+                               int64_t w1_stride_row, const void* w2, int64_t w2_stride_e,
+                               int64_t w2_stride_row, int32_t dtype, int32_t num_tokens,
+                               int32_t hidden, int32_t ffn, int32_t num_experts, int32_t topk,
+                               int32_t renormalize, int64_t* topk_idx, float* topk_weights,
+                               void* out, int64_t ldo, void* workspace, int64_t workspace_bytes,
+                               int32_t* status, void* stream);
+
+/*
  * DeepEP's get_dispatch_layout (thirdParty/DeepEP/deep_ep/buffer.py:293-319,
  * kernels/layout.cu:10-121): tokens per rank (each token counted once per rank),
  * tokens per expert and is_token_in_rank [num_tokens][world] (bool, 1 byte).

@@ -14,6 +14,7 @@ from .gemm import (
     tile_list,
 )
 from ._lib import MoeError, check_status
+from .few_tokens import experts_few_tokens, moe_few_tokens
 from .fp8 import dequantize_fp8, quantize_fp8
 from .router import router_topk
 
@@ -25,6 +26,8 @@ __all__ = [
     "reference_grouped_gemm",
     "tile_list",
     "router_topk",
+    "moe_few_tokens",
+    "experts_few_tokens",
     "quantize_fp8",
     "dequantize_fp8",
     "MoeError",

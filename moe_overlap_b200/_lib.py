@@ -185,6 +185,15 @@ SIGNATURES: dict[str, tuple] = {
         [_c_void_p, _c_void_p, _c_void_p, _i32, _i32, _i32, _i32,  # probs, idx, dw, T, E, k, renorm
          _c_void_p, _c_void_p],  # grad_logits, stream
     ),
+    "moe_few_tokens_workspace": (_i64, [_i32, _i32, _i32, _i32, _i32]),
+    "moe_few_tokens": (
+        _i32,
+        [_c_void_p, _i64, _c_void_p, _i64, _c_void_p,  # x, ldx, router_w, ldr, router_bias
+         _c_void_p, _i64, _i64, _c_void_p, _i64, _i64,  # w1, strides e/row, w2, strides e/row
+         _i32, _i32, _i32, _i32, _i32, _i32, _i32,  # dtype, T, H, F, E, k, renormalize
+         _c_void_p, _c_void_p, _c_void_p, _i64,  # topk_idx, topk_weights, out, ldo
+         _c_void_p, _i64, _c_void_p, _c_void_p],  # workspace, bytes, status, stream
+    ),
     "moe_ep_dispatch_layout": (
         _i32, [_c_void_p, _i32, _i32, _i32, _i32, _c_void_p, _c_void_p, _c_void_p, _c_void_p]),
     "moe_ipc_export": (_i32, [_c_void_p, _c_void_p]),

@@ -32,6 +32,7 @@ import torch
 import torch.distributed as dist
 
 from .deep_ep_comm import DeepEPDispatcher
+from .few_tokens import experts_few_tokens, moe_few_tokens
 from .fp8 import dequantize_fp8, quantize_fp8
 from .gemm import grouped_gemm, grouped_gemm_wgrad
 from .router import router_topk
@@ -380,6 +381,25 @@ class MoELayer:
         return out, stats
 
     __call__ = forward
+
+    def forward_few(self, x: torch.Tensor, routing=None, out: Optional[torch.Tensor] = None):
+        """The layer for a decode batch of at most 128 tokens: (out, topk_idx, topk_w).
+
+        One pass over the weights of the experts taken, on the caller's stream, with
+        no exchange (few_tokens.moe_few_tokens), so one rank must hold every expert.
+        ``routing`` = (topk_idx, topk_w) to reuse; slots of -1 (padding) add nothing.
+        Unlike ``route``, which rounds the gate's logits to bf16, the logits keep
+        64 bits here.  Forward only.
+        """
+        if self.world != 1 or self._slot_of_expert is not None:
+            raise ValueError("forward_few needs every expert on this rank, in contiguous placement")
+        x = x.to(torch.bfloat16)
+        w1, w2 = self.w1.detach(), self.w2.detach()
+        if routing is not None:
+            idx, w = routing
+            return experts_few_tokens(x, w1, w2, idx, w, out=out), idx, w
+        return moe_few_tokens(x, self.router_w.detach(), w1, w2, self.top_k,
+                              router_bias=self.router_b, renormalize=self.renormalize, out=out)
 
     def forward_serialized(self, x: torch.Tensor, routing,
                            host_cover_cycles: int = 2_000_000) -> tuple[torch.Tensor, dict]:
