@@ -14,6 +14,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "../../include/moe_overlap.h"
 #include "host_common.h"
@@ -42,6 +43,9 @@ __device__ __forceinline__ T from_f(float v) {
     return __float2half_rn(v);
 }
 
+template <typename T>
+constexpr float kMaxOf = std::is_same<T, __nv_bfloat16>::value ? 3.38953139e38f : 65504.0f;
+
 __device__ __forceinline__ double warp_sum(double v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -54,17 +58,18 @@ __device__ __forceinline__ float warp_sum(float v) {
 }
 
 // Dot product of two rows of `n` elements (a multiple of 8, 16-byte aligned) over one
-// warp; every 8 products (exact in fp32 for bf16 and fp16) are summed in Acc.
-template <typename T, typename Acc>
-__device__ __forceinline__ Acc warp_dot(const T* a, const T* b, int n, int lane) {
-  Acc s = 0;
+// warp.  A product of two bf16 or fp16 values is exact in fp32; the sum is fp64.
+template <typename T>
+__device__ __forceinline__ double warp_dot(const T* a, const T* b, int n, int lane) {
+  double s = 0;
+#pragma unroll 4
   for (int i = lane * 8; i < n; i += 256) {
     const uint4 ua = *reinterpret_cast<const uint4*>(a + i);
     const uint4 ub = *reinterpret_cast<const uint4*>(b + i);
     const T* pa = reinterpret_cast<const T*>(&ua);
     const T* pb = reinterpret_cast<const T*>(&ub);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) s += static_cast<Acc>(to_f(pa[j]) * to_f(pb[j]));
+    for (int j = 0; j < 8; ++j) s += static_cast<double>(to_f(pa[j]) * to_f(pb[j]));
   }
   return warp_sum(s);
 }
@@ -139,73 +144,639 @@ __device__ __forceinline__ void warp_topk(const double* z, int E, int k, bool re
   }
 }
 
+// One cluster of 8 CTAs a token: CTA r sums the logits of experts r, r + 8, ..., its
+// warps split over those experts and, when they are few, over parts of hidden; the
+// first CTA gathers the logits and takes the top k.  Also zeroes the counters of the
+// experts' kernel, which is allowed to start at once and waits for this one's end.
+constexpr int kGateCluster = 8;
+
 template <typename T>
-__global__ void __launch_bounds__(32 * kWarps)
+__global__ void __cluster_dims__(kGateCluster, 1, 1) __launch_bounds__(32 * kWarps)
     gate_kernel(const T* x, int64_t ldx, const T* rw, int64_t ldr, const float* bias, int H, int E,
-                int k, int renorm, int64_t* idx, float* w) {
+                int k, int renorm, int64_t* idx, float* w, int32_t* count, int n_count) {
   __shared__ double z[kMaxE];
+  __shared__ double partial[kMaxE / kGateCluster][kWarps];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int t = blockIdx.x;
-  for (int e = warp; e < E; e += kWarps) {
-    const double d = warp_dot<T, double>(x + t * ldx, rw + e * ldr, H, lane);
-    if (lane == 0) z[e] = bias != nullptr ? d + static_cast<double>(bias[e]) : d;
+  const int rank = static_cast<int>(cluster_ctarank()), t = blockIdx.x / kGateCluster;
+  if (blockIdx.x == 0)
+    for (int i = threadIdx.x; i < n_count; i += 32 * kWarps) count[i] = 0;
+  const int mine = (E - rank + kGateCluster - 1) / kGateCluster;  // experts of this CTA (may be 0)
+  const int parts = mine > 0 && mine < kWarps ? kWarps / mine : 1;
+  const int cols = ((H + parts - 1) / parts + 7) / 8 * 8;
+  for (int u = warp; u < mine * parts; u += kWarps) {
+    const int i = u / parts, c0 = (u % parts) * cols;
+    const int n = min(cols, H - c0);  // <= 0: an empty part
+    const double d = warp_dot(x + t * ldx + c0, rw + int64_t(rank + i * kGateCluster) * ldr + c0, n, lane);
+    if (lane == 0) partial[i][u % parts] = d;
   }
   __syncthreads();
-  if (warp == 0) warp_topk(z, E, k, renorm != 0, lane, idx + int64_t(t) * k, w + int64_t(t) * k);
-}
-
-__device__ __forceinline__ int slot_expert(const int64_t* idx, int slot, int E, int32_t* status) {
-  const int64_t e = idx[slot];
-  if (e < -1 || e >= E) {
-    record_status(status, MOE_ERR_INVALID_ARG);
-    return -1;
+  if (threadIdx.x < mine) {
+    const int e = rank + static_cast<int>(threadIdx.x) * kGateCluster;
+    double d = 0;
+    for (int i = 0; i < parts; ++i) d += partial[threadIdx.x][i];
+    if (bias != nullptr) d += static_cast<double>(bias[e]);
+    asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(mapa_shared(smem_u32(&z[e]), 0)), "d"(d)
+                 : "memory");
   }
-  return static_cast<int>(e);
+  cluster_sync_all();
+  if (rank == 0 && warp == 0)
+    warp_topk(z, E, k, renorm != 0, lane, idx + int64_t(t) * k, w + int64_t(t) * k);
 }
 
-template <typename T>
-__global__ void __launch_bounds__(32 * kWarps)
-    up_kernel(const T* x, int64_t ldx, const T* w1, int64_t w1_se, int64_t w1_sr, const int64_t* idx,
-              int H, int F, int E, int k, T* h, int32_t* status) {
-  const int lane = threadIdx.x & 31, f = blockIdx.x * kWarps + (threadIdx.x >> 5);
-  const int slot = blockIdx.y, e = slot_expert(idx, slot, E, status);
-  if (f >= F || e < 0) return;
-  const float a = warp_dot<T, float>(x + (slot / k) * ldx, w1 + e * w1_se + f * w1_sr, H, lane);
-  if (lane == 0)
-    h[int64_t(slot) * F + f] = from_f<T>(0.5f * a * (1.0f + erff(a * 0.70710678118654752440f)));
-}
+// ------------------------------------------------------------ the experts --
+// One persistent kernel streams the weights of the experts taken exactly once.
+// A work item is BM rows of W1[e] (all of hidden) for one group of at most 8 J slots
+// of expert e, or BM rows of W2[e] (one of KS parts of ffn) for such a group.  Items
+// are taken from a ticket counter, all of W1's before any of W2's; the items of W2
+// wait (bounded) until their group's h is complete.  Whoever holds an earlier ticket
+// is running and waits for nothing later, so the waits end whatever else the GPU
+// does, and no grid-wide barrier is needed.
+//
+// Warp 0 fetches weights: TMA boxes of BM rows x 64 columns into a ring of stages of
+// 16 KB.  The weights do not depend on h, so the ring runs ahead into W2 while h is
+// still being finished.  Warp 1 copies the slots' columns of the same stage beside
+// them (rows of x picked by token, or rows of h).  Two sets of 8 warps multiply, on
+// items in turn, so that one set's sums, stores and fences (several microseconds'
+// worth of latency an item) pass under the other's products: a stage is R tiles of 16 rows x C = 8/R slices of 64 columns, one (tile, slice) per warp,
+// m16n8k16 with the weights as the 16-row side and the slots as the 8-column side.
+// (tcgen05's 128-row tiles would leave too few items for 148 SMs at one token, and
+// the tensor work here is a few percent of the time either way.)  The order of k
+// inside a slice is free, so lane (g, q) takes the 16 contiguous columns 16q.. of its
+// rows and of its slot: both come by conflict-free 16-byte shared loads.
+constexpr int kConsumers = 8;
+constexpr int kSets = 2;         // of consumers, on items in turn
+constexpr int kThreads = 32 * (2 + kSets * kConsumers);
+constexpr int kStageBytes = 16 * 1024;
+constexpr int kRedStride = 20;  // floats between slots in the reduction buffer: no bank conflicts
+constexpr int kMaxSlots = kMaxTokens * kMaxK;
+constexpr int kQueue = 8;
+
+// Shared memory of one variant.  A stage's slots: 8 J rows of 64 C columns, twice (h
+// comes in two parts).
+template <int R, int J>
+struct Cfg {
+  static constexpr int BM = 16 * R, C = kConsumers / R, BKS = 64 * C, NT = 8 * J;
+  static constexpr int kSlotBytes = NT * BKS * 2;
+  static constexpr int kFull = kStageBytes + 2 * kSlotBytes;
+  static constexpr int kRed = C > 1 ? kSets * kConsumers * NT * kRedStride * 4 : 0;
+  static constexpr int kStages = (200 * 1024 - kRed) / kFull;
+  static constexpr int kBytes = kStages * kFull + kRed;
+};
+
+__host__ __device__ constexpr int max_groups(int J, int E) { return E + kMaxSlots / (8 * J); }
+
+struct Params {
+  const void* x;
+  int64_t ldx;
+  const int64_t* idx;
+  const float* w;
+  void* out;
+  int64_t ldo;
+  void* h;         // [2][slots][F]: h in slot order by expert, rounded, and what the rounding left
+  float* part;     // [KS * C][slots][H]
+  int32_t* count;  // ticket, then per group its finished W1 items, then per 16 rows of H its finished parts
+  int32_t* status;
+  int T, H, F, E, k, KS;
+};
+
+struct Plan {  // in shared memory; every CTA derives the same one from idx
+  int n_groups, n_slots;
+  int16_t expert_of_slot[kMaxSlots];  // -1: none
+  uint16_t slot_at[kMaxSlots];        // slots ordered by expert
+  uint16_t pos_of[kMaxSlots];         // place of a slot in that order, 0xffff: none
+};
+
+struct Ctrl {
+  uint64_t full[12], empty[12], qfull[kQueue], qempty[kQueue], turn[kSets];
+  int item[kQueue];
+};
 
 template <typename T>
-__global__ void __launch_bounds__(32 * kWarps)
-    down_kernel(const T* h, const T* w2, int64_t w2_se, int64_t w2_sr, const int64_t* idx,
-                const float* w, int H, int F, int E, int k, T* out, int64_t ldo) {
-  const int lane = threadIdx.x & 31, col = blockIdx.x * kWarps + (threadIdx.x >> 5);
-  const int t = blockIdx.y;
-  if (col >= H) return;
-  float s = 0.0f;
-  for (int j = 0; j < k; ++j) {
-    const int slot = t * k + j, e = slot_expert(idx, slot, E, nullptr);
-    if (e >= 0)
-      s += w[slot] * warp_dot<T, float>(h + int64_t(slot) * F, w2 + e * w2_se + col * w2_sr, F, lane);
+__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                    uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void ld_shared_v4(uint32_t addr, uint32_t* r) {
+  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+// 16 bytes to shared memory, zeros when `bytes` is 0 (nothing is read then).
+__device__ __forceinline__ void copy_async_16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
+               : "memory");
+}
+// Arrives on `bar` when this thread's earlier copies have landed.
+__device__ __forceinline__ void copies_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ int ld_acquire_gpu(const int* p) {
+  int v;
+  asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ void red_release_gpu(int* p, int v) {
+  asm volatile("red.release.gpu.global.add.s32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
+}
+__device__ __forceinline__ int add_acq_rel_gpu(int* p, int v) {
+  int r;
+  asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], %2;" : "=r"(r) : "l"(p), "r"(v) : "memory");
+  return r;
+}
+// The 8 warps of one set.
+__device__ __forceinline__ void set_sync(int set) {
+  asm volatile("bar.sync %0, 256;" ::"r"(1 + set) : "memory");
+}
+
+// The slots by expert and the groups of at most NT of them: grp holds
+// expert << 16 | place of the group's first slot.
+__device__ __forceinline__ void build_plan(const Params& p, int NT, Plan* pl, int* grp, int* cnt,
+                                           int* grp_first) {
+  const int tid = threadIdx.x, S = p.T * p.k;
+  for (int i = tid; i < S; i += kThreads) {
+    const int64_t e = p.idx[i];
+    if (e < -1 || e >= p.E) record_status(p.status, MOE_ERR_INVALID_ARG);
+    pl->expert_of_slot[i] = (e >= 0 && e < p.E) ? static_cast<int16_t>(e) : int16_t(-1);
+    pl->pos_of[i] = 0xffff;
   }
-  if (lane == 0) out[t * ldo + col] = from_f<T>(s);
+  __syncthreads();
+  if (tid < p.E) {
+    int c = 0;
+    for (int i = 0; i < S; ++i) c += pl->expert_of_slot[i] == tid;
+    cnt[tid] = c;
+  }
+  __syncthreads();
+  if (tid < 32) {  // prefix sums over the experts: slots and groups
+    int run_s = 0, run_g = 0;
+    for (int b = 0; b < p.E; b += 32) {
+      const int e = b + tid;
+      const int c = e < p.E ? cnt[e] : 0, g = (c + NT - 1) / NT;
+      int is = c, ig = g;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int vs = __shfl_up_sync(0xffffffffu, is, o), vg = __shfl_up_sync(0xffffffffu, ig, o);
+        if (tid >= o) {
+          is += vs;
+          ig += vg;
+        }
+      }
+      if (e < p.E) {
+        cnt[e] = run_s + is - c;
+        grp_first[e] = run_g + ig - g;
+      }
+      run_s += __shfl_sync(0xffffffffu, is, 31);
+      run_g += __shfl_sync(0xffffffffu, ig, 31);
+    }
+    if (tid == 0) {
+      pl->n_slots = run_s;
+      pl->n_groups = run_g;
+    }
+  }
+  __syncthreads();
+  if (tid < p.E) {
+    const int s0 = cnt[tid];
+    int at = s0, g = grp_first[tid];
+    for (int i = 0; i < S; ++i)
+      if (pl->expert_of_slot[i] == tid) {
+        if ((at - s0) % NT == 0) grp[g++] = (tid << 16) | at;
+        pl->slot_at[at] = static_cast<uint16_t>(i);
+        pl->pos_of[i] = static_cast<uint16_t>(at);
+        ++at;
+      }
+  }
+  __syncthreads();
+}
+
+// One work item, decoded from its ticket.
+struct Item {
+  bool down;
+  int g, blk, ks, c0, c1;  // group, row block, part of ffn, its columns [c0, c1)
+};
+
+template <typename T, int R, int J>
+__global__ void __launch_bounds__(kThreads, 1)
+    experts_kernel(const __grid_constant__ CUtensorMap map1, const __grid_constant__ CUtensorMap map2,
+                   const __grid_constant__ Params p) {
+  using K = Cfg<R, J>;
+  constexpr int BM = K::BM, C = K::C, BKS = K::BKS, NT = K::NT, kStages = K::kStages;
+  constexpr int kSliceBytes = BM * 128;
+  extern __shared__ char smem_raw[];
+  char* base = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  // Stages' weights, then their slots, then two reduction buffers.
+  char* slots = base + kStages * kStageBytes;
+  float* red = reinterpret_cast<float*>(slots + kStages * 2 * K::kSlotBytes);
+  Ctrl* ctrl = reinterpret_cast<Ctrl*>(base + K::kBytes);
+  Plan* plan = reinterpret_cast<Plan*>(ctrl + 1);
+  int* grp = reinterpret_cast<int*>(plan + 1);
+  int* cnt = grp + max_groups(J, p.E);
+  int* grp_first = cnt + p.E;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(smem_u32(&ctrl->full[s]), 1 + 32);
+      mbar_init(smem_u32(&ctrl->empty[s]), kConsumers);
+    }
+    for (int s = 0; s < kSets; ++s) mbar_init(smem_u32(&ctrl->turn[s]), kConsumers);
+    for (int s = 0; s < kQueue; ++s) {
+      mbar_init(smem_u32(&ctrl->qfull[s]), 1);
+      mbar_init(smem_u32(&ctrl->qempty[s]), 1 + kSets * kConsumers);
+    }
+    fence_mbar_init();
+    tma_prefetch_desc(&map1);
+    tma_prefetch_desc(&map2);
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the gate's idx, w and counters
+  build_plan(p, NT, plan, grp, cnt, grp_first);
+  const int G = plan->n_groups, S = plan->n_slots;
+  const int FB = (p.F + BM - 1) / BM, HB = (p.H + BM - 1) / BM;
+  if (G == 0) {  // no slot is routed: zeros
+    T* out = static_cast<T*>(p.out);
+    for (int i = blockIdx.x * kThreads + tid; i < p.T * p.H; i += gridDim.x * kThreads)
+      out[(i / p.H) * p.ldo + i % p.H] = from_f<T>(0.0f);
+    return;
+  }
+  const int up_items = G * FB, items = up_items + G * HB * p.KS;
+  int* ready = p.count + 1;
+  int* done = ready + G;
+  // columns of F that one part of a W2 item covers (a multiple of a stage's)
+  const int part_cols = ((p.F + p.KS - 1) / p.KS + BKS - 1) / BKS * BKS;
+  auto decode = [&](int item) {
+    Item it;
+    it.down = item >= up_items;
+    const int q = it.down ? item - up_items : item, per = it.down ? HB * p.KS : FB;
+    it.g = q / per;
+    const int r = q - it.g * per;
+    it.blk = it.down ? r / p.KS : r;
+    it.ks = it.down ? r - it.blk * p.KS : 0;
+    it.c0 = it.ks * part_cols;
+    it.c1 = it.down ? min(it.c0 + part_cols, p.F) : p.H;
+    return it;
+  };
+  // Takes the queue's next item; -1 at the end (or when the wait ran out).
+  auto pop = [&](int n) {
+    const int slot = n % kQueue;
+    int item = -1;
+    if (mbar_wait(smem_u32(&ctrl->qfull[slot]), (n / kQueue) & 1, nullptr))
+      item = ctrl->item[slot];
+    else
+      record_status(p.status, MOE_ERR_TIMEOUT);
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(&ctrl->qempty[slot]));
+    return item;
+  };
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      int next = atomicAdd(p.count, 1);
+      for (int n = 0;; ++n) {
+        const int item = next;
+        const bool end = item >= items;
+        if (!end) next = atomicAdd(p.count, 1);
+        const int slot = n % kQueue;
+        if (!mbar_wait(smem_u32(&ctrl->qempty[slot]), ((n / kQueue) & 1) ^ 1, nullptr)) {
+          record_status(p.status, MOE_ERR_TIMEOUT);
+          return;
+        }
+        ctrl->item[slot] = end ? -1 : item;
+        mbar_arrive(smem_u32(&ctrl->qfull[slot]));
+        if (end) return;
+        const Item it = decode(item);
+        const int e = grp[it.g] >> 16;
+        const CUtensorMap* map = it.down ? &map2 : &map1;
+        for (int c = it.c0; c < it.c1; c += BKS) {
+          const uint32_t full = smem_u32(&ctrl->full[stage]);
+          if (!mbar_wait(smem_u32(&ctrl->empty[stage]), phase ^ 1, nullptr)) {
+            record_status(p.status, MOE_ERR_TIMEOUT);
+            return;
+          }
+          mbar_arrive_expect_tx(full, kStageBytes);
+          const uint32_t dst = smem_u32(base + stage * kStageBytes);
+#pragma unroll
+          for (int i = 0; i < C; ++i)
+            tma_load_3d(dst + i * kSliceBytes, map, full, c + 64 * i, it.blk * BM, e);
+          if (++stage == kStages) stage = 0, phase ^= 1;
+        }
+      }
+    }
+    return;
+  }
+
+  const T* x = static_cast<const T*>(p.x);
+  T* h = static_cast<T*>(p.h);
+  T* h_lo = h + int64_t(p.T) * p.k * p.F;
+  if (warp == 1) {
+    // A stage's slots: row nn of slice s at (s NT + nn) * 128, its 16-byte pieces
+    // XOR-ed with nn & 7 like the weights' TMA swizzle.
+    constexpr int kPieces = BKS / 8;              // of 16 bytes in a row
+    constexpr int kPasses = NT * kPieces / 32;
+    uint32_t off[kPasses];
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+      const int nn = (lane + 32 * i) / kPieces, piece = (lane + 32 * i) % kPieces;
+      off[i] = ((piece >> 3) * NT + nn) * 128 + (((piece & 7) ^ (nn & 7)) << 4);
+    }
+    const int piece8 = lane % kPieces * 8;  // (32 is a multiple of kPieces: the same in every pass)
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int n = 0;; ++n) {
+      const int item = pop(n);
+      if (item < 0) return;
+      const Item it = decode(item);
+      const int pos0 = grp[it.g] & 0xffff;
+      const int rows = (it.g + 1 < G ? (grp[it.g + 1] & 0xffff) : S) - pos0;
+      if (it.down) {  // this group's h, complete and visible to this thread
+        const long long t0 = clock64();
+        while (ld_acquire_gpu(ready + it.g) < FB * kConsumers)
+          if (clock64() - t0 > kWaitBudgetCycles) {
+            record_status(p.status, MOE_ERR_TIMEOUT);
+            break;  // carry on with what is there: the pipeline still ends
+          }
+      }
+      const T* src[kPasses];
+#pragma unroll
+      for (int i = 0; i < kPasses; ++i) {
+        const int nn = (lane + 32 * i) / kPieces;
+        src[i] = nullptr;
+        if (nn < rows)
+          src[i] = (it.down ? h + int64_t(pos0 + nn) * p.F
+                            : x + (plan->slot_at[pos0 + nn] / p.k) * p.ldx) +
+                   piece8;
+      }
+      for (int c = it.c0; c < it.c1; c += BKS) {
+        const uint32_t full = smem_u32(&ctrl->full[stage]);
+        if (!mbar_wait(smem_u32(&ctrl->empty[stage]), phase ^ 1, nullptr)) {
+          record_status(p.status, MOE_ERR_TIMEOUT);
+          return;
+        }
+        const uint32_t dst = smem_u32(slots + stage * 2 * K::kSlotBytes);
+        const int bytes = c + piece8 < it.c1 ? 16 : 0;
+        const int from = bytes ? c : it.c0;
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i) {
+          if (i * 32 / kPieces >= rows) break;
+          if (src[i] != nullptr) {
+            copy_async_16(dst + off[i], src[i] + from, bytes);
+            if (it.down) copy_async_16(dst + off[i] + K::kSlotBytes, src[i] + from + (h_lo - h), bytes);
+          }
+        }
+        copies_arrive(full);
+        if (++stage == kStages) stage = 0, phase ^= 1;
+      }
+    }
+  }
+
+  const int set = (warp - 2) / kConsumers, cw = (warp - 2) % kConsumers;
+  const int rt = cw % R, cs = cw / R, g8 = lane >> 2, q4 = lane & 3;
+  const uint32_t a_base = smem_u32(base) + cs * kSliceBytes + (rt * 16 + g8) * 128;
+  const uint32_t b_base = smem_u32(slots) + (cs * NT + g8) * 128;
+  const uint32_t off0 = ((2 * q4) ^ g8) * 16, off1 = ((2 * q4 + 1) ^ g8) * 16;
+  int stage = 0;
+  uint32_t phase = 0;
+  for (int n = 0;; ++n) {
+    const int item = pop(n);
+    if (item < 0) return;
+    const Item it = decode(item);
+    if (n % kSets != set) {  // the other set's item: past its stages
+      stage += (it.c1 - it.c0 + BKS - 1) / BKS;
+      while (stage >= kStages) stage -= kStages, phase ^= 1;
+      continue;
+    }
+    // The other set has used every stage before this item's: a parity wait on a stage
+    // is only sound within one turn of the ring.
+    if (!mbar_wait(smem_u32(&ctrl->turn[set]), ((n / kSets) & 1) ^ (set == 0), nullptr)) {
+      record_status(p.status, MOE_ERR_TIMEOUT);
+      return;
+    }
+    const int pos0 = grp[it.g] & 0xffff;
+    const int rows = (it.g + 1 < G ? (grp[it.g + 1] & 0xffff) : S) - pos0;
+    float acc[J][4];
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[j][i] = 0.0f;
+
+    for (int c = it.c0; c < it.c1; c += BKS) {
+      if (!mbar_wait(smem_u32(&ctrl->full[stage]), phase, nullptr)) {
+        record_status(p.status, MOE_ERR_TIMEOUT);
+        return;
+      }
+      uint32_t a[2][8];  // rows g8 and g8 + 8, 16 columns each
+      const uint32_t sa = a_base + stage * kStageBytes;
+      ld_shared_v4(sa + off0, &a[0][0]);
+      ld_shared_v4(sa + off1, &a[0][4]);
+      ld_shared_v4(sa + 1024 + off0, &a[1][0]);
+      ld_shared_v4(sa + 1024 + off1, &a[1][4]);
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        if (j * 8 < rows) {
+          const uint32_t sb = b_base + stage * 2 * K::kSlotBytes + j * 1024;
+          uint32_t b[8];
+          ld_shared_v4(sb + off0, &b[0]);
+          ld_shared_v4(sb + off1, &b[4]);
+#pragma unroll
+          for (int s = 0; s < 4; ++s)
+            mma<T>(acc[j], a[0][2 * s], a[1][2 * s], a[0][2 * s + 1], a[1][2 * s + 1], b[2 * s],
+                   b[2 * s + 1]);
+          if (it.down) {
+            ld_shared_v4(sb + K::kSlotBytes + off0, &b[0]);
+            ld_shared_v4(sb + K::kSlotBytes + off1, &b[4]);
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+              mma<T>(acc[j], a[0][2 * s], a[1][2 * s], a[0][2 * s + 1], a[1][2 * s + 1], b[2 * s],
+                     b[2 * s + 1]);
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&ctrl->empty[stage]));
+      if (++stage == kStages) stage = 0, phase ^= 1;
+    }
+
+    if (lane == 0) mbar_arrive(smem_u32(&ctrl->turn[set ^ 1]));
+
+    if (!it.down) {
+      auto put_h = [&](int nn, int row, float v) {
+        const float a = 0.5f * v * (1.0f + erff(v * 0.70710678118654752440f));
+        // what is beyond the type's largest value goes to the second part as well
+        const T hi = from_f<T>(fminf(fmaxf(a, -kMaxOf<T>), kMaxOf<T>));
+        h[int64_t(pos0 + nn) * p.F + row] = hi;
+        h_lo[int64_t(pos0 + nn) * p.F + row] = from_f<T>(a - to_f(hi));
+      };
+      if constexpr (C == 1) {
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int nn = j * 8 + 2 * q4 + (i & 1), row = it.blk * BM + rt * 16 + g8 + 8 * (i >> 1);
+            if (nn < rows && row < p.F) put_h(nn, row, acc[j][i]);
+          }
+      } else {  // the C column slices' sums, through shared memory
+        float* rb = red + (set * kConsumers + cw) * (NT * kRedStride);
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            rb[(j * 8 + 2 * q4 + (i & 1)) * kRedStride + g8 + 8 * (i >> 1)] = acc[j][i];
+        set_sync(set);
+        const float* rs = red + set * kConsumers * (NT * kRedStride);
+        for (int o = cw * 32 + lane; o < BM * rows; o += 32 * kConsumers) {
+          const int m = o % BM, nn = o / BM, row = it.blk * BM + m;
+          float v = 0.0f;
+#pragma unroll
+          for (int i = 0; i < C; ++i)
+            v += rs[(i * R + m / 16) * (NT * kRedStride) + nn * kRedStride + m % 16];
+          if (row < p.F) put_h(nn, row, v);
+        }
+        set_sync(set);  // the buffer is free again
+      }
+      __syncwarp();
+      if (lane == 0) red_release_gpu(ready + it.g, 1);
+      continue;
+    }
+
+    // This warp's part of 16 rows of W2; whoever brings the last part of them adds the
+    // slots' parts in a fixed order.
+    const int row16 = it.blk * BM + rt * 16;
+    if (row16 >= p.H) continue;
+    float* part = p.part + (int64_t(it.ks * C + cs) * p.T * p.k + pos0) * p.H + row16;
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int nn = j * 8 + 2 * q4 + (i & 1), m = g8 + 8 * (i >> 1);
+        if (nn < rows && row16 + m < p.H) part[int64_t(nn) * p.H + m] = acc[j][i];
+      }
+    __syncwarp();
+    int before = 0;
+    if (lane == 0) before = add_acq_rel_gpu(done + it.blk * R + rt, 1);
+    before = __shfl_sync(0xffffffffu, before, 0);
+    if (before != G * p.KS * C - 1) continue;
+    const int col = row16 + (lane & 3) * 4;  // 4 columns of 8 tokens at a time (H: multiple of 8)
+    if (col >= p.H) continue;
+    const int64_t part_stride = int64_t(p.T) * p.k * p.H;
+    for (int t = lane >> 2; t < p.T; t += 8) {
+      float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      for (int j = 0; j < p.k; ++j) {
+        const int pos = plan->pos_of[t * p.k + j];
+        if (pos == 0xffff) continue;
+        float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        const float* src = p.part + int64_t(pos) * p.H + col;
+#pragma unroll 4
+        for (int i = 0; i < p.KS * C; ++i) {
+          const float4 u = __ldcg(reinterpret_cast<const float4*>(src + i * part_stride));
+          y.x += u.x, y.y += u.y, y.z += u.z, y.w += u.w;
+        }
+        const float wt = p.w[t * p.k + j];
+        v[0] += wt * y.x, v[1] += wt * y.y, v[2] += wt * y.z, v[3] += wt * y.w;
+      }
+      T o[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] = from_f<T>(v[i]);
+      *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + t * p.ldo + col) =
+          *reinterpret_cast<const uint2*>(o);
+    }
+  }
+}
+
+// Parts of F in W2's items, of about 1024 columns, fewer when there are many slots (then
+// there are many groups, and the parts' sums cost more than their balance gains).
+inline int k_splits(int F, int64_t S) {
+  const int64_t fine = (F + 1023) / 1024, most = S < 1 || S >= 1024 ? 1 : 1024 / S;
+  return static_cast<int>(fine < most ? fine : most);
+}
+
+struct Workspace {
+  int64_t part, count, total;
+  Workspace(int T, int H, int F, int E, int k) {
+    const int64_t S = int64_t(T) * k;
+    part = (S * F * 4 + 15) / 16 * 16;
+    // a variant with column slices splits each part into up to 4
+    count = part + (S * H * 4 * k_splits(F, S) * 4 + 15) / 16 * 16;
+    total = count + 4 * (int64_t(1) + max_groups(1, E) + (H + 15) / 16);
+  }
+  int64_t count_bytes() const { return total - count; }
+};
+
+template <typename T, int R, int J>
+int launch_experts(const Params& p, const void* w1, int64_t w1_se, int64_t w1_sr, const void* w2,
+                   int64_t w2_se, int64_t w2_sr, bool after_gate, int sms, cudaStream_t s) {
+  using K = Cfg<R, J>;
+  CUtensorMap m1, m2;
+  const CUtensorMapDataType dt = std::is_same<T, __nv_bfloat16>::value
+                                     ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                     : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  const uint32_t box[3] = {64, K::BM, 1};
+  const uint64_t d1[3] = {uint64_t(p.H), uint64_t(p.F), uint64_t(p.E)};
+  const uint64_t d2[3] = {uint64_t(p.F), uint64_t(p.H), uint64_t(p.E)};
+  const uint64_t s1[2] = {uint64_t(w1_sr) * 2, uint64_t(p.E > 1 ? w1_se : w1_sr * p.F) * 2};
+  const uint64_t s2[2] = {uint64_t(w2_sr) * 2, uint64_t(p.E > 1 ? w2_se : w2_sr * p.H) * 2};
+  int rc = encode_tiled(&m1, dt, 3, w1, d1, s1, box);
+  if (rc == MOE_OK) rc = encode_tiled(&m2, dt, 3, w2, d2, s2, box);
+  if (rc != MOE_OK) return rc;
+  const int smem = 1024 + K::kBytes + int(sizeof(Ctrl)) + int(sizeof(Plan)) +
+                   4 * (max_groups(J, p.E) + 2 * p.E);
+  static_assert(K::kStages <= 12 && 1024 + K::kBytes + int(sizeof(Ctrl)) + int(sizeof(Plan)) +
+                        4 * (max_groups(J, kMaxE) + 2 * kMaxE) <= 227 * 1024,
+                "shared memory");
+  auto kern = &experts_kernel<T, R, J>;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    return MOE_ERR_CUDA;
+  // No more CTAs than there can be items: every slot in a group of its own.
+  const int64_t most = int64_t(p.T) * p.k * ((p.F + K::BM - 1) / K::BM + (p.H + K::BM - 1) / K::BM * p.KS);
+  const int grid = static_cast<int>(most < sms ? most : sms);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute early{};  // set up beside the gate's kernel
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &early;
+  cfg.numAttrs = after_gate ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kern, m1, m2, p) == cudaSuccess ? MOE_OK : MOE_ERR_CUDA;
 }
 
 template <typename T>
-int launch(const void* x, int64_t ldx, const void* rw, int64_t ldr, const float* bias,
-           const void* w1, int64_t w1_se, int64_t w1_sr, const void* w2, int64_t w2_se,
-           int64_t w2_sr, int T_, int H, int F, int E, int k, int renorm, int64_t* idx, float* w,
-           void* out, int64_t ldo, void* ws, int32_t* status, cudaStream_t s) {
-  const T* xt = static_cast<const T*>(x);
-  if (rw != nullptr)
-    gate_kernel<T><<<T_, 32 * kWarps, 0, s>>>(xt, ldx, static_cast<const T*>(rw), ldr, bias, H, E, k,
-                                              renorm, idx, w);
-  T* h = static_cast<T*>(ws);
-  up_kernel<T><<<dim3((F + kWarps - 1) / kWarps, T_ * k), 32 * kWarps, 0, s>>>(
-      xt, ldx, static_cast<const T*>(w1), w1_se, w1_sr, idx, H, F, E, k, h, status);
-  down_kernel<T><<<dim3((H + kWarps - 1) / kWarps, T_), 32 * kWarps, 0, s>>>(
-      h, static_cast<const T*>(w2), w2_se, w2_sr, idx, w, H, F, E, k, static_cast<T*>(out), ldo);
-  return cudaGetLastError() == cudaSuccess ? MOE_OK : MOE_ERR_CUDA;
+int launch(Params p, const void* rw, int64_t ldr, const float* bias, const void* w1, int64_t w1_se,
+           int64_t w1_sr, const void* w2, int64_t w2_se, int64_t w2_sr, int renorm, int64_t* idx,
+           float* w, void* ws, int sms, cudaStream_t s) {
+  const Workspace lay(p.T, p.H, p.F, p.E, p.k);
+  p.idx = idx;
+  p.w = w;
+  p.h = ws;
+  p.part = reinterpret_cast<float*>(static_cast<char*>(ws) + lay.part);
+  p.count = reinterpret_cast<int32_t*>(static_cast<char*>(ws) + lay.count);
+  p.KS = k_splits(p.F, int64_t(p.T) * p.k);
+  if (rw != nullptr) {
+    gate_kernel<T><<<p.T * kGateCluster, 32 * kWarps, 0, s>>>(
+        static_cast<const T*>(p.x), p.ldx, static_cast<const T*>(rw), ldr, bias, p.H, p.E, p.k, renorm,
+        idx, w, p.count, static_cast<int>(lay.count_bytes() / 4));
+    if (cudaGetLastError() != cudaSuccess) return MOE_ERR_CUDA;
+  } else if (cudaMemsetAsync(p.count, 0, lay.count_bytes(), s) != cudaSuccess) {
+    return MOE_ERR_CUDA;
+  }
+  // Narrow row blocks give a few tokens' few experts enough items for every SM; with
+  // more tokens, blocks of 128 rows need no sums across warps and fetch each slot's
+  // columns once for all 8 (one token of 16 x 2048 x 4096, R = 4 against 8: 32.5 and
+  // 34.1 us; 16 tokens of 16 x 2048 x 8192: 166 and 149 us).
+  return p.T <= 8 ? launch_experts<T, 4, 1>(p, w1, w1_se, w1_sr, w2, w2_se, w2_sr, rw != nullptr, sms, s)
+                  : launch_experts<T, 8, 2>(p, w1, w1_se, w1_sr, w2, w2_se, w2_sr, rw != nullptr, sms, s);
 }
 
 }  // namespace few
@@ -226,7 +797,7 @@ bool rows_ok(const void* p, int64_t ld, int64_t width) {
 extern "C" int64_t moe_few_tokens_workspace(int32_t num_tokens, int32_t hidden, int32_t ffn,
                                             int32_t num_experts, int32_t topk) {
   if (!sizes_ok(num_tokens, hidden, ffn, num_experts, topk)) return -1;
-  return int64_t(num_tokens) * topk * ffn * 2;
+  return moe::few::Workspace(num_tokens, hidden, ffn, num_experts, topk).total;
 }
 
 extern "C" int32_t moe_few_tokens(const void* x, int64_t ldx, const void* router_w, int64_t ldr,
@@ -255,8 +826,11 @@ extern "C" int32_t moe_few_tokens(const void* x, int64_t ldx, const void* router
   const int rc = moe::current_device_info(&dev, &info);
   if (rc != MOE_OK) return rc;
   if (info.major != 10) return MOE_ERR_UNSUPPORTED;
+  moe::few::Params p{};
+  p.x = x, p.ldx = ldx, p.out = out, p.ldo = ldo, p.status = status;
+  p.T = num_tokens, p.H = hidden, p.F = ffn, p.E = num_experts, p.k = topk;
   auto fn = dtype == MOE_DTYPE_BF16 ? &moe::few::launch<__nv_bfloat16> : &moe::few::launch<__half>;
-  return fn(x, ldx, router_w, ldr, router_bias, w1, w1_stride_e, w1_stride_row, w2, w2_stride_e,
-            w2_stride_row, num_tokens, hidden, ffn, num_experts, topk, renormalize, topk_idx,
-            topk_weights, out, ldo, workspace, status, static_cast<cudaStream_t>(stream));
+  return fn(p, router_w, ldr, router_bias, w1, w1_stride_e, w1_stride_row, w2, w2_stride_e,
+            w2_stride_row, renormalize, topk_idx, topk_weights, workspace, info.sm_count,
+            static_cast<cudaStream_t>(stream));
 }
