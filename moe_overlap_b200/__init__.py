@@ -16,6 +16,7 @@ from .gemm import (
 from ._lib import MoeError, check_status
 from .few_tokens import experts_few_tokens, moe_few_tokens
 from .fp8 import dequantize_fp8, quantize_fp8
+from .lora import lora_linear
 from .router import router_topk
 
 __all__ = [
@@ -28,6 +29,7 @@ __all__ = [
     "router_topk",
     "moe_few_tokens",
     "experts_few_tokens",
+    "lora_linear",
     "quantize_fp8",
     "dequantize_fp8",
     "MoeError",

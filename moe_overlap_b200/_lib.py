@@ -194,6 +194,26 @@ SIGNATURES: dict[str, tuple] = {
          _c_void_p, _c_void_p, _c_void_p, _i64,  # topk_idx, topk_weights, out, ldo
          _c_void_p, _i64, _c_void_p, _c_void_p],  # workspace, bytes, status, stream
     ),
+    "moe_lora_plan": (
+        _i32, [_c_void_p, _i32, _i64, _i32, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p]),
+    "moe_lora_shrink": (
+        _i32,
+        [_c_void_p, _i64, _c_void_p, _i64, _i64, _i32,  # x, ldx, w, strides l/row, transposed
+         _c_void_p, _c_void_p, _i32, _i64, _i64, _i32, _i32,  # perm, offs, dtype, m, k, adapters, rank
+         _c_void_p, _c_void_p],  # s, stream
+    ),
+    "moe_lora_expand": (
+        _i32,
+        [_c_void_p, _c_void_p, _i64, _i64, _i32, _c_void_p,  # s, w, strides l/row, transposed, scale
+         _c_void_p, _c_void_p, _i32, _i64, _i64, _i32, _i32,  # perm, offs, dtype, m, n, adapters, rank
+         _c_void_p, _i64, _c_void_p],  # y, ldy, stream
+    ),
+    "moe_lora_grad": (
+        _i32,
+        [_c_void_p, _c_void_p, _i64, _c_void_p,  # s, z, ldz, scale
+         _c_void_p, _c_void_p, _i32, _i64, _i64, _i32, _i32,  # perm, offs, dtype, m, n, adapters, rank
+         _c_void_p, _i64, _i64, _i32, _c_void_p],  # g, strides l/row, transposed, stream
+    ),
     "moe_ep_dispatch_layout": (
         _i32, [_c_void_p, _i32, _i32, _i32, _i32, _c_void_p, _c_void_p, _c_void_p, _c_void_p]),
     "moe_ipc_export": (_i32, [_c_void_p, _c_void_p]),
