@@ -579,7 +579,9 @@ MOE_API int32_t moe_few_tokens(const void* x, int64_t ldx, const void* router_w,
  *                   in perm; base_offs [2]: {0, m}, expert_offsets of the shared
  *                   product.  An id outside [-1, adapters) counts as -1 and records
  *                   MOE_ERR_INVALID_ARG in `status`.
- * moe_lora_shrink   s[p][j] = sum_k x[perm[p]][k] w_i(j, k)                (fp32 [m][rank])
+ * moe_lora_shrink   s[p][j] = sum_k x[perm[p]][k] w_i(j, k), held as two arrays
+ *                   [m][rank] of `dtype`, one behind the other: the rounded value and
+ *                   what the rounding left
  * moe_lora_expand   y[perm[p]][c] += scale[i] sum_j s[p][j] w_i(c, j); other rows stay
  * moe_lora_grad     g_i(c, j) = scale[i] sum_p s[p][j] z[perm[p]][c] over the rows of i,
  *                   zeros for an adapter without rows
@@ -594,13 +596,13 @@ MOE_API int32_t moe_lora_plan(const void* ids, int32_t ids_int64, int64_t m, int
 MOE_API int32_t moe_lora_shrink(const void* x, int64_t ldx, const void* w, int64_t w_stride_l,
                                 int64_t w_stride_row, int32_t w_transposed, const int32_t* perm,
                                 const int32_t* offs, int32_t dtype, int64_t m, int64_t k,
-                                int32_t adapters, int32_t rank, float* s, void* stream);
-MOE_API int32_t moe_lora_expand(const float* s, const void* w, int64_t w_stride_l,
+                                int32_t adapters, int32_t rank, void* s, void* stream);
+MOE_API int32_t moe_lora_expand(const void* s, const void* w, int64_t w_stride_l,
                                 int64_t w_stride_row, int32_t w_transposed, const float* scale,
                                 const int32_t* perm, const int32_t* offs, int32_t dtype, int64_t m,
                                 int64_t n, int32_t adapters, int32_t rank, void* y, int64_t ldy,
                                 void* stream);
-MOE_API int32_t moe_lora_grad(const float* s, const void* z, int64_t ldz, const float* scale,
+MOE_API int32_t moe_lora_grad(const void* s, const void* z, int64_t ldz, const float* scale,
                               const int32_t* perm, const int32_t* offs, int32_t dtype, int64_t m,
                               int64_t n, int32_t adapters, int32_t rank, void* g, int64_t g_stride_l,
                               int64_t g_stride_row, int32_t g_transposed, void* stream);

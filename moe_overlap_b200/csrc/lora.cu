@@ -9,7 +9,8 @@
 //   shrink  s[p] = x[perm[p]] A[i]^T           (also dy B[i], with B read along rows)
 //   expand  y[perm[p]] += scale[i] s[p] B[i]^T (also dx += scale[i] (dy B[i]) A[i])
 //   grad    dB[i] = scale[i] sum_p dy[perm[p]]^T s[p]  (also dA[i])
-// s is held in fp32.
+// s is held as two values of the inputs' type, the rounded one and what the rounding
+// left (16 bits or more in all): the operand of a second tensor-core product.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -41,25 +42,6 @@ __device__ __forceinline__ T from_f(float v) {
   else
     return __float2half_rn(v);
 }
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-
-// Adapter of sorted place p: the last i with offs[i] <= p.
-__device__ __forceinline__ int adapter_of(const int32_t* offs, int L, int p) {
-  int lo = 0, hi = L - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) / 2;
-    if (offs[mid] <= p)
-      lo = mid;
-    else
-      hi = mid - 1;
-  }
-  return lo;
-}
-
 // One block per adapter: it counts the rows of smaller adapters (its segment's start)
 // and writes its own rows in order.  No block depends on another and the order is
 // always the same.
@@ -112,54 +94,528 @@ __global__ void __launch_bounds__(1024) plan_kernel(const void* ids, int ids64, 
   }
 }
 
-// s[p][j] = sum_k x[perm[p]][k] W_i(j, k): one warp an element.  W_i(j, k) is at
-// w + i*sl + j*sr + k, or with kT at w + i*sl + k*sr + j.
-template <typename T, bool kT>
-__global__ void __launch_bounds__(256) shrink_kernel(const T* x, int64_t ldx, const T* w, int64_t sl,
-                                                     int64_t sr, const int32_t* perm,
-                                                     const int32_t* offs, int L, int K, int r, float* s) {
-  const int64_t e = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31, j = static_cast<int>(e % r);
-  const int64_t p = e / r;
-  if (p >= offs[L]) return;
-  const T* xr = x + perm[p] * ldx;
-  const T* wi = w + adapter_of(offs, L, static_cast<int>(p)) * sl;
-  float v = 0.0f;
-  for (int k = lane; k < K; k += 32) v += to_f(xr[k]) * to_f(kT ? wi[k * sr + j] : wi[j * sr + k]);
-  v = warp_sum(v);
-  if (lane == 0) s[p * r + j] = v;
+// ---------------------------------------------------------- tensor-core tiles --
+// All three products move far more bytes than they need arithmetic for at the ranks
+// of adapters, so they run on m16n8k16 from shared memory filled by cp.async: rows
+// are gathered through perm, which whole-tile TMA boxes cannot do.  Rows of shared
+// memory are 16 bytes longer than a multiple of 32, so that ldmatrix meets no bank
+// twice.  RP is the rank rounded up to 16, 32, 64 or 128.
+constexpr int kThreads = 256;
+
+template <typename T>
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <bool kTrans>
+__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
+  if constexpr (kTrans)
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+  else
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+// 16 bytes to shared memory, zeros (and nothing read) unless `in`.
+__device__ __forceinline__ void copy_async_16(uint32_t dst, const void* src, bool in) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kLeft>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory");
+}
+__device__ __forceinline__ float ld_shared_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
 }
 
-// y[perm[p]][n] += scale[i] sum_j s[p][j] W_i(n, j): one thread an element.  W_i(n, j)
-// is at w + i*sl + n*sr + j, or with kT at w + i*sl + j*sr + n.
-template <typename T, bool kT>
-__global__ void __launch_bounds__(256) expand_kernel(const float* s, const T* w, int64_t sl, int64_t sr,
-                                                     const float* scale, const int32_t* perm,
-                                                     const int32_t* offs, int L, int N, int r, T* y,
-                                                     int64_t ldy) {
-  const int n = blockIdx.y * 256 + threadIdx.x;
-  const int p = blockIdx.x;
-  if (p >= offs[L] || n >= N) return;
-  const int i = adapter_of(offs, L, p);
-  const T* wi = w + i * sl;
-  float v = 0.0f;
-  for (int j = 0; j < r; ++j) v += s[int64_t(p) * r + j] * to_f(kT ? wi[j * sr + n] : wi[n * sr + j]);
-  T* at = y + perm[p] * ldy + n;
-  *at = from_f<T>(to_f(*at) + scale[i] * v);
+// Block `tile` of at most TILE rows of one adapter: its adapter (-1: no such block), first
+// place and rows.  Called by a whole CTA; every warp finds it for itself.
+struct Tile {
+  int i, p0, rows;
+};
+__device__ __forceinline__ Tile find_tile(const int32_t* offs, int L, int tile, int TILE) {
+  const int lane = threadIdx.x & 31;
+  Tile t{-1, 0, 0};
+  int before = 0;
+  for (int b = 0; b < L; b += 32) {
+    const int i = b + lane;
+    const int o0 = i < L ? offs[i] : 0, n = i < L ? offs[i + 1] - o0 : 0;
+    const int blocks = (n + TILE - 1) / TILE;
+    int incl = blocks;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    const int k = tile - before - (incl - blocks);  // block of this adapter
+    const unsigned hit = __ballot_sync(0xffffffffu, k >= 0 && k < blocks);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      t.i = b + src;
+      const int kk = __shfl_sync(0xffffffffu, k, src);
+      const int o = __shfl_sync(0xffffffffu, o0, src), nn = __shfl_sync(0xffffffffu, n, src);
+      t.p0 = o + kk * TILE;
+      t.rows = min(TILE, nn - kk * TILE);
+      return t;
+    }
+    before += __shfl_sync(0xffffffffu, incl, 31);
+  }
+  return t;
 }
 
-// g_i(n, j) = scale[i] sum_p s[p][j] z[perm[p]][n] over adapter i's rows (zeros without
-// rows), at g + i*gl + n*gr + j, or with kT at g + i*gl + j*gr + n.
-template <typename T, bool kT>
-__global__ void __launch_bounds__(256) grad_kernel(const float* s, const T* z, int64_t ldz,
-                                                   const float* scale, const int32_t* perm,
-                                                   const int32_t* offs, int n, int r, T* g, int64_t gl,
-                                                   int64_t gr) {
-  const int col = blockIdx.x * 256 + threadIdx.x, j = blockIdx.y, i = blockIdx.z;
-  if (col >= n) return;
-  float v = 0.0f;
-  for (int p = offs[i]; p < offs[i + 1]; ++p) v += s[int64_t(p) * r + j] * to_f(z[perm[p] * ldz + col]);
-  g[i * gl + (kT ? j * gr + col : col * gr + j)] = from_f<T>(scale[i] * v);
+// A value as two of type T: rounded, and what the rounding left (what is beyond the
+// type's largest value goes to the second part as well).
+template <typename T>
+__device__ __forceinline__ void split(float v, T* hi, T* lo) {
+  const float big = std::is_same<T, __nv_bfloat16>::value ? 3.38953139e38f : 65504.0f;
+  *hi = from_f<T>(fminf(fmaxf(v, -big), big));
+  *lo = from_f<T>(v - to_f(*hi));
+}
+
+// shrink.  A CTA forms 128 rows x RP of s over one part of k; the CTAs of a cluster
+// share the rows and add their parts through distributed shared memory, in order.
+// Bound by reading x once (and w once a block of 128 rows).
+constexpr int kShrinkRows = 128;
+constexpr int kShrinkCols = 64;  // of k, a stage
+constexpr int kShrinkPitch = kShrinkCols * 2 + 16;
+
+template <bool kT, int RP>
+struct ShrinkCfg {
+  static constexpr int kW = kT ? kShrinkCols * (RP * 2 + 16) : RP * kShrinkPitch;
+  static constexpr int kStage = kShrinkRows * kShrinkPitch + kW;
+  static constexpr int kStages = RP == 128 ? 3 : 4;
+  static constexpr int kBytes = kStages * kStage;
+  static_assert(kShrinkRows * (RP + 4) * 4 <= kBytes, "the sums reuse the stages");
+};
+
+template <typename T, bool kT, int RP>
+__global__ void __launch_bounds__(kThreads, 2)
+    shrink_kernel(const T* x, int64_t ldx, const T* w, int64_t sl, int64_t sr, const int32_t* perm,
+                  const int32_t* offs, int L, int K, int r, int64_t part_stride, T* s) {
+  using C = ShrinkCfg<kT, RP>;
+  extern __shared__ __align__(128) char smem[];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const Tile t = find_tile(offs, L, blockIdx.x, kShrinkRows);
+  if (t.i < 0) return;  // the same in every CTA of the cluster
+  const int parts = gridDim.y, part = blockIdx.y;
+  const int cols = ((K + parts - 1) / parts + kShrinkCols - 1) / kShrinkCols * kShrinkCols;
+  const int k0 = min(K, part * cols), k1 = min(K, k0 + cols);
+  const int steps = (k1 - k0 + kShrinkCols - 1) / kShrinkCols;
+  const T* wi = w + t.i * sl;
+  const T* row[4];  // the rows that this thread copies: tid / 8 + 32 q
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int m = tid / 8 + 32 * q;
+    row[q] = m < t.rows ? x + perm[t.p0 + m] * ldx : nullptr;
+  }
+  auto fetch = [&](int step) {
+    if (step < steps) {
+      const uint32_t xs = smem_u32(smem) + (step % C::kStages) * C::kStage;
+      const uint32_t ws = xs + kShrinkRows * kShrinkPitch;
+      const int c = k0 + step * kShrinkCols, k = c + (tid & 7) * 8;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const bool in = row[q] != nullptr && k < k1;
+        copy_async_16(xs + (tid / 8 + 32 * q) * kShrinkPitch + (tid & 7) * 16, in ? row[q] + k : x, in);
+      }
+      if constexpr (kT) {
+        for (int e = tid; e < kShrinkCols * (RP / 8); e += kThreads) {
+          const int kk = e / (RP / 8), j = e % (RP / 8) * 8;
+          const bool in = c + kk < k1 && j < r;
+          copy_async_16(ws + kk * (RP * 2 + 16) + j * 2, in ? wi + int64_t(c + kk) * sr + j : w, in);
+        }
+      } else {
+        for (int e = tid; e < RP * 8; e += kThreads) {
+          const int j = e / 8;
+          const bool in = j < r && k < k1;
+          copy_async_16(ws + j * kShrinkPitch + (tid & 7) * 16, in ? wi + j * sr + k : w, in);
+        }
+      }
+    }
+    copies_commit();
+  };
+  float acc[RP / 8][4];
+#pragma unroll
+  for (int n = 0; n < RP / 8; ++n)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) acc[n][q] = 0.0f;
+#pragma unroll
+  for (int q = 0; q < C::kStages - 1; ++q) fetch(q);
+  for (int step = 0; step < steps; ++step) {
+    copies_wait<C::kStages - 2>();
+    __syncthreads();
+    fetch(step + C::kStages - 1);
+    const uint32_t xs = smem_u32(smem) + (step % C::kStages) * C::kStage;
+    const uint32_t ws = xs + kShrinkRows * kShrinkPitch;
+#pragma unroll
+    for (int kk = 0; kk < kShrinkCols; kk += 16) {
+      uint32_t a[4];
+      ldmatrix_x4<false>(a, xs + (warp * 16 + (lane & 15)) * kShrinkPitch + (kk + (lane >> 4) * 8) * 2);
+#pragma unroll
+      for (int n = 0; n < RP / 8; n += 2) {
+        uint32_t b[4];
+        if constexpr (kT)
+          ldmatrix_x4<true>(b, ws + (kk + (lane & 15)) * (RP * 2 + 16) + (n + (lane >> 4)) * 16);
+        else
+          ldmatrix_x4<false>(b, ws + (n * 8 + (lane >> 4) * 8 + (lane & 7)) * kShrinkPitch +
+                                    (kk + ((lane >> 3) & 1) * 8) * 2);
+        mma<T>(acc[n], a, b[0], b[1]);
+        mma<T>(acc[n + 1], a, b[2], b[3]);
+      }
+    }
+  }
+  copies_wait<0>();
+  __syncthreads();
+  constexpr int kPitch = RP + 4;
+  float* sums = reinterpret_cast<float*>(smem);
+#pragma unroll
+  for (int n = 0; n < RP / 8; ++n)
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      sums[(warp * 16 + (lane >> 2) + 8 * (q >> 1)) * kPitch + n * 8 + (lane & 3) * 2 + (q & 1)] = acc[n][q];
+  if (parts > 1)
+    cluster_sync_all();
+  else
+    __syncthreads();
+  const int share = kShrinkRows / parts;  // rows that this CTA finishes
+  for (int e = tid; e < share * r; e += kThreads) {
+    const int m = part * share + e / r, j = e % r;
+    if (m >= t.rows) break;
+    float v = 0.0f;
+    if (parts > 1) {
+      const uint32_t at = smem_u32(sums + m * kPitch + j);
+      for (int q = 0; q < parts; ++q) v += ld_shared_cluster(mapa_shared(at, q));
+    } else {
+      v = sums[m * kPitch + j];
+    }
+    T* out = s + int64_t(t.p0 + m) * r + j;
+    split(v, out, out + part_stride);
+  }
+  if (parts > 1) cluster_sync_all();  // no CTA leaves while another reads its sums
+}
+
+// expand.  A CTA holds 64 rows of s in registers (both parts) and runs over blocks of
+// 256 columns: 4 groups of 16 rows x 2 halves of 128 columns, one per warp.  Bound by
+// reading and writing y; y's 16-byte pieces are loaded before the products.  For W in
+// rows of n the columns are placed so that a lane's results of 4 column tiles are 8
+// neighbours; read along n they go through a patch of shared memory for that.
+constexpr int kExpandRows = 64;
+constexpr int kExpandCols = 256;
+constexpr int kPatchPitch = 36;  // floats
+
+template <bool kT, int RP>
+struct ExpandCfg {
+  static constexpr int kW = kT ? RP * (kExpandCols * 2 + 16) : kExpandCols * (RP * 2 + 16);
+  static constexpr int kPatch = kT ? 8 * 16 * kPatchPitch * 4 : 0;
+  static constexpr int kBytes = kW + kPatch;
+};
+
+template <typename T, bool kT, int RP>
+__global__ void __launch_bounds__(kThreads, RP == 128 ? 1 : 2)
+    expand_kernel(const T* s, int64_t part_stride, const T* w, int64_t sl, int64_t sr,
+                  const float* scale, const int32_t* perm, const int32_t* offs, int L, int N, int r,
+                  T* y, int64_t ldy) {
+  using C = ExpandCfg<kT, RP>;
+  extern __shared__ __align__(128) char smem[];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, q4 = lane & 3;
+  const Tile t = find_tile(offs, L, blockIdx.x, kExpandRows);
+  if (t.i < 0) return;
+  const int mg = warp & 3, half = warp >> 2;
+  const T* wi = w + t.i * sl;
+  const float c = scale[t.i];
+  // A fragments straight from s: rows mg*16 + g8 and + 8, pairs of columns.
+  uint32_t a[2][RP / 16][4];
+  int64_t yrow[2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int m = mg * 16 + g8 + 8 * u;
+    yrow[u] = m < t.rows ? perm[t.p0 + m] * ldy : -1;
+#pragma unroll
+    for (int k = 0; k < RP / 16; ++k)
+#pragma unroll
+      for (int v = 0; v < 2; ++v) {
+        const int j = k * 16 + v * 8 + q4 * 2;
+        const bool in = m < t.rows && j < r;
+        const T* at = s + int64_t(t.p0 + m) * r + j;
+        a[0][k][u + 2 * v] = in ? *reinterpret_cast<const uint32_t*>(at) : 0u;
+        a[1][k][u + 2 * v] = in ? *reinterpret_cast<const uint32_t*>(at + part_stride) : 0u;
+      }
+  }
+  for (int n0 = blockIdx.y * kExpandCols; n0 < N; n0 += gridDim.y * kExpandCols) {
+    const uint32_t ws = smem_u32(smem);
+    if constexpr (kT) {
+      for (int e = tid; e < RP * (kExpandCols / 8); e += kThreads) {
+        const int j = e / (kExpandCols / 8), n = e % (kExpandCols / 8) * 8;
+        const bool in = j < r && n0 + n < N;
+        copy_async_16(ws + j * (kExpandCols * 2 + 16) + n * 2, in ? wi + j * sr + n0 + n : w, in);
+      }
+    } else {
+      for (int e = tid; e < kExpandCols * (RP / 8); e += kThreads) {
+        const int n = e / (RP / 8), j = e % (RP / 8) * 8;
+        // column 8 q + 2 t + o of a group of 32 goes to row 8 t + 2 q + o
+        const int at = (n & ~31) + ((n >> 1) & 3) * 8 + ((n >> 3) & 3) * 2 + (n & 1);
+        const bool in = j < r && n0 + n < N;
+        copy_async_16(ws + at * (RP * 2 + 16) + j * 2, in ? wi + (n0 + n) * sr + j : w, in);
+      }
+    }
+    copies_commit();
+    uint4 yv[4][2];  // 4 groups of 32 columns, 8 of them a lane
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int n = n0 + half * 128 + g * 32 + q4 * 8;
+        if (yrow[u] >= 0 && n < N) yv[g][u] = *reinterpret_cast<const uint4*>(y + yrow[u] + n);
+      }
+    copies_wait<0>();
+    __syncthreads();
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      float acc[4][4];
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) acc[n][q] = 0.0f;
+      const int col = half * 128 + g * 32;
+#pragma unroll
+      for (int k = 0; k < RP / 16; ++k)
+#pragma unroll
+        for (int n = 0; n < 4; n += 2) {
+          uint32_t b[4];
+          if constexpr (kT)
+            ldmatrix_x4<true>(b, ws + (k * 16 + (lane & 15)) * (kExpandCols * 2 + 16) +
+                                     (col + (n + (lane >> 4)) * 8) * 2);
+          else
+            ldmatrix_x4<false>(b, ws + (col + n * 8 + (lane >> 4) * 8 + (lane & 7)) * (RP * 2 + 16) +
+                                      (k * 16 + ((lane >> 3) & 1) * 8) * 2);
+#pragma unroll
+          for (int part = 0; part < 2; ++part) {
+            mma<T>(acc[n], a[part][k], b[0], b[1]);
+            mma<T>(acc[n + 1], a[part][k], b[2], b[3]);
+          }
+        }
+      float add[2][8];  // this lane's 8 neighbouring columns of its two rows
+      if constexpr (kT) {
+        float* patch = reinterpret_cast<float*>(smem + C::kW) + warp * 16 * kPatchPitch;
+        __syncwarp();
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+            *reinterpret_cast<float2*>(patch + (g8 + 8 * u) * kPatchPitch + n * 8 + q4 * 2) =
+                make_float2(acc[n][2 * u], acc[n][2 * u + 1]);
+        __syncwarp();
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int v = 0; v < 2; ++v)
+            *reinterpret_cast<float4*>(&add[u][4 * v]) =
+                *reinterpret_cast<const float4*>(patch + (g8 + 8 * u) * kPatchPitch + q4 * 8 + 4 * v);
+      } else {
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) add[q >> 1][2 * n + (q & 1)] = acc[n][q];
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int n = n0 + col + q4 * 8;
+        if (yrow[u] < 0 || n >= N) continue;
+        T* v = reinterpret_cast<T*>(&yv[g][u]);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] = from_f<T>(to_f(v[q]) + c * add[u][q]);
+        *reinterpret_cast<uint4*>(y + yrow[u] + n) = yv[g][u];
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// grad.  A CTA forms 128 MT columns of z x RP of one adapter's gradient over one part
+// of its rows, 32 at a time: z^T by ldmatrix.trans as the 16-row side, s as the
+// 8-column side.  The CTAs of a cluster take the parts of the rows and add their sums
+// through distributed shared memory, in order.  Bound by reading z once.
+constexpr int kGradRows = 32;
+
+template <int RP>
+struct GradCfg {
+  static constexpr int MT = RP == 128 ? 1 : 2;  // 16-column tiles of z a warp
+  static constexpr int kCols = 128 * MT;
+  static constexpr int kZPitch = kCols * 2 + 16, kSPitch = RP * 2 + 16;
+  static constexpr int kStage = kGradRows * (kZPitch + 2 * kSPitch);
+  static constexpr int kStages = 4;
+  static constexpr int kSums = kCols * (RP + 4) * 4;
+  static constexpr int kBytes = kStages * kStage > kSums ? kStages * kStage : kSums;
+};
+
+template <typename T, bool kT, int RP>
+__global__ void __launch_bounds__(kThreads, 2)
+    grad_kernel(const T* s, int64_t part_stride, const T* z, int64_t ldz, const float* scale,
+                const int32_t* perm, const int32_t* offs, int n, int r, T* g, int64_t gl, int64_t gr) {
+  using C = GradCfg<RP>;
+  constexpr int MT = C::MT;
+  extern __shared__ __align__(128) char smem[];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int parts = gridDim.x, part = blockIdx.x, n0 = blockIdx.y * C::kCols, i = blockIdx.z;
+  const int o0 = offs[i], rows = offs[i + 1] - o0;
+  const int share = ((rows + parts - 1) / parts + kGradRows - 1) / kGradRows * kGradRows;
+  const int p0 = min(rows, part * share), p1 = min(rows, p0 + share);
+  const int steps = (p1 - p0 + kGradRows - 1) / kGradRows;
+  auto fetch = [&](int step) {
+    if (step < steps) {
+      const uint32_t zs = smem_u32(smem) + (step % C::kStages) * C::kStage;
+      const uint32_t ss = zs + kGradRows * C::kZPitch;
+      const int p = p0 + step * kGradRows;
+      constexpr int kPieces = C::kCols / 8;
+#pragma unroll
+      for (int q = 0; q < kGradRows * kPieces / kThreads; ++q) {
+        const int e = tid + q * kThreads, m = e / kPieces, c = e % kPieces * 8;
+        const bool in = p + m < p1 && n0 + c < n;
+        copy_async_16(zs + m * C::kZPitch + c * 2, in ? z + perm[o0 + p + m] * ldz + n0 + c : z, in);
+      }
+      for (int e = tid; e < kGradRows * (RP / 8) * 2; e += kThreads) {
+        const int half = e / (kGradRows * (RP / 8)), f = e % (kGradRows * (RP / 8));
+        const int m = f / (RP / 8), j = f % (RP / 8) * 8;
+        const bool in = p + m < p1 && j < r;
+        copy_async_16(ss + (half * kGradRows + m) * C::kSPitch + j * 2,
+                      in ? s + half * part_stride + int64_t(o0 + p + m) * r + j : s, in);
+      }
+    }
+    copies_commit();
+  };
+  float acc[MT][RP / 8][4];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int k = 0; k < RP / 8; ++k)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) acc[m][k][q] = 0.0f;
+#pragma unroll
+  for (int q = 0; q < C::kStages - 1; ++q) fetch(q);
+  for (int step = 0; step < steps; ++step) {
+    copies_wait<C::kStages - 2>();
+    __syncthreads();
+    fetch(step + C::kStages - 1);
+    const uint32_t zs = smem_u32(smem) + (step % C::kStages) * C::kStage;
+    const uint32_t ss = zs + kGradRows * C::kZPitch;
+#pragma unroll
+    for (int kk = 0; kk < kGradRows; kk += 16) {
+      uint32_t a[MT][4];
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+        ldmatrix_x4<true>(a[m], zs + (kk + (lane & 7) + (lane >> 4) * 8) * C::kZPitch +
+                                    ((warp * MT + m) * 16 + ((lane >> 3) & 1) * 8) * 2);
+#pragma unroll
+      for (int k = 0; k < RP / 8; k += 2)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          uint32_t b[4];
+          ldmatrix_x4<true>(b, ss + (half * kGradRows + kk + (lane & 15)) * C::kSPitch +
+                                   (k + (lane >> 4)) * 16);
+#pragma unroll
+          for (int m = 0; m < MT; ++m) {
+            mma<T>(acc[m][k], a[m], b[0], b[1]);
+            mma<T>(acc[m][k + 1], a[m], b[2], b[3]);
+          }
+        }
+    }
+  }
+  copies_wait<0>();
+  __syncthreads();
+  constexpr int kPitch = RP + 4;
+  float* sums = reinterpret_cast<float*>(smem);
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int k = 0; k < RP / 8; ++k)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        sums[((warp * MT + m) * 16 + (lane >> 2) + 8 * (q >> 1)) * kPitch + k * 8 + (lane & 3) * 2 + (q & 1)] =
+            acc[m][k][q];
+  if (parts > 1)
+    cluster_sync_all();
+  else
+    __syncthreads();
+  const float c = scale[i];
+  const int cols = C::kCols / parts;  // that this CTA finishes
+  for (int e = tid; e < cols * r; e += kThreads) {
+    const int col = part * cols + (kT ? e % cols : e / r), j = kT ? e / cols : e % r;
+    if (n0 + col >= n) continue;
+    float v = 0.0f;
+    if (parts > 1) {
+      const uint32_t at = smem_u32(sums + col * kPitch + j);
+      for (int q = 0; q < parts; ++q) v += ld_shared_cluster(mapa_shared(at, q));
+    } else {
+      v = sums[col * kPitch + j];
+    }
+    g[i * gl + (kT ? j * gr + n0 + col : (n0 + col) * gr + j)] = from_f<T>(c * v);
+  }
+  if (parts > 1) cluster_sync_all();
+}
+
+template <typename K, typename... A>
+int launch(K kern, dim3 grid, dim3 cluster, int smem, cudaStream_t stream, A... args) {
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    return MOE_ERR_CUDA;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = cluster.x;
+  attr.val.clusterDim.y = cluster.y;
+  attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = cluster.x * cluster.y > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kern, args...) == cudaSuccess ? MOE_OK : MOE_ERR_CUDA;
+}
+
+// Calls fn(T(), transposed, RP) with the compile-time values for this call.
+template <typename Fn>
+int dispatch(int dtype, bool transposed, int rank, Fn fn) {
+  auto by_rank = [&](auto t, auto tr) {
+    if (rank <= 16) return fn(t, tr, std::integral_constant<int, 16>());
+    if (rank <= 32) return fn(t, tr, std::integral_constant<int, 32>());
+    if (rank <= 64) return fn(t, tr, std::integral_constant<int, 64>());
+    return fn(t, tr, std::integral_constant<int, 128>());
+  };
+  auto by_layout = [&](auto t) {
+    return transposed ? by_rank(t, std::true_type()) : by_rank(t, std::false_type());
+  };
+  return dtype == MOE_DTYPE_BF16 ? by_layout(__nv_bfloat16()) : by_layout(__half());
+}
+
+// The most blocks of `tile` rows that m rows of `adapters` adapters can make.
+inline int64_t most_tiles(int64_t m, int adapters, int tile) {
+  const int64_t t = (m + tile - 1) / tile + adapters;
+  return t < m ? t : m;
+}
+// A power of two up to 8 that brings `blocks` to about two CTAs an SM, while each part
+// keeps at least `least` of `length`.
+inline int cluster_parts(int64_t blocks, int64_t length, int64_t least) {
+  int parts = 1;
+  while (parts < 8 && blocks * parts < 296 && length / (parts * 2) >= least) parts *= 2;
+  return parts;
 }
 
 }  // namespace lora
@@ -199,28 +655,28 @@ extern "C" int32_t moe_lora_plan(const void* ids, int32_t ids_int64, int64_t m, 
 extern "C" int32_t moe_lora_shrink(const void* x, int64_t ldx, const void* w, int64_t w_stride_l,
                                    int64_t w_stride_row, int32_t w_transposed, const int32_t* perm,
                                    const int32_t* offs, int32_t dtype, int64_t m, int64_t k,
-                                   int32_t adapters, int32_t rank, float* s, void* stream) {
+                                   int32_t adapters, int32_t rank, void* s, void* stream) {
   if (!dims_ok(dtype, m, k, adapters, rank)) return MOE_ERR_INVALID_ARG;
   if (m == 0) return MOE_OK;
   if (!rows_ok(x, ldx, k) || perm == nullptr || offs == nullptr || s == nullptr || !aligned16(s) ||
       !(w_transposed ? weights_ok(w, w_stride_l, w_stride_row, k, rank, adapters)
                      : weights_ok(w, w_stride_l, w_stride_row, rank, k, adapters)))
     return MOE_ERR_INVALID_ARG;
-  auto go = [&](auto t, auto tr) {
+  return lora::dispatch(dtype, w_transposed != 0, rank, [&](auto t, auto tr, auto rp) {
     using T = decltype(t);
-    lora::shrink_kernel<T, decltype(tr)::value>
-        <<<static_cast<unsigned>((m * rank + 7) / 8), 256, 0, static_cast<cudaStream_t>(stream)>>>(
-            static_cast<const T*>(x), ldx, static_cast<const T*>(w), w_stride_l, w_stride_row, perm,
-            offs, adapters, static_cast<int>(k), rank, s);
-  };
-  if (dtype == MOE_DTYPE_BF16)
-    w_transposed ? go(__nv_bfloat16(), std::true_type()) : go(__nv_bfloat16(), std::false_type());
-  else
-    w_transposed ? go(__half(), std::true_type()) : go(__half(), std::false_type());
-  return launched();
+    constexpr bool kT = decltype(tr)::value;
+    constexpr int RP = decltype(rp)::value;
+    const unsigned tiles = static_cast<unsigned>(lora::most_tiles(m, adapters, lora::kShrinkRows));
+    const unsigned parts = lora::cluster_parts(tiles, k, 256);
+    return lora::launch(lora::shrink_kernel<T, kT, RP>, dim3(tiles, parts), dim3(1, parts),
+                        lora::ShrinkCfg<kT, RP>::kBytes, static_cast<cudaStream_t>(stream),
+                        static_cast<const T*>(x), ldx, static_cast<const T*>(w), w_stride_l,
+                        w_stride_row, perm, offs, static_cast<int>(adapters), static_cast<int>(k),
+                        static_cast<int>(rank), m * rank, static_cast<T*>(s));
+  });
 }
 
-extern "C" int32_t moe_lora_expand(const float* s, const void* w, int64_t w_stride_l,
+extern "C" int32_t moe_lora_expand(const void* s, const void* w, int64_t w_stride_l,
                                    int64_t w_stride_row, int32_t w_transposed, const float* scale,
                                    const int32_t* perm, const int32_t* offs, int32_t dtype, int64_t m,
                                    int64_t n, int32_t adapters, int32_t rank, void* y, int64_t ldy,
@@ -232,22 +688,23 @@ extern "C" int32_t moe_lora_expand(const float* s, const void* w, int64_t w_stri
       !(w_transposed ? weights_ok(w, w_stride_l, w_stride_row, rank, n, adapters)
                      : weights_ok(w, w_stride_l, w_stride_row, n, rank, adapters)))
     return MOE_ERR_INVALID_ARG;
-  auto go = [&](auto t, auto tr) {
+  return lora::dispatch(dtype, w_transposed != 0, rank, [&](auto t, auto tr, auto rp) {
     using T = decltype(t);
-    lora::expand_kernel<T, decltype(tr)::value>
-        <<<dim3(static_cast<unsigned>(m), static_cast<unsigned>((n + 255) / 256)), 256, 0,
-           static_cast<cudaStream_t>(stream)>>>(s, static_cast<const T*>(w), w_stride_l, w_stride_row,
-                                                scale, perm, offs, adapters, static_cast<int>(n), rank,
-                                                static_cast<T*>(y), ldy);
-  };
-  if (dtype == MOE_DTYPE_BF16)
-    w_transposed ? go(__nv_bfloat16(), std::true_type()) : go(__nv_bfloat16(), std::false_type());
-  else
-    w_transposed ? go(__half(), std::true_type()) : go(__half(), std::false_type());
-  return launched();
+    constexpr bool kT = decltype(tr)::value;
+    constexpr int RP = decltype(rp)::value;
+    const int64_t tiles = lora::most_tiles(m, adapters, lora::kExpandRows);
+    const int64_t blocks = (n + lora::kExpandCols - 1) / lora::kExpandCols;
+    const int64_t want = (1200 + tiles - 1) / tiles;  // about four CTAs a place on the SMs
+    return lora::launch(lora::expand_kernel<T, kT, RP>,
+                        dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(want < blocks ? want : blocks)),
+                        dim3(1, 1), lora::ExpandCfg<kT, RP>::kBytes, static_cast<cudaStream_t>(stream),
+                        static_cast<const T*>(s), m * rank, static_cast<const T*>(w), w_stride_l,
+                        w_stride_row, scale, perm, offs, static_cast<int>(adapters), static_cast<int>(n),
+                        static_cast<int>(rank), static_cast<T*>(y), ldy);
+  });
 }
 
-extern "C" int32_t moe_lora_grad(const float* s, const void* z, int64_t ldz, const float* scale,
+extern "C" int32_t moe_lora_grad(const void* s, const void* z, int64_t ldz, const float* scale,
                                  const int32_t* perm, const int32_t* offs, int32_t dtype, int64_t m,
                                  int64_t n, int32_t adapters, int32_t rank, void* g, int64_t g_stride_l,
                                  int64_t g_stride_row, int32_t g_transposed, void* stream) {
@@ -257,17 +714,16 @@ extern "C" int32_t moe_lora_grad(const float* s, const void* z, int64_t ldz, con
       !(g_transposed ? weights_ok(g, g_stride_l, g_stride_row, rank, n, adapters)
                      : weights_ok(g, g_stride_l, g_stride_row, n, rank, adapters)))
     return MOE_ERR_INVALID_ARG;
-  auto go = [&](auto t, auto tr) {
+  return lora::dispatch(dtype, g_transposed != 0, rank, [&](auto t, auto tr, auto rp) {
     using T = decltype(t);
-    lora::grad_kernel<T, decltype(tr)::value>
-        <<<dim3(static_cast<unsigned>((n + 255) / 256), rank, adapters), 256, 0,
-           static_cast<cudaStream_t>(stream)>>>(s, static_cast<const T*>(z), ldz, scale, perm, offs,
-                                                static_cast<int>(n), rank, static_cast<T*>(g),
-                                                g_stride_l, g_stride_row);
-  };
-  if (dtype == MOE_DTYPE_BF16)
-    g_transposed ? go(__nv_bfloat16(), std::true_type()) : go(__nv_bfloat16(), std::false_type());
-  else
-    g_transposed ? go(__half(), std::true_type()) : go(__half(), std::false_type());
-  return launched();
+    constexpr bool kT = decltype(tr)::value;
+    constexpr int RP = decltype(rp)::value;
+    using C = lora::GradCfg<RP>;
+    const unsigned blocks = static_cast<unsigned>((n + C::kCols - 1) / C::kCols);
+    const unsigned parts = lora::cluster_parts(int64_t(blocks) * adapters, m / adapters, 64);
+    return lora::launch(lora::grad_kernel<T, kT, RP>, dim3(parts, blocks, adapters), dim3(parts, 1),
+                        C::kBytes, static_cast<cudaStream_t>(stream), static_cast<const T*>(s), m * rank,
+                        static_cast<const T*>(z), ldz, scale, perm, offs, static_cast<int>(n),
+                        static_cast<int>(rank), static_cast<T*>(g), g_stride_l, g_stride_row);
+  });
 }

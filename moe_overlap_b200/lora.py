@@ -66,7 +66,7 @@ def _shared(x, w, stride_k, stride_n, n, plan):
 
 def _shrink(x, w, transposed, plan, rank):
     m, k = x.shape
-    s = torch.empty(m, rank, dtype=torch.float32, device=x.device)
+    s = torch.empty(2, m, rank, dtype=x.dtype, device=x.device)
     rc = _lib.load().moe_lora_shrink(x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), w.stride(1),
                                      int(transposed), plan.perm.data_ptr(), plan.offs.data_ptr(),
                                      _DTYPE_CODE[x.dtype], m, k, w.shape[0], rank, s.data_ptr(),
@@ -80,7 +80,7 @@ def _expand(s, w, transposed, scale, plan, y):
     rc = _lib.load().moe_lora_expand(s.data_ptr(), w.data_ptr(), w.stride(0), w.stride(1),
                                      int(transposed), scale.data_ptr(), plan.perm.data_ptr(),
                                      plan.offs.data_ptr(), _DTYPE_CODE[y.dtype], m, n, w.shape[0],
-                                     s.shape[1], y.data_ptr(), y.stride(0), _lib.stream_handle(y.device))
+                                     s.shape[2], y.data_ptr(), y.stride(0), _lib.stream_handle(y.device))
     _lib.check_call(rc, "moe_lora_expand")
 
 
@@ -89,7 +89,7 @@ def _grad(s, z, scale, plan, like, transposed):
     m, n = z.shape
     rc = _lib.load().moe_lora_grad(s.data_ptr(), z.data_ptr(), z.stride(0), scale.data_ptr(),
                                    plan.perm.data_ptr(), plan.offs.data_ptr(), _DTYPE_CODE[z.dtype],
-                                   m, n, like.shape[0], s.shape[1], g.data_ptr(), g.stride(0),
+                                   m, n, like.shape[0], s.shape[2], g.data_ptr(), g.stride(0),
                                    g.stride(1), int(transposed), _lib.stream_handle(z.device))
     _lib.check_call(rc, "moe_lora_grad")
     return g
@@ -175,8 +175,8 @@ def lora_linear(x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor, lor
     at a later call.  ``scale`` is a number or a float tensor [L].
 
     Differentiable in ``x``, ``lora_a`` and ``lora_b`` (sums in fp32, the gradients in
-    the inputs' type; the two products of rank r are held in fp32 between them); the
-    shared weight is frozen.  Sizes that are not multiples of 8, and rows that do not
+    the inputs' type; the product of rank r between the two is held in two parts of that
+    type); the shared weight is frozen.  Sizes that are not multiples of 8, and rows that do not
     start on 16 bytes, are copied with padding on every call.
 
     A training step can be captured into a CUDA graph (forward and backward together);
