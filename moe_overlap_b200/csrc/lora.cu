@@ -100,7 +100,8 @@ __global__ void __launch_bounds__(1024) plan_kernel(const void* ids, int ids64, 
 // are gathered through perm, which whole-tile TMA boxes cannot do.  Rows of shared
 // memory are 16 bytes longer than a multiple of 32, so that ldmatrix meets no bank
 // twice.  RP is the rank rounded up to 16, 32, 64 or 128.
-constexpr int kThreads = 256;
+constexpr int kThreads = 256;        // expand and grad
+constexpr int kShrinkThreads = 128;  // 4 warps of 32 rows: each reads all of w's tile from shared memory
 
 template <typename T>
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -140,10 +141,24 @@ template <int kLeft>
 __device__ __forceinline__ void copies_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory");
 }
-__device__ __forceinline__ float ld_shared_cluster(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  return v;
+// The sum over the cluster's CTAs, in their order, of 4 floats at this CTA's address
+// `at`; every CTA's load is under way before the first is used.
+__device__ __forceinline__ float4 cluster_sum4(const float* at, int parts) {
+  if (parts == 1) return *reinterpret_cast<const float4*>(at);
+  const uint32_t mine = smem_u32(at);
+  float4 v[8];
+#pragma unroll
+  for (int q = 0; q < 8; ++q)
+    if (q < parts)
+      asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+                   : "=f"(v[q].x), "=f"(v[q].y), "=f"(v[q].z), "=f"(v[q].w)
+                   : "r"(mapa_shared(mine, q))
+                   : "memory");
+  float4 s = v[0];
+#pragma unroll
+  for (int q = 1; q < 8; ++q)
+    if (q < parts) s.x += v[q].x, s.y += v[q].y, s.z += v[q].z, s.w += v[q].w;
+  return s;
 }
 
 // Block `tile` of at most TILE rows of one adapter: its adapter (-1: no such block), first
@@ -207,7 +222,7 @@ struct ShrinkCfg {
 };
 
 template <typename T, bool kT, int RP>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kShrinkThreads, 2)
     shrink_kernel(const T* x, int64_t ldx, const T* w, int64_t sl, int64_t sr, const int32_t* perm,
                   const int32_t* offs, int L, int K, int r, int64_t part_stride, T* s) {
   using C = ShrinkCfg<kT, RP>;
@@ -220,10 +235,11 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int k0 = min(K, part * cols), k1 = min(K, k0 + cols);
   const int steps = (k1 - k0 + kShrinkCols - 1) / kShrinkCols;
   const T* wi = w + t.i * sl;
-  const T* row[4];  // the rows that this thread copies: tid / 8 + 32 q
+  constexpr int kRowSteps = kShrinkThreads / 8;  // rows that all threads copy at a time
+  const T* row[kShrinkRows / kRowSteps];
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const int m = tid / 8 + 32 * q;
+  for (int q = 0; q < kShrinkRows / kRowSteps; ++q) {
+    const int m = tid / 8 + kRowSteps * q;
     row[q] = m < t.rows ? x + perm[t.p0 + m] * ldx : nullptr;
   }
   auto fetch = [&](int step) {
@@ -232,19 +248,22 @@ __global__ void __launch_bounds__(kThreads, 2)
       const uint32_t ws = xs + kShrinkRows * kShrinkPitch;
       const int c = k0 + step * kShrinkCols, k = c + (tid & 7) * 8;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
+      for (int q = 0; q < kShrinkRows / kRowSteps; ++q) {
         const bool in = row[q] != nullptr && k < k1;
-        copy_async_16(xs + (tid / 8 + 32 * q) * kShrinkPitch + (tid & 7) * 16, in ? row[q] + k : x, in);
+        copy_async_16(xs + (tid / 8 + kRowSteps * q) * kShrinkPitch + (tid & 7) * 16,
+                      in ? row[q] + k : x, in);
       }
       if constexpr (kT) {
-        for (int e = tid; e < kShrinkCols * (RP / 8); e += kThreads) {
-          const int kk = e / (RP / 8), j = e % (RP / 8) * 8;
+#pragma unroll
+        for (int q = 0; q < kShrinkCols * (RP / 8) / kShrinkThreads; ++q) {
+          const int e = tid + q * kShrinkThreads, kk = e / (RP / 8), j = e % (RP / 8) * 8;
           const bool in = c + kk < k1 && j < r;
           copy_async_16(ws + kk * (RP * 2 + 16) + j * 2, in ? wi + int64_t(c + kk) * sr + j : w, in);
         }
       } else {
-        for (int e = tid; e < RP * 8; e += kThreads) {
-          const int j = e / 8;
+#pragma unroll
+        for (int q = 0; q < RP * 8 / kShrinkThreads; ++q) {
+          const int j = tid / 8 + q * kRowSteps;
           const bool in = j < r && k < k1;
           copy_async_16(ws + j * kShrinkPitch + (tid & 7) * 16, in ? wi + j * sr + k : w, in);
         }
@@ -252,23 +271,30 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
     copies_commit();
   };
-  float acc[RP / 8][4];
+  float acc[2][RP / 8][4];
 #pragma unroll
-  for (int n = 0; n < RP / 8; ++n)
+  for (int m = 0; m < 2; ++m)
 #pragma unroll
-    for (int q = 0; q < 4; ++q) acc[n][q] = 0.0f;
+    for (int n = 0; n < RP / 8; ++n)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) acc[m][n][q] = 0.0f;
 #pragma unroll
   for (int q = 0; q < C::kStages - 1; ++q) fetch(q);
+  const bool busy = warp * 32 < t.rows;  // a warp without rows only copies
   for (int step = 0; step < steps; ++step) {
     copies_wait<C::kStages - 2>();
     __syncthreads();
     fetch(step + C::kStages - 1);
     const uint32_t xs = smem_u32(smem) + (step % C::kStages) * C::kStage;
     const uint32_t ws = xs + kShrinkRows * kShrinkPitch;
+    if (!busy) continue;
 #pragma unroll
     for (int kk = 0; kk < kShrinkCols; kk += 16) {
-      uint32_t a[4];
-      ldmatrix_x4<false>(a, xs + (warp * 16 + (lane & 15)) * kShrinkPitch + (kk + (lane >> 4) * 8) * 2);
+      uint32_t a[2][4];
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+        ldmatrix_x4<false>(a[m], xs + (warp * 32 + m * 16 + (lane & 15)) * kShrinkPitch +
+                                     (kk + (lane >> 4) * 8) * 2);
 #pragma unroll
       for (int n = 0; n < RP / 8; n += 2) {
         uint32_t b[4];
@@ -277,8 +303,11 @@ __global__ void __launch_bounds__(kThreads, 2)
         else
           ldmatrix_x4<false>(b, ws + (n * 8 + (lane >> 4) * 8 + (lane & 7)) * kShrinkPitch +
                                     (kk + ((lane >> 3) & 1) * 8) * 2);
-        mma<T>(acc[n], a, b[0], b[1]);
-        mma<T>(acc[n + 1], a, b[2], b[3]);
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          mma<T>(acc[m][n], a[m], b[0], b[1]);
+          mma<T>(acc[m][n + 1], a[m], b[2], b[3]);
+        }
       }
     }
   }
@@ -287,49 +316,50 @@ __global__ void __launch_bounds__(kThreads, 2)
   constexpr int kPitch = RP + 4;
   float* sums = reinterpret_cast<float*>(smem);
 #pragma unroll
-  for (int n = 0; n < RP / 8; ++n)
+  for (int m = 0; m < 2; ++m)
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-      sums[(warp * 16 + (lane >> 2) + 8 * (q >> 1)) * kPitch + n * 8 + (lane & 3) * 2 + (q & 1)] = acc[n][q];
+    for (int n = 0; n < RP / 8; ++n)
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+        *reinterpret_cast<float2*>(sums + (warp * 32 + m * 16 + (lane >> 2) + 8 * q) * kPitch + n * 8 +
+                                   (lane & 3) * 2) = make_float2(acc[m][n][2 * q], acc[m][n][2 * q + 1]);
   if (parts > 1)
     cluster_sync_all();
   else
     __syncthreads();
   const int share = kShrinkRows / parts;  // rows that this CTA finishes
-  for (int e = tid; e < share * r; e += kThreads) {
-    const int m = part * share + e / r, j = e % r;
-    if (m >= t.rows) break;
-    float v = 0.0f;
-    if (parts > 1) {
-      const uint32_t at = smem_u32(sums + m * kPitch + j);
-      for (int q = 0; q < parts; ++q) v += ld_shared_cluster(mapa_shared(at, q));
-    } else {
-      v = sums[m * kPitch + j];
-    }
+  for (int e = tid; e < share * (RP / 4); e += kShrinkThreads) {
+    const int m = part * share + e / (RP / 4), j = e % (RP / 4) * 4;
+    if (m >= t.rows || j >= r) continue;
+    const float4 v = cluster_sum4(sums + m * kPitch + j, parts);
+    T hi[4], lo[4];
+    split(v.x, hi, lo), split(v.y, hi + 1, lo + 1), split(v.z, hi + 2, lo + 2), split(v.w, hi + 3, lo + 3);
     T* out = s + int64_t(t.p0 + m) * r + j;
-    split(v, out, out + part_stride);
+    *reinterpret_cast<uint2*>(out) = *reinterpret_cast<const uint2*>(hi);
+    *reinterpret_cast<uint2*>(out + part_stride) = *reinterpret_cast<const uint2*>(lo);
   }
   if (parts > 1) cluster_sync_all();  // no CTA leaves while another reads its sums
 }
 
 // expand.  A CTA holds 64 rows of s in registers (both parts) and runs over blocks of
-// 256 columns: 4 groups of 16 rows x 2 halves of 128 columns, one per warp.  Bound by
-// reading and writing y; y's 16-byte pieces are loaded before the products.  For W in
-// rows of n the columns are placed so that a lane's results of 4 column tiles are 8
-// neighbours; read along n they go through a patch of shared memory for that.
+// 128 columns: 4 groups of 16 rows x 2 halves of 64 columns, one per warp.  Bound by
+// reading and writing y; y's 16-byte pieces and w's rows of the next block are loaded
+// under the products of this one.  For w in rows of n the columns are placed so that a
+// lane's results of 4 column tiles are 8 neighbours; read along n they go through a
+// patch of shared memory for that.
 constexpr int kExpandRows = 64;
-constexpr int kExpandCols = 256;
+constexpr int kExpandCols = 128;
 constexpr int kPatchPitch = 36;  // floats
 
 template <bool kT, int RP>
 struct ExpandCfg {
   static constexpr int kW = kT ? RP * (kExpandCols * 2 + 16) : kExpandCols * (RP * 2 + 16);
   static constexpr int kPatch = kT ? 8 * 16 * kPatchPitch * 4 : 0;
-  static constexpr int kBytes = kW + kPatch;
+  static constexpr int kBytes = 2 * kW + kPatch;
 };
 
 template <typename T, bool kT, int RP>
-__global__ void __launch_bounds__(kThreads, RP == 128 ? 1 : 2)
+__global__ void __launch_bounds__(kThreads, 2)
     expand_kernel(const T* s, int64_t part_stride, const T* w, int64_t sl, int64_t sr,
                   const float* scale, const int32_t* perm, const int32_t* offs, int L, int N, int r,
                   T* y, int64_t ldy) {
@@ -340,14 +370,53 @@ __global__ void __launch_bounds__(kThreads, RP == 128 ? 1 : 2)
   if (t.i < 0) return;
   const int mg = warp & 3, half = warp >> 2;
   const T* wi = w + t.i * sl;
+  const int step = gridDim.y * kExpandCols;
+  auto fetch_w = [&](int n0, int buf) {
+    if (n0 < N) {
+      const uint32_t ws = smem_u32(smem) + buf * C::kW;
+      constexpr int kPieces = RP * kExpandCols / 8 / kThreads;
+#pragma unroll
+      for (int q = 0; q < kPieces; ++q) {
+        const int e = tid + q * kThreads;
+        if constexpr (kT) {
+          const int j = e / (kExpandCols / 8), n = e % (kExpandCols / 8) * 8;
+          const bool in = j < r && n0 + n < N;
+          copy_async_16(ws + j * (kExpandCols * 2 + 16) + n * 2, in ? wi + j * sr + n0 + n : w, in);
+        } else {
+          const int n = e / (RP / 8), j = e % (RP / 8) * 8;
+          // column 8 q + 2 t + o of a group of 32 goes to row 8 t + 2 q + o
+          const int at = (n & ~31) + ((n >> 1) & 3) * 8 + ((n >> 3) & 3) * 2 + (n & 1);
+          const bool in = j < r && n0 + n < N;
+          copy_async_16(ws + at * (RP * 2 + 16) + j * 2, in ? wi + (n0 + n) * sr + j : w, in);
+        }
+      }
+    }
+    copies_commit();
+  };
+  fetch_w(blockIdx.y * kExpandCols, 0);
   const float c = scale[t.i];
-  // A fragments straight from s: rows mg*16 + g8 and + 8, pairs of columns.
-  uint32_t a[2][RP / 16][4];
-  int64_t yrow[2];
+  T* yrow[2];
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     const int m = mg * 16 + g8 + 8 * u;
-    yrow[u] = m < t.rows ? perm[t.p0 + m] * ldy : -1;
+    yrow[u] = m < t.rows ? y + perm[t.p0 + m] * ldy + half * 64 + q4 * 8 : nullptr;
+  }
+  const int ncol = half * 64 + q4 * 8;  // this lane's first column of a block; + 32 for the second
+  auto fetch_y = [&](int n0, uint4(&v)[2][2]) {
+#pragma unroll
+    for (int g = 0; g < 2; ++g)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        if (yrow[u] != nullptr && n0 + ncol + g * 32 < N)
+          v[g][u] = *reinterpret_cast<const uint4*>(yrow[u] + n0 + g * 32);
+  };
+  uint4 yv[2][2], yn[2][2];
+  fetch_y(blockIdx.y * kExpandCols, yv);
+  // A fragments straight from s: rows mg*16 + g8 and + 8, pairs of columns.
+  uint32_t a[2][RP / 16][4];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int m = mg * 16 + g8 + 8 * u;
 #pragma unroll
     for (int k = 0; k < RP / 16; ++k)
 #pragma unroll
@@ -359,42 +428,21 @@ __global__ void __launch_bounds__(kThreads, RP == 128 ? 1 : 2)
         a[1][k][u + 2 * v] = in ? *reinterpret_cast<const uint32_t*>(at + part_stride) : 0u;
       }
   }
-  for (int n0 = blockIdx.y * kExpandCols; n0 < N; n0 += gridDim.y * kExpandCols) {
-    const uint32_t ws = smem_u32(smem);
-    if constexpr (kT) {
-      for (int e = tid; e < RP * (kExpandCols / 8); e += kThreads) {
-        const int j = e / (kExpandCols / 8), n = e % (kExpandCols / 8) * 8;
-        const bool in = j < r && n0 + n < N;
-        copy_async_16(ws + j * (kExpandCols * 2 + 16) + n * 2, in ? wi + j * sr + n0 + n : w, in);
-      }
-    } else {
-      for (int e = tid; e < kExpandCols * (RP / 8); e += kThreads) {
-        const int n = e / (RP / 8), j = e % (RP / 8) * 8;
-        // column 8 q + 2 t + o of a group of 32 goes to row 8 t + 2 q + o
-        const int at = (n & ~31) + ((n >> 1) & 3) * 8 + ((n >> 3) & 3) * 2 + (n & 1);
-        const bool in = j < r && n0 + n < N;
-        copy_async_16(ws + at * (RP * 2 + 16) + j * 2, in ? wi + (n0 + n) * sr + j : w, in);
-      }
-    }
-    copies_commit();
-    uint4 yv[4][2];  // 4 groups of 32 columns, 8 of them a lane
-#pragma unroll
-    for (int g = 0; g < 4; ++g)
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int n = n0 + half * 128 + g * 32 + q4 * 8;
-        if (yrow[u] >= 0 && n < N) yv[g][u] = *reinterpret_cast<const uint4*>(y + yrow[u] + n);
-      }
-    copies_wait<0>();
+  int buf = 0;
+  for (int n0 = blockIdx.y * kExpandCols; n0 < N; n0 += step) {
+    fetch_w(n0 + step, buf ^ 1);
+    fetch_y(n0 + step, yn);
+    copies_wait<1>();
     __syncthreads();
+    const uint32_t ws = smem_u32(smem) + buf * C::kW;
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
+    for (int g = 0; g < 2; ++g) {
       float acc[4][4];
 #pragma unroll
       for (int n = 0; n < 4; ++n)
 #pragma unroll
         for (int q = 0; q < 4; ++q) acc[n][q] = 0.0f;
-      const int col = half * 128 + g * 32;
+      const int col = half * 64 + g * 32;
 #pragma unroll
       for (int k = 0; k < RP / 16; ++k)
 #pragma unroll
@@ -414,7 +462,7 @@ __global__ void __launch_bounds__(kThreads, RP == 128 ? 1 : 2)
         }
       float add[2][8];  // this lane's 8 neighbouring columns of its two rows
       if constexpr (kT) {
-        float* patch = reinterpret_cast<float*>(smem + C::kW) + warp * 16 * kPatchPitch;
+        float* patch = reinterpret_cast<float*>(smem + 2 * C::kW) + warp * 16 * kPatchPitch;
         __syncwarp();
 #pragma unroll
         for (int n = 0; n < 4; ++n)
@@ -437,16 +485,21 @@ __global__ void __launch_bounds__(kThreads, RP == 128 ? 1 : 2)
       }
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const int n = n0 + col + q4 * 8;
-        if (yrow[u] < 0 || n >= N) continue;
+        if (yrow[u] == nullptr || n0 + ncol + g * 32 >= N) continue;
         T* v = reinterpret_cast<T*>(&yv[g][u]);
 #pragma unroll
         for (int q = 0; q < 8; ++q) v[q] = from_f<T>(to_f(v[q]) + c * add[u][q]);
-        *reinterpret_cast<uint4*>(y + yrow[u] + n) = yv[g][u];
+        *reinterpret_cast<uint4*>(yrow[u] + n0 + g * 32) = yv[g][u];
       }
     }
     __syncthreads();
+#pragma unroll
+    for (int g = 0; g < 2; ++g)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) yv[g][u] = yn[g][u];
+    buf ^= 1;
   }
+  copies_wait<0>();
 }
 
 // grad.  A CTA forms 128 MT columns of z x RP of one adapter's gradient over one part
@@ -462,7 +515,7 @@ struct GradCfg {
   static constexpr int kZPitch = kCols * 2 + 16, kSPitch = RP * 2 + 16;
   static constexpr int kStage = kGradRows * (kZPitch + 2 * kSPitch);
   static constexpr int kStages = 4;
-  static constexpr int kSums = kCols * (RP + 4) * 4;
+  static constexpr int kSums = (kCols + 4) * (RP + 4) * 4;
   static constexpr int kBytes = kStages * kStage > kSums ? kStages * kStage : kSums;
 };
 
@@ -479,18 +532,31 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int share = ((rows + parts - 1) / parts + kGradRows - 1) / kGradRows * kGradRows;
   const int p0 = min(rows, part * share), p1 = min(rows, p0 + share);
   const int steps = (p1 - p0 + kGradRows - 1) / kGradRows;
+  constexpr int kPieces = C::kCols / 8;  // 16-byte pieces of a row of z
+  constexpr int kCopies = kGradRows * kPieces / kThreads;
+  const int zc = tid % kPieces * 8;
+  int next_row[kCopies];  // perm's entries for the next fetch: known before they are used
+  auto look_up = [&](int step) {
+#pragma unroll
+    for (int q = 0; q < kCopies; ++q) {
+      const int p = p0 + step * kGradRows + tid / kPieces + q * (kThreads / kPieces);
+      next_row[q] = p < p1 && n0 + zc < n ? perm[o0 + p] : -1;
+    }
+  };
+  look_up(0);
   auto fetch = [&](int step) {
     if (step < steps) {
       const uint32_t zs = smem_u32(smem) + (step % C::kStages) * C::kStage;
       const uint32_t ss = zs + kGradRows * C::kZPitch;
       const int p = p0 + step * kGradRows;
-      constexpr int kPieces = C::kCols / 8;
 #pragma unroll
-      for (int q = 0; q < kGradRows * kPieces / kThreads; ++q) {
-        const int e = tid + q * kThreads, m = e / kPieces, c = e % kPieces * 8;
-        const bool in = p + m < p1 && n0 + c < n;
-        copy_async_16(zs + m * C::kZPitch + c * 2, in ? z + perm[o0 + p + m] * ldz + n0 + c : z, in);
+      for (int q = 0; q < kCopies; ++q) {
+        const int m = tid / kPieces + q * (kThreads / kPieces);
+        const bool in = next_row[q] >= 0;
+        copy_async_16(zs + m * C::kZPitch + zc * 2, in ? z + next_row[q] * ldz + n0 + zc : z, in);
       }
+      look_up(step + 1);
+#pragma unroll
       for (int e = tid; e < kGradRows * (RP / 8) * 2; e += kThreads) {
         const int half = e / (kGradRows * (RP / 8)), f = e % (kGradRows * (RP / 8));
         const int m = f / (RP / 8), j = f % (RP / 8) * 8;
@@ -540,44 +606,43 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
   copies_wait<0>();
   __syncthreads();
-  constexpr int kPitch = RP + 4;
+  // The sums lie as the gradient does: [column][rank], or [rank][column] with kT.
+  constexpr int kPitch = kT ? C::kCols + 4 : RP + 4;
   float* sums = reinterpret_cast<float*>(smem);
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
     for (int k = 0; k < RP / 8; ++k)
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        sums[((warp * MT + m) * 16 + (lane >> 2) + 8 * (q >> 1)) * kPitch + k * 8 + (lane & 3) * 2 + (q & 1)] =
-            acc[m][k][q];
+      for (int q = 0; q < 4; ++q) {
+        const int col = (warp * MT + m) * 16 + (lane >> 2) + 8 * (q >> 1), j = k * 8 + (lane & 3) * 2 + (q & 1);
+        sums[kT ? j * kPitch + col : col * kPitch + j] = acc[m][k][q];
+      }
   if (parts > 1)
     cluster_sync_all();
   else
     __syncthreads();
   const float c = scale[i];
-  const int cols = C::kCols / parts;  // that this CTA finishes
-  for (int e = tid; e < cols * r; e += kThreads) {
-    const int col = part * cols + (kT ? e % cols : e / r), j = kT ? e / cols : e % r;
-    if (n0 + col >= n) continue;
-    float v = 0.0f;
-    if (parts > 1) {
-      const uint32_t at = smem_u32(sums + col * kPitch + j);
-      for (int q = 0; q < parts; ++q) v += ld_shared_cluster(mapa_shared(at, q));
-    } else {
-      v = sums[col * kPitch + j];
-    }
-    g[i * gl + (kT ? j * gr + n0 + col : (n0 + col) * gr + j)] = from_f<T>(c * v);
+  // Four neighbours of a row at a time; the CTAs take the rows in turn.
+  constexpr int kRows = kT ? RP : C::kCols, kQuads = (kT ? C::kCols : RP) / 4;
+  for (int e = tid; e < kRows / parts * kQuads; e += kThreads) {
+    const int row = e / kQuads * parts + part, at = e % kQuads * 4;
+    if (kT ? row >= r || n0 + at >= n : n0 + row >= n || at >= r) continue;
+    const float4 v = cluster_sum4(sums + row * kPitch + at, parts);
+    const T o[4] = {from_f<T>(c * v.x), from_f<T>(c * v.y), from_f<T>(c * v.z), from_f<T>(c * v.w)};
+    T* out = g + i * gl + (kT ? row * gr + n0 + at : (n0 + row) * gr + at);
+    *reinterpret_cast<uint2*>(out) = *reinterpret_cast<const uint2*>(o);
   }
   if (parts > 1) cluster_sync_all();
 }
 
 template <typename K, typename... A>
-int launch(K kern, dim3 grid, dim3 cluster, int smem, cudaStream_t stream, A... args) {
+int launch(K kern, dim3 grid, int threads, dim3 cluster, int smem, cudaStream_t stream, A... args) {
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return MOE_ERR_CUDA;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr{};
@@ -610,11 +675,11 @@ inline int64_t most_tiles(int64_t m, int adapters, int tile) {
   const int64_t t = (m + tile - 1) / tile + adapters;
   return t < m ? t : m;
 }
-// A power of two up to 8 that brings `blocks` to about two CTAs an SM, while each part
-// keeps at least `least` of `length`.
-inline int cluster_parts(int64_t blocks, int64_t length, int64_t least) {
+// A power of two up to 8 that keeps blocks * parts at most `most` and gives each part
+// at least `least` of `length`.
+inline int cluster_parts(int64_t blocks, int64_t most, int64_t length, int64_t least) {
   int parts = 1;
-  while (parts < 8 && blocks * parts < 296 && length / (parts * 2) >= least) parts *= 2;
+  while (parts < 8 && blocks * parts * 2 <= most && length / (parts * 2) >= least) parts *= 2;
   return parts;
 }
 
@@ -667,8 +732,9 @@ extern "C" int32_t moe_lora_shrink(const void* x, int64_t ldx, const void* w, in
     constexpr bool kT = decltype(tr)::value;
     constexpr int RP = decltype(rp)::value;
     const unsigned tiles = static_cast<unsigned>(lora::most_tiles(m, adapters, lora::kShrinkRows));
-    const unsigned parts = lora::cluster_parts(tiles, k, 256);
-    return lora::launch(lora::shrink_kernel<T, kT, RP>, dim3(tiles, parts), dim3(1, parts),
+    const unsigned parts = lora::cluster_parts(tiles, 2 * 148, k, 256);
+    return lora::launch(lora::shrink_kernel<T, kT, RP>, dim3(tiles, parts),
+                        lora::kShrinkThreads, dim3(1, parts),
                         lora::ShrinkCfg<kT, RP>::kBytes, static_cast<cudaStream_t>(stream),
                         static_cast<const T*>(x), ldx, static_cast<const T*>(w), w_stride_l,
                         w_stride_row, perm, offs, static_cast<int>(adapters), static_cast<int>(k),
@@ -697,7 +763,7 @@ extern "C" int32_t moe_lora_expand(const void* s, const void* w, int64_t w_strid
     const int64_t want = (1200 + tiles - 1) / tiles;  // about four CTAs a place on the SMs
     return lora::launch(lora::expand_kernel<T, kT, RP>,
                         dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(want < blocks ? want : blocks)),
-                        dim3(1, 1), lora::ExpandCfg<kT, RP>::kBytes, static_cast<cudaStream_t>(stream),
+                        lora::kThreads, dim3(1, 1), lora::ExpandCfg<kT, RP>::kBytes, static_cast<cudaStream_t>(stream),
                         static_cast<const T*>(s), m * rank, static_cast<const T*>(w), w_stride_l,
                         w_stride_row, scale, perm, offs, static_cast<int>(adapters), static_cast<int>(n),
                         static_cast<int>(rank), static_cast<T*>(y), ldy);
@@ -720,8 +786,10 @@ extern "C" int32_t moe_lora_grad(const void* s, const void* z, int64_t ldz, cons
     constexpr int RP = decltype(rp)::value;
     using C = lora::GradCfg<RP>;
     const unsigned blocks = static_cast<unsigned>((n + C::kCols - 1) / C::kCols);
-    const unsigned parts = lora::cluster_parts(int64_t(blocks) * adapters, m / adapters, 64);
-    return lora::launch(lora::grad_kernel<T, kT, RP>, dim3(parts, blocks, adapters), dim3(parts, 1),
+    // Adapters' rows are uneven, so many small parts: the largest adapter's rows spread.
+    const unsigned parts = lora::cluster_parts(int64_t(blocks) * adapters, 8 * 2 * 148, m / adapters, 64);
+    return lora::launch(lora::grad_kernel<T, kT, RP>, dim3(parts, blocks, adapters),
+                        lora::kThreads, dim3(parts, 1),
                         C::kBytes, static_cast<cudaStream_t>(stream), static_cast<const T*>(s), m * rank,
                         static_cast<const T*>(z), ldz, scale, perm, offs, static_cast<int>(n),
                         static_cast<int>(rank), static_cast<T*>(g), g_stride_l, g_stride_row);
