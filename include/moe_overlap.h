@@ -567,45 +567,42 @@ MOE_API int32_t moe_few_tokens(const void* x, int64_t ldx, const void* router_w,
                                int32_t* status, void* stream);
 
 /*
- * Low-rank adapters of many requests beside a shared projection.  With the shared
- * product y = x W^T from moe_grouped_gemm (one expert), row m of adapter i = ids[m]
- * gets y[m] += scale[i] (x[m] A[i]^T) B[i]^T; -1 is a row without adapter.  The
- * calls of one forward:  plan, shrink (x, A), expand (B);  of its backward:  shrink
- * (dy, B transposed), expand (A transposed) onto dx, grad (dy, s) for dB and grad (x,
- * the second shrink's s) for dA.
- *
- * moe_lora_plan     ids [m] int32 / int64 -> perm [m]: the rows with an adapter, by
- *                   adapter, in row order; offs [adapters + 1]: the adapters' places
- *                   in perm; base_offs [2]: {0, m}, expert_offsets of the shared
- *                   product.  An id outside [-1, adapters) counts as -1 and records
- *                   MOE_ERR_INVALID_ARG in `status`.
- * moe_lora_shrink   s[p][j] = sum_k x[perm[p]][k] w_i(j, k), held as two arrays
- *                   [m][rank] of `dtype`, one behind the other: the rounded value and
- *                   what the rounding left
- * moe_lora_expand   y[perm[p]][c] += scale[i] sum_j s[p][j] w_i(c, j); other rows stay
- * moe_lora_grad     g_i(c, j) = scale[i] sum_p s[p][j] z[perm[p]][c] over the rows of i,
- *                   zeros for an adapter without rows
- * for p < offs[adapters] and i the adapter of place p.  w_i(j, k) is stored at
- * w + i*stride_l + j*stride_row + k, or transposed at w + i*stride_l + k*stride_row + j;
- * likewise w_i(c, j) and g_i(c, j) with c in j's place.  Rows start on 16 bytes; k, n
- * and rank are multiples of 8; rank <= 128; adapters <= 1024.  Sums are fp32.
+ * A projection with the low-rank adapter of each row's request beside it:
+ *   y[r] = x[r] W^T + scale[i] (x[r] A[i]^T) B[i]^T,   i = ids[r], -1: no adapter
+ * and its gradients for a frozen W.
+ *   x [m, k], weight [n, k], y [m, n]   row strides in elements
+ *   lora_a [adapters, rank, k], lora_b [adapters, n, rank]
+ *                   adapter and row strides in elements
+ *   ids [m]         int32, or int64 if ids_int64; an id outside [-1, adapters) counts
+ *                   as -1 and records MOE_ERR_INVALID_ARG in `status`
+ *   scale           float[adapters], or NULL: scale_all for every adapter
+ *   plan            int32 [m + adapters + 3], out: the rows by adapter
+ *   s               2 m rank elements of `dtype`, out: x[r] A[i]^T in plan order, the
+ *                   rounded values and what the rounding left
+ * dtype is MOE_DTYPE_BF16 or MOE_DTYPE_F16.  Rows start on 16 bytes; k, n and rank are
+ * multiples of 8; rank <= 128; adapters <= 1024.  Sums are fp32.
  */
-MOE_API int32_t moe_lora_plan(const void* ids, int32_t ids_int64, int64_t m, int32_t adapters,
-                              int32_t* perm, int32_t* offs, int32_t* base_offs, int32_t* status,
-                              void* stream);
-MOE_API int32_t moe_lora_shrink(const void* x, int64_t ldx, const void* w, int64_t w_stride_l,
-                                int64_t w_stride_row, int32_t w_transposed, const int32_t* perm,
-                                const int32_t* offs, int32_t dtype, int64_t m, int64_t k,
-                                int32_t adapters, int32_t rank, void* s, void* stream);
-MOE_API int32_t moe_lora_expand(const void* s, const void* w, int64_t w_stride_l,
-                                int64_t w_stride_row, int32_t w_transposed, const float* scale,
-                                const int32_t* perm, const int32_t* offs, int32_t dtype, int64_t m,
-                                int64_t n, int32_t adapters, int32_t rank, void* y, int64_t ldy,
-                                void* stream);
-MOE_API int32_t moe_lora_grad(const void* s, const void* z, int64_t ldz, const float* scale,
-                              const int32_t* perm, const int32_t* offs, int32_t dtype, int64_t m,
-                              int64_t n, int32_t adapters, int32_t rank, void* g, int64_t g_stride_l,
-                              int64_t g_stride_row, int32_t g_transposed, void* stream);
+MOE_API int32_t moe_lora_forward(const void* x, int64_t ldx, const void* weight, int64_t ldw,
+                                 const void* lora_a, int64_t a_stride_l, int64_t a_stride_row,
+                                 const void* lora_b, int64_t b_stride_l, int64_t b_stride_row,
+                                 const void* ids, int32_t ids_int64, const float* scale,
+                                 float scale_all, int32_t dtype, int64_t m, int64_t k, int64_t n,
+                                 int32_t adapters, int32_t rank, void* y, int64_t ldy, int32_t* plan,
+                                 void* s, int32_t* status, void* stream);
+
+/*
+ * Gradients of moe_lora_forward, from its plan and s: dx [m, k], da [adapters, rank, k]
+ * and db [adapters, n, rank], the last two contiguous; a NULL one is not formed.  An
+ * adapter without rows gets zeros.  t: workspace like s, needed for dx and da.
+ */
+MOE_API int32_t moe_lora_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx,
+                                  const void* weight, int64_t ldw, const void* lora_a,
+                                  int64_t a_stride_l, int64_t a_stride_row, const void* lora_b,
+                                  int64_t b_stride_l, int64_t b_stride_row, const float* scale,
+                                  float scale_all, int32_t dtype, int64_t m, int64_t k, int64_t n,
+                                  int32_t adapters, int32_t rank, int32_t* plan, const void* s, void* t,
+                                  void* dx, int64_t lddx, void* da, void* db, int32_t* status,
+                                  void* stream);
 
 /*
  * DeepEP's get_dispatch_layout (thirdParty/DeepEP/deep_ep/buffer.py:293-319,

@@ -12,6 +12,7 @@ raised at the next call (like CUDA's own asynchronous error reporting), and
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -194,25 +195,21 @@ SIGNATURES: dict[str, tuple] = {
          _c_void_p, _c_void_p, _c_void_p, _i64,  # topk_idx, topk_weights, out, ldo
          _c_void_p, _i64, _c_void_p, _c_void_p],  # workspace, bytes, status, stream
     ),
-    "moe_lora_plan": (
-        _i32, [_c_void_p, _i32, _i64, _i32, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p]),
-    "moe_lora_shrink": (
+    "moe_lora_forward": (
         _i32,
-        [_c_void_p, _i64, _c_void_p, _i64, _i64, _i32,  # x, ldx, w, strides l/row, transposed
-         _c_void_p, _c_void_p, _i32, _i64, _i64, _i32, _i32,  # perm, offs, dtype, m, k, adapters, rank
-         _c_void_p, _c_void_p],  # s, stream
+        [_c_void_p, _i64, _c_void_p, _i64,  # x, ldx, weight, ldw
+         _c_void_p, _i64, _i64, _c_void_p, _i64, _i64,  # lora_a, strides l/row, lora_b, strides l/row
+         _c_void_p, _i32, _c_void_p, ctypes.c_float,  # ids, ids_int64, scale, scale_all
+         _i32, _i64, _i64, _i64, _i32, _i32,  # dtype, m, k, n, adapters, rank
+         _c_void_p, _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p],  # y, ldy, plan, s, status, stream
     ),
-    "moe_lora_expand": (
+    "moe_lora_backward": (
         _i32,
-        [_c_void_p, _c_void_p, _i64, _i64, _i32, _c_void_p,  # s, w, strides l/row, transposed, scale
-         _c_void_p, _c_void_p, _i32, _i64, _i64, _i32, _i32,  # perm, offs, dtype, m, n, adapters, rank
-         _c_void_p, _i64, _c_void_p],  # y, ldy, stream
-    ),
-    "moe_lora_grad": (
-        _i32,
-        [_c_void_p, _c_void_p, _i64, _c_void_p,  # s, z, ldz, scale
-         _c_void_p, _c_void_p, _i32, _i64, _i64, _i32, _i32,  # perm, offs, dtype, m, n, adapters, rank
-         _c_void_p, _i64, _i64, _i32, _c_void_p],  # g, strides l/row, transposed, stream
+        [_c_void_p, _i64, _c_void_p, _i64, _c_void_p, _i64,  # dy, lddy, x, ldx, weight, ldw
+         _c_void_p, _i64, _i64, _c_void_p, _i64, _i64,  # lora_a, strides l/row, lora_b, strides l/row
+         _c_void_p, ctypes.c_float, _i32, _i64, _i64, _i64, _i32, _i32,  # scale, .., rank
+         _c_void_p, _c_void_p, _c_void_p,  # plan, s, t
+         _c_void_p, _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p],  # dx, lddx, da, db, status, stream
     ),
     "moe_ep_dispatch_layout": (
         _i32, [_c_void_p, _i32, _i32, _i32, _i32, _c_void_p, _c_void_p, _c_void_p, _c_void_p]),
@@ -224,6 +221,7 @@ SIGNATURES: dict[str, tuple] = {
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
 _status_words: dict[int, torch.Tensor] = {}
+_status_views: dict[int, ctypes.c_int32] = {}  # the same words, read without a torch call
 
 
 class MoeError(RuntimeError):
@@ -268,6 +266,7 @@ def status_word(device: torch.device) -> torch.Tensor:
             w = _status_words.get(idx)
             if w is None:
                 w = torch.zeros(1, dtype=torch.int32, pin_memory=True)
+                _status_views[idx] = ctypes.c_int32.from_address(w.data_ptr())
                 _status_words[idx] = w
     return w
 
@@ -278,11 +277,26 @@ def check_status(device: torch.device | None = None, sync: bool = False) -> None
         device = torch.device("cuda", torch.cuda.current_device())
     if sync:
         torch.cuda.synchronize(device)
-    w = status_word(device)
-    code = int(w[0])
+    status_address(device)
+    view = _status_views[device.index if device.index is not None else torch.cuda.current_device()]
+    code = view.value
     if code != 0:
-        w.zero_()
+        view.value = 0
         raise MoeError(code, "device-side error from an earlier moe_overlap_b200 kernel")
+
+
+def status_address(device: torch.device) -> int:
+    """Address of ``device``'s status word, for the C entry points."""
+    view = _status_views.get(device.index)
+    return ctypes.addressof(view) if view is not None else status_word(device).data_ptr()
+
+
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def on_device(device: torch.device):
+    """Makes ``device`` current for a ``with`` block; free when it already is."""
+    return _SAME_DEVICE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def check_call(code: int, where: str) -> None:

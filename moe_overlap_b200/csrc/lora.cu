@@ -42,6 +42,13 @@ __device__ __forceinline__ T from_f(float v) {
   else
     return __float2half_rn(v);
 }
+// One number for each adapter, or one for all.
+struct Scale {
+  const float* each;
+  float all;
+  __device__ float of(int i) const { return each != nullptr ? each[i] : all; }
+};
+
 // One block per adapter: it counts the rows of smaller adapters (its segment's start)
 // and writes its own rows in order.  No block depends on another and the order is
 // always the same.
@@ -361,7 +368,7 @@ struct ExpandCfg {
 template <typename T, bool kT, int RP>
 __global__ void __launch_bounds__(kThreads, 2)
     expand_kernel(const T* s, int64_t part_stride, const T* w, int64_t sl, int64_t sr,
-                  const float* scale, const int32_t* perm, const int32_t* offs, int L, int N, int r,
+                  Scale scale, const int32_t* perm, const int32_t* offs, int L, int N, int r,
                   T* y, int64_t ldy) {
   using C = ExpandCfg<kT, RP>;
   extern __shared__ __align__(128) char smem[];
@@ -394,7 +401,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     copies_commit();
   };
   fetch_w(blockIdx.y * kExpandCols, 0);
-  const float c = scale[t.i];
+  const float c = scale.of(t.i);
   T* yrow[2];
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
@@ -521,7 +528,7 @@ struct GradCfg {
 
 template <typename T, bool kT, int RP>
 __global__ void __launch_bounds__(kThreads, 2)
-    grad_kernel(const T* s, int64_t part_stride, const T* z, int64_t ldz, const float* scale,
+    grad_kernel(const T* s, int64_t part_stride, const T* z, int64_t ldz, Scale scale,
                 const int32_t* perm, const int32_t* offs, int n, int r, T* g, int64_t gl, int64_t gr) {
   using C = GradCfg<RP>;
   constexpr int MT = C::MT;
@@ -622,7 +629,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     cluster_sync_all();
   else
     __syncthreads();
-  const float c = scale[i];
+  const float c = scale.of(i);
   // Four neighbours of a row at a time; the CTAs take the rows in turn.
   constexpr int kRows = kT ? RP : C::kCols, kQuads = (kT ? C::kCols : RP) / 4;
   for (int e = tid; e < kRows / parts * kQuads; e += kThreads) {
@@ -683,115 +690,157 @@ inline int cluster_parts(int64_t blocks, int64_t most, int64_t length, int64_t l
   return parts;
 }
 
+// The caller's plan buffer: perm [m], offs [adapters + 1] and {0, m}.
+struct PlanView {
+  int32_t *perm, *offs, *base;
+  PlanView(int32_t* plan, int64_t m, int adapters)
+      : perm(plan), offs(plan + m), base(plan + m + adapters + 1) {}
+};
+struct Weights {  // of all adapters
+  const void* p;
+  int64_t stride_l, stride_row;
+};
+
+// s = x w^T by adapter, w in rows of k (transposed: in rows of the rank).
+int shrink(const void* x, int64_t ldx, Weights w, bool transposed, PlanView plan, int dtype, int64_t m,
+           int64_t k, int adapters, int rank, void* s, cudaStream_t stream) {
+  return dispatch(dtype, transposed, rank, [&](auto t, auto tr, auto rp) {
+    using T = decltype(t);
+    constexpr bool kT = decltype(tr)::value;
+    constexpr int RP = decltype(rp)::value;
+    const unsigned tiles = static_cast<unsigned>(most_tiles(m, adapters, kShrinkRows));
+    const unsigned parts = cluster_parts(tiles, 2 * 148, k, 256);
+    return launch(shrink_kernel<T, kT, RP>, dim3(tiles, parts), kShrinkThreads, dim3(1, parts),
+                  ShrinkCfg<kT, RP>::kBytes, stream, static_cast<const T*>(x), ldx,
+                  static_cast<const T*>(w.p), w.stride_l, w.stride_row, plan.perm, plan.offs, adapters,
+                  static_cast<int>(k), rank, m * rank, static_cast<T*>(s));
+  });
+}
+
+// y += scale s w^T, w in rows of the rank (transposed: in rows of n).
+int expand(const void* s, Weights w, bool transposed, Scale scale, PlanView plan, int dtype, int64_t m,
+           int64_t n, int adapters, int rank, void* y, int64_t ldy, cudaStream_t stream) {
+  return dispatch(dtype, transposed, rank, [&](auto t, auto tr, auto rp) {
+    using T = decltype(t);
+    constexpr bool kT = decltype(tr)::value;
+    constexpr int RP = decltype(rp)::value;
+    const int64_t tiles = most_tiles(m, adapters, kExpandRows);
+    const int64_t blocks = (n + kExpandCols - 1) / kExpandCols;
+    const int64_t want = (1200 + tiles - 1) / tiles;  // about four CTAs a place on the SMs
+    return launch(expand_kernel<T, kT, RP>,
+                  dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(want < blocks ? want : blocks)),
+                  kThreads, dim3(1, 1), ExpandCfg<kT, RP>::kBytes, stream, static_cast<const T*>(s),
+                  m * rank, static_cast<const T*>(w.p), w.stride_l, w.stride_row, scale, plan.perm,
+                  plan.offs, adapters, static_cast<int>(n), rank, static_cast<T*>(y), ldy);
+  });
+}
+
+// g [adapters, n, rank] (transposed: [adapters, rank, n]) = scale z^T s by adapter.
+int grad(const void* s, const void* z, int64_t ldz, bool transposed, Scale scale, PlanView plan, int dtype,
+         int64_t m, int64_t n, int adapters, int rank, void* g, cudaStream_t stream) {
+  return dispatch(dtype, transposed, rank, [&](auto t, auto tr, auto rp) {
+    using T = decltype(t);
+    constexpr bool kT = decltype(tr)::value;
+    constexpr int RP = decltype(rp)::value;
+    using C = GradCfg<RP>;
+    const unsigned blocks = static_cast<unsigned>((n + C::kCols - 1) / C::kCols);
+    // Adapters' rows are uneven, so many small parts: the largest adapter's rows spread.
+    const unsigned parts = cluster_parts(int64_t(blocks) * adapters, 8 * 2 * 148, m / adapters, 64);
+    return launch(grad_kernel<T, kT, RP>, dim3(parts, blocks, adapters), kThreads, dim3(parts, 1),
+                  C::kBytes, stream, static_cast<const T*>(s), m * rank, static_cast<const T*>(z), ldz,
+                  scale, plan.perm, plan.offs, static_cast<int>(n), rank, static_cast<T*>(g), n * rank,
+                  kT ? n : int64_t(rank));
+  });
+}
+
 }  // namespace lora
 }  // namespace moe
 
 using namespace moe;
 
 namespace {
-bool dims_ok(int32_t dtype, int64_t m, int64_t n, int32_t adapters, int32_t rank) {
-  return (dtype == MOE_DTYPE_BF16 || dtype == MOE_DTYPE_F16) && m >= 0 && m <= INT32_MAX / 2 && n >= 8 &&
-         n % 8 == 0 && n <= INT32_MAX / 2 && adapters >= 1 && adapters <= lora::kMaxAdapters && rank >= 8 &&
-         rank % 8 == 0 && rank <= lora::kMaxRank;
+bool dims_ok(int32_t dtype, int64_t m, int64_t k, int64_t n, int32_t adapters, int32_t rank) {
+  const int64_t most = INT32_MAX / 2;
+  return (dtype == MOE_DTYPE_BF16 || dtype == MOE_DTYPE_F16) && m >= 0 && m <= most && k >= 8 &&
+         k % 8 == 0 && k <= most && n >= 8 && n % 8 == 0 && n <= most && adapters >= 1 &&
+         adapters <= lora::kMaxAdapters && rank >= 8 && rank % 8 == 0 && rank <= lora::kMaxRank;
 }
-// Adapter weights: rows of `width` at 16-byte starts, one adapter after another.
-bool weights_ok(const void* w, int64_t stride_l, int64_t stride_row, int64_t rows, int64_t width,
-                int32_t adapters) {
-  return w != nullptr && aligned16(w) && stride_row >= width && stride_row % 8 == 0 &&
-         (adapters == 1 || (stride_l % 8 == 0 && stride_l >= (rows - 1) * stride_row + width));
-}
+// Rows of `width` at 16-byte starts; of several adapters, one behind another.
 bool rows_ok(const void* p, int64_t ld, int64_t width) {
   return p != nullptr && aligned16(p) && ld >= width && ld % 8 == 0;
 }
-int launched() { return cudaGetLastError() == cudaSuccess ? MOE_OK : MOE_ERR_CUDA; }
+bool weights_ok(lora::Weights w, int64_t rows, int64_t width, int32_t adapters) {
+  return rows_ok(w.p, w.stride_row, width) &&
+         (adapters == 1 || (w.stride_l % 8 == 0 && w.stride_l >= (rows - 1) * w.stride_row + width));
+}
+int shared_product(const void* x, int64_t ldx, const void* w, int64_t stride_k, int64_t stride_n, void* y,
+                   int64_t ldy, const int32_t* base, int64_t m, int64_t k, int64_t n, int32_t dtype,
+                   int32_t* status, void* stream) {
+  int dev;
+  DeviceInfo info;
+  const int rc = current_device_info(&dev, &info);
+  if (rc != MOE_OK) return rc;
+  return moe_grouped_gemm(x, ldx, w, 0, stride_k, stride_n, y, ldy, base, 0, m, k, n, 1, dtype,
+                          MOE_ACT_NONE, info.sm_count, 0, nullptr, status, stream);
+}
 }  // namespace
 
-extern "C" int32_t moe_lora_plan(const void* ids, int32_t ids_int64, int64_t m, int32_t adapters,
-                                 int32_t* perm, int32_t* offs, int32_t* base_offs, int32_t* status,
-                                 void* stream) {
-  if (m < 0 || m > INT32_MAX / 2 || adapters < 1 || adapters > lora::kMaxAdapters || offs == nullptr ||
-      base_offs == nullptr || (m > 0 && (ids == nullptr || perm == nullptr)))
+extern "C" int32_t moe_lora_forward(const void* x, int64_t ldx, const void* weight, int64_t ldw,
+                                    const void* lora_a, int64_t a_stride_l, int64_t a_stride_row,
+                                    const void* lora_b, int64_t b_stride_l, int64_t b_stride_row,
+                                    const void* ids, int32_t ids_int64, const float* scale,
+                                    float scale_all, int32_t dtype, int64_t m, int64_t k, int64_t n,
+                                    int32_t adapters, int32_t rank, void* y, int64_t ldy, int32_t* plan,
+                                    void* s, int32_t* status, void* stream) {
+  const lora::Weights a{lora_a, a_stride_l, a_stride_row}, b{lora_b, b_stride_l, b_stride_row};
+  if (!dims_ok(dtype, m, k, n, adapters, rank) || plan == nullptr || !rows_ok(weight, ldw, k) ||
+      !weights_ok(a, rank, k, adapters) || !weights_ok(b, n, rank, adapters) ||
+      (m > 0 && (!rows_ok(x, ldx, k) || !rows_ok(y, ldy, n) || ids == nullptr || s == nullptr || !aligned16(s))))
     return MOE_ERR_INVALID_ARG;
-  lora::plan_kernel<<<adapters, 1024, 0, static_cast<cudaStream_t>(stream)>>>(
-      ids, ids_int64, static_cast<int>(m), adapters, perm, offs, base_offs, status);
-  return launched();
-}
-
-extern "C" int32_t moe_lora_shrink(const void* x, int64_t ldx, const void* w, int64_t w_stride_l,
-                                   int64_t w_stride_row, int32_t w_transposed, const int32_t* perm,
-                                   const int32_t* offs, int32_t dtype, int64_t m, int64_t k,
-                                   int32_t adapters, int32_t rank, void* s, void* stream) {
-  if (!dims_ok(dtype, m, k, adapters, rank)) return MOE_ERR_INVALID_ARG;
+  const lora::PlanView pv(plan, m, adapters);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  lora::plan_kernel<<<adapters, 1024, 0, st>>>(ids, ids_int64, static_cast<int>(m), adapters, pv.perm,
+                                               pv.offs, pv.base, status);
+  if (cudaGetLastError() != cudaSuccess) return MOE_ERR_CUDA;
   if (m == 0) return MOE_OK;
-  if (!rows_ok(x, ldx, k) || perm == nullptr || offs == nullptr || s == nullptr || !aligned16(s) ||
-      !(w_transposed ? weights_ok(w, w_stride_l, w_stride_row, k, rank, adapters)
-                     : weights_ok(w, w_stride_l, w_stride_row, rank, k, adapters)))
-    return MOE_ERR_INVALID_ARG;
-  return lora::dispatch(dtype, w_transposed != 0, rank, [&](auto t, auto tr, auto rp) {
-    using T = decltype(t);
-    constexpr bool kT = decltype(tr)::value;
-    constexpr int RP = decltype(rp)::value;
-    const unsigned tiles = static_cast<unsigned>(lora::most_tiles(m, adapters, lora::kShrinkRows));
-    const unsigned parts = lora::cluster_parts(tiles, 2 * 148, k, 256);
-    return lora::launch(lora::shrink_kernel<T, kT, RP>, dim3(tiles, parts),
-                        lora::kShrinkThreads, dim3(1, parts),
-                        lora::ShrinkCfg<kT, RP>::kBytes, static_cast<cudaStream_t>(stream),
-                        static_cast<const T*>(x), ldx, static_cast<const T*>(w), w_stride_l,
-                        w_stride_row, perm, offs, static_cast<int>(adapters), static_cast<int>(k),
-                        static_cast<int>(rank), m * rank, static_cast<T*>(s));
-  });
+  int rc = lora::shrink(x, ldx, a, false, pv, dtype, m, k, adapters, rank, s, st);
+  if (rc == MOE_OK)
+    rc = shared_product(x, ldx, weight, 1, ldw, y, ldy, pv.base, m, k, n, dtype, status, stream);
+  if (rc == MOE_OK)
+    rc = lora::expand(s, b, false, lora::Scale{scale, scale_all}, pv, dtype, m, n, adapters, rank, y, ldy, st);
+  return rc;
 }
 
-extern "C" int32_t moe_lora_expand(const void* s, const void* w, int64_t w_stride_l,
-                                   int64_t w_stride_row, int32_t w_transposed, const float* scale,
-                                   const int32_t* perm, const int32_t* offs, int32_t dtype, int64_t m,
-                                   int64_t n, int32_t adapters, int32_t rank, void* y, int64_t ldy,
-                                   void* stream) {
-  if (!dims_ok(dtype, m, n, adapters, rank)) return MOE_ERR_INVALID_ARG;
-  if (m == 0) return MOE_OK;
-  if (!rows_ok(y, ldy, n) || perm == nullptr || offs == nullptr || scale == nullptr || s == nullptr ||
-      !aligned16(s) ||
-      !(w_transposed ? weights_ok(w, w_stride_l, w_stride_row, rank, n, adapters)
-                     : weights_ok(w, w_stride_l, w_stride_row, n, rank, adapters)))
+extern "C" int32_t moe_lora_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx,
+                                     const void* weight, int64_t ldw, const void* lora_a,
+                                     int64_t a_stride_l, int64_t a_stride_row, const void* lora_b,
+                                     int64_t b_stride_l, int64_t b_stride_row, const float* scale,
+                                     float scale_all, int32_t dtype, int64_t m, int64_t k, int64_t n,
+                                     int32_t adapters, int32_t rank, int32_t* plan, const void* s, void* t,
+                                     void* dx, int64_t lddx, void* da, void* db, int32_t* status,
+                                     void* stream) {
+  const lora::Weights a{lora_a, a_stride_l, a_stride_row}, b{lora_b, b_stride_l, b_stride_row};
+  if (!dims_ok(dtype, m, k, n, adapters, rank) || plan == nullptr || !rows_ok(weight, ldw, k) ||
+      !weights_ok(a, rank, k, adapters) || !weights_ok(b, n, rank, adapters) ||
+      (da != nullptr && !aligned16(da)) || (db != nullptr && !aligned16(db)) ||
+      (m > 0 && (!rows_ok(dy, lddy, n) || !rows_ok(x, ldx, k) || s == nullptr || !aligned16(s) ||
+                 ((dx != nullptr || da != nullptr) && (t == nullptr || !aligned16(t))) ||
+                 (dx != nullptr && !rows_ok(dx, lddx, k)))))
     return MOE_ERR_INVALID_ARG;
-  return lora::dispatch(dtype, w_transposed != 0, rank, [&](auto t, auto tr, auto rp) {
-    using T = decltype(t);
-    constexpr bool kT = decltype(tr)::value;
-    constexpr int RP = decltype(rp)::value;
-    const int64_t tiles = lora::most_tiles(m, adapters, lora::kExpandRows);
-    const int64_t blocks = (n + lora::kExpandCols - 1) / lora::kExpandCols;
-    const int64_t want = (1200 + tiles - 1) / tiles;  // about four CTAs a place on the SMs
-    return lora::launch(lora::expand_kernel<T, kT, RP>,
-                        dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(want < blocks ? want : blocks)),
-                        lora::kThreads, dim3(1, 1), lora::ExpandCfg<kT, RP>::kBytes, static_cast<cudaStream_t>(stream),
-                        static_cast<const T*>(s), m * rank, static_cast<const T*>(w), w_stride_l,
-                        w_stride_row, scale, perm, offs, static_cast<int>(adapters), static_cast<int>(n),
-                        static_cast<int>(rank), static_cast<T*>(y), ldy);
-  });
-}
-
-extern "C" int32_t moe_lora_grad(const void* s, const void* z, int64_t ldz, const float* scale,
-                                 const int32_t* perm, const int32_t* offs, int32_t dtype, int64_t m,
-                                 int64_t n, int32_t adapters, int32_t rank, void* g, int64_t g_stride_l,
-                                 int64_t g_stride_row, int32_t g_transposed, void* stream) {
-  if (!dims_ok(dtype, m, n, adapters, rank)) return MOE_ERR_INVALID_ARG;
-  if (offs == nullptr || scale == nullptr ||
-      (m > 0 && (!rows_ok(z, ldz, n) || perm == nullptr || s == nullptr || !aligned16(s))) ||
-      !(g_transposed ? weights_ok(g, g_stride_l, g_stride_row, rank, n, adapters)
-                     : weights_ok(g, g_stride_l, g_stride_row, n, rank, adapters)))
-    return MOE_ERR_INVALID_ARG;
-  return lora::dispatch(dtype, g_transposed != 0, rank, [&](auto t, auto tr, auto rp) {
-    using T = decltype(t);
-    constexpr bool kT = decltype(tr)::value;
-    constexpr int RP = decltype(rp)::value;
-    using C = lora::GradCfg<RP>;
-    const unsigned blocks = static_cast<unsigned>((n + C::kCols - 1) / C::kCols);
-    // Adapters' rows are uneven, so many small parts: the largest adapter's rows spread.
-    const unsigned parts = lora::cluster_parts(int64_t(blocks) * adapters, 8 * 2 * 148, m / adapters, 64);
-    return lora::launch(lora::grad_kernel<T, kT, RP>, dim3(parts, blocks, adapters),
-                        lora::kThreads, dim3(parts, 1),
-                        C::kBytes, static_cast<cudaStream_t>(stream), static_cast<const T*>(s), m * rank,
-                        static_cast<const T*>(z), ldz, scale, perm, offs, static_cast<int>(n),
-                        static_cast<int>(rank), static_cast<T*>(g), g_stride_l, g_stride_row);
-  });
+  const lora::PlanView pv(plan, m, adapters);
+  const lora::Scale sc{scale, scale_all};
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  int rc = MOE_OK;
+  if (m > 0 && (dx != nullptr || da != nullptr))
+    rc = lora::shrink(dy, lddy, b, true, pv, dtype, m, n, adapters, rank, t, st);
+  if (rc == MOE_OK && m > 0 && dx != nullptr) {
+    rc = shared_product(dy, lddy, weight, ldw, 1, dx, lddx, pv.base, m, n, k, dtype, status, stream);
+    if (rc == MOE_OK)
+      rc = lora::expand(t, a, true, sc, pv, dtype, m, k, adapters, rank, dx, lddx, st);
+  }
+  if (rc == MOE_OK && da != nullptr)
+    rc = lora::grad(t, x, ldx, true, sc, pv, dtype, m, k, adapters, rank, da, st);
+  if (rc == MOE_OK && db != nullptr)
+    rc = lora::grad(s, dy, lddy, false, sc, pv, dtype, m, n, adapters, rank, db, st);
+  return rc;
 }

@@ -72,7 +72,7 @@ def _run(x, router_w, router_bias, w1, w2, top_k, renormalize, idx, w, out):
     if nbytes < 0:
         raise _lib.MoeError(_lib.MOE_ERR_INVALID_ARG, "moe_few_tokens_workspace")
     ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
+    with _lib.on_device(dev):
         rc = lib.moe_few_tokens(
             x.data_ptr(), x.stride(0),
             router_w.data_ptr() if router_w is not None else None,
@@ -81,7 +81,7 @@ def _run(x, router_w, router_bias, w1, w2, top_k, renormalize, idx, w, out):
             w1.data_ptr(), w1.stride(0), w1.stride(1), w2.data_ptr(), w2.stride(0), w2.stride(1),
             _DTYPE_CODE[dt], tokens, hidden, ffn, experts, top_k, 1 if renormalize else 0,
             idx.data_ptr(), w.data_ptr(), out.data_ptr(), out.stride(0), ws.data_ptr(), ws.numel(),
-            _lib.status_word(dev).data_ptr(), _lib.stream_handle(dev))
+            _lib.status_address(dev), _lib.stream_handle(dev))
     _lib.check_call(rc, "moe_few_tokens")
     if _lib.sync_check_enabled():
         _lib.check_status(dev, sync=True)

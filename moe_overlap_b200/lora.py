@@ -25,6 +25,8 @@ MAX_ADAPTERS = 1024
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """``t`` with unit-stride rows (and adapters) that start on 16 bytes, copied if needed."""
+    if t.is_contiguous() and t.shape[-1] % 8 == 0 and t.data_ptr() % 16 == 0:
+        return t
     ok = t.stride(-1) == 1 and t.stride(-2) % 8 == 0 and t.stride(-2) >= t.shape[-1]
     if t.dim() == 3 and t.shape[0] > 1:
         ok = ok and t.stride(0) % 8 == 0 and t.stride(0) >= t.stride(1) * t.shape[1]
@@ -33,66 +35,28 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t.clone(memory_format=torch.contiguous_format)
 
 
-class _Plan:
-    """The batch's rows by adapter: ``perm`` [M], ``offs`` [L + 1] and ``base`` {0, M}."""
-
-    def __init__(self, ids: torch.Tensor, adapters: int):
-        m, dev = ids.shape[0], ids.device
-        buf = torch.empty(m + adapters + 3, dtype=torch.int32, device=dev)
-        self.perm, self.offs, self.base = buf[:m], buf[m:m + adapters + 1], buf[m + adapters + 1:]
-        rc = _lib.load().moe_lora_plan(ids.data_ptr(), int(ids.dtype == torch.int64), m, adapters,
-                                       self.perm.data_ptr(), self.offs.data_ptr(),
-                                       self.base.data_ptr(), _lib.status_word(dev).data_ptr(),
-                                       _lib.stream_handle(dev))
-        _lib.check_call(rc, "moe_lora_plan")
+def _scale_args(scale):
+    return (scale.data_ptr(), 0.0) if isinstance(scale, torch.Tensor) else (None, scale)
 
 
-def _shared(x, w, stride_k, stride_n, n, plan):
-    """The shared product as the grouped GEMM of one expert, w[k, n] at the given strides.
-
-    The C entry directly: a bad adapter id, which the plan may just have recorded, is
-    raised by a later call and not by the middle of this one."""
-    m, k = x.shape
-    y = torch.empty(m, n, dtype=x.dtype, device=x.device)
-    sms = torch.cuda.get_device_properties(x.device).multi_processor_count
-    rc = _lib.load().moe_grouped_gemm(x.data_ptr(), x.stride(0), w.data_ptr(), 0, stride_k, stride_n,
-                                      y.data_ptr(), n, plan.base.data_ptr(), 0, m, k, n, 1,
-                                      _DTYPE_CODE[x.dtype], _lib.MOE_ACT_NONE, sms, 0, None,
-                                      _lib.status_word(x.device).data_ptr(),
-                                      _lib.stream_handle(x.device))
-    _lib.check_call(rc, "moe_grouped_gemm")
-    return y
-
-
-def _shrink(x, w, transposed, plan, rank):
-    m, k = x.shape
-    s = torch.empty(2, m, rank, dtype=x.dtype, device=x.device)
-    rc = _lib.load().moe_lora_shrink(x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), w.stride(1),
-                                     int(transposed), plan.perm.data_ptr(), plan.offs.data_ptr(),
-                                     _DTYPE_CODE[x.dtype], m, k, w.shape[0], rank, s.data_ptr(),
-                                     _lib.stream_handle(x.device))
-    _lib.check_call(rc, "moe_lora_shrink")
-    return s
-
-
-def _expand(s, w, transposed, scale, plan, y):
-    m, n = y.shape
-    rc = _lib.load().moe_lora_expand(s.data_ptr(), w.data_ptr(), w.stride(0), w.stride(1),
-                                     int(transposed), scale.data_ptr(), plan.perm.data_ptr(),
-                                     plan.offs.data_ptr(), _DTYPE_CODE[y.dtype], m, n, w.shape[0],
-                                     s.shape[2], y.data_ptr(), y.stride(0), _lib.stream_handle(y.device))
-    _lib.check_call(rc, "moe_lora_expand")
-
-
-def _grad(s, z, scale, plan, like, transposed):
-    g = torch.empty(like.shape, dtype=like.dtype, device=like.device)
-    m, n = z.shape
-    rc = _lib.load().moe_lora_grad(s.data_ptr(), z.data_ptr(), z.stride(0), scale.data_ptr(),
-                                   plan.perm.data_ptr(), plan.offs.data_ptr(), _DTYPE_CODE[z.dtype],
-                                   m, n, like.shape[0], s.shape[2], g.data_ptr(), g.stride(0),
-                                   g.stride(1), int(transposed), _lib.stream_handle(z.device))
-    _lib.check_call(rc, "moe_lora_grad")
-    return g
+def _forward(x, weight, lora_a, lora_b, ids, scale):
+    """(y, the buffer with the rows by adapter and x A^T that the backward needs)."""
+    (m, k), n = x.shape, weight.shape[0]
+    adapters, rank, _ = lora_a.shape
+    dev = x.device
+    y = torch.empty(m, n, dtype=x.dtype, device=dev)
+    low = 4 * m * rank  # bytes of x A^T: two parts of 16 bits; the plan stands behind it
+    kept = torch.empty(low + 4 * (m + adapters + 3), dtype=torch.uint8, device=dev)
+    at = kept.data_ptr()
+    with _lib.on_device(dev):
+        rc = _lib.load().moe_lora_forward(
+            x.data_ptr(), x.stride(0), weight.data_ptr(), weight.stride(0),
+            lora_a.data_ptr(), lora_a.stride(0), lora_a.stride(1),
+            lora_b.data_ptr(), lora_b.stride(0), lora_b.stride(1),
+            ids.data_ptr(), ids.dtype == torch.int64, *_scale_args(scale), _DTYPE_CODE[x.dtype], m, k, n,
+            adapters, rank, y.data_ptr(), n, at + low, at, _lib.status_address(dev), _lib.stream_handle(dev))
+    _lib.check_call(rc, "moe_lora_forward")
+    return y, kept
 
 
 class LoraLinear(torch.autograd.Function):
@@ -101,33 +65,36 @@ class LoraLinear(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, lora_a, lora_b, ids, scale):
-        with torch.cuda.device(x.device):
-            plan = _Plan(ids, lora_a.shape[0])
-            s = _shrink(x, lora_a, False, plan, lora_a.shape[1])
-            y = _shared(x, weight, 1, weight.stride(0), weight.shape[0], plan)
-            _expand(s, lora_b, False, scale, plan, y)
-        ctx.save_for_backward(x, weight, lora_a, lora_b, scale, s)
-        ctx.plan = plan
+        y, kept = _forward(x, weight, lora_a, lora_b, ids, scale)
+        ctx.save_for_backward(x, weight, lora_a, lora_b, kept)
+        ctx.scale = scale
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, weight, lora_a, lora_b, scale, s = ctx.saved_tensors
-        plan = ctx.plan
+        x, weight, lora_a, lora_b, kept = ctx.saved_tensors
         need_x, _, need_a, need_b, _, _ = ctx.needs_input_grad
-        dx = da = db = None
+        (m, k), n = x.shape, weight.shape[0]
+        adapters, rank, _ = lora_a.shape
+        dev, dt = x.device, x.dtype
         dy = _rows(dy)
-        with torch.cuda.device(x.device):
-            if need_x or need_a:
-                back = _shrink(dy, lora_b, True, plan, lora_a.shape[1])
-            if need_x:
-                dx = _shared(dy, weight, weight.stride(0), 1, weight.shape[1], plan)
-                _expand(back, lora_a, True, scale, plan, dx)
-            if need_a:
-                da = _grad(back, x, scale, plan, lora_a, True)
-            if need_b:
-                db = _grad(s, dy, scale, plan, lora_b, False)
+        dx = torch.empty(m, k, dtype=dt, device=dev) if need_x else None
+        da = torch.empty(adapters, rank, k, dtype=dt, device=dev) if need_a else None
+        db = torch.empty(adapters, n, rank, dtype=dt, device=dev) if need_b else None
+        low = 4 * m * rank
+        t = torch.empty(low, dtype=torch.uint8, device=dev) if need_x or need_a else None
+        at = kept.data_ptr()
+        with _lib.on_device(dev):
+            rc = _lib.load().moe_lora_backward(
+                dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0), weight.data_ptr(),
+                weight.stride(0), lora_a.data_ptr(), lora_a.stride(0), lora_a.stride(1),
+                lora_b.data_ptr(), lora_b.stride(0), lora_b.stride(1), *_scale_args(ctx.scale),
+                _DTYPE_CODE[dt], m, k, n, adapters, rank, at + low, at,
+                *(v.data_ptr() if v is not None else None for v in (t, dx)), k,
+                *(v.data_ptr() if v is not None else None for v in (da, db)),
+                _lib.status_address(dev), _lib.stream_handle(dev))
+        _lib.check_call(rc, "moe_lora_backward")
         return dx, None, da, db, None, None
 
 
@@ -143,8 +110,6 @@ def _leaf_nodes(*tensors):
     captured backward and break the capture in the autograd engine, so such a call
     marks it, and a call under capture that finds the mark is refused here instead.
     """
-    if not torch.is_grad_enabled():
-        return []
     capturing = torch.cuda.is_current_stream_capturing()
     nodes = [torch.autograd.graph.get_gradient_edge(t).node for t in tensors
              if t.requires_grad and t.is_leaf]
@@ -211,13 +176,17 @@ def lora_linear(x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor, lor
             raise ValueError("lora_linear gives the scale no gradient")
         scale = scale.to(device=x.device, dtype=torch.float32).contiguous()
     else:
-        scale = torch.full((adapters,), float(scale), dtype=torch.float32, device=x.device)
+        scale = float(scale)
     _lib.check_status(x.device)
-    nodes = _leaf_nodes(x, lora_a, lora_b)
     pk, pn, pr = -k % 8, -n % 8, -rank % 8
-    y = LoraLinear.apply(_rows(_pad(x, pk)), _rows(_pad(weight, pk, pn)), _rows(_pad(lora_a, pk, pr)),
-                         _rows(_pad(lora_b, pr, pn)), adapter_ids.contiguous(), scale)
-    del nodes
+    args = (_rows(_pad(x, pk)), _rows(_pad(weight, pk, pn)), _rows(_pad(lora_a, pk, pr)),
+            _rows(_pad(lora_b, pr, pn)), adapter_ids.contiguous(), scale)
+    if torch.is_grad_enabled() and (x.requires_grad or lora_a.requires_grad or lora_b.requires_grad):
+        nodes = _leaf_nodes(x, lora_a, lora_b)
+        y = LoraLinear.apply(*args)
+        del nodes
+    else:
+        y, _ = _forward(*args)
     if _lib.sync_check_enabled():
         _lib.check_status(x.device, sync=True)
     return y[:, :n] if pn else y
