@@ -103,44 +103,43 @@ __device__ __forceinline__ void warp_topk(const double* z, int E, int k, bool re
   }
   // The exponent's argument is a difference of fp64 logits, rounded once to fp32.
   float s = 0.0f;
+  // Order-preserving words for the search: a larger word is a larger logit (+0 and -0
+  // are one); 0 is below every logit's word and marks no candidate.
+  uint64_t key[kPer];
 #pragma unroll
-  for (int i = 0; i < kPer; ++i)
-    if (lane + 32 * i < E) s += expf(static_cast<float>(v[i] - m));
-  s = warp_sum(s);
-  uint32_t taken = 0;  // bit i: this lane's expert i is taken
-  float my_w = 0.0f, wsum = 0.0f;
-  int my_e = 0;
-  for (int j = 0; j < k; ++j) {
-    double best = -INFINITY;
-    int be = 0x7fffffff;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int e = lane + 32 * i;
-      if (e < E && !(taken >> i & 1u) && (be == 0x7fffffff || v[i] > best)) {
-        best = v[i];
-        be = e;
-      }
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const double ob = __shfl_xor_sync(0xffffffffu, best, o);
-      const int oe = __shfl_xor_sync(0xffffffffu, be, o);
-      if (oe != 0x7fffffff && (be == 0x7fffffff || ob > best || (ob == best && oe < be))) {
-        best = ob;
-        be = oe;
-      }
-    }
-    if ((be & 31) == lane) taken |= 1u << (be >> 5);
-    const float p = expf(static_cast<float>(best - m)) / s;
-    wsum += p;
-    if (lane == j) {
-      my_w = p;
-      my_e = be;
+  for (int i = 0; i < kPer; ++i) {
+    key[i] = 0;
+    if (lane + 32 * i < E) {
+      s += expf(static_cast<float>(v[i] - m));
+      const uint64_t b = static_cast<uint64_t>(__double_as_longlong(v[i] + 0.0));
+      key[i] = (b >> 63) ? ~b : b | (1ull << 63);
     }
   }
+  s = warp_sum(s);
+  double my_z = 0.0;
+  int my_e = 0;
+  for (int j = 0; j < k; ++j) {
+    uint64_t best = key[0];
+    int be = lane;
+#pragma unroll
+    for (int i = 1; i < kPer; ++i)
+      if (key[i] > best) best = key[i], be = lane + 32 * i;
+    const uint32_t hi = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(best >> 32));
+    const uint32_t lo = __reduce_max_sync(
+        0xffffffffu, static_cast<uint32_t>(best >> 32) == hi ? static_cast<uint32_t>(best) : 0u);
+    const bool mine = best == ((static_cast<uint64_t>(hi) << 32) | lo);
+    be = static_cast<int>(__reduce_min_sync(0xffffffffu, mine ? static_cast<uint32_t>(be) : 0xffffffffu));
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (lane + 32 * i == be) key[i] = 0;
+    if (lane == j) my_e = be;
+  }
+  if (lane < k) my_z = z[my_e];
+  const float p = lane < k ? expf(static_cast<float>(my_z - m)) / s : 0.0f;
+  const float sum = renorm ? warp_sum(p) : 1.0f;
   if (lane < k) {
     idx_out[lane] = my_e;
-    w_out[lane] = renorm ? my_w / wsum : my_w;
+    w_out[lane] = p / sum;
   }
 }
 
@@ -310,17 +309,21 @@ __device__ __forceinline__ void build_plan(const Params& p, int NT, Plan* pl, in
     const int64_t e = p.idx[i];
     if (e < -1 || e >= p.E) record_status(p.status, MOE_ERR_INVALID_ARG);
     pl->expert_of_slot[i] = (e >= 0 && e < p.E) ? static_cast<int16_t>(e) : int16_t(-1);
-    pl->pos_of[i] = 0xffff;
   }
+  for (int e = tid; e < p.E; e += kThreads) cnt[e] = 0;
   __syncthreads();
-  if (tid < p.E) {
-    int c = 0;
-    for (int i = 0; i < S; ++i) c += pl->expert_of_slot[i] == tid;
-    cnt[tid] = c;
-  }
-  __syncthreads();
-  if (tid < 32) {  // prefix sums over the experts: slots and groups
-    int run_s = 0, run_g = 0;
+  if (tid < 32) {
+    // Each slot's rank among its expert's, 32 slots at a time in slot order.
+    for (int b = 0; b < S; b += 32) {
+      const int i = b + tid, e = i < S ? pl->expert_of_slot[i] : -1;
+      const unsigned same = __match_any_sync(0xffffffffu, e);
+      const int before = e >= 0 ? cnt[e] : 0;
+      if (i < S) pl->pos_of[i] = static_cast<uint16_t>(before + __popc(same & ((1u << tid) - 1u)));
+      __syncwarp();
+      if (e >= 0 && (same >> tid) == 1u) cnt[e] = before + __popc(same);
+      __syncwarp();
+    }
+    int run_s = 0, run_g = 0;  // prefix sums over the experts: slots and groups
     for (int b = 0; b < p.E; b += 32) {
       const int e = b + tid;
       const int c = e < p.E ? cnt[e] : 0, g = (c + NT - 1) / NT;
@@ -346,16 +349,16 @@ __device__ __forceinline__ void build_plan(const Params& p, int NT, Plan* pl, in
     }
   }
   __syncthreads();
-  if (tid < p.E) {
-    const int s0 = cnt[tid];
-    int at = s0, g = grp_first[tid];
-    for (int i = 0; i < S; ++i)
-      if (pl->expert_of_slot[i] == tid) {
-        if ((at - s0) % NT == 0) grp[g++] = (tid << 16) | at;
-        pl->slot_at[at] = static_cast<uint16_t>(i);
-        pl->pos_of[i] = static_cast<uint16_t>(at);
-        ++at;
-      }
+  for (int i = tid; i < S; i += kThreads) {
+    const int e = pl->expert_of_slot[i], rank = pl->pos_of[i];
+    if (e < 0) {
+      pl->pos_of[i] = 0xffff;
+      continue;
+    }
+    const int at = cnt[e] + rank;
+    if (rank % NT == 0) grp[grp_first[e] + rank / NT] = (e << 16) | at;
+    pl->slot_at[at] = static_cast<uint16_t>(i);
+    pl->pos_of[i] = static_cast<uint16_t>(at);
   }
   __syncthreads();
 }
@@ -399,6 +402,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     tma_prefetch_desc(&map2);
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");  // the gate's idx, w and counters
+  int ticket = 0;  // the fetching thread's first, on its way while the plan is made
+  if (tid == 0) ticket = atomicAdd(p.count, 1);
   build_plan(p, NT, plan, grp, cnt, grp_first);
   const int G = plan->n_groups, S = plan->n_slots;
   const int FB = (p.F + BM - 1) / BM, HB = (p.H + BM - 1) / BM;
@@ -442,7 +447,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 0) {
       int stage = 0;
       uint32_t phase = 0;
-      int next = atomicAdd(p.count, 1);
+      int next = ticket;
       for (int n = 0;; ++n) {
         const int item = next;
         const bool end = item >= items;
@@ -669,20 +674,26 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int col = row16 + (lane & 3) * 4;  // 4 columns of 8 tokens at a time (H: multiple of 8)
     if (col >= p.H) continue;
     const int64_t part_stride = int64_t(p.T) * p.k * p.H;
+    const int parts = p.KS * C, terms = p.k * parts;
     for (int t = lane >> 2; t < p.T; t += 8) {
       float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      for (int j = 0; j < p.k; ++j) {
-        const int pos = plan->pos_of[t * p.k + j];
-        if (pos == 0xffff) continue;
-        float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        const float* src = p.part + int64_t(pos) * p.H + col;
-#pragma unroll 4
-        for (int i = 0; i < p.KS * C; ++i) {
-          const float4 u = __ldcg(reinterpret_cast<const float4*>(src + i * part_stride));
-          y.x += u.x, y.y += u.y, y.z += u.z, y.w += u.w;
+      for (int b = 0; b < terms; b += 8) {  // 8 loads under way at a time
+        float4 u[8];
+        float wt[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          const int j = (b + q) / parts, i = (b + q) - j * parts;
+          const int pos = b + q < terms ? plan->pos_of[t * p.k + j] : 0xffff;
+          u[q] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          wt[q] = 0.0f;
+          if (pos != 0xffff) {
+            u[q] = __ldcg(reinterpret_cast<const float4*>(p.part + i * part_stride + int64_t(pos) * p.H + col));
+            wt[q] = p.w[t * p.k + j];
+          }
         }
-        const float wt = p.w[t * p.k + j];
-        v[0] += wt * y.x, v[1] += wt * y.y, v[2] += wt * y.z, v[3] += wt * y.w;
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+          v[0] += wt[q] * u[q].x, v[1] += wt[q] * u[q].y, v[2] += wt[q] * u[q].z, v[3] += wt[q] * u[q].w;
       }
       T o[4];
 #pragma unroll
