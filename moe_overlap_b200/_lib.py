@@ -305,7 +305,8 @@ def check_call(code: int, where: str) -> None:
 
 
 def stream_handle(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(
+        device.index if device.index is not None else torch.cuda.current_device())
 
 
 def sync_check_enabled() -> bool:

@@ -290,11 +290,6 @@ __device__ __forceinline__ int ld_acquire_gpu(const int* p) {
 __device__ __forceinline__ void red_release_gpu(int* p, int v) {
   asm volatile("red.release.gpu.global.add.s32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
 }
-__device__ __forceinline__ int add_acq_rel_gpu(int* p, int v) {
-  int r;
-  asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], %2;" : "=r"(r) : "l"(p), "r"(v) : "memory");
-  return r;
-}
 // The 8 warps of one set.
 __device__ __forceinline__ void set_sync(int set) {
   asm volatile("bar.sync %0, 256;" ::"r"(1 + set) : "memory");
@@ -554,7 +549,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint32_t phase = 0;
   for (int n = 0;; ++n) {
     const int item = pop(n);
-    if (item < 0) return;
+    if (item < 0) break;
     const Item it = decode(item);
     if (n % kSets != set) {  // the other set's item: past its stages
       stage += (it.c1 - it.c0 + BKS - 1) / BKS;
@@ -654,8 +649,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       continue;
     }
 
-    // This warp's part of 16 rows of W2; whoever brings the last part of them adds the
-    // slots' parts in a fixed order.
+    // This warp's part of 16 rows of W2.
     const int row16 = it.blk * BM + rt * 16;
     if (row16 >= p.H) continue;
     float* part = p.part + (int64_t(it.ks * C + cs) * p.T * p.k + pos0) * p.H + row16;
@@ -667,47 +661,56 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (nn < rows && row16 + m < p.H) part[int64_t(nn) * p.H + m] = acc[j][i];
       }
     __syncwarp();
-    int before = 0;
-    if (lane == 0) before = add_acq_rel_gpu(done + it.blk * R + rt, 1);
-    before = __shfl_sync(0xffffffffu, before, 0);
-    if (before != G * p.KS * C - 1) continue;
-    const int col = row16 + (lane & 3) * 4;  // 4 columns of 8 tokens at a time (H: multiple of 8)
-    if (col >= p.H) continue;
-    const int64_t part_stride = int64_t(p.T) * p.k * p.H;
-    const int parts = p.KS * C, terms = p.k * parts;
-    for (int t = lane >> 2; t < p.T; t += 8) {
-      float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      for (int b = 0; b < terms; b += 8) {  // 8 loads under way at a time
-        float4 u[8];
-        float wt[8];
-#pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          const int j = (b + q) / parts, i = (b + q) - j * parts;
-          const int pos = b + q < terms ? plan->pos_of[t * p.k + j] : 0xffff;
-          u[q] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-          wt[q] = 0.0f;
-          if (pos != 0xffff) {
-            u[q] = __ldcg(reinterpret_cast<const float4*>(p.part + i * part_stride + int64_t(pos) * p.H + col));
-            wt[q] = p.w[t * p.k + j];
-          }
-        }
-#pragma unroll
-        for (int q = 0; q < 8; ++q)
-          v[0] += wt[q] * u[q].x, v[1] += wt[q] * u[q].y, v[2] += wt[q] * u[q].z, v[3] += wt[q] * u[q].w;
+    if (lane == 0) red_release_gpu(done + it.blk * R + rt, 1);
+  }
+
+  // The weighted sums over the slots and their parts, in a fixed order: every warp of
+  // the grid takes blocks of 16 columns x 8 tokens.  The items are all taken by now, by
+  // CTAs that run, so the waits for their parts end.
+  const int t_groups = (p.T + 7) / 8, units = (p.H + 15) / 16 * t_groups;
+  const int parts = p.KS * C, terms = p.k * parts;
+  const int64_t part_stride = int64_t(p.T) * p.k * p.H;
+  for (int u = (warp - 2) * gridDim.x + blockIdx.x; u < units; u += kSets * kConsumers * gridDim.x) {
+    const int blk16 = u / t_groups, t = u % t_groups * 8 + (lane >> 2);
+    const int col = blk16 * 16 + (lane & 3) * 4;  // 4 columns of one token a lane (H: a multiple of 8)
+    const long long t0 = clock64();
+    while (ld_acquire_gpu(done + blk16) < G * parts)
+      if (clock64() - t0 > kWaitBudgetCycles) {
+        record_status(p.status, MOE_ERR_TIMEOUT);
+        break;
       }
-      T o[4];
+    if (t >= p.T || col >= p.H) continue;
+    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    int j = 0, i = 0;
+    for (int b = 0; b < terms; b += 8) {  // 8 loads under way at a time
+      float4 y[8];
+      float wt[8];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = from_f<T>(v[i]);
-      *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + t * p.ldo + col) =
-          *reinterpret_cast<const uint2*>(o);
+      for (int q = 0; q < 8; ++q) {
+        y[q] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        wt[q] = 0.0f;
+        const int pos = b + q < terms ? plan->pos_of[t * p.k + j] : 0xffff;
+        if (pos != 0xffff) {
+          y[q] = __ldcg(reinterpret_cast<const float4*>(p.part + i * part_stride + int64_t(pos) * p.H + col));
+          wt[q] = p.w[t * p.k + j];
+        }
+        if (++i == parts) i = 0, ++j;
+      }
+#pragma unroll
+      for (int q = 0; q < 8; ++q)
+        v[0] += wt[q] * y[q].x, v[1] += wt[q] * y[q].y, v[2] += wt[q] * y[q].z, v[3] += wt[q] * y[q].w;
     }
+    T o[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) o[q] = from_f<T>(v[q]);
+    *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + t * p.ldo + col) = *reinterpret_cast<const uint2*>(o);
   }
 }
 
-// Parts of F in W2's items, of about 1024 columns, fewer when there are many slots (then
+// Parts of F in W2's items, of about 2048 columns, fewer when there are many slots (then
 // there are many groups, and the parts' sums cost more than their balance gains).
 inline int k_splits(int F, int64_t S) {
-  const int64_t fine = (F + 1023) / 1024, most = S < 1 || S >= 1024 ? 1 : 1024 / S;
+  const int64_t fine = (F + 2047) / 2048, most = S < 1 || S >= 1024 ? 1 : 1024 / S;
   return static_cast<int>(fine < most ? fine : most);
 }
 
@@ -782,12 +785,22 @@ int launch(Params p, const void* rw, int64_t ldr, const float* bias, const void*
   } else if (cudaMemsetAsync(p.count, 0, lay.count_bytes(), s) != cudaSuccess) {
     return MOE_ERR_CUDA;
   }
-  // Narrow row blocks give a few tokens' few experts enough items for every SM; with
-  // more tokens, blocks of 128 rows need no sums across warps and fetch each slot's
-  // columns once for all 8 (one token of 16 x 2048 x 4096, R = 4 against 8: 32.5 and
-  // 34.1 us; 16 tokens of 16 x 2048 x 8192: 166 and 149 us).
-  return p.T <= 8 ? launch_experts<T, 4, 1>(p, w1, w1_se, w1_sr, w2, w2_se, w2_sr, rw != nullptr, sms, s)
-                  : launch_experts<T, 8, 2>(p, w1, w1_se, w1_sr, w2, w2_se, w2_sr, rw != nullptr, sms, s);
+  auto go = [&](auto r, auto j) {
+    return launch_experts<T, decltype(r)::value, decltype(j)::value>(p, w1, w1_se, w1_sr, w2, w2_se, w2_sr,
+                                                                     rw != nullptr, sms, s);
+  };
+  using std::integral_constant;
+  // Blocks of 128 rows need no sums across warps and fetch each slot's columns once for
+  // all 8 warps; a few tokens' few experts make too few of them for every SM and get
+  // blocks of 32 rows (one token of 16 experts of 2048 x 4096: 28.6 us with 32 rows,
+  // 33.5 with 128; 37 tokens of 64 experts of 2048 x 1024, 174 and 98 us).
+  const int64_t S = int64_t(p.T) * p.k, groups = S < p.E ? S : p.E;
+  const bool narrow = groups * ((p.F + 127) / 128) < sms;
+  if (p.T <= 8)  // no expert has more than 8 slots, unless it is repeated
+    return narrow ? go(integral_constant<int, 2>(), integral_constant<int, 1>())
+                  : go(integral_constant<int, 8>(), integral_constant<int, 1>());
+  return narrow ? go(integral_constant<int, 2>(), integral_constant<int, 2>())
+                : go(integral_constant<int, 8>(), integral_constant<int, 2>());
 }
 
 }  // namespace few

@@ -101,25 +101,27 @@ class LoraLinear(torch.autograd.Function):
 _EAGER = "moe_overlap_b200.lora_linear ran outside a capture"
 
 
-def _leaf_nodes(*tensors):
-    """The gradient accumulators of the leaves among ``tensors``, to be held until the
-    forward's graph holds them.
+def _guard_capture(y, inputs, given):
+    """Refuses a capture that could not be used.
 
-    An accumulator belongs to the stream that it was made on and lives as long as any
-    graph of its leaf.  One left from a call outside would pull that stream into a
-    captured backward and break the capture in the autograd engine, so such a call
-    marks it, and a call under capture that finds the mark is refused here instead.
+    The gradient accumulator of a leaf belongs to the stream that it was made on and
+    lives as long as any graph of the leaf.  One left from a call outside would pull
+    that stream into a captured backward and break the capture in the autograd engine;
+    so a call outside marks the accumulators, and a call under capture that finds the
+    mark is refused here instead.
     """
     capturing = torch.cuda.is_current_stream_capturing()
-    nodes = [torch.autograd.graph.get_gradient_edge(t).node for t in tensors
-             if t.requires_grad and t.is_leaf]
-    for node in nodes:
+    edges = y.grad_fn.next_functions
+    for at in (0, 2, 3):  # x, lora_a, lora_b
+        t = given[at]
+        if not (t.requires_grad and t.is_leaf):
+            continue
+        node = edges[at][0] if inputs[at] is t else torch.autograd.graph.get_gradient_edge(t).node
         if not capturing:
             node.metadata[_EAGER] = True
         elif _EAGER in node.metadata:
             raise RuntimeError("lora_linear: a graph of the same inputs from a call outside the capture "
                                "is alive; drop its outputs before capturing a training step")
-    return nodes
 
 
 def _pad(t: torch.Tensor, *by: int) -> torch.Tensor:
@@ -148,25 +150,26 @@ def lora_linear(x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor, lor
     as for every autograd graph, no graph of the same leaves from before the capture
     may be alive then.
     """
-    if x.device.type != "cuda":
+    dev, dt = x.device, x.dtype
+    if dev.type != "cuda":
         raise ValueError("lora_linear requires CUDA tensors.")
     if x.dim() != 2 or weight.dim() != 2 or lora_a.dim() != 3 or lora_b.dim() != 3:
         raise ValueError("Shapes must be x [M, K], weight [N, K], lora_a [L, r, K], lora_b [L, N, r].")
     (m, k), n = x.shape, weight.shape[0]
-    adapters, rank, _ = lora_a.shape
-    if weight.shape != (n, k) or lora_a.shape[2] != k or lora_b.shape != (adapters, n, rank):
+    adapters, rank, width = lora_a.shape
+    if weight.shape != (n, k) or width != k or lora_b.shape != (adapters, n, rank):
         raise ValueError("Shapes must be x [M, K], weight [N, K], lora_a [L, r, K], lora_b [L, N, r].")
     if k == 0 or n == 0 or not 1 <= rank <= MAX_RANK or not 1 <= adapters <= MAX_ADAPTERS:
         raise ValueError(f"ranks go from 1 to {MAX_RANK}, adapters from 1 to {MAX_ADAPTERS}, and K "
                          "and N must not be 0")
-    if x.dtype not in _DTYPE_CODE:
+    if dt not in _DTYPE_CODE:
         raise ValueError("x dtype must be bf16/fp16.")
     for name, t in (("weight", weight), ("lora_a", lora_a), ("lora_b", lora_b)):
-        if t.dtype != x.dtype or t.device != x.device:
-            raise ValueError(f"{name} must be a {x.dtype} tensor on {x.device}")
-    if adapter_ids.shape != (m,) or adapter_ids.device != x.device or \
+        if t.dtype != dt or t.device != dev:
+            raise ValueError(f"{name} must be a {dt} tensor on {dev}")
+    if adapter_ids.shape != (m,) or adapter_ids.device != dev or \
             adapter_ids.dtype not in (torch.int32, torch.int64):
-        raise ValueError(f"adapter_ids must be an int32 or int64 tensor [M] on {x.device}")
+        raise ValueError(f"adapter_ids must be an int32 or int64 tensor [M] on {dev}")
     if weight.requires_grad and torch.is_grad_enabled():
         raise ValueError("the shared weight is frozen: lora_linear gives it no gradient")
     if isinstance(scale, torch.Tensor):
@@ -177,14 +180,16 @@ def lora_linear(x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor, lor
         scale = scale.to(device=x.device, dtype=torch.float32).contiguous()
     else:
         scale = float(scale)
-    _lib.check_status(x.device)
+    _lib.check_status(dev)
     pk, pn, pr = -k % 8, -n % 8, -rank % 8
-    args = (_rows(_pad(x, pk)), _rows(_pad(weight, pk, pn)), _rows(_pad(lora_a, pk, pr)),
-            _rows(_pad(lora_b, pr, pn)), adapter_ids.contiguous(), scale)
+    if pk or pn or pr:
+        args = (_rows(_pad(x, pk)), _rows(_pad(weight, pk, pn)), _rows(_pad(lora_a, pk, pr)),
+                _rows(_pad(lora_b, pr, pn)), adapter_ids.contiguous(), scale)
+    else:
+        args = (_rows(x), _rows(weight), _rows(lora_a), _rows(lora_b), adapter_ids.contiguous(), scale)
     if torch.is_grad_enabled() and (x.requires_grad or lora_a.requires_grad or lora_b.requires_grad):
-        nodes = _leaf_nodes(x, lora_a, lora_b)
         y = LoraLinear.apply(*args)
-        del nodes
+        _guard_capture(y, args, (x, weight, lora_a, lora_b))
     else:
         y, _ = _forward(*args)
     if _lib.sync_check_enabled():
