@@ -576,9 +576,11 @@ MOE_API int32_t moe_few_tokens(const void* x, int64_t ldx, const void* router_w,
  *   ids [m]         int32, or int64 if ids_int64; an id outside [-1, adapters) counts
  *                   as -1 and records MOE_ERR_INVALID_ARG in `status`
  *   scale           float[adapters], or NULL: scale_all for every adapter
+ *   for_backward    nonzero: plan and s are kept for moe_lora_backward; 0: they are
+ *                   workspace, and few rows take kernels of their own
  *   plan            int32 [m + adapters + 3], out: the rows by adapter
- *   s               2 m rank elements of `dtype`, out: x[r] A[i]^T in plan order, the
- *                   rounded values and what the rounding left
+ *   s               4 m rank bytes, out: x[r] A[i]^T in plan order, two elements of
+ *                   `dtype`, the rounded values and then what the rounding left
  * dtype is MOE_DTYPE_BF16 or MOE_DTYPE_F16.  Rows start on 16 bytes; k, n and rank are
  * multiples of 8; rank <= 128; adapters <= 1024.  Sums are fp32.
  */
@@ -587,8 +589,8 @@ MOE_API int32_t moe_lora_forward(const void* x, int64_t ldx, const void* weight,
                                  const void* lora_b, int64_t b_stride_l, int64_t b_stride_row,
                                  const void* ids, int32_t ids_int64, const float* scale,
                                  float scale_all, int32_t dtype, int64_t m, int64_t k, int64_t n,
-                                 int32_t adapters, int32_t rank, void* y, int64_t ldy, int32_t* plan,
-                                 void* s, int32_t* status, void* stream);
+                                 int32_t adapters, int32_t rank, int32_t for_backward, void* y,
+                                 int64_t ldy, int32_t* plan, void* s, int32_t* status, void* stream);
 
 /*
  * Gradients of moe_lora_forward, from its plan and s: dx [m, k], da [adapters, rank, k]

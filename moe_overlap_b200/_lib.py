@@ -200,7 +200,7 @@ SIGNATURES: dict[str, tuple] = {
         [_c_void_p, _i64, _c_void_p, _i64,  # x, ldx, weight, ldw
          _c_void_p, _i64, _i64, _c_void_p, _i64, _i64,  # lora_a, strides l/row, lora_b, strides l/row
          _c_void_p, _i32, _c_void_p, ctypes.c_float,  # ids, ids_int64, scale, scale_all
-         _i32, _i64, _i64, _i64, _i32, _i32,  # dtype, m, k, n, adapters, rank
+         _i32, _i64, _i64, _i64, _i32, _i32, _i32,  # dtype, m, k, n, adapters, rank, for_backward
          _c_void_p, _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p],  # y, ldy, plan, s, status, stream
     ),
     "moe_lora_backward": (

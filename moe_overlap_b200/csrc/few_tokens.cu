@@ -9,8 +9,6 @@
 // A slot with expert -1 adds nothing; a token without any expert gets zeros.
 // Sums are fp32, h is rounded to the input type (the matrix operand of the second
 // product, as in the layer's own path), the output is rounded once.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -18,6 +16,7 @@
 
 #include "../../include/moe_overlap.h"
 #include "host_common.h"
+#include "mma16.cuh"
 #include "ptx.cuh"
 
 namespace moe {
@@ -27,35 +26,6 @@ constexpr int kMaxTokens = 128;
 constexpr int kMaxE = 256;
 constexpr int kMaxK = 16;
 constexpr int kWarps = 8;
-
-template <typename T>
-__device__ __forceinline__ float to_f(T v) {
-  if constexpr (sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value)
-    return __bfloat162float(v);
-  else
-    return __half2float(v);
-}
-template <typename T>
-__device__ __forceinline__ T from_f(float v) {
-  if constexpr (std::is_same<T, __nv_bfloat16>::value)
-    return __float2bfloat16_rn(v);
-  else
-    return __float2half_rn(v);
-}
-
-template <typename T>
-constexpr float kMaxOf = std::is_same<T, __nv_bfloat16>::value ? 3.38953139e38f : 65504.0f;
-
-__device__ __forceinline__ double warp_sum(double v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
 
 // Dot product of two rows of `n` elements (a multiple of 8, 16-byte aligned) over one
 // warp.  A product of two bf16 or fp16 values is exact in fp32; the sum is fp64.
@@ -155,7 +125,7 @@ __global__ void __cluster_dims__(kGateCluster, 1, 1) __launch_bounds__(32 * kWar
                 int k, int renorm, int64_t* idx, float* w, int32_t* count, int n_count) {
   __shared__ double z[kMaxE];
   __shared__ double partial[kMaxE / kGateCluster][kWarps];
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  let_next_kernel_start();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int rank = static_cast<int>(cluster_ctarank()), t = blockIdx.x / kGateCluster;
   if (blockIdx.x == 0)
@@ -251,45 +221,6 @@ struct Ctrl {
   int item[kQueue];
 };
 
-template <typename T>
-__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                    uint32_t b0, uint32_t b1) {
-  if constexpr (std::is_same<T, __nv_bfloat16>::value)
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-        "{%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-  else
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-        "{%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
-__device__ __forceinline__ void ld_shared_v4(uint32_t addr, uint32_t* r) {
-  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr));
-}
-// 16 bytes to shared memory, zeros when `bytes` is 0 (nothing is read then).
-__device__ __forceinline__ void copy_async_16(uint32_t dst, const void* src, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
-               : "memory");
-}
-// Arrives on `bar` when this thread's earlier copies have landed.
-__device__ __forceinline__ void copies_arrive(uint32_t bar) {
-  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ int ld_acquire_gpu(const int* p) {
-  int v;
-  asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
-  return v;
-}
-__device__ __forceinline__ void red_release_gpu(int* p, int v) {
-  asm volatile("red.release.gpu.global.add.s32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
-}
 // The 8 warps of one set.
 __device__ __forceinline__ void set_sync(int set) {
   asm volatile("bar.sync %0, 256;" ::"r"(1 + set) : "memory");
@@ -396,7 +327,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tma_prefetch_desc(&map1);
     tma_prefetch_desc(&map2);
   }
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // the gate's idx, w and counters
+  wait_for_previous_kernel();  // the gate's idx, w and counters
   int ticket = 0;  // the fetching thread's first, on its way while the plan is made
   if (tid == 0) ticket = atomicAdd(p.count, 1);
   build_plan(p, NT, plan, grp, cnt, grp_first);
@@ -524,14 +455,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           return;
         }
         const uint32_t dst = smem_u32(slots + stage * 2 * K::kSlotBytes);
-        const int bytes = c + piece8 < it.c1 ? 16 : 0;
-        const int from = bytes ? c : it.c0;
+        const bool in = c + piece8 < it.c1;
+        const int from = in ? c : it.c0;
 #pragma unroll
         for (int i = 0; i < kPasses; ++i) {
           if (i * 32 / kPieces >= rows) break;
           if (src[i] != nullptr) {
-            copy_async_16(dst + off[i], src[i] + from, bytes);
-            if (it.down) copy_async_16(dst + off[i] + K::kSlotBytes, src[i] + from + (h_lo - h), bytes);
+            copy_async_16(dst + off[i], src[i] + from, in);
+            if (it.down) copy_async_16(dst + off[i] + K::kSlotBytes, src[i] + from + (h_lo - h), in);
           }
         }
         copies_arrive(full);
@@ -612,10 +543,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (!it.down) {
       auto put_h = [&](int nn, int row, float v) {
         const float a = 0.5f * v * (1.0f + erff(v * 0.70710678118654752440f));
-        // what is beyond the type's largest value goes to the second part as well
-        const T hi = from_f<T>(fminf(fmaxf(a, -kMaxOf<T>), kMaxOf<T>));
-        h[int64_t(pos0 + nn) * p.F + row] = hi;
-        h_lo[int64_t(pos0 + nn) * p.F + row] = from_f<T>(a - to_f(hi));
+        const int64_t at = int64_t(pos0 + nn) * p.F + row;
+        split(a, h + at, h_lo + at);
       };
       if constexpr (C == 1) {
 #pragma unroll

@@ -11,8 +11,6 @@
 //   grad    dB[i] = scale[i] sum_p dy[perm[p]]^T s[p]  (also dA[i])
 // s is held as two values of the inputs' type, the rounded one and what the rounding
 // left (16 bits or more in all): the operand of a second tensor-core product.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -20,6 +18,8 @@
 
 #include "../../include/moe_overlap.h"
 #include "host_common.h"
+#include "lora.cuh"
+#include "mma16.cuh"
 #include "ptx.cuh"
 
 namespace moe {
@@ -27,27 +27,6 @@ namespace lora {
 
 constexpr int kMaxAdapters = 1024;
 constexpr int kMaxRank = 128;
-
-template <typename T>
-__device__ __forceinline__ float to_f(T v) {
-  if constexpr (std::is_same<T, __nv_bfloat16>::value)
-    return __bfloat162float(v);
-  else
-    return __half2float(v);
-}
-template <typename T>
-__device__ __forceinline__ T from_f(float v) {
-  if constexpr (std::is_same<T, __nv_bfloat16>::value)
-    return __float2bfloat16_rn(v);
-  else
-    return __float2half_rn(v);
-}
-// One number for each adapter, or one for all.
-struct Scale {
-  const float* each;
-  float all;
-  __device__ float of(int i) const { return each != nullptr ? each[i] : all; }
-};
 
 // One block per adapter: it counts the rows of smaller adapters (its segment's start)
 // and writes its own rows in order.  No block depends on another and the order is
@@ -110,44 +89,6 @@ __global__ void __launch_bounds__(1024) plan_kernel(const void* ids, int ids64, 
 constexpr int kThreads = 256;        // expand and grad
 constexpr int kShrinkThreads = 128;  // 4 warps of 32 rows: each reads all of w's tile from shared memory
 
-template <typename T>
-__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if constexpr (std::is_same<T, __nv_bfloat16>::value)
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-        "{%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-        "{%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-template <bool kTrans>
-__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
-  if constexpr (kTrans)
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(addr)
-                 : "memory");
-  else
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(addr)
-                 : "memory");
-}
-// 16 bytes to shared memory, zeros (and nothing read) unless `in`.
-__device__ __forceinline__ void copy_async_16(uint32_t dst, const void* src, bool in) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0)
-               : "memory");
-}
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int kLeft>
-__device__ __forceinline__ void copies_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory");
-}
 // The sum over the cluster's CTAs, in their order, of 4 floats at this CTA's address
 // `at`; every CTA's load is under way before the first is used.
 __device__ __forceinline__ float4 cluster_sum4(const float* at, int parts) {
@@ -201,15 +142,6 @@ __device__ __forceinline__ Tile find_tile(const int32_t* offs, int L, int tile, 
     before += __shfl_sync(0xffffffffu, incl, 31);
   }
   return t;
-}
-
-// A value as two of type T: rounded, and what the rounding left (what is beyond the
-// type's largest value goes to the second part as well).
-template <typename T>
-__device__ __forceinline__ void split(float v, T* hi, T* lo) {
-  const float big = std::is_same<T, __nv_bfloat16>::value ? 3.38953139e38f : 65504.0f;
-  *hi = from_f<T>(fminf(fmaxf(v, -big), big));
-  *lo = from_f<T>(v - to_f(*hi));
 }
 
 // shrink.  A CTA forms 128 rows x RP of s over one part of k; the CTAs of a cluster
@@ -696,11 +628,6 @@ struct PlanView {
   PlanView(int32_t* plan, int64_t m, int adapters)
       : perm(plan), offs(plan + m), base(plan + m + adapters + 1) {}
 };
-struct Weights {  // of all adapters
-  const void* p;
-  int64_t stride_l, stride_row;
-};
-
 // s = x w^T by adapter, w in rows of k (transposed: in rows of the rank).
 int shrink(const void* x, int64_t ldx, Weights w, bool transposed, PlanView plan, int dtype, int64_t m,
            int64_t k, int adapters, int rank, void* s, cudaStream_t stream) {
@@ -790,8 +717,8 @@ extern "C" int32_t moe_lora_forward(const void* x, int64_t ldx, const void* weig
                                     const void* lora_b, int64_t b_stride_l, int64_t b_stride_row,
                                     const void* ids, int32_t ids_int64, const float* scale,
                                     float scale_all, int32_t dtype, int64_t m, int64_t k, int64_t n,
-                                    int32_t adapters, int32_t rank, void* y, int64_t ldy, int32_t* plan,
-                                    void* s, int32_t* status, void* stream) {
+                                    int32_t adapters, int32_t rank, int32_t for_backward, void* y,
+                                    int64_t ldy, int32_t* plan, void* s, int32_t* status, void* stream) {
   const lora::Weights a{lora_a, a_stride_l, a_stride_row}, b{lora_b, b_stride_l, b_stride_row};
   if (!dims_ok(dtype, m, k, n, adapters, rank) || plan == nullptr || !rows_ok(weight, ldw, k) ||
       !weights_ok(a, rank, k, adapters) || !weights_ok(b, n, rank, adapters) ||
@@ -799,6 +726,10 @@ extern "C" int32_t moe_lora_forward(const void* x, int64_t ldx, const void* weig
     return MOE_ERR_INVALID_ARG;
   const lora::PlanView pv(plan, m, adapters);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (!for_backward && m > 0 && m <= lora::kFewRows)
+    return lora::forward_few_rows(x, ldx, weight, ldw, a, b, ids, ids_int64, lora::Scale{scale, scale_all},
+                                  dtype, static_cast<int>(m), static_cast<int>(k), static_cast<int>(n),
+                                  adapters, rank, y, ldy, static_cast<float*>(s), status, st);
   lora::plan_kernel<<<adapters, 1024, 0, st>>>(ids, ids_int64, static_cast<int>(m), adapters, pv.perm,
                                                pv.offs, pv.base, status);
   if (cudaGetLastError() != cudaSuccess) return MOE_ERR_CUDA;

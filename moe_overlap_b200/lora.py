@@ -39,7 +39,7 @@ def _scale_args(scale):
     return (scale.data_ptr(), 0.0) if isinstance(scale, torch.Tensor) else (None, scale)
 
 
-def _forward(x, weight, lora_a, lora_b, ids, scale):
+def _forward(x, weight, lora_a, lora_b, ids, scale, for_backward):
     """(y, the buffer with the rows by adapter and x A^T that the backward needs)."""
     (m, k), n = x.shape, weight.shape[0]
     adapters, rank, _ = lora_a.shape
@@ -54,7 +54,7 @@ def _forward(x, weight, lora_a, lora_b, ids, scale):
             lora_a.data_ptr(), lora_a.stride(0), lora_a.stride(1),
             lora_b.data_ptr(), lora_b.stride(0), lora_b.stride(1),
             ids.data_ptr(), ids.dtype == torch.int64, *_scale_args(scale), _DTYPE_CODE[x.dtype], m, k, n,
-            adapters, rank, y.data_ptr(), n, at + low, at, _lib.status_address(dev), _lib.stream_handle(dev))
+            adapters, rank, for_backward, y.data_ptr(), n, at + low, at, _lib.status_address(dev), _lib.stream_handle(dev))
     _lib.check_call(rc, "moe_lora_forward")
     return y, kept
 
@@ -65,7 +65,7 @@ class LoraLinear(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, lora_a, lora_b, ids, scale):
-        y, kept = _forward(x, weight, lora_a, lora_b, ids, scale)
+        y, kept = _forward(x, weight, lora_a, lora_b, ids, scale, True)
         ctx.save_for_backward(x, weight, lora_a, lora_b, kept)
         ctx.scale = scale
         return y
@@ -191,7 +191,7 @@ def lora_linear(x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor, lor
         y = LoraLinear.apply(*args)
         _guard_capture(y, args, (x, weight, lora_a, lora_b))
     else:
-        y, _ = _forward(*args)
+        y, _ = _forward(*args, False)
     if _lib.sync_check_enabled():
         _lib.check_status(x.device, sync=True)
     return y[:, :n] if pn else y

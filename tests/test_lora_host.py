@@ -16,8 +16,8 @@ def test_cpu_tensors_are_refused():
 
 def _forward(**kw):
     a = dict(x=16, ldx=64, w=16, ldw=64, a=16, asl=8 * 64, asr=64, b=16, bsl=72 * 8, bsr=8, ids=16, ids64=1,
-             scale=16, scale_all=1.0, dtype=0, m=4, k=64, n=72, L=3, r=8, y=16, ldy=72, plan=16, s=16,
-             status=None, stream=None)
+             scale=16, scale_all=1.0, dtype=0, m=4, k=64, n=72, L=3, r=8, keep=1, y=16, ldy=72, plan=16,
+             s=16, status=None, stream=None)
     a.update(kw)
     return _lib.load().moe_lora_forward(*a.values())
 
