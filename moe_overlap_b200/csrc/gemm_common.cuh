@@ -34,6 +34,21 @@ struct ArrivalWait {
   uint64_t wait_ns;         // bound on each wait
 };
 
+// Adapters' products added in the accumulator of a one-expert product: for each of the
+// first count[t] adapters list[t] of row tile t (256 rows), the product of `rows` (256
+// x rank for each of the tile's kPerTile places, zeros in rows of other adapters) and
+// that adapter's matrix w_i, stored in the direction of B (one matrix behind another,
+// `stride_l` apart, rows `stride_row` apart).
+struct Adapters {
+  static constexpr int kPerTile = 4;
+  const void* rows;      // [row tiles][kPerTile][256][rank], the inputs' type
+  const int32_t* count;  // [row tiles]
+  const int4* list;      // [row tiles]
+  const void* w;
+  int64_t stride_l, stride_row;
+  int rank, adapters;
+};
+
 struct Params {
   void* c;
   int64_t ldc;
@@ -311,7 +326,8 @@ int grouped_gemm_launch(const void* a, int64_t lda, const void* b, int64_t b_str
                         int32_t activation, int32_t num_sms, int32_t use_atomic_queue,
                         int32_t* work_counter, const float* row_scale, const void* aux_in,
                         void* aux_out, int64_t ld_aux, int32_t* status, cudaStream_t stream,
-                        const PushTarget* push, const ArrivalWait* arrival = nullptr);
+                        const PushTarget* push, const ArrivalWait* arrival = nullptr,
+                        const Adapters* adapters = nullptr);
 
 // Launches the 2-SM (CTA pair) kernel; grid must be even.  `ta_half` is A's map with
 // 64-row boxes (the rows a swapped tile of N <= 128 reads per CTA); `tc` is the 2-D {N, m_total}
@@ -319,7 +335,16 @@ int grouped_gemm_launch(const void* a, int64_t lda, const void* b, int64_t b_str
 // Returns a MOE_* code.
 int launch_pair_kernel(bool bf16, bool b_mn, const CUtensorMap& ta, const CUtensorMap& ta_half,
                        const CUtensorMap& tb, const CUtensorMap& tc, const Params& p, int grid,
-                       cudaStream_t stream);
+                       cudaStream_t stream, const struct AdapterMaps* adapters = nullptr);
+
+// The tensor maps of Adapters and what the pair kernel reads beside them.
+struct AdapterMaps {
+  CUtensorMap rows, rows_half;  // boxes as A's and its half
+  CUtensorMap w;                // boxes as B's
+  const int32_t* count;
+  const int4* list;
+  int k_blocks;  // of 64 in the rank
+};
 
 }  // namespace gg
 }  // namespace moe

@@ -405,7 +405,8 @@ int moe::gg::grouped_gemm_launch(const void* a, int64_t lda, const void* b, int6
                                  int32_t activation, int32_t num_sms, int32_t use_atomic_queue,
                                  int32_t* work_counter, const float* row_scale, const void* aux_in,
                                  void* aux_out, int64_t ld_aux, int32_t* status, cudaStream_t stream,
-                                 const PushTarget* push, const ArrivalWait* arrival) {
+                                 const PushTarget* push, const ArrivalWait* arrival,
+                                 const Adapters* adapters) {
   using namespace moe::gg;
   const bool pushing = push != nullptr && push->src != nullptr;
   if (dtype != MOE_DTYPE_BF16 && dtype != MOE_DTYPE_F16) return MOE_ERR_INVALID_ARG;
@@ -522,11 +523,35 @@ int moe::gg::grouped_gemm_launch(const void* a, int64_t lda, const void* b, int6
     p.c_tma = 1;
   }
 
+  AdapterMaps extra;
+  if (adapters != nullptr) {
+    // The pair kernel's row tiles, with one expert, are the adapters' tiles.
+    if (!use_pair || num_experts != 1) return MOE_ERR_UNSUPPORTED;
+    const uint64_t r = uint64_t(adapters->rank);
+    const uint64_t tiles = uint64_t((m_total + 255) / 256);
+    const uint64_t rdims[2] = {r, tiles * Adapters::kPerTile * 256};
+    const uint64_t rstrides[1] = {r * 2};
+    const uint32_t rbox[2] = {BK, BM}, rbox_half[2] = {BK, BM / 2};
+    if (int rc = encode_tiled(&extra.rows, dt, 2, adapters->rows, rdims, rstrides, rbox); rc != MOE_OK) return rc;
+    if (int rc = encode_tiled(&extra.rows_half, dt, 2, adapters->rows, rdims, rstrides, rbox_half); rc != MOE_OK)
+      return rc;
+    const uint64_t wdims[3] = {b_mn ? uint64_t(n) : r, b_mn ? r : uint64_t(n), uint64_t(adapters->adapters)};
+    const uint64_t row = uint64_t(adapters->stride_row) * 2;
+    const uint64_t wstrides[2] = {row, adapters->adapters > 1 ? uint64_t(adapters->stride_l) * 2 : row * wdims[1]};
+    const uint32_t wbox[3] = {64, b_mn ? uint32_t(BK) : uint32_t(BN / 2), 1};
+    if (int rc = encode_tiled(&extra.w, dt, 3, adapters->w, wdims, wstrides, wbox); rc != MOE_OK) return rc;
+    extra.count = adapters->count;
+    extra.list = adapters->list;
+    extra.k_blocks = (adapters->rank + BK - 1) / BK;
+  }
+
   if (p.use_atomic &&
       cudaMemsetAsync(work_counter, 0, sizeof(int32_t), stream) != cudaSuccess)
     return MOE_ERR_CUDA;
   const bool bf16 = dtype == MOE_DTYPE_BF16;
-  if (use_pair) return launch_pair_kernel(bf16, b_mn, ta, ta_half, tb, tc, p, grid, stream);
+  if (use_pair)
+    return launch_pair_kernel(bf16, b_mn, ta, ta_half, tb, tc, p, grid, stream,
+                              adapters != nullptr ? &extra : nullptr);
   if (bf16 && b_mn) return launch<true, true>(ta, tb, p, grid, stream);
   if (bf16 && !b_mn) return launch<true, false>(ta, tb, p, grid, stream);
   if (!bf16 && b_mn) return launch<false, true>(ta, tb, p, grid, stream);

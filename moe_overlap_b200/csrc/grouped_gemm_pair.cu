@@ -31,11 +31,17 @@
 // so the tensor work follows the rows.  Each CTA's TMEM then holds its 128 output
 // columns in its lanes and the tile's rows in N accumulator columns; the epilogue
 // stores them transposed (plain or GELU epilogues only).
+// Adapters (ADAPTERS, one expert): behind a tile's own k-blocks come, for each adapter of
+// its rows, the k-blocks of the adapter's rank, A from the tile's rows of x A_i^T (zeros in
+// other adapters' rows) and B from the adapter's second matrix; boxes past the rank are
+// zero-filled, so any rank fills whole k-blocks.  The sum stays in the accumulator and is
+// rounded once.
 // No load uses cluster multicast; the pair exchanges only barrier arrivals and
 // the tile ring entries through shared::cluster addresses.
 #include <algorithm>
 #include <cstdint>
 #include <mutex>
+#include <type_traits>
 
 #include "gemm_common.cuh"
 #include "host_common.h"
@@ -231,12 +237,16 @@ __device__ __forceinline__ bool issue_tile(Ctrl* ctrl, uint8_t* sA, uint8_t* sB,
 // warp per sub-partition of a 4-warp exchange block at <= 80 registers, so the
 // dispatch/combine kernels run beside this persistent kernel.  PUSH compiles the
 // expert-parallel combine push into the epilogue (rows go to their source ranks).
-template <bool BF16, bool B_MN_MAJOR, bool PUSH>
+struct NoAdapters {};
+
+template <bool BF16, bool B_MN_MAJOR, bool PUSH, class EXTRA>
 __global__ void __cluster_dims__(2, 1, 1) __maxnreg__(kMaxRegs)
     grouped_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a,
                              const __grid_constant__ CUtensorMap tmap_a_half,
                              const __grid_constant__ CUtensorMap tmap_b,
-                             const __grid_constant__ CUtensorMap tmap_c, const Params p) {
+                             const __grid_constant__ CUtensorMap tmap_c, const Params p,
+                             const __grid_constant__ EXTRA extra) {
+  constexpr bool ADAPTERS = !std::is_same<EXTRA, NoAdapters>::value;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
@@ -324,6 +334,8 @@ __global__ void __cluster_dims__(2, 1, 1) __maxnreg__(kMaxRegs)
             const TileCoord tc = decode_tile(t, p.num_experts, tile_prefix, seg_start, seg_rows,
                                              BM, tiles_n, p.tile_order);
             s = make_int4(tc.row0, tc.rows, tc.tile_n * BN, tc.expert);
+            // the only expert is 0: its place carries the tile's adapters
+            if constexpr (ADAPTERS) s.w = extra.count[tc.row0 / BM];
           }
           ctrl->slot[q] = s;
           st_shared_cluster_v4(mapa_shared(smem_u32(&ctrl->slot[q]), 1), s);
@@ -342,12 +354,20 @@ __global__ void __cluster_dims__(2, 1, 1) __maxnreg__(kMaxRegs)
           qphase ^= 1;
         }
         if (s.z < 0) break;
-        if (s.w != ready_expert) {  // expert-ordered dispatch: this expert's rows have landed
-          if (!wait_expert_rows(p, s.w)) {
+        int expert = s.w;
+        int4 list = make_int4(0, 0, 0, 0);
+        int extra_kb = 0;
+        if constexpr (ADAPTERS) {
+          expert = 0;
+          extra_kb = s.w * extra.k_blocks;
+          if (extra_kb > 0) list = extra.list[s.x / BM];
+        }
+        if (expert != ready_expert) {  // expert-ordered dispatch: this expert's rows have landed
+          if (!wait_expert_rows(p, expert)) {
             failed = true;
             break;
           }
-          ready_expert = s.w;
+          ready_expert = expert;
         }
         // A swapped tile of N rows takes N/2 of them from each CTA (the MMA's N side),
         // CTA c from row c*N/2, through the 64-row map into the first half of the A
@@ -359,7 +379,7 @@ __global__ void __cluster_dims__(2, 1, 1) __maxnreg__(kMaxRegs)
         const CUtensorMap* map_a = half_box ? &tmap_a_half : &tmap_a;
         const uint32_t stage_tx = half_box ? PAIR_TX_BYTES_SWAPPED : PAIR_TX_BYTES;
         const int n_b = s.z + static_cast<int>(crank) * BN_CTA;
-        for (int kb = 0; kb < num_kb; ++kb) {
+        for (int kb = 0; kb < num_kb + extra_kb; ++kb) {
           if (!mbar_wait_cluster(smem_u32(&ctrl->empty[stage]), phase ^ 1, abort_flag)) {
             failed = true;
             break;
@@ -367,15 +387,27 @@ __global__ void __cluster_dims__(2, 1, 1) __maxnreg__(kMaxRegs)
           const uint32_t full_local = smem_u32(&ctrl->full[stage]);
           if (leader) mbar_arrive_expect_tx(full_local, stage_tx);
           const uint32_t full_leader = mapa_shared(full_local, 0);
-          tma_load_2d_pair(smem_u32(sA + stage * A_STAGE_BYTES), map_a, full_leader, kb * BK, row_a);
+          const CUtensorMap* ka = map_a;
+          const CUtensorMap* kb_map = &tmap_b;
+          int k0 = kb * BK, a_row = row_a, b_matrix = expert;
+          if constexpr (ADAPTERS) {
+            if (kb >= num_kb) {
+              const int at = (kb - num_kb) / extra.k_blocks;
+              k0 = (kb - num_kb - at * extra.k_blocks) * BK;
+              a_row = ((s.x / BM) * Adapters::kPerTile + at) * BM + (row_a - s.x);
+              b_matrix = at == 0 ? list.x : at == 1 ? list.y : at == 2 ? list.z : list.w;
+              ka = half_box ? &extra.rows_half : &extra.rows;
+              kb_map = &extra.w;
+            }
+          }
+          tma_load_2d_pair(smem_u32(sA + stage * A_STAGE_BYTES), ka, full_leader, k0, a_row);
           const uint32_t b_dst = smem_u32(sB + stage * B_STAGE_BYTES);
           if constexpr (B_MN_MAJOR) {
 #pragma unroll
             for (int j = 0; j < BN_CTA / 64; ++j)
-              tma_load_3d_pair(b_dst + j * B_SLAB_BYTES, &tmap_b, full_leader, n_b + 64 * j, kb * BK,
-                               s.w);
+              tma_load_3d_pair(b_dst + j * B_SLAB_BYTES, kb_map, full_leader, n_b + 64 * j, k0, b_matrix);
           } else {
-            tma_load_3d_pair(b_dst, &tmap_b, full_leader, kb * BK, n_b, s.w);
+            tma_load_3d_pair(b_dst, kb_map, full_leader, k0, n_b, b_matrix);
           }
           if (++stage == STAGES) {
             stage = 0;
@@ -423,13 +455,15 @@ __global__ void __cluster_dims__(2, 1, 1) __maxnreg__(kMaxRegs)
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + uint32_t(acc * BN);
         const int n_sw = swapped_n(p, s.y);
+        int tile_kb = num_kb;
+        if constexpr (ADAPTERS) tile_kb += s.w * extra.k_blocks;
         // Two instantiations of the k-block loop, so that the usual tile's loop
         // carries no per-MMA choice between the two operand arrangements.
         const bool ok =
-            n_sw > 0 ? issue_tile<BF16, B_MN_MAJOR, true>(ctrl, sA, sB, d_tmem, num_kb, stage, phase,
+            n_sw > 0 ? issue_tile<BF16, B_MN_MAJOR, true>(ctrl, sA, sB, d_tmem, tile_kb, stage, phase,
                                                           abort_flag, issued_any,
                                                           idesc_f16(BF16, BM, n_sw, B_MN_MAJOR, false))
-                     : issue_tile<BF16, B_MN_MAJOR, false>(ctrl, sA, sB, d_tmem, num_kb, stage, phase,
+                     : issue_tile<BF16, B_MN_MAJOR, false>(ctrl, sA, sB, d_tmem, tile_kb, stage, phase,
                                                            abort_flag, issued_any, 0u);
         if (!ok) failed = true;
         if (failed) break;
@@ -518,10 +552,11 @@ __global__ void __cluster_dims__(2, 1, 1) __maxnreg__(kMaxRegs)
   }
 }
 
-template <bool BF16, bool B_MN, bool PUSH = false>
+template <bool BF16, bool B_MN, bool PUSH = false, class EXTRA = NoAdapters>
 int launch(const CUtensorMap& ta, const CUtensorMap& ta_half, const CUtensorMap& tb,
-           const CUtensorMap& tc, const Params& p, int grid, cudaStream_t stream) {
-  auto kern = grouped_gemm_pair_kernel<BF16, B_MN, PUSH>;
+           const CUtensorMap& tc, const Params& p, int grid, cudaStream_t stream,
+           const EXTRA& extra = EXTRA()) {
+  auto kern = grouped_gemm_pair_kernel<BF16, B_MN, PUSH, EXTRA>;
   static std::once_flag once[kMaxDevices];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return MOE_ERR_CUDA;
@@ -531,7 +566,7 @@ int launch(const CUtensorMap& ta, const CUtensorMap& ta_half, const CUtensorMap&
                                     static_cast<int>(smem_bytes(kMaxExperts)));
   });
   if (attr_err != cudaSuccess) return MOE_ERR_CUDA;
-  kern<<<grid, NUM_THREADS, smem_bytes(p.num_experts), stream>>>(ta, ta_half, tb, tc, p);
+  kern<<<grid, NUM_THREADS, smem_bytes(p.num_experts), stream>>>(ta, ta_half, tb, tc, p, extra);
   return cudaGetLastError() == cudaSuccess ? MOE_OK : MOE_ERR_CUDA;
 }
 
@@ -539,8 +574,16 @@ int launch(const CUtensorMap& ta, const CUtensorMap& ta_half, const CUtensorMap&
 
 int launch_pair_kernel(bool bf16, bool b_mn, const CUtensorMap& ta, const CUtensorMap& ta_half,
                        const CUtensorMap& tb, const CUtensorMap& tc, const Params& p, int grid,
-                       cudaStream_t stream) {
+                       cudaStream_t stream, const AdapterMaps* adapters) {
   if (grid < 2 || grid % 2 != 0) return MOE_ERR_INVALID_ARG;
+  if (adapters != nullptr) {
+    using X = AdapterMaps;
+    if (p.push.src != nullptr) return MOE_ERR_INVALID_ARG;
+    if (bf16 && b_mn) return pair::launch<true, true, false, X>(ta, ta_half, tb, tc, p, grid, stream, *adapters);
+    if (bf16) return pair::launch<true, false, false, X>(ta, ta_half, tb, tc, p, grid, stream, *adapters);
+    if (b_mn) return pair::launch<false, true, false, X>(ta, ta_half, tb, tc, p, grid, stream, *adapters);
+    return pair::launch<false, false, false, X>(ta, ta_half, tb, tc, p, grid, stream, *adapters);
+  }
   if (p.push.src != nullptr) {  // combine push (bf16 only)
     if (!bf16) return MOE_ERR_INVALID_ARG;
     return b_mn ? pair::launch<true, true, true>(ta, ta_half, tb, tc, p, grid, stream)

@@ -2,21 +2,27 @@
 //
 //   y[m] = x[m] W^T + scale[i] (x[m] A[i]^T) B[i]^T,   i = ids[m] (-1: no adapter)
 //
-// The shared product is the grouped GEMM of one expert; the kernels here add the
-// adapters' part and form its gradients.  Rows are taken in adapter order through a
-// permutation, so each adapter is read once per block of its rows:
-//   plan    perm (the rows with an adapter, by adapter, in row order) and offs
+// The shared product is the grouped GEMM of one expert, which can take the adapters'
+// second product into its accumulator; the kernels here prepare that and form the
+// gradients.  Rows are taken in adapter order through a permutation, so each adapter is
+// read once per block of its rows:
+//   plan    perm (the rows with an adapter, by adapter, in row order), offs, and for each
+//           tile of 256 rows the adapters in it
 //   shrink  s[p] = x[perm[p]] A[i]^T           (also dy B[i], with B read along rows)
-//   expand  y[perm[p]] += scale[i] s[p] B[i]^T (also dx += scale[i] (dy B[i]) A[i])
+//   expand  y[perm[p]] += scale[i] s[p] B[i]^T (also dx += scale[i] (dy B[i]) A[i]) for the
+//           rows of tiles with more adapters than the shared product takes
 //   grad    dB[i] = scale[i] sum_p dy[perm[p]]^T s[p]  (also dA[i])
-// s is held as two values of the inputs' type, the rounded one and what the rounding
-// left (16 bits or more in all): the operand of a second tensor-core product.
+// For the gradients and for expand s is held as two values of the inputs' type, the
+// rounded one and what the rounding left (16 bits or more in all).  The shared product
+// takes scale[i] s rounded to the type, like every operand of it; the sum with the
+// shared part is then rounded once, where expand rounds it a second time.
 #include <cuda_runtime.h>
 
 #include <cstdint>
 #include <type_traits>
 
 #include "../../include/moe_overlap.h"
+#include "gemm_common.cuh"
 #include "host_common.h"
 #include "lora.cuh"
 #include "mma16.cuh"
@@ -28,55 +34,139 @@ namespace lora {
 constexpr int kMaxAdapters = 1024;
 constexpr int kMaxRank = 128;
 
-// One block per adapter: it counts the rows of smaller adapters (its segment's start)
-// and writes its own rows in order.  No block depends on another and the order is
-// always the same.
-__global__ void __launch_bounds__(1024) plan_kernel(const void* ids, int ids64, int M, int L,
-                                                    int32_t* perm, int32_t* offs, int32_t* base_offs,
+constexpr int kTileRows = 256;  // of the shared product
+using gg::Adapters;
+
+// The caller's plan buffer (int32, 16-byte aligned): what depends on the ids alone.
+struct PlanView {
+  int32_t* list;   // [tiles][kPerTile] adapters of a tile, ascending
+  int32_t* count;  // [tiles] how many; 0 also for a tile with too many
+  int32_t* place;  // [m] block of the row in the tiles' blocks, -1: left to expand
+  int32_t* perm;   // [m]
+  int32_t* offs;   // [adapters + 1]
+  int32_t* base;   // {0, m}
+  static int64_t tiles(int64_t m) { return (m + kTileRows - 1) / kTileRows; }
+  static int64_t ints(int64_t m, int adapters) {
+    return tiles(m) * (Adapters::kPerTile + 1) + 2 * m + adapters + 3;
+  }
+  PlanView(void* plan, int64_t m, int adapters) {
+    list = static_cast<int32_t*>(plan);
+    count = list + tiles(m) * Adapters::kPerTile;
+    place = count + tiles(m);
+    perm = place + m;
+    offs = perm + m;
+    base = offs + adapters + 1;
+  }
+};
+
+__device__ __forceinline__ int id_at(const void* ids, int ids64, int m, int L) {
+  const int64_t v = ids64 ? static_cast<const int64_t*>(ids)[m]
+                          : static_cast<int64_t>(static_cast<const int32_t*>(ids)[m]);
+  return v < 0 || v >= L ? (v == -1 ? -1 : -2) : static_cast<int>(v);  // -2: a bad id
+}
+
+// Blocks 0 .. L-1 each take one adapter: they count the rows of smaller adapters (the
+// segment's start) and write their own rows in order.  Blocks L .. take one row tile each:
+// the adapters in it, its rows' places, and zeros in its blocks for the rows of others.
+// No block depends on another and the order is always the same.
+__global__ void __launch_bounds__(1024) plan_kernel(const void* ids, int ids64, int M, int L, int r,
+                                                    PlanView plan, int per_tile, uint4* blocks,
                                                     int32_t* status) {
-  __shared__ int less[32], equal[32];
-  const int i = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  auto id_at = [&](int m) -> int {
-    const int64_t v = ids64 ? static_cast<const int64_t*>(ids)[m]
-                            : static_cast<int64_t>(static_cast<const int32_t*>(ids)[m]);
-    if (v < -1 || v >= L) {
-      if (i == 0) record_status(status, MOE_ERR_INVALID_ARG);
-      return -1;
-    }
-    return static_cast<int>(v);
-  };
-  const int per = ((M + 31) / 32 + 31) / 32 * 32;  // rows of a warp
-  const int m0 = warp * per, m1 = min(M, m0 + per);
-  int nl = 0, ne = 0;
-  for (int m = m0 + lane; m < m1; m += 32) {
-    const int v = id_at(m);
-    nl += v >= 0 && v < i;
-    ne += v == i;
-  }
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tid = threadIdx.x;
+  if (static_cast<int>(blockIdx.x) < L) {
+    __shared__ int less[32], equal[32];
+    constexpr int kBatch = 8;  // loads under way at a time
+    const int i = blockIdx.x;
+    const int per = ((M + 31) / 32 + 31) / 32 * 32;  // rows of a warp
+    const int m0 = warp * per, m1 = min(M, m0 + per);
+    int nl = 0, ne = 0;
+    bool bad = false;
+    for (int b = m0; b < m1; b += 32 * kBatch) {
+      int v[kBatch];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    nl += __shfl_xor_sync(0xffffffffu, nl, o);
-    ne += __shfl_xor_sync(0xffffffffu, ne, o);
+      for (int q = 0; q < kBatch; ++q) {
+        const int m = b + 32 * q + lane;
+        v[q] = m < m1 ? id_at(ids, ids64, m, L) : -1;
+      }
+#pragma unroll
+      for (int q = 0; q < kBatch; ++q) {
+        nl += v[q] >= 0 && v[q] < i;
+        ne += v[q] == i;
+        bad |= v[q] == -2;
+      }
+    }
+    if (bad && i == 0) record_status(status, MOE_ERR_INVALID_ARG);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      nl += __shfl_xor_sync(0xffffffffu, nl, o);
+      ne += __shfl_xor_sync(0xffffffffu, ne, o);
+    }
+    if (lane == 0) less[warp] = nl, equal[warp] = ne;
+    __syncthreads();
+    int start = 0, at = 0, all = 0;
+#pragma unroll
+    for (int k = 0; k < 32; ++k) {
+      start += less[k];
+      at += k < warp ? equal[k] : 0;
+      all += equal[k];
+    }
+    if (tid == 0) {
+      plan.offs[i] = start;
+      if (i == L - 1) plan.offs[L] = start + all;
+      if (i == 0) plan.base[0] = 0, plan.base[1] = M;
+    }
+    if (all == 0) return;
+    at += start;
+    for (int b = m0; b < m1; b += 32 * kBatch) {
+      bool mine[kBatch];
+#pragma unroll
+      for (int q = 0; q < kBatch; ++q) {
+        const int m = b + 32 * q + lane;
+        mine[q] = m < m1 && id_at(ids, ids64, m, L) == i;
+      }
+#pragma unroll
+      for (int q = 0; q < kBatch; ++q) {
+        const unsigned votes = __ballot_sync(0xffffffffu, mine[q]);
+        if (mine[q]) plan.perm[at + __popc(votes & ((1u << lane) - 1u))] = b + 32 * q + lane;
+        at += __popc(votes);
+      }
+    }
+    return;
   }
-  if (lane == 0) less[warp] = nl, equal[warp] = ne;
+  __shared__ unsigned present[kMaxAdapters / 32];  // a bit for each adapter
+  __shared__ int before[kMaxAdapters / 32 + 1];
+  static_assert(kMaxAdapters / 32 == 32, "one word a lane");
+  const int t = blockIdx.x - L, m = t * kTileRows + tid;
+  const int id = tid < kTileRows && m < M ? id_at(ids, ids64, m, L) : -1;
+  if (tid < 32) present[tid] = 0;
   __syncthreads();
-  int start = 0, at = 0, all = 0;
-  for (int k = 0; k < 32; ++k) {
-    start += less[k];
-    at += k < warp ? equal[k] : 0;
-    all += equal[k];
+  if (id >= 0) atomicOr(&present[id >> 5], 1u << (id & 31));
+  __syncthreads();
+  if (tid < 32) {
+    const int n = __popc(present[tid]);
+    int incl = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (tid >= o) incl += v;
+    }
+    before[tid] = incl - n;
+    if (tid == 31) before[32] = incl;
   }
-  if (threadIdx.x == 0) {
-    offs[i] = start;
-    if (i == L - 1) offs[L] = start + all;
-    if (i == 0) base_offs[0] = 0, base_offs[1] = M;
+  __syncthreads();
+  const int n = before[32];
+  const bool taken = n <= per_tile;
+  if (tid == 0) plan.count[t] = taken ? n : 0;
+  if (tid < kTileRows && m < M) {
+    const int rank = id >= 0 ? before[id >> 5] + __popc(present[id >> 5] & ((1u << (id & 31)) - 1u)) : 0;
+    plan.place[m] = taken && id >= 0 ? t * Adapters::kPerTile + rank : -1;
+    // every row of the adapter writes the same word
+    if (taken && id >= 0) plan.list[t * Adapters::kPerTile + rank] = id;
   }
-  at += start;
-  for (int b = m0; b < m1; b += 32) {
-    const bool mine = b + lane < m1 && id_at(b + lane) == i;
-    const unsigned votes = __ballot_sync(0xffffffffu, mine);
-    if (mine) perm[at + __popc(votes & ((1u << lane) - 1u))] = b + lane;
-    at += __popc(votes);
+  if (taken) {
+    const int words = kTileRows * r / 8;  // of 16 bytes in one block
+    uint4* mine = blocks + int64_t(t) * Adapters::kPerTile * words;
+    for (int q = tid; q < n * words; q += 1024) mine[q] = make_uint4(0, 0, 0, 0);
   }
 }
 
@@ -163,7 +253,8 @@ struct ShrinkCfg {
 template <typename T, bool kT, int RP>
 __global__ void __launch_bounds__(kShrinkThreads, 2)
     shrink_kernel(const T* x, int64_t ldx, const T* w, int64_t sl, int64_t sr, const int32_t* perm,
-                  const int32_t* offs, int L, int K, int r, int64_t part_stride, T* s) {
+                  const int32_t* offs, int L, int K, int r, int64_t part_stride, T* s, Scale scale,
+                  const int32_t* place, T* blocks) {
   using C = ShrinkCfg<kT, RP>;
   extern __shared__ __align__(128) char smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -266,6 +357,7 @@ __global__ void __launch_bounds__(kShrinkThreads, 2)
     cluster_sync_all();
   else
     __syncthreads();
+  const float c = scale.of(t.i);
   const int share = kShrinkRows / parts;  // rows that this CTA finishes
   for (int e = tid; e < share * (RP / 4); e += kShrinkThreads) {
     const int m = part * share + e / (RP / 4), j = e % (RP / 4) * 4;
@@ -276,6 +368,12 @@ __global__ void __launch_bounds__(kShrinkThreads, 2)
     T* out = s + int64_t(t.p0 + m) * r + j;
     *reinterpret_cast<uint2*>(out) = *reinterpret_cast<const uint2*>(hi);
     *reinterpret_cast<uint2*>(out + part_stride) = *reinterpret_cast<const uint2*>(lo);
+    const int row = perm[t.p0 + m], at = place[row];
+    if (at >= 0) {  // the shared product takes this row's
+      const T o[4] = {from_f<T>(c * v.x), from_f<T>(c * v.y), from_f<T>(c * v.z), from_f<T>(c * v.w)};
+      *reinterpret_cast<uint2*>(blocks + (int64_t(at) * kTileRows + row % kTileRows) * r + j) =
+          *reinterpret_cast<const uint2*>(o);
+    }
   }
   if (parts > 1) cluster_sync_all();  // no CTA leaves while another reads its sums
 }
@@ -300,14 +398,21 @@ struct ExpandCfg {
 template <typename T, bool kT, int RP>
 __global__ void __launch_bounds__(kThreads, 2)
     expand_kernel(const T* s, int64_t part_stride, const T* w, int64_t sl, int64_t sr,
-                  Scale scale, const int32_t* perm, const int32_t* offs, int L, int N, int r,
-                  T* y, int64_t ldy) {
+                  Scale scale, const int32_t* perm, const int32_t* offs, const int32_t* place, int L,
+                  int N, int r, T* y, int64_t ldy) {
   using C = ExpandCfg<kT, RP>;
   extern __shared__ __align__(128) char smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, q4 = lane & 3;
   const Tile t = find_tile(offs, L, blockIdx.x, kExpandRows);
   if (t.i < 0) return;
   const int mg = warp & 3, half = warp >> 2;
+  T* yrow[2];  // rows mg*16 + g8 and + 8; null for those that the shared product has taken
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int m = mg * 16 + g8 + 8 * u, row = m < t.rows ? perm[t.p0 + m] : -1;
+    yrow[u] = row >= 0 && place[row] < 0 ? y + row * ldy + half * 64 + q4 * 8 : nullptr;
+  }
+  if (!__syncthreads_or(yrow[0] != nullptr || yrow[1] != nullptr)) return;
   const T* wi = w + t.i * sl;
   const int step = gridDim.y * kExpandCols;
   auto fetch_w = [&](int n0, int buf) {
@@ -334,12 +439,6 @@ __global__ void __launch_bounds__(kThreads, 2)
   };
   fetch_w(blockIdx.y * kExpandCols, 0);
   const float c = scale.of(t.i);
-  T* yrow[2];
-#pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    const int m = mg * 16 + g8 + 8 * u;
-    yrow[u] = m < t.rows ? y + perm[t.p0 + m] * ldy + half * 64 + q4 * 8 : nullptr;
-  }
   const int ncol = half * 64 + q4 * 8;  // this lane's first column of a block; + 32 for the second
   auto fetch_y = [&](int n0, uint4(&v)[2][2]) {
 #pragma unroll
@@ -622,15 +721,10 @@ inline int cluster_parts(int64_t blocks, int64_t most, int64_t length, int64_t l
   return parts;
 }
 
-// The caller's plan buffer: perm [m], offs [adapters + 1] and {0, m}.
-struct PlanView {
-  int32_t *perm, *offs, *base;
-  PlanView(int32_t* plan, int64_t m, int adapters)
-      : perm(plan), offs(plan + m), base(plan + m + adapters + 1) {}
-};
-// s = x w^T by adapter, w in rows of k (transposed: in rows of the rank).
-int shrink(const void* x, int64_t ldx, Weights w, bool transposed, PlanView plan, int dtype, int64_t m,
-           int64_t k, int adapters, int rank, void* s, cudaStream_t stream) {
+// s = x w^T by adapter, w in rows of k (transposed: in rows of the rank); scale s also
+// into the blocks of the shared product's row tiles.
+int shrink(const void* x, int64_t ldx, Weights w, bool transposed, Scale scale, const PlanView& plan, int dtype,
+           int64_t m, int64_t k, int adapters, int rank, void* s, void* blocks, cudaStream_t stream) {
   return dispatch(dtype, transposed, rank, [&](auto t, auto tr, auto rp) {
     using T = decltype(t);
     constexpr bool kT = decltype(tr)::value;
@@ -640,13 +734,15 @@ int shrink(const void* x, int64_t ldx, Weights w, bool transposed, PlanView plan
     return launch(shrink_kernel<T, kT, RP>, dim3(tiles, parts), kShrinkThreads, dim3(1, parts),
                   ShrinkCfg<kT, RP>::kBytes, stream, static_cast<const T*>(x), ldx,
                   static_cast<const T*>(w.p), w.stride_l, w.stride_row, plan.perm, plan.offs, adapters,
-                  static_cast<int>(k), rank, m * rank, static_cast<T*>(s));
+                  static_cast<int>(k), rank, m * rank, static_cast<T*>(s), scale, plan.place,
+                  static_cast<T*>(blocks));
   });
 }
 
-// y += scale s w^T, w in rows of the rank (transposed: in rows of n).
-int expand(const void* s, Weights w, bool transposed, Scale scale, PlanView plan, int dtype, int64_t m,
-           int64_t n, int adapters, int rank, void* y, int64_t ldy, cudaStream_t stream) {
+// y += scale s w^T for the rows that the shared product has left, w in rows of the rank
+// (transposed: in rows of n).
+int expand(const void* s, Weights w, bool transposed, Scale scale, const PlanView& plan, int dtype,
+           int64_t m, int64_t n, int adapters, int rank, void* y, int64_t ldy, cudaStream_t stream) {
   return dispatch(dtype, transposed, rank, [&](auto t, auto tr, auto rp) {
     using T = decltype(t);
     constexpr bool kT = decltype(tr)::value;
@@ -658,13 +754,13 @@ int expand(const void* s, Weights w, bool transposed, Scale scale, PlanView plan
                   dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(want < blocks ? want : blocks)),
                   kThreads, dim3(1, 1), ExpandCfg<kT, RP>::kBytes, stream, static_cast<const T*>(s),
                   m * rank, static_cast<const T*>(w.p), w.stride_l, w.stride_row, scale, plan.perm,
-                  plan.offs, adapters, static_cast<int>(n), rank, static_cast<T*>(y), ldy);
+                  plan.offs, plan.place, adapters, static_cast<int>(n), rank, static_cast<T*>(y), ldy);
   });
 }
 
 // g [adapters, n, rank] (transposed: [adapters, rank, n]) = scale z^T s by adapter.
-int grad(const void* s, const void* z, int64_t ldz, bool transposed, Scale scale, PlanView plan, int dtype,
-         int64_t m, int64_t n, int adapters, int rank, void* g, cudaStream_t stream) {
+int grad(const void* s, const void* z, int64_t ldz, bool transposed, Scale scale, const PlanView& plan,
+         int dtype, int64_t m, int64_t n, int adapters, int rank, void* g, cudaStream_t stream) {
   return dispatch(dtype, transposed, rank, [&](auto t, auto tr, auto rp) {
     using T = decltype(t);
     constexpr bool kT = decltype(tr)::value;
@@ -700,17 +796,37 @@ bool weights_ok(lora::Weights w, int64_t rows, int64_t width, int32_t adapters) 
   return rows_ok(w.p, w.stride_row, width) &&
          (adapters == 1 || (w.stride_l % 8 == 0 && w.stride_l >= (rows - 1) * w.stride_row + width));
 }
+// y = x w^T, w(k, n) at the given strides, with the adapters' second product of the rows
+// that have a place.
 int shared_product(const void* x, int64_t ldx, const void* w, int64_t stride_k, int64_t stride_n, void* y,
-                   int64_t ldy, const int32_t* base, int64_t m, int64_t k, int64_t n, int32_t dtype,
-                   int32_t* status, void* stream) {
+                   int64_t ldy, const lora::PlanView& plan, lora::Weights second, const void* blocks,
+                   int64_t m, int64_t k, int64_t n, int adapters, int rank, int dtype, int32_t* status,
+                   cudaStream_t stream) {
   int dev;
   DeviceInfo info;
   const int rc = current_device_info(&dev, &info);
   if (rc != MOE_OK) return rc;
-  return moe_grouped_gemm(x, ldx, w, 0, stride_k, stride_n, y, ldy, base, 0, m, k, n, 1, dtype,
-                          MOE_ACT_NONE, info.sm_count, 0, nullptr, status, stream);
+  const gg::Adapters extra{blocks, plan.count, reinterpret_cast<const int4*>(plan.list), second.p,
+                           second.stride_l, second.stride_row, rank, adapters};
+  return gg::grouped_gemm_launch(x, ldx, w, 0, stride_k, stride_n, y, ldy, plan.base, 0, m, k, n, 1, dtype,
+                                 MOE_ACT_NONE, info.sm_count, 0, nullptr, nullptr, nullptr, nullptr, 0, status,
+                                 stream, nullptr, nullptr, force_single_sm_kernel() ? nullptr : &extra);
 }
+// Adapters that the shared product takes in a tile of rows; none on the 1-SM kernel.
+int per_tile() { return force_single_sm_kernel() ? 0 : gg::Adapters::kPerTile; }
+int64_t low_bytes(int64_t m, int32_t rank) { return 4 * m * rank; }
 }  // namespace
+
+extern "C" int64_t moe_lora_kept_bytes(int64_t m, int32_t adapters, int32_t rank) {
+  if (!dims_ok(MOE_DTYPE_BF16, m, 8, 8, adapters, rank)) return -1;
+  return low_bytes(m, rank) + 4 * lora::PlanView::ints(m, adapters);
+}
+
+extern "C" int64_t moe_lora_workspace_bytes(int64_t m, int32_t adapters, int32_t rank) {
+  if (!dims_ok(MOE_DTYPE_BF16, m, 8, 8, adapters, rank)) return -1;
+  return low_bytes(m, rank) +
+         lora::PlanView::tiles(m) * gg::Adapters::kPerTile * lora::kTileRows * int64_t(rank) * 2;
+}
 
 extern "C" int32_t moe_lora_forward(const void* x, int64_t ldx, const void* weight, int64_t ldw,
                                     const void* lora_a, int64_t a_stride_l, int64_t a_stride_row,
@@ -718,27 +834,33 @@ extern "C" int32_t moe_lora_forward(const void* x, int64_t ldx, const void* weig
                                     const void* ids, int32_t ids_int64, const float* scale,
                                     float scale_all, int32_t dtype, int64_t m, int64_t k, int64_t n,
                                     int32_t adapters, int32_t rank, int32_t for_backward, void* y,
-                                    int64_t ldy, int32_t* plan, void* s, int32_t* status, void* stream) {
+                                    int64_t ldy, void* kept, void* workspace, int32_t* status,
+                                    void* stream) {
   const lora::Weights a{lora_a, a_stride_l, a_stride_row}, b{lora_b, b_stride_l, b_stride_row};
-  if (!dims_ok(dtype, m, k, n, adapters, rank) || plan == nullptr || !rows_ok(weight, ldw, k) ||
-      !weights_ok(a, rank, k, adapters) || !weights_ok(b, n, rank, adapters) ||
-      (m > 0 && (!rows_ok(x, ldx, k) || !rows_ok(y, ldy, n) || ids == nullptr || s == nullptr || !aligned16(s))))
+  if (!dims_ok(dtype, m, k, n, adapters, rank) || kept == nullptr || !aligned16(kept) ||
+      !rows_ok(weight, ldw, k) || !weights_ok(a, rank, k, adapters) || !weights_ok(b, n, rank, adapters) ||
+      (m > 0 && (!rows_ok(x, ldx, k) || !rows_ok(y, ldy, n) || ids == nullptr || workspace == nullptr ||
+                 !aligned16(workspace))))
     return MOE_ERR_INVALID_ARG;
-  const lora::PlanView pv(plan, m, adapters);
+  const lora::PlanView plan(static_cast<char*>(kept) + low_bytes(m, rank), m, adapters);
+  const lora::Scale sc{scale, scale_all};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (!for_backward && m > 0 && m <= lora::kFewRows)
-    return lora::forward_few_rows(x, ldx, weight, ldw, a, b, ids, ids_int64, lora::Scale{scale, scale_all},
-                                  dtype, static_cast<int>(m), static_cast<int>(k), static_cast<int>(n),
-                                  adapters, rank, y, ldy, static_cast<float*>(s), status, st);
-  lora::plan_kernel<<<adapters, 1024, 0, st>>>(ids, ids_int64, static_cast<int>(m), adapters, pv.perm,
-                                               pv.offs, pv.base, status);
+    return lora::forward_few_rows(x, ldx, weight, ldw, a, b, ids, ids_int64, sc, dtype,
+                                  static_cast<int>(m), static_cast<int>(k), static_cast<int>(n), adapters,
+                                  rank, y, ldy, static_cast<float*>(kept), status, st);
+  char* blocks = static_cast<char*>(workspace) + low_bytes(m, rank);
+  lora::plan_kernel<<<static_cast<unsigned>(adapters + lora::PlanView::tiles(m)), 1024, 0, st>>>(
+      ids, ids_int64, static_cast<int>(m), adapters, rank, plan, per_tile(), reinterpret_cast<uint4*>(blocks),
+      status);
   if (cudaGetLastError() != cudaSuccess) return MOE_ERR_CUDA;
   if (m == 0) return MOE_OK;
-  int rc = lora::shrink(x, ldx, a, false, pv, dtype, m, k, adapters, rank, s, st);
+  int rc = lora::shrink(x, ldx, a, false, sc, plan, dtype, m, k, adapters, rank, kept, blocks, st);
   if (rc == MOE_OK)
-    rc = shared_product(x, ldx, weight, 1, ldw, y, ldy, pv.base, m, k, n, dtype, status, stream);
+    rc = shared_product(x, ldx, weight, 1, ldw, y, ldy, plan, b, blocks, m, k, n, adapters, rank, dtype, status,
+                        st);
   if (rc == MOE_OK)
-    rc = lora::expand(s, b, false, lora::Scale{scale, scale_all}, pv, dtype, m, n, adapters, rank, y, ldy, st);
+    rc = lora::expand(kept, b, false, sc, plan, dtype, m, n, adapters, rank, y, ldy, st);
   return rc;
 }
 
@@ -747,31 +869,38 @@ extern "C" int32_t moe_lora_backward(const void* dy, int64_t lddy, const void* x
                                      int64_t a_stride_l, int64_t a_stride_row, const void* lora_b,
                                      int64_t b_stride_l, int64_t b_stride_row, const float* scale,
                                      float scale_all, int32_t dtype, int64_t m, int64_t k, int64_t n,
-                                     int32_t adapters, int32_t rank, int32_t* plan, const void* s, void* t,
+                                     int32_t adapters, int32_t rank, const void* kept, void* workspace,
                                      void* dx, int64_t lddx, void* da, void* db, int32_t* status,
                                      void* stream) {
   const lora::Weights a{lora_a, a_stride_l, a_stride_row}, b{lora_b, b_stride_l, b_stride_row};
-  if (!dims_ok(dtype, m, k, n, adapters, rank) || plan == nullptr || !rows_ok(weight, ldw, k) ||
-      !weights_ok(a, rank, k, adapters) || !weights_ok(b, n, rank, adapters) ||
+  if (!dims_ok(dtype, m, k, n, adapters, rank) || kept == nullptr || !aligned16(kept) ||
+      !rows_ok(weight, ldw, k) || !weights_ok(a, rank, k, adapters) || !weights_ok(b, n, rank, adapters) ||
       (da != nullptr && !aligned16(da)) || (db != nullptr && !aligned16(db)) ||
-      (m > 0 && (!rows_ok(dy, lddy, n) || !rows_ok(x, ldx, k) || s == nullptr || !aligned16(s) ||
-                 ((dx != nullptr || da != nullptr) && (t == nullptr || !aligned16(t))) ||
+      (m > 0 && (!rows_ok(dy, lddy, n) || !rows_ok(x, ldx, k) ||
+                 ((dx != nullptr || da != nullptr) && (workspace == nullptr || !aligned16(workspace))) ||
                  (dx != nullptr && !rows_ok(dx, lddx, k)))))
     return MOE_ERR_INVALID_ARG;
-  const lora::PlanView pv(plan, m, adapters);
+  const lora::PlanView plan(const_cast<char*>(static_cast<const char*>(kept)) + low_bytes(m, rank), m, adapters);
   const lora::Scale sc{scale, scale_all};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  char* blocks = static_cast<char*>(workspace) + low_bytes(m, rank);
   int rc = MOE_OK;
-  if (m > 0 && (dx != nullptr || da != nullptr))
-    rc = lora::shrink(dy, lddy, b, true, pv, dtype, m, n, adapters, rank, t, st);
+  if (m > 0 && (dx != nullptr || da != nullptr)) {
+    // The blocks' rows of other adapters are zeros again: the forward's may be gone.
+    if (dx != nullptr && cudaMemsetAsync(blocks, 0, moe_lora_workspace_bytes(m, adapters, rank) - low_bytes(m, rank),
+                                         st) != cudaSuccess)
+      return MOE_ERR_CUDA;
+    rc = lora::shrink(dy, lddy, b, true, sc, plan, dtype, m, n, adapters, rank, workspace, blocks, st);
+  }
   if (rc == MOE_OK && m > 0 && dx != nullptr) {
-    rc = shared_product(dy, lddy, weight, ldw, 1, dx, lddx, pv.base, m, n, k, dtype, status, stream);
+    rc = shared_product(dy, lddy, weight, ldw, 1, dx, lddx, plan, a, blocks, m, n, k, adapters, rank, dtype,
+                        status, st);
     if (rc == MOE_OK)
-      rc = lora::expand(t, a, true, sc, pv, dtype, m, k, adapters, rank, dx, lddx, st);
+      rc = lora::expand(workspace, a, true, sc, plan, dtype, m, k, adapters, rank, dx, lddx, st);
   }
   if (rc == MOE_OK && da != nullptr)
-    rc = lora::grad(t, x, ldx, true, sc, pv, dtype, m, k, adapters, rank, da, st);
+    rc = lora::grad(workspace, x, ldx, true, sc, plan, dtype, m, k, adapters, rank, da, st);
   if (rc == MOE_OK && db != nullptr)
-    rc = lora::grad(s, dy, lddy, false, sc, pv, dtype, m, n, adapters, rank, db, st);
+    rc = lora::grad(kept, dy, lddy, false, sc, plan, dtype, m, n, adapters, rank, db, st);
   return rc;
 }

@@ -61,7 +61,7 @@ __global__ void __launch_bounds__(32 * kLowWarps)
 // side.  The order of k inside a slice is free: lane (g, q) takes the 16 contiguous
 // columns 16q.. of its rows, so both operands come by 16-byte conflict-free loads.
 constexpr int kConsumers = 8;
-constexpr int kThreads = 32 * (1 + kConsumers);
+constexpr int kThreads = 32 * (2 + kConsumers);
 constexpr int kStageBytes = 16 * 1024;
 constexpr int kRedStride = 20;
 
@@ -108,7 +108,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint32_t phase = 0;
 
   if (warp == 0) {
-    if (lane == 0)
+    if (lane == 0) {
       for (int blk = blockIdx.x; blk < blocks; blk += gridDim.x)
         for (int c = 0; c < K; c += BKS) {
           const uint32_t full = smem_u32(&ctrl->full[stage]);
@@ -126,6 +126,18 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           if (++stage == kStages) stage = 0, phase ^= 1;
         }
+    }
+    return;
+  }
+  if (warp == 1 + kConsumers) {  // the epilogues' rows of B, on their way to L2 by then
+    for (int blk = blockIdx.x; blk < blocks; blk += gridDim.x)
+      for (int m = 0; m < M; ++m) {
+        const int i = ctrl->id[m];
+        if (i < 0) continue;
+        for (int row = blk * BM + lane; row < min(N, (blk + 1) * BM); row += 32)
+          for (int j = 0; j < r; j += 64)
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(b + i * sl + row * sr + j));
+      }
     return;
   }
   const int cw = warp - 1, rt = cw % R, cs = cw / R, g8 = lane >> 2, q4 = lane & 3;
@@ -150,18 +162,19 @@ __global__ void __launch_bounds__(kThreads, 1)
       ld_shared_v4(sa + off1, &a[0][4]);
       ld_shared_v4(sa + 1024 + off0, &a[1][0]);
       ld_shared_v4(sa + 1024 + off1, &a[1][4]);
+      uint32_t v[J][8];
 #pragma unroll
       for (int j = 0; j < J; ++j) {
-        if (j * 8 < M) {
-          const uint32_t sb = b_base + stage * Q::kSlotBytes + j * 1024;
-          uint32_t v[8];
-          ld_shared_v4(sb + off0, &v[0]);
-          ld_shared_v4(sb + off1, &v[4]);
-#pragma unroll
-          for (int s = 0; s < 4; ++s)
-            mma<T>(acc[j], a[0][2 * s], a[1][2 * s], a[0][2 * s + 1], a[1][2 * s + 1], v[2 * s], v[2 * s + 1]);
-        }
+        const uint32_t sb = b_base + stage * Q::kSlotBytes + j * 1024;
+        ld_shared_v4(sb + off0, &v[j][0]);
+        ld_shared_v4(sb + off1, &v[j][4]);
       }
+#pragma unroll
+      for (int s = 0; s < 4; ++s)  // J independent sums between two products of one
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+          mma<T>(acc[j], a[0][2 * s], a[1][2 * s], a[0][2 * s + 1], a[1][2 * s + 1], v[j][2 * s],
+                 v[j][2 * s + 1]);
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&ctrl->empty[stage]));
       if (++stage == kStages) stage = 0, phase ^= 1;
@@ -175,9 +188,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("bar.sync 1, 256;" ::: "memory");
     if (!waited) wait_for_previous_kernel();  // for `low`
     waited = true;
-    // One column of W a thread (row n of the block) and every 256 / BM-th row of x, four at
+    // One column of W a thread (row n of the block) and every 256 / BM-th row of x, eight at
     // a time so that their adapters' rows are under way together.
-    constexpr int kStep = 32 * kConsumers / BM, kTogether = 4;
+    constexpr int kStep = 32 * kConsumers / BM, kTogether = 8;
     const int n = (cw * 32 + lane) % BM, row = blk * BM + n;
     if (row < N)
       for (int m0 = (cw * 32 + lane) / BM; m0 < M; m0 += kTogether * kStep) {
@@ -191,7 +204,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           lr[u] = low + m * r;
           add[u] = 0.0f;
         }
-#pragma unroll 2
+#pragma unroll 1
         for (int j = 0; j < r; j += 8) {
           uint4 ub[kTogether];
 #pragma unroll
@@ -276,7 +289,9 @@ int forward(const void* x, int64_t ldx, const void* weight, int64_t ldw, Weights
     using std::integral_constant;
     if (m <= 8) return go(rr, integral_constant<int, 1>());
     if (m <= 16) return go(rr, integral_constant<int, 2>());
+    if (m <= 24) return go(wide, integral_constant<int, 3>());
     if (m <= 32) return go(wide, integral_constant<int, 4>());
+    if (m <= 48) return go(wide, integral_constant<int, 6>());
     return go(wide, integral_constant<int, 8>());
   };
   // The widest row blocks that still give most SMs one; with more rows of x the narrow

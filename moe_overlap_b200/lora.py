@@ -21,6 +21,7 @@ __all__ = ["lora_linear"]
 _DTYPE_CODE = {torch.bfloat16: _lib.MOE_DTYPE_BF16, torch.float16: _lib.MOE_DTYPE_F16}
 MAX_RANK = 128
 MAX_ADAPTERS = 1024
+FEW_ROWS = 64  # a batch of so many rows without gradients takes the decode kernels
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -40,21 +41,24 @@ def _scale_args(scale):
 
 
 def _forward(x, weight, lora_a, lora_b, ids, scale, for_backward):
-    """(y, the buffer with the rows by adapter and x A^T that the backward needs)."""
+    """(y, what the backward needs: x A^T and the rows by adapter)."""
     (m, k), n = x.shape, weight.shape[0]
     adapters, rank, _ = lora_a.shape
     dev = x.device
+    lib = _lib.load()
     y = torch.empty(m, n, dtype=x.dtype, device=dev)
-    low = 4 * m * rank  # bytes of x A^T: two parts of 16 bits; the plan stands behind it
-    kept = torch.empty(low + 4 * (m + adapters + 3), dtype=torch.uint8, device=dev)
-    at = kept.data_ptr()
+    kept = torch.empty(lib.moe_lora_kept_bytes(m, adapters, rank), dtype=torch.uint8, device=dev)
+    ws = kept  # a decode batch needs no more
+    if for_backward or m > FEW_ROWS:
+        ws = torch.empty(lib.moe_lora_workspace_bytes(m, adapters, rank), dtype=torch.uint8, device=dev)
     with _lib.on_device(dev):
-        rc = _lib.load().moe_lora_forward(
+        rc = lib.moe_lora_forward(
             x.data_ptr(), x.stride(0), weight.data_ptr(), weight.stride(0),
             lora_a.data_ptr(), lora_a.stride(0), lora_a.stride(1),
             lora_b.data_ptr(), lora_b.stride(0), lora_b.stride(1),
             ids.data_ptr(), ids.dtype == torch.int64, *_scale_args(scale), _DTYPE_CODE[x.dtype], m, k, n,
-            adapters, rank, for_backward, y.data_ptr(), n, at + low, at, _lib.status_address(dev), _lib.stream_handle(dev))
+            adapters, rank, for_backward, y.data_ptr(), n, kept.data_ptr(), ws.data_ptr(),
+            _lib.status_address(dev), _lib.stream_handle(dev))
     _lib.check_call(rc, "moe_lora_forward")
     return y, kept
 
@@ -78,20 +82,21 @@ class LoraLinear(torch.autograd.Function):
         (m, k), n = x.shape, weight.shape[0]
         adapters, rank, _ = lora_a.shape
         dev, dt = x.device, x.dtype
+        lib = _lib.load()
         dy = _rows(dy)
         dx = torch.empty(m, k, dtype=dt, device=dev) if need_x else None
         da = torch.empty(adapters, rank, k, dtype=dt, device=dev) if need_a else None
         db = torch.empty(adapters, n, rank, dtype=dt, device=dev) if need_b else None
-        low = 4 * m * rank
-        t = torch.empty(low, dtype=torch.uint8, device=dev) if need_x or need_a else None
-        at = kept.data_ptr()
+        ws = None
+        if need_x or need_a:
+            ws = torch.empty(lib.moe_lora_workspace_bytes(m, adapters, rank), dtype=torch.uint8, device=dev)
         with _lib.on_device(dev):
-            rc = _lib.load().moe_lora_backward(
+            rc = lib.moe_lora_backward(
                 dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0), weight.data_ptr(),
                 weight.stride(0), lora_a.data_ptr(), lora_a.stride(0), lora_a.stride(1),
                 lora_b.data_ptr(), lora_b.stride(0), lora_b.stride(1), *_scale_args(ctx.scale),
-                _DTYPE_CODE[dt], m, k, n, adapters, rank, at + low, at,
-                *(v.data_ptr() if v is not None else None for v in (t, dx)), k,
+                _DTYPE_CODE[dt], m, k, n, adapters, rank, kept.data_ptr(),
+                *(v.data_ptr() if v is not None else None for v in (ws, dx)), k,
                 *(v.data_ptr() if v is not None else None for v in (da, db)),
                 _lib.status_address(dev), _lib.stream_handle(dev))
         _lib.check_call(rc, "moe_lora_backward")

@@ -6,8 +6,9 @@ the type's least subnormal):
                product's operand (two parts of the type):
                |ds| <= K v (|x| |A|^T) + 2^-16 |s| + tiny
   y            the shared product may be rounded to the type before the adapters' part
-               is added: |dy| <= u |y| + u |x W^T| + K v (|x| |W|^T)
-                                 + c ((|ds| + (r + 4) v |s|) |B|^T) + tiny
+               is added, or take s rounded to the type (half a step, u |s|) into its sum:
+               |dy| <= u |y| + u |x W^T| + K v (|x| |W|^T)
+                       + c ((|ds| + (u + (r + 4) v) |s|) |B|^T) + tiny
   dx           the same with dy, B for A, A for B, N for K
   dA, dB       sums over the R rows of the adapter:
                |dA| <= u |dA| + c (|dT| + (R + 4) v |T|)^T |x| + tiny
@@ -57,9 +58,9 @@ def reference(x, w, a, b, dy, scale, ids):
         s, ds = low(x[rows], a[i], K, tiny)
         t, dt_ = low(dy[rows], b[i].t(), N, tiny)
         y[rows] += c * (s @ b[i].t())
-        ty[rows] += c * ((ds + (r + 4) * V * s.abs()) @ b[i].abs().t())
+        ty[rows] += c * ((ds + (u + (r + 4) * V) * s.abs()) @ b[i].abs().t())
         dx[rows] += c * (t @ a[i])
-        tx[rows] += c * ((dt_ + (r + 4) * V * t.abs()) @ a[i].abs())
+        tx[rows] += c * ((dt_ + (u + (r + 4) * V) * t.abs()) @ a[i].abs())
         da[i] = c * (t.t() @ x[rows])
         ta[i] += c * ((dt_ + (R + 4) * V * t.abs()).t() @ x[rows].abs())
         db[i] = c * (dy[rows].t() @ s)
@@ -93,6 +94,27 @@ def test_forward_matches_64_bit_reference(cuda_device, M, K, N, L, r, dtype):
     assert y.dtype == dtype
     assert_close(y, reference(x, w, a, b, dy, scale, ids)[0])
     assert torch.equal(mo.lora_linear(x, w, a, b, ids.to(torch.int32), scale=scale), y)
+
+
+@pytest.mark.parametrize("M,K,N,L,r,dtype", [
+    (900, 256, 520, 9, 16, torch.bfloat16), (515, 136, 264, 30, 128, torch.bfloat16),
+    (1290, 520, 136, 6, 72, torch.float16), (256, 64, 512, 1000, 8, torch.bfloat16),
+    (300, 192, 256, 5, 64, torch.float16)])
+def test_rows_in_runs_and_tiles_of_many_adapters(cuda_device, M, K, N, L, r, dtype):
+    """Rows of an adapter together, so that most tiles of 256 rows hold few adapters, with
+    one stretch of rows in which every row has another one, and a short last tile."""
+    x, w, a, b, dy, scale, _ = make(M, K, N, L, r, dtype, seed=M + L, device=cuda_device)
+    ids = torch.arange(M) // 97 % L
+    ids[300:420] = torch.arange(len(ids[300:420])) % L
+    ids[40:60] = -1
+    ids = ids.to(cuda_device)
+    for t in (x, a, b):
+        t.requires_grad_(True)
+    y = mo.lora_linear(x, w, a, b, ids, scale=scale)
+    grads = torch.autograd.grad(y, (x, a, b), dy)
+    mo.check_status(cuda_device, sync=True)
+    for got, want in zip((y, *grads), reference(x, w, a, b, dy, scale, ids)):
+        assert_close(got, want)
 
 
 @pytest.mark.parametrize("M,K,N,L,r,dtype", SHAPES)
