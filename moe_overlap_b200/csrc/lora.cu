@@ -41,18 +41,20 @@ using gg::Adapters;
 struct PlanView {
   int32_t* list;   // [tiles][kPerTile] adapters of a tile, ascending
   int32_t* count;  // [tiles] how many; 0 also for a tile with too many
+  int32_t* left;   // [tiles] whether the tile's adapters are left to expand
   int32_t* place;  // [m] block of the row in the tiles' blocks, -1: left to expand
   int32_t* perm;   // [m]
   int32_t* offs;   // [adapters + 1]
   int32_t* base;   // {0, m}
   static int64_t tiles(int64_t m) { return (m + kTileRows - 1) / kTileRows; }
   static int64_t ints(int64_t m, int adapters) {
-    return tiles(m) * (Adapters::kPerTile + 1) + 2 * m + adapters + 3;
+    return tiles(m) * (Adapters::kPerTile + 2) + 2 * m + adapters + 3;
   }
   PlanView(void* plan, int64_t m, int adapters) {
     list = static_cast<int32_t*>(plan);
     count = list + tiles(m) * Adapters::kPerTile;
-    place = count + tiles(m);
+    left = count + tiles(m);
+    place = left + tiles(m);
     perm = place + m;
     offs = perm + m;
     base = offs + adapters + 1;
@@ -156,7 +158,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(const void* ids, int ids64, 
   __syncthreads();
   const int n = before[32];
   const bool taken = n <= per_tile;
-  if (tid == 0) plan.count[t] = taken ? n : 0;
+  if (tid == 0) plan.count[t] = taken ? n : 0, plan.left[t] = !taken;
   if (tid < kTileRows && m < M) {
     const int rank = id >= 0 ? before[id >> 5] + __popc(present[id >> 5] & ((1u << (id & 31)) - 1u)) : 0;
     plan.place[m] = taken && id >= 0 ? t * Adapters::kPerTile + rank : -1;
@@ -176,8 +178,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(const void* ids, int ids64, 
 // are gathered through perm, which whole-tile TMA boxes cannot do.  Rows of shared
 // memory are 16 bytes longer than a multiple of 32, so that ldmatrix meets no bank
 // twice.  RP is the rank rounded up to 16, 32, 64 or 128.
-constexpr int kThreads = 256;        // expand and grad
-constexpr int kShrinkThreads = 128;  // 4 warps of 32 rows: each reads all of w's tile from shared memory
+constexpr int kThreads = 256;
 
 // The sum over the cluster's CTAs, in their order, of 4 floats at this CTA's address
 // `at`; every CTA's load is under way before the first is used.
@@ -234,7 +235,8 @@ __device__ __forceinline__ Tile find_tile(const int32_t* offs, int L, int tile, 
   return t;
 }
 
-// shrink.  A CTA forms 128 rows x RP of s over one part of k; the CTAs of a cluster
+// shrink.  A CTA forms 128 rows x RP of s over one part of k: 4 warps of 32 rows (each
+// reads all of w's tile from shared memory) for each half of a stage's columns; the CTAs of a cluster
 // share the rows and add their parts through distributed shared memory, in order.
 // Bound by reading x once (and w once a block of 128 rows).
 constexpr int kShrinkRows = 128;
@@ -251,7 +253,7 @@ struct ShrinkCfg {
 };
 
 template <typename T, bool kT, int RP>
-__global__ void __launch_bounds__(kShrinkThreads, 2)
+__global__ void __launch_bounds__(kThreads, 2)
     shrink_kernel(const T* x, int64_t ldx, const T* w, int64_t sl, int64_t sr, const int32_t* perm,
                   const int32_t* offs, int L, int K, int r, int64_t part_stride, T* s, Scale scale,
                   const int32_t* place, T* blocks) {
@@ -265,7 +267,7 @@ __global__ void __launch_bounds__(kShrinkThreads, 2)
   const int k0 = min(K, part * cols), k1 = min(K, k0 + cols);
   const int steps = (k1 - k0 + kShrinkCols - 1) / kShrinkCols;
   const T* wi = w + t.i * sl;
-  constexpr int kRowSteps = kShrinkThreads / 8;  // rows that all threads copy at a time
+  constexpr int kRowSteps = kThreads / 8;  // rows that all threads copy at a time
   const T* row[kShrinkRows / kRowSteps];
 #pragma unroll
   for (int q = 0; q < kShrinkRows / kRowSteps; ++q) {
@@ -285,15 +287,15 @@ __global__ void __launch_bounds__(kShrinkThreads, 2)
       }
       if constexpr (kT) {
 #pragma unroll
-        for (int q = 0; q < kShrinkCols * (RP / 8) / kShrinkThreads; ++q) {
-          const int e = tid + q * kShrinkThreads, kk = e / (RP / 8), j = e % (RP / 8) * 8;
+        for (int e = tid; e < kShrinkCols * (RP / 8); e += kThreads) {
+          const int kk = e / (RP / 8), j = e % (RP / 8) * 8;
           const bool in = c + kk < k1 && j < r;
           copy_async_16(ws + kk * (RP * 2 + 16) + j * 2, in ? wi + int64_t(c + kk) * sr + j : w, in);
         }
       } else {
 #pragma unroll
-        for (int q = 0; q < RP * 8 / kShrinkThreads; ++q) {
-          const int j = tid / 8 + q * kRowSteps;
+        for (int e = tid; e < RP * 8; e += kThreads) {
+          const int j = e / 8;
           const bool in = j < r && k < k1;
           copy_async_16(ws + j * kShrinkPitch + (tid & 7) * 16, in ? wi + j * sr + k : w, in);
         }
@@ -310,7 +312,8 @@ __global__ void __launch_bounds__(kShrinkThreads, 2)
       for (int q = 0; q < 4; ++q) acc[m][n][q] = 0.0f;
 #pragma unroll
   for (int q = 0; q < C::kStages - 1; ++q) fetch(q);
-  const bool busy = warp * 32 < t.rows;  // a warp without rows only copies
+  const int mg = warp & 3, kg = warp >> 2;
+  const bool busy = mg * 32 < t.rows;  // a warp without rows only copies
   for (int step = 0; step < steps; ++step) {
     copies_wait<C::kStages - 2>();
     __syncthreads();
@@ -319,11 +322,12 @@ __global__ void __launch_bounds__(kShrinkThreads, 2)
     const uint32_t ws = xs + kShrinkRows * kShrinkPitch;
     if (!busy) continue;
 #pragma unroll
-    for (int kk = 0; kk < kShrinkCols; kk += 16) {
+    for (int q = 0; q < kShrinkCols / 2; q += 16) {
+      const int kk = kg * (kShrinkCols / 2) + q;
       uint32_t a[2][4];
 #pragma unroll
       for (int m = 0; m < 2; ++m)
-        ldmatrix_x4<false>(a[m], xs + (warp * 32 + m * 16 + (lane & 15)) * kShrinkPitch +
+        ldmatrix_x4<false>(a[m], xs + (mg * 32 + m * 16 + (lane & 15)) * kShrinkPitch +
                                      (kk + (lane >> 4) * 8) * 2);
 #pragma unroll
       for (int n = 0; n < RP / 8; n += 2) {
@@ -346,20 +350,29 @@ __global__ void __launch_bounds__(kShrinkThreads, 2)
   constexpr int kPitch = RP + 4;
   float* sums = reinterpret_cast<float*>(smem);
 #pragma unroll
-  for (int m = 0; m < 2; ++m)
+  for (int half = 0; half < 2; ++half) {  // the second half's warps add to the first's
+    if (kg == half)
 #pragma unroll
-    for (int n = 0; n < RP / 8; ++n)
+      for (int m = 0; m < 2; ++m)
 #pragma unroll
-      for (int q = 0; q < 2; ++q)
-        *reinterpret_cast<float2*>(sums + (warp * 32 + m * 16 + (lane >> 2) + 8 * q) * kPitch + n * 8 +
-                                   (lane & 3) * 2) = make_float2(acc[m][n][2 * q], acc[m][n][2 * q + 1]);
+        for (int n = 0; n < RP / 8; ++n)
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            float2* at = reinterpret_cast<float2*>(sums + (mg * 32 + m * 16 + (lane >> 2) + 8 * q) * kPitch +
+                                                   n * 8 + (lane & 3) * 2);
+            float2 v = make_float2(acc[m][n][2 * q], acc[m][n][2 * q + 1]);
+            if (half == 1) v.x += at->x, v.y += at->y;
+            *at = v;
+          }
+    if (half == 0) __syncthreads();
+  }
   if (parts > 1)
     cluster_sync_all();
   else
     __syncthreads();
   const float c = scale.of(t.i);
   const int share = kShrinkRows / parts;  // rows that this CTA finishes
-  for (int e = tid; e < share * (RP / 4); e += kShrinkThreads) {
+  for (int e = tid; e < share * (RP / 4); e += kThreads) {
     const int m = part * share + e / (RP / 4), j = e % (RP / 4) * 4;
     if (m >= t.rows || j >= r) continue;
     const float4 v = cluster_sum4(sums + m * kPitch + j, parts);
@@ -398,23 +411,29 @@ struct ExpandCfg {
 template <typename T, bool kT, int RP>
 __global__ void __launch_bounds__(kThreads, 2)
     expand_kernel(const T* s, int64_t part_stride, const T* w, int64_t sl, int64_t sr,
-                  Scale scale, const int32_t* perm, const int32_t* offs, const int32_t* place, int L,
-                  int N, int r, T* y, int64_t ldy) {
+                  Scale scale, const int32_t* perm, const int32_t* offs, const int32_t* place,
+                  const int32_t* left, int tiles, int splits, int L, int N, int r, T* y, int64_t ldy) {
   using C = ExpandCfg<kT, RP>;
   extern __shared__ __align__(128) char smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, q4 = lane & 3;
-  const Tile t = find_tile(offs, L, blockIdx.x, kExpandRows);
-  if (t.i < 0) return;
+  // Usually the shared product has taken every row.
+  bool any = false;
+  for (int q = tid; q < tiles; q += kThreads) any |= left[q] != 0;
+  if (!__syncthreads_or(any)) return;
   const int mg = warp & 3, half = warp >> 2;
+  for (int unit = blockIdx.x;; unit += gridDim.x) {
+  const Tile t = find_tile(offs, L, unit / splits, kExpandRows);
+  if (t.i < 0) return;
+  const int first = unit % splits * kExpandCols;
   T* yrow[2];  // rows mg*16 + g8 and + 8; null for those that the shared product has taken
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     const int m = mg * 16 + g8 + 8 * u, row = m < t.rows ? perm[t.p0 + m] : -1;
     yrow[u] = row >= 0 && place[row] < 0 ? y + row * ldy + half * 64 + q4 * 8 : nullptr;
   }
-  if (!__syncthreads_or(yrow[0] != nullptr || yrow[1] != nullptr)) return;
+  if (!__syncthreads_or(yrow[0] != nullptr || yrow[1] != nullptr)) continue;
   const T* wi = w + t.i * sl;
-  const int step = gridDim.y * kExpandCols;
+  const int step = splits * kExpandCols;
   auto fetch_w = [&](int n0, int buf) {
     if (n0 < N) {
       const uint32_t ws = smem_u32(smem) + buf * C::kW;
@@ -437,7 +456,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
     copies_commit();
   };
-  fetch_w(blockIdx.y * kExpandCols, 0);
+  fetch_w(first, 0);
   const float c = scale.of(t.i);
   const int ncol = half * 64 + q4 * 8;  // this lane's first column of a block; + 32 for the second
   auto fetch_y = [&](int n0, uint4(&v)[2][2]) {
@@ -449,7 +468,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           v[g][u] = *reinterpret_cast<const uint4*>(yrow[u] + n0 + g * 32);
   };
   uint4 yv[2][2], yn[2][2];
-  fetch_y(blockIdx.y * kExpandCols, yv);
+  fetch_y(first, yv);
   // A fragments straight from s: rows mg*16 + g8 and + 8, pairs of columns.
   uint32_t a[2][RP / 16][4];
 #pragma unroll
@@ -467,7 +486,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
   }
   int buf = 0;
-  for (int n0 = blockIdx.y * kExpandCols; n0 < N; n0 += step) {
+  for (int n0 = first; n0 < N; n0 += step) {
     fetch_w(n0 + step, buf ^ 1);
     fetch_y(n0 + step, yn);
     copies_wait<1>();
@@ -538,6 +557,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     buf ^= 1;
   }
   copies_wait<0>();
+  }
 }
 
 // grad.  A CTA forms 128 MT columns of z x RP of one adapter's gradient over one part
@@ -731,7 +751,7 @@ int shrink(const void* x, int64_t ldx, Weights w, bool transposed, Scale scale, 
     constexpr int RP = decltype(rp)::value;
     const unsigned tiles = static_cast<unsigned>(most_tiles(m, adapters, kShrinkRows));
     const unsigned parts = cluster_parts(tiles, 2 * 148, k, 256);
-    return launch(shrink_kernel<T, kT, RP>, dim3(tiles, parts), kShrinkThreads, dim3(1, parts),
+    return launch(shrink_kernel<T, kT, RP>, dim3(tiles, parts), kThreads, dim3(1, parts),
                   ShrinkCfg<kT, RP>::kBytes, stream, static_cast<const T*>(x), ldx,
                   static_cast<const T*>(w.p), w.stride_l, w.stride_row, plan.perm, plan.offs, adapters,
                   static_cast<int>(k), rank, m * rank, static_cast<T*>(s), scale, plan.place,
@@ -747,14 +767,16 @@ int expand(const void* s, Weights w, bool transposed, Scale scale, const PlanVie
     using T = decltype(t);
     constexpr bool kT = decltype(tr)::value;
     constexpr int RP = decltype(rp)::value;
-    const int64_t tiles = most_tiles(m, adapters, kExpandRows);
     const int64_t blocks = (n + kExpandCols - 1) / kExpandCols;
-    const int64_t want = (1200 + tiles - 1) / tiles;  // about four CTAs a place on the SMs
-    return launch(expand_kernel<T, kT, RP>,
-                  dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(want < blocks ? want : blocks)),
+    // Work for about four CTAs a place on the SMs, if every row were left.
+    const int64_t tiles = most_tiles(m, adapters, kExpandRows), want = (1200 + tiles - 1) / tiles;
+    const int splits = static_cast<int>(want < blocks ? want : blocks);
+    const int64_t units = tiles * splits, places = 2 * 148;
+    return launch(expand_kernel<T, kT, RP>, dim3(static_cast<unsigned>(units < places ? units : places)),
                   kThreads, dim3(1, 1), ExpandCfg<kT, RP>::kBytes, stream, static_cast<const T*>(s),
                   m * rank, static_cast<const T*>(w.p), w.stride_l, w.stride_row, scale, plan.perm,
-                  plan.offs, plan.place, adapters, static_cast<int>(n), rank, static_cast<T*>(y), ldy);
+                  plan.offs, plan.place, plan.left, static_cast<int>(PlanView::tiles(m)), splits, adapters,
+                  static_cast<int>(n), rank, static_cast<T*>(y), ldy);
   });
 }
 
