@@ -267,39 +267,51 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int k0 = min(K, part * cols), k1 = min(K, k0 + cols);
   const int steps = (k1 - k0 + kShrinkCols - 1) / kShrinkCols;
   const T* wi = w + t.i * sl;
-  constexpr int kRowSteps = kThreads / 8;  // rows that all threads copy at a time
-  const T* row[kShrinkRows / kRowSteps];
+  // What this thread copies: a 16-byte piece of 4 rows of x and of some rows of w, at
+  // pointers that move on by a stage each time (rows that are not there stay at their
+  // base and copy nothing).
+  constexpr int kRowSteps = kThreads / 8, kXCopies = kShrinkRows / kRowSteps;
+  constexpr int kWPieces = kT ? RP / 8 : kShrinkCols / 8, kWRows = kT ? kShrinkCols : RP;
+  constexpr int kWCopies = (kWRows * kWPieces + kThreads - 1) / kThreads;
+  const int piece = (tid & 7) * 8;
+  const T* xp[kXCopies];
+  uint32_t x_there = 0, w_there = 0;
 #pragma unroll
-  for (int q = 0; q < kShrinkRows / kRowSteps; ++q) {
+  for (int q = 0; q < kXCopies; ++q) {
     const int m = tid / 8 + kRowSteps * q;
-    row[q] = m < t.rows ? x + perm[t.p0 + m] * ldx : nullptr;
+    const bool there = m < t.rows;
+    xp[q] = x + (there ? perm[t.p0 + m] * ldx : 0) + k0 + piece;
+    x_there |= uint32_t(there) << q;
   }
-  auto fetch = [&](int step) {
-    if (step < steps) {
-      const uint32_t xs = smem_u32(smem) + (step % C::kStages) * C::kStage;
-      const uint32_t ws = xs + kShrinkRows * kShrinkPitch;
-      const int c = k0 + step * kShrinkCols, k = c + (tid & 7) * 8;
+  const T* wp[kWCopies];
 #pragma unroll
-      for (int q = 0; q < kShrinkRows / kRowSteps; ++q) {
-        const bool in = row[q] != nullptr && k < k1;
-        copy_async_16(xs + (tid / 8 + kRowSteps * q) * kShrinkPitch + (tid & 7) * 16,
-                      in ? row[q] + k : x, in);
+  for (int q = 0; q < kWCopies; ++q) {
+    const int e = tid + q * kThreads, row = e / kWPieces, c = e % kWPieces * 8;
+    const bool there = row < kWRows && (kT ? c : row) < r;
+    wp[q] = wi + (there ? (kT ? int64_t(k0 + row) * sr + c : row * sr + k0 + c) : 0);
+    w_there |= uint32_t(there) << q;
+  }
+  const int64_t w_step = kT ? kShrinkCols * sr : kShrinkCols;
+  int ck = k0, at = 0;  // the column and the stage of the next fetch
+  auto fetch = [&]() {
+    if (ck < k1) {
+      const uint32_t xs = smem_u32(smem) + at * C::kStage + tid / 8 * kShrinkPitch + piece * 2;
+      const uint32_t ws = smem_u32(smem) + at * C::kStage + kShrinkRows * kShrinkPitch;
+      const bool k_in = ck + piece < k1;
+#pragma unroll
+      for (int q = 0; q < kXCopies; ++q) {
+        copy_async_16(xs + kRowSteps * q * kShrinkPitch, xp[q], k_in && (x_there >> q & 1));
+        xp[q] += kShrinkCols;
       }
-      if constexpr (kT) {
 #pragma unroll
-        for (int e = tid; e < kShrinkCols * (RP / 8); e += kThreads) {
-          const int kk = e / (RP / 8), j = e % (RP / 8) * 8;
-          const bool in = c + kk < k1 && j < r;
-          copy_async_16(ws + kk * (RP * 2 + 16) + j * 2, in ? wi + int64_t(c + kk) * sr + j : w, in);
-        }
-      } else {
-#pragma unroll
-        for (int e = tid; e < RP * 8; e += kThreads) {
-          const int j = e / 8;
-          const bool in = j < r && k < k1;
-          copy_async_16(ws + j * kShrinkPitch + (tid & 7) * 16, in ? wi + j * sr + k : w, in);
-        }
+      for (int q = 0; q < kWCopies; ++q) {
+        const int e = tid + q * kThreads, row = e / kWPieces, c = e % kWPieces;
+        const bool in = (w_there >> q & 1) && (kT ? ck + row < k1 : k_in);
+        if (row < kWRows) copy_async_16(ws + row * (kT ? RP * 2 + 16 : kShrinkPitch) + c * 16, wp[q], in);
+        wp[q] += w_step;
       }
+      ck += kShrinkCols;
+      if (++at == C::kStages) at = 0;
     }
     copies_commit();
   };
@@ -311,14 +323,14 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
       for (int q = 0; q < 4; ++q) acc[m][n][q] = 0.0f;
 #pragma unroll
-  for (int q = 0; q < C::kStages - 1; ++q) fetch(q);
+  for (int q = 0; q < C::kStages - 1; ++q) fetch();
   const int mg = warp & 3, kg = warp >> 2;
   const bool busy = mg * 32 < t.rows;  // a warp without rows only copies
-  for (int step = 0; step < steps; ++step) {
+  for (int step = 0, stage = 0; step < steps; ++step, stage = stage + 1 == C::kStages ? 0 : stage + 1) {
     copies_wait<C::kStages - 2>();
     __syncthreads();
-    fetch(step + C::kStages - 1);
-    const uint32_t xs = smem_u32(smem) + (step % C::kStages) * C::kStage;
+    fetch();
+    const uint32_t xs = smem_u32(smem) + stage * C::kStage;
     const uint32_t ws = xs + kShrinkRows * kShrinkPitch;
     if (!busy) continue;
 #pragma unroll
@@ -602,26 +614,38 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
   };
   look_up(0);
-  auto fetch = [&](int step) {
-    if (step < steps) {
-      const uint32_t zs = smem_u32(smem) + (step % C::kStages) * C::kStage;
+  // s: pieces of both parts, at pointers that move on by 32 rows.
+  constexpr int kSPieces = RP / 8, kSCopies = (2 * kGradRows * kSPieces + kThreads - 1) / kThreads;
+  const T* sp[kSCopies];
+#pragma unroll
+  for (int q = 0; q < kSCopies; ++q) {
+    const int e = tid + q * kThreads, half = e / (kGradRows * kSPieces), f = e % (kGradRows * kSPieces);
+    const int j = f % kSPieces * 8;
+    sp[q] = s + (j < r && half < 2 ? half * part_stride + int64_t(o0 + p0 + f / kSPieces) * r + j : 0);
+  }
+  int step_f = 0, at = 0;  // the step and the stage of the next fetch
+  auto fetch = [&]() {
+    if (step_f < steps) {
+      const uint32_t zs = smem_u32(smem) + at * C::kStage;
       const uint32_t ss = zs + kGradRows * C::kZPitch;
-      const int p = p0 + step * kGradRows;
+      const int p = p0 + step_f * kGradRows;
 #pragma unroll
       for (int q = 0; q < kCopies; ++q) {
         const int m = tid / kPieces + q * (kThreads / kPieces);
         const bool in = next_row[q] >= 0;
-        copy_async_16(zs + m * C::kZPitch + zc * 2, in ? z + next_row[q] * ldz + n0 + zc : z, in);
+        copy_async_16(zs + m * C::kZPitch + zc * 2, z + (in ? next_row[q] * ldz + n0 + zc : 0), in);
       }
-      look_up(step + 1);
+      ++step_f;
+      look_up(step_f);
 #pragma unroll
-      for (int e = tid; e < kGradRows * (RP / 8) * 2; e += kThreads) {
-        const int half = e / (kGradRows * (RP / 8)), f = e % (kGradRows * (RP / 8));
-        const int m = f / (RP / 8), j = f % (RP / 8) * 8;
-        const bool in = p + m < p1 && j < r;
-        copy_async_16(ss + (half * kGradRows + m) * C::kSPitch + j * 2,
-                      in ? s + half * part_stride + int64_t(o0 + p + m) * r + j : s, in);
+      for (int q = 0; q < kSCopies; ++q) {
+        const int e = tid + q * kThreads, half = e / (kGradRows * kSPieces), f = e % (kGradRows * kSPieces);
+        const int m = f / kSPieces, j = f % kSPieces;
+        const bool in = p + m < p1 && j * 8 < r;
+        if (half < 2) copy_async_16(ss + (half * kGradRows + m) * C::kSPitch + j * 16, sp[q], in);
+        sp[q] += kGradRows * r;
       }
+      if (++at == C::kStages) at = 0;
     }
     copies_commit();
   };
@@ -633,12 +657,12 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
       for (int q = 0; q < 4; ++q) acc[m][k][q] = 0.0f;
 #pragma unroll
-  for (int q = 0; q < C::kStages - 1; ++q) fetch(q);
-  for (int step = 0; step < steps; ++step) {
+  for (int q = 0; q < C::kStages - 1; ++q) fetch();
+  for (int step = 0, stage = 0; step < steps; ++step, stage = stage + 1 == C::kStages ? 0 : stage + 1) {
     copies_wait<C::kStages - 2>();
     __syncthreads();
-    fetch(step + C::kStages - 1);
-    const uint32_t zs = smem_u32(smem) + (step % C::kStages) * C::kStage;
+    fetch();
+    const uint32_t zs = smem_u32(smem) + stage * C::kStage;
     const uint32_t ss = zs + kGradRows * C::kZPitch;
 #pragma unroll
     for (int kk = 0; kk < kGradRows; kk += 16) {
@@ -789,8 +813,8 @@ int grad(const void* s, const void* z, int64_t ldz, bool transposed, Scale scale
     constexpr int RP = decltype(rp)::value;
     using C = GradCfg<RP>;
     const unsigned blocks = static_cast<unsigned>((n + C::kCols - 1) / C::kCols);
-    // Adapters' rows are uneven, so many small parts: the largest adapter's rows spread.
-    const unsigned parts = cluster_parts(int64_t(blocks) * adapters, 8 * 2 * 148, m / adapters, 64);
+    // Adapters' rows are uneven, so several CTAs a place on the SMs: the largest's rows spread.
+    const unsigned parts = cluster_parts(int64_t(blocks) * adapters, 4 * 2 * 148, m / adapters, 64);
     return launch(grad_kernel<T, kT, RP>, dim3(parts, blocks, adapters), kThreads, dim3(parts, 1),
                   C::kBytes, stream, static_cast<const T*>(s), m * rank, static_cast<const T*>(z), ldz,
                   scale, plan.perm, plan.offs, static_cast<int>(n), rank, static_cast<T*>(g), n * rank,
