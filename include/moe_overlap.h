@@ -576,39 +576,35 @@ MOE_API int32_t moe_few_tokens(const void* x, int64_t ldx, const void* router_w,
  *   ids [m]         int32, or int64 if ids_int64; an id outside [-1, adapters) counts
  *                   as -1 and records MOE_ERR_INVALID_ARG in `status`
  *   scale           float[adapters], or NULL: scale_all for every adapter
- *   for_backward    nonzero: `kept` is for moe_lora_backward; 0: it is workspace too, and
- *                   at most 64 rows take kernels of their own
- *   kept            moe_lora_kept_bytes(...) bytes: x[r] A[i]^T in two parts, and the rows
- *                   by adapter
- *   workspace       moe_lora_workspace_bytes(...) bytes, of this call alone
- * dtype is MOE_DTYPE_BF16 or MOE_DTYPE_F16.  Rows, kept and workspace start on 16 bytes;
- * k, n and rank are multiples of 8; rank <= 128; adapters <= 1024.  Sums are fp32.  Both
- * sizes are -1 for sizes out of these bounds.
+ *   for_backward    nonzero: `kept` is for moe_lora_backward; 0: it is workspace, and at
+ *                   most 64 rows take kernels of their own
+ *   kept            moe_lora_kept_bytes(...) bytes (-1: sizes out of bounds), of this call
+ *                   and its backward passes alone; its contents need no set-up
+ * dtype is MOE_DTYPE_BF16 or MOE_DTYPE_F16.  Rows and kept start on 16 bytes; k, n and
+ * rank are multiples of 8; rank <= 128; adapters <= 1024.  Sums are fp32.
  */
-MOE_API int64_t moe_lora_kept_bytes(int64_t m, int32_t adapters, int32_t rank);
-MOE_API int64_t moe_lora_workspace_bytes(int64_t m, int32_t adapters, int32_t rank);
+MOE_API int64_t moe_lora_kept_bytes(int64_t m, int32_t adapters, int32_t rank, int32_t for_backward);
 MOE_API int32_t moe_lora_forward(const void* x, int64_t ldx, const void* weight, int64_t ldw,
                                  const void* lora_a, int64_t a_stride_l, int64_t a_stride_row,
                                  const void* lora_b, int64_t b_stride_l, int64_t b_stride_row,
                                  const void* ids, int32_t ids_int64, const float* scale,
                                  float scale_all, int32_t dtype, int64_t m, int64_t k, int64_t n,
                                  int32_t adapters, int32_t rank, int32_t for_backward, void* y,
-                                 int64_t ldy, void* kept, void* workspace, int32_t* status,
-                                 void* stream);
+                                 int64_t ldy, void* kept, int32_t* status, void* stream);
 
 /*
  * Gradients of moe_lora_forward, from what it kept: dx [m, k], da [adapters, rank, k]
  * and db [adapters, n, rank], the last two contiguous; a NULL one is not formed.  An
- * adapter without rows gets zeros.  workspace as above, needed for dx and da.
+ * adapter without rows gets zeros.  May be repeated on the same `kept`, one at a time
+ * (it holds this pass's workspace as well).
  */
 MOE_API int32_t moe_lora_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx,
                                   const void* weight, int64_t ldw, const void* lora_a,
                                   int64_t a_stride_l, int64_t a_stride_row, const void* lora_b,
                                   int64_t b_stride_l, int64_t b_stride_row, const float* scale,
                                   float scale_all, int32_t dtype, int64_t m, int64_t k, int64_t n,
-                                  int32_t adapters, int32_t rank, const void* kept, void* workspace,
-                                  void* dx, int64_t lddx, void* da, void* db, int32_t* status,
-                                  void* stream);
+                                  int32_t adapters, int32_t rank, void* kept, void* dx, int64_t lddx,
+                                  void* da, void* db, int32_t* status, void* stream);
 
 /*
  * DeepEP's get_dispatch_layout (thirdParty/DeepEP/deep_ep/buffer.py:293-319,

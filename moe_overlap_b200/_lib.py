@@ -195,23 +195,22 @@ SIGNATURES: dict[str, tuple] = {
          _c_void_p, _c_void_p, _c_void_p, _i64,  # topk_idx, topk_weights, out, ldo
          _c_void_p, _i64, _c_void_p, _c_void_p],  # workspace, bytes, status, stream
     ),
-    "moe_lora_kept_bytes": (_i64, [_i64, _i32, _i32]),
-    "moe_lora_workspace_bytes": (_i64, [_i64, _i32, _i32]),
+    "moe_lora_kept_bytes": (_i64, [_i64, _i32, _i32, _i32]),
     "moe_lora_forward": (
         _i32,
         [_c_void_p, _i64, _c_void_p, _i64,  # x, ldx, weight, ldw
          _c_void_p, _i64, _i64, _c_void_p, _i64, _i64,  # lora_a, strides l/row, lora_b, strides l/row
          _c_void_p, _i32, _c_void_p, ctypes.c_float,  # ids, ids_int64, scale, scale_all
          _i32, _i64, _i64, _i64, _i32, _i32, _i32,  # dtype, m, k, n, adapters, rank, for_backward
-         _c_void_p, _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p],  # y, ldy, kept, workspace, ..
+         _c_void_p, _i64, _c_void_p, _c_void_p, _c_void_p],  # y, ldy, kept, status, stream
     ),
     "moe_lora_backward": (
         _i32,
         [_c_void_p, _i64, _c_void_p, _i64, _c_void_p, _i64,  # dy, lddy, x, ldx, weight, ldw
          _c_void_p, _i64, _i64, _c_void_p, _i64, _i64,  # lora_a, strides l/row, lora_b, strides l/row
          _c_void_p, ctypes.c_float, _i32, _i64, _i64, _i64, _i32, _i32,  # scale, .., rank
-         _c_void_p, _c_void_p,  # kept, workspace
-         _c_void_p, _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p],  # dx, lddx, da, db, status, stream
+         _c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p,  # kept, dx, lddx, da, db
+         _c_void_p, _c_void_p],  # status, stream
     ),
     "moe_ep_dispatch_layout": (
         _i32, [_c_void_p, _i32, _i32, _i32, _i32, _c_void_p, _c_void_p, _c_void_p, _c_void_p]),

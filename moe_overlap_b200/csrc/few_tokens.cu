@@ -671,14 +671,12 @@ int launch_experts(const Params& p, const void* w1, int64_t w1_se, int64_t w1_sr
   int rc = encode_tiled(&m1, dt, 3, w1, d1, s1, box);
   if (rc == MOE_OK) rc = encode_tiled(&m2, dt, 3, w2, d2, s2, box);
   if (rc != MOE_OK) return rc;
-  const int smem = 1024 + K::kBytes + int(sizeof(Ctrl)) + int(sizeof(Plan)) +
-                   4 * (max_groups(J, p.E) + 2 * p.E);
-  static_assert(K::kStages <= 12 && 1024 + K::kBytes + int(sizeof(Ctrl)) + int(sizeof(Plan)) +
-                        4 * (max_groups(J, kMaxE) + 2 * kMaxE) <= 227 * 1024,
-                "shared memory");
-  auto kern = &experts_kernel<T, R, J>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-    return MOE_ERR_CUDA;
+  constexpr int kFixed = 1024 + K::kBytes + int(sizeof(Ctrl)) + int(sizeof(Plan));
+  const int smem = kFixed + 4 * (max_groups(J, p.E) + 2 * p.E);
+  constexpr int kMost = kFixed + 4 * (max_groups(J, kMaxE) + 2 * kMaxE);
+  static_assert(K::kStages <= 12 && kMost <= 227 * 1024, "shared memory");
+  constexpr auto kern = &experts_kernel<T, R, J>;
+  if (!allow_shared_memory<kern>(kMost)) return MOE_ERR_CUDA;
   // No more CTAs than there can be items: every slot in a group of its own.
   const int64_t most = int64_t(p.T) * p.k * ((p.F + K::BM - 1) / K::BM + (p.H + K::BM - 1) / K::BM * p.KS);
   const int grid = static_cast<int>(most < sms ? most : sms);

@@ -718,13 +718,12 @@ __global__ void __launch_bounds__(kThreads, 2)
   if (parts > 1) cluster_sync_all();
 }
 
-template <typename K, typename... A>
-int launch(K kern, dim3 grid, int threads, dim3 cluster, int smem, cudaStream_t stream, A... args) {
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-    return MOE_ERR_CUDA;
+template <auto kern, typename... A>
+int launch(dim3 grid, dim3 cluster, int smem, cudaStream_t stream, A... args) {
+  if (!allow_shared_memory<kern>(smem)) return MOE_ERR_CUDA;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
+  cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr{};
@@ -775,7 +774,7 @@ int shrink(const void* x, int64_t ldx, Weights w, bool transposed, Scale scale, 
     constexpr int RP = decltype(rp)::value;
     const unsigned tiles = static_cast<unsigned>(most_tiles(m, adapters, kShrinkRows));
     const unsigned parts = cluster_parts(tiles, 2 * 148, k, 256);
-    return launch(shrink_kernel<T, kT, RP>, dim3(tiles, parts), kThreads, dim3(1, parts),
+    return launch<&shrink_kernel<T, kT, RP>>(dim3(tiles, parts), dim3(1, parts),
                   ShrinkCfg<kT, RP>::kBytes, stream, static_cast<const T*>(x), ldx,
                   static_cast<const T*>(w.p), w.stride_l, w.stride_row, plan.perm, plan.offs, adapters,
                   static_cast<int>(k), rank, m * rank, static_cast<T*>(s), scale, plan.place,
@@ -796,8 +795,8 @@ int expand(const void* s, Weights w, bool transposed, Scale scale, const PlanVie
     const int64_t tiles = most_tiles(m, adapters, kExpandRows), want = (1200 + tiles - 1) / tiles;
     const int splits = static_cast<int>(want < blocks ? want : blocks);
     const int64_t units = tiles * splits, places = 2 * 148;
-    return launch(expand_kernel<T, kT, RP>, dim3(static_cast<unsigned>(units < places ? units : places)),
-                  kThreads, dim3(1, 1), ExpandCfg<kT, RP>::kBytes, stream, static_cast<const T*>(s),
+    return launch<&expand_kernel<T, kT, RP>>(dim3(static_cast<unsigned>(units < places ? units : places)),
+                  dim3(1, 1), ExpandCfg<kT, RP>::kBytes, stream, static_cast<const T*>(s),
                   m * rank, static_cast<const T*>(w.p), w.stride_l, w.stride_row, scale, plan.perm,
                   plan.offs, plan.place, plan.left, static_cast<int>(PlanView::tiles(m)), splits, adapters,
                   static_cast<int>(n), rank, static_cast<T*>(y), ldy);
@@ -815,7 +814,7 @@ int grad(const void* s, const void* z, int64_t ldz, bool transposed, Scale scale
     const unsigned blocks = static_cast<unsigned>((n + C::kCols - 1) / C::kCols);
     // Adapters' rows are uneven, so several CTAs a place on the SMs: the largest's rows spread.
     const unsigned parts = cluster_parts(int64_t(blocks) * adapters, 4 * 2 * 148, m / adapters, 64);
-    return launch(grad_kernel<T, kT, RP>, dim3(parts, blocks, adapters), kThreads, dim3(parts, 1),
+    return launch<&grad_kernel<T, kT, RP>>(dim3(parts, blocks, adapters), dim3(parts, 1),
                   C::kBytes, stream, static_cast<const T*>(s), m * rank, static_cast<const T*>(z), ldz,
                   scale, plan.perm, plan.offs, static_cast<int>(n), rank, static_cast<T*>(g), n * rank,
                   kT ? n : int64_t(rank));
@@ -861,17 +860,28 @@ int shared_product(const void* x, int64_t ldx, const void* w, int64_t stride_k, 
 // Adapters that the shared product takes in a tile of rows; none on the 1-SM kernel.
 int per_tile() { return force_single_sm_kernel() ? 0 : gg::Adapters::kPerTile; }
 int64_t low_bytes(int64_t m, int32_t rank) { return 4 * m * rank; }
+// The caller's buffer: x A^T by adapter and dy B by adapter (two parts each), the row
+// tiles' blocks, the plan.
+struct Buffers {
+  char *s, *t, *blocks, *plan;
+  int64_t bytes;
+  Buffers(void* kept, int64_t m, int32_t adapters, int32_t rank) {
+    const int64_t low = low_bytes(m, rank);
+    const int64_t in_blocks =
+        lora::PlanView::tiles(m) * gg::Adapters::kPerTile * lora::kTileRows * int64_t(rank) * 2;
+    s = static_cast<char*>(kept);
+    t = s + low;
+    blocks = t + low;
+    plan = blocks + in_blocks;
+    bytes = 2 * low + in_blocks + 4 * lora::PlanView::ints(m, adapters);
+  }
+};
 }  // namespace
 
-extern "C" int64_t moe_lora_kept_bytes(int64_t m, int32_t adapters, int32_t rank) {
+extern "C" int64_t moe_lora_kept_bytes(int64_t m, int32_t adapters, int32_t rank, int32_t for_backward) {
   if (!dims_ok(MOE_DTYPE_BF16, m, 8, 8, adapters, rank)) return -1;
-  return low_bytes(m, rank) + 4 * lora::PlanView::ints(m, adapters);
-}
-
-extern "C" int64_t moe_lora_workspace_bytes(int64_t m, int32_t adapters, int32_t rank) {
-  if (!dims_ok(MOE_DTYPE_BF16, m, 8, 8, adapters, rank)) return -1;
-  return low_bytes(m, rank) +
-         lora::PlanView::tiles(m) * gg::Adapters::kPerTile * lora::kTileRows * int64_t(rank) * 2;
+  if (!for_backward && m <= lora::kFewRows) return low_bytes(m, rank);
+  return Buffers(nullptr, m, adapters, rank).bytes;
 }
 
 extern "C" int32_t moe_lora_forward(const void* x, int64_t ldx, const void* weight, int64_t ldw,
@@ -880,33 +890,31 @@ extern "C" int32_t moe_lora_forward(const void* x, int64_t ldx, const void* weig
                                     const void* ids, int32_t ids_int64, const float* scale,
                                     float scale_all, int32_t dtype, int64_t m, int64_t k, int64_t n,
                                     int32_t adapters, int32_t rank, int32_t for_backward, void* y,
-                                    int64_t ldy, void* kept, void* workspace, int32_t* status,
-                                    void* stream) {
+                                    int64_t ldy, void* kept, int32_t* status, void* stream) {
   const lora::Weights a{lora_a, a_stride_l, a_stride_row}, b{lora_b, b_stride_l, b_stride_row};
   if (!dims_ok(dtype, m, k, n, adapters, rank) || kept == nullptr || !aligned16(kept) ||
       !rows_ok(weight, ldw, k) || !weights_ok(a, rank, k, adapters) || !weights_ok(b, n, rank, adapters) ||
-      (m > 0 && (!rows_ok(x, ldx, k) || !rows_ok(y, ldy, n) || ids == nullptr || workspace == nullptr ||
-                 !aligned16(workspace))))
+      (m > 0 && (!rows_ok(x, ldx, k) || !rows_ok(y, ldy, n) || ids == nullptr)))
     return MOE_ERR_INVALID_ARG;
-  const lora::PlanView plan(static_cast<char*>(kept) + low_bytes(m, rank), m, adapters);
   const lora::Scale sc{scale, scale_all};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (!for_backward && m > 0 && m <= lora::kFewRows)
     return lora::forward_few_rows(x, ldx, weight, ldw, a, b, ids, ids_int64, sc, dtype,
                                   static_cast<int>(m), static_cast<int>(k), static_cast<int>(n), adapters,
                                   rank, y, ldy, static_cast<float*>(kept), status, st);
-  char* blocks = static_cast<char*>(workspace) + low_bytes(m, rank);
+  const Buffers buf(kept, m, adapters, rank);
+  const lora::PlanView plan(buf.plan, m, adapters);
   lora::plan_kernel<<<static_cast<unsigned>(adapters + lora::PlanView::tiles(m)), 1024, 0, st>>>(
-      ids, ids_int64, static_cast<int>(m), adapters, rank, plan, per_tile(), reinterpret_cast<uint4*>(blocks),
-      status);
+      ids, ids_int64, static_cast<int>(m), adapters, rank, plan, per_tile(),
+      reinterpret_cast<uint4*>(buf.blocks), status);
   if (cudaGetLastError() != cudaSuccess) return MOE_ERR_CUDA;
   if (m == 0) return MOE_OK;
-  int rc = lora::shrink(x, ldx, a, false, sc, plan, dtype, m, k, adapters, rank, kept, blocks, st);
+  int rc = lora::shrink(x, ldx, a, false, sc, plan, dtype, m, k, adapters, rank, buf.s, buf.blocks, st);
   if (rc == MOE_OK)
-    rc = shared_product(x, ldx, weight, 1, ldw, y, ldy, plan, b, blocks, m, k, n, adapters, rank, dtype, status,
+    rc = shared_product(x, ldx, weight, 1, ldw, y, ldy, plan, b, buf.blocks, m, k, n, adapters, rank, dtype, status,
                         st);
   if (rc == MOE_OK)
-    rc = lora::expand(kept, b, false, sc, plan, dtype, m, n, adapters, rank, y, ldy, st);
+    rc = lora::expand(buf.s, b, false, sc, plan, dtype, m, n, adapters, rank, y, ldy, st);
   return rc;
 }
 
@@ -915,38 +923,31 @@ extern "C" int32_t moe_lora_backward(const void* dy, int64_t lddy, const void* x
                                      int64_t a_stride_l, int64_t a_stride_row, const void* lora_b,
                                      int64_t b_stride_l, int64_t b_stride_row, const float* scale,
                                      float scale_all, int32_t dtype, int64_t m, int64_t k, int64_t n,
-                                     int32_t adapters, int32_t rank, const void* kept, void* workspace,
-                                     void* dx, int64_t lddx, void* da, void* db, int32_t* status,
-                                     void* stream) {
+                                     int32_t adapters, int32_t rank, void* kept, void* dx, int64_t lddx,
+                                     void* da, void* db, int32_t* status, void* stream) {
   const lora::Weights a{lora_a, a_stride_l, a_stride_row}, b{lora_b, b_stride_l, b_stride_row};
   if (!dims_ok(dtype, m, k, n, adapters, rank) || kept == nullptr || !aligned16(kept) ||
       !rows_ok(weight, ldw, k) || !weights_ok(a, rank, k, adapters) || !weights_ok(b, n, rank, adapters) ||
       (da != nullptr && !aligned16(da)) || (db != nullptr && !aligned16(db)) ||
-      (m > 0 && (!rows_ok(dy, lddy, n) || !rows_ok(x, ldx, k) ||
-                 ((dx != nullptr || da != nullptr) && (workspace == nullptr || !aligned16(workspace))) ||
-                 (dx != nullptr && !rows_ok(dx, lddx, k)))))
+      (m > 0 && (!rows_ok(dy, lddy, n) || !rows_ok(x, ldx, k) || (dx != nullptr && !rows_ok(dx, lddx, k)))))
     return MOE_ERR_INVALID_ARG;
-  const lora::PlanView plan(const_cast<char*>(static_cast<const char*>(kept)) + low_bytes(m, rank), m, adapters);
+  const Buffers buf(kept, m, adapters, rank);
+  const lora::PlanView plan(buf.plan, m, adapters);
   const lora::Scale sc{scale, scale_all};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  char* blocks = static_cast<char*>(workspace) + low_bytes(m, rank);
   int rc = MOE_OK;
-  if (m > 0 && (dx != nullptr || da != nullptr)) {
-    // The blocks' rows of other adapters are zeros again: the forward's may be gone.
-    if (dx != nullptr && cudaMemsetAsync(blocks, 0, moe_lora_workspace_bytes(m, adapters, rank) - low_bytes(m, rank),
-                                         st) != cudaSuccess)
-      return MOE_ERR_CUDA;
-    rc = lora::shrink(dy, lddy, b, true, sc, plan, dtype, m, n, adapters, rank, workspace, blocks, st);
-  }
+  // The rows of the blocks that the forward left zero are those of this pass too.
+  if (m > 0 && (dx != nullptr || da != nullptr))
+    rc = lora::shrink(dy, lddy, b, true, sc, plan, dtype, m, n, adapters, rank, buf.t, buf.blocks, st);
   if (rc == MOE_OK && m > 0 && dx != nullptr) {
-    rc = shared_product(dy, lddy, weight, ldw, 1, dx, lddx, plan, a, blocks, m, n, k, adapters, rank, dtype,
+    rc = shared_product(dy, lddy, weight, ldw, 1, dx, lddx, plan, a, buf.blocks, m, n, k, adapters, rank, dtype,
                         status, st);
     if (rc == MOE_OK)
-      rc = lora::expand(workspace, a, true, sc, plan, dtype, m, k, adapters, rank, dx, lddx, st);
+      rc = lora::expand(buf.t, a, true, sc, plan, dtype, m, k, adapters, rank, dx, lddx, st);
   }
   if (rc == MOE_OK && da != nullptr)
-    rc = lora::grad(workspace, x, ldx, true, sc, plan, dtype, m, k, adapters, rank, da, st);
+    rc = lora::grad(buf.t, x, ldx, true, sc, plan, dtype, m, k, adapters, rank, da, st);
   if (rc == MOE_OK && db != nullptr)
-    rc = lora::grad(kept, dy, lddy, false, sc, plan, dtype, m, n, adapters, rank, db, st);
+    rc = lora::grad(buf.s, dy, lddy, false, sc, plan, dtype, m, n, adapters, rank, db, st);
   return rc;
 }

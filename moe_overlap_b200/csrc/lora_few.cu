@@ -250,11 +250,10 @@ int project(const T* x, int64_t ldx, const void* weight, int64_t ldw, Weights b,
   int rc = encode_tiled(&wmap, dt, 2, weight, wdims, wstrides, wbox);
   if (rc == MOE_OK) rc = encode_tiled(&xmap, dt, 2, x, xdims, xstrides, xbox);
   if (rc != MOE_OK) return rc;
-  auto kern = &project_kernel<T, R, J>;
+  constexpr auto kern = &project_kernel<T, R, J>;
   constexpr int kSmem = 1024 + Q::kBytes + int(sizeof(Ctrl));
   static_assert(kSmem <= 227 * 1024, "shared memory");
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess)
-    return MOE_ERR_CUDA;
+  if (!allow_shared_memory<kern>(kSmem)) return MOE_ERR_CUDA;
   const int blocks = (n + Q::BM - 1) / Q::BM;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(blocks < sms ? blocks : sms);

@@ -21,7 +21,6 @@ __all__ = ["lora_linear"]
 _DTYPE_CODE = {torch.bfloat16: _lib.MOE_DTYPE_BF16, torch.float16: _lib.MOE_DTYPE_F16}
 MAX_RANK = 128
 MAX_ADAPTERS = 1024
-FEW_ROWS = 64  # a batch of so many rows without gradients takes the decode kernels
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -36,28 +35,21 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t.clone(memory_format=torch.contiguous_format)
 
 
-def _scale_args(scale):
-    return (scale.data_ptr(), 0.0) if isinstance(scale, torch.Tensor) else (None, scale)
-
-
 def _forward(x, weight, lora_a, lora_b, ids, scale, for_backward):
-    """(y, what the backward needs: x A^T and the rows by adapter)."""
+    """(y, the buffer that the backward needs)."""
     (m, k), n = x.shape, weight.shape[0]
     adapters, rank, _ = lora_a.shape
-    dev = x.device
+    dev, dt = x.device, x.dtype
     lib = _lib.load()
-    y = torch.empty(m, n, dtype=x.dtype, device=dev)
-    kept = torch.empty(lib.moe_lora_kept_bytes(m, adapters, rank), dtype=torch.uint8, device=dev)
-    ws = kept  # a decode batch needs no more
-    if for_backward or m > FEW_ROWS:
-        ws = torch.empty(lib.moe_lora_workspace_bytes(m, adapters, rank), dtype=torch.uint8, device=dev)
+    sa, sb = lora_a.stride(), lora_b.stride()
+    each, all_ = (scale.data_ptr(), 0.0) if isinstance(scale, torch.Tensor) else (None, scale)
+    y = torch.empty(m, n, dtype=dt, device=dev)
+    kept = torch.empty(lib.moe_lora_kept_bytes(m, adapters, rank, for_backward), dtype=torch.uint8, device=dev)
     with _lib.on_device(dev):
         rc = lib.moe_lora_forward(
-            x.data_ptr(), x.stride(0), weight.data_ptr(), weight.stride(0),
-            lora_a.data_ptr(), lora_a.stride(0), lora_a.stride(1),
-            lora_b.data_ptr(), lora_b.stride(0), lora_b.stride(1),
-            ids.data_ptr(), ids.dtype == torch.int64, *_scale_args(scale), _DTYPE_CODE[x.dtype], m, k, n,
-            adapters, rank, for_backward, y.data_ptr(), n, kept.data_ptr(), ws.data_ptr(),
+            x.data_ptr(), x.stride(0), weight.data_ptr(), weight.stride(0), lora_a.data_ptr(), sa[0], sa[1],
+            lora_b.data_ptr(), sb[0], sb[1], ids.data_ptr(), ids.dtype == torch.int64, each, all_,
+            _DTYPE_CODE[dt], m, k, n, adapters, rank, for_backward, y.data_ptr(), n, kept.data_ptr(),
             _lib.status_address(dev), _lib.stream_handle(dev))
     _lib.check_call(rc, "moe_lora_forward")
     return y, kept
@@ -78,27 +70,23 @@ class LoraLinear(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         x, weight, lora_a, lora_b, kept = ctx.saved_tensors
-        need_x, _, need_a, need_b, _, _ = ctx.needs_input_grad
+        need = ctx.needs_input_grad
         (m, k), n = x.shape, weight.shape[0]
         adapters, rank, _ = lora_a.shape
-        dev, dt = x.device, x.dtype
-        lib = _lib.load()
+        dev, dt, scale = x.device, x.dtype, ctx.scale
+        sa, sb = lora_a.stride(), lora_b.stride()
+        each, all_ = (scale.data_ptr(), 0.0) if isinstance(scale, torch.Tensor) else (None, scale)
         dy = _rows(dy)
-        dx = torch.empty(m, k, dtype=dt, device=dev) if need_x else None
-        da = torch.empty(adapters, rank, k, dtype=dt, device=dev) if need_a else None
-        db = torch.empty(adapters, n, rank, dtype=dt, device=dev) if need_b else None
-        ws = None
-        if need_x or need_a:
-            ws = torch.empty(lib.moe_lora_workspace_bytes(m, adapters, rank), dtype=torch.uint8, device=dev)
+        dx = torch.empty(m, k, dtype=dt, device=dev) if need[0] else None
+        da = torch.empty(adapters, rank, k, dtype=dt, device=dev) if need[2] else None
+        db = torch.empty(adapters, n, rank, dtype=dt, device=dev) if need[3] else None
         with _lib.on_device(dev):
-            rc = lib.moe_lora_backward(
-                dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0), weight.data_ptr(),
-                weight.stride(0), lora_a.data_ptr(), lora_a.stride(0), lora_a.stride(1),
-                lora_b.data_ptr(), lora_b.stride(0), lora_b.stride(1), *_scale_args(ctx.scale),
+            rc = _lib.load().moe_lora_backward(
+                dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0), weight.data_ptr(), weight.stride(0),
+                lora_a.data_ptr(), sa[0], sa[1], lora_b.data_ptr(), sb[0], sb[1], each, all_,
                 _DTYPE_CODE[dt], m, k, n, adapters, rank, kept.data_ptr(),
-                *(v.data_ptr() if v is not None else None for v in (ws, dx)), k,
-                *(v.data_ptr() if v is not None else None for v in (da, db)),
-                _lib.status_address(dev), _lib.stream_handle(dev))
+                dx.data_ptr() if dx is not None else None, k, da.data_ptr() if da is not None else None,
+                db.data_ptr() if db is not None else None, _lib.status_address(dev), _lib.stream_handle(dev))
         _lib.check_call(rc, "moe_lora_backward")
         return dx, None, da, db, None, None
 
@@ -182,12 +170,17 @@ def lora_linear(x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor, lor
             raise ValueError("scale must be a number or a float tensor [L]")
         if scale.requires_grad and torch.is_grad_enabled():
             raise ValueError("lora_linear gives the scale no gradient")
-        scale = scale.to(device=x.device, dtype=torch.float32).contiguous()
+        if scale.dtype != torch.float32 or scale.device != dev or not scale.is_contiguous():
+            scale = scale.to(device=dev, dtype=torch.float32).contiguous()
     else:
         scale = float(scale)
     _lib.check_status(dev)
     pk, pn, pr = -k % 8, -n % 8, -rank % 8
-    if pk or pn or pr:
+    if not (pk or pn or pr) and x.is_contiguous() and weight.is_contiguous() and lora_a.is_contiguous() \
+            and lora_b.is_contiguous() and adapter_ids.is_contiguous() \
+            and not (x.data_ptr() | weight.data_ptr() | lora_a.data_ptr() | lora_b.data_ptr()) & 15:
+        args = (x, weight, lora_a, lora_b, adapter_ids, scale)
+    elif pk or pn or pr:
         args = (_rows(_pad(x, pk)), _rows(_pad(weight, pk, pn)), _rows(_pad(lora_a, pk, pr)),
                 _rows(_pad(lora_b, pr, pn)), adapter_ids.contiguous(), scale)
     else:
