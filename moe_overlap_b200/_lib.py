@@ -12,7 +12,6 @@ raised at the next call (like CUDA's own asynchronous error reporting), and
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import os
 import threading
@@ -22,6 +21,8 @@ import torch
 
 LIB_NAME = "libmoe_overlap_b200.so"
 LIB_PATH = Path(__file__).resolve().with_name(LIB_NAME)
+# The torch extension in front of some of its entry points (csrc/torch_ops.cpp).
+TORCH_OPS_PATH = Path(__file__).resolve().with_name("_torch_ops.so")
 
 MOE_OK = 0
 MOE_ERR_INVALID_ARG = 1
@@ -221,6 +222,7 @@ SIGNATURES: dict[str, tuple] = {
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
+_torch_ops = None
 _status_words: dict[int, torch.Tensor] = {}
 _status_views: dict[int, ctypes.c_int32] = {}  # the same words, read without a torch call
 
@@ -254,6 +256,28 @@ def load() -> ctypes.CDLL:
     return _lib
 
 
+def torch_ops():
+    """The torch extension module, loaded once and bound to the library's entry points."""
+    global _torch_ops
+    if _torch_ops is not None:
+        return _torch_ops
+    lib = load()
+    with _lock:
+        if _torch_ops is None:
+            if not TORCH_OPS_PATH.exists():
+                raise RuntimeError(f"{TORCH_OPS_PATH.name} is not built (expected at {TORCH_OPS_PATH}); "
+                                   "run `python -m moe_overlap_b200.build`")
+            from . import _torch_ops as ops
+
+            ops.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value
+                       for name in ("moe_few_tokens", "moe_few_tokens_workspace", "moe_lora_forward",
+                                    "moe_lora_backward", "moe_lora_kept_bytes")))
+            for idx, w in _status_words.items():
+                ops.set_status_word(idx, w.data_ptr())
+            _torch_ops = ops
+    return _torch_ops
+
+
 def status_string(code: int) -> str:
     return load().moe_status_string(int(code)).decode()
 
@@ -268,6 +292,8 @@ def status_word(device: torch.device) -> torch.Tensor:
             if w is None:
                 w = torch.zeros(1, dtype=torch.int32, pin_memory=True)
                 _status_views[idx] = ctypes.c_int32.from_address(w.data_ptr())
+                if _torch_ops is not None:
+                    _torch_ops.set_status_word(idx, w.data_ptr())
                 _status_words[idx] = w
     return w
 
@@ -278,26 +304,12 @@ def check_status(device: torch.device | None = None, sync: bool = False) -> None
         device = torch.device("cuda", torch.cuda.current_device())
     if sync:
         torch.cuda.synchronize(device)
-    status_address(device)
+    status_word(device)
     view = _status_views[device.index if device.index is not None else torch.cuda.current_device()]
     code = view.value
     if code != 0:
         view.value = 0
         raise MoeError(code, "device-side error from an earlier moe_overlap_b200 kernel")
-
-
-def status_address(device: torch.device) -> int:
-    """Address of ``device``'s status word, for the C entry points."""
-    view = _status_views.get(device.index)
-    return ctypes.addressof(view) if view is not None else status_word(device).data_ptr()
-
-
-_SAME_DEVICE = contextlib.nullcontext()
-
-
-def on_device(device: torch.device):
-    """Makes ``device`` current for a ``with`` block; free when it already is."""
-    return _SAME_DEVICE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def check_call(code: int, where: str) -> None:

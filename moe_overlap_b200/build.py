@@ -16,6 +16,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
@@ -25,6 +26,7 @@ INCLUDE = REPO_DIR / "include"
 BUILD_DIR = REPO_DIR / "_build"
 LIB_NAME = "libmoe_overlap_b200.so"
 LIB_PATH = PKG_DIR / LIB_NAME
+TORCH_OPS_PATH = PKG_DIR / "_torch_ops.so"
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = [
@@ -68,14 +70,40 @@ def _compile(src: Path, force: bool, verbose: bool) -> tuple[Path, str]:
     return obj, (proc.stdout + proc.stderr) if verbose else ""
 
 
+def _build_torch_ops(force: bool) -> None:
+    """The C++ extension that puts torch tensors and autograd in front of the C ABI."""
+    src = CSRC / "torch_ops.cpp"
+    newest = max(f.stat().st_mtime for f in (src, *INCLUDE.glob("*.h")))
+    if not force and TORCH_OPS_PATH.exists() and TORCH_OPS_PATH.stat().st_mtime >= newest:
+        return
+    import torch
+    from torch.utils import cpp_extension
+
+    torch_lib = Path(torch.__file__).resolve().parent / "lib"
+    includes = [*cpp_extension.include_paths("cuda"), sysconfig.get_paths()["include"], str(INCLUDE)]
+    tmp = TORCH_OPS_PATH.with_suffix(".so.tmp")
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           "-DTORCH_EXTENSION_NAME=_torch_ops", "-DTORCH_API_INCLUDE_EXTENSION_H",
+           *(f"-isystem{p}" for p in includes), str(src), "-o", str(tmp), f"-L{torch_lib}",
+           f"-Wl,-rpath,{torch_lib}", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_python"]
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError(f"g++ failed for {src.name}:\n{proc.stdout}\n{proc.stderr}")
+    os.replace(tmp, TORCH_OPS_PATH)
+
+
 def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compiles (if stale) and links the library; returns its path."""
+    """Compiles (if stale) and links the library and the torch extension; returns the
+    library's path."""
     BUILD_DIR.mkdir(exist_ok=True)
     sources = sorted(CSRC.glob("*.cu"))
     if not sources:
         raise RuntimeError(f"no CUDA sources under {CSRC}")
     with cf.ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as ex:
+        torch_ops = ex.submit(_build_torch_ops, force)
         results = list(ex.map(lambda s: _compile(s, force, verbose), sources))
+        torch_ops.result()
     objs = [o for o, _ in results]
     for _, log in results:
         if log:

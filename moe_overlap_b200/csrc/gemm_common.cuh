@@ -35,15 +35,17 @@ struct ArrivalWait {
 };
 
 // Adapters' products added in the accumulator of a one-expert product: for each of the
-// first count[t] adapters list[t] of row tile t (256 rows), the product of `rows` (256
+// first count[t] adapters of row tile t's list (256 rows), the product of `rows` (256
 // x rank for each of the tile's kPerTile places, zeros in rows of other adapters) and
 // that adapter's matrix w_i, stored in the direction of B (one matrix behind another,
 // `stride_l` apart, rows `stride_row` apart).
 struct Adapters {
-  static constexpr int kPerTile = 4;
+  // Each costs ceil(rank / 64) k-blocks in every tile; left out, its rows of C are read
+  // and written once more instead.  At k = 2048 and rank 64 eight add a quarter to a tile.
+  static constexpr int kPerTile = 8;
   const void* rows;      // [row tiles][kPerTile][256][rank], the inputs' type
   const int32_t* count;  // [row tiles]
-  const int4* list;      // [row tiles]
+  const int32_t* list;   // [row tiles][kPerTile]
   const void* w;
   int64_t stride_l, stride_row;
   int rank, adapters;
@@ -342,7 +344,7 @@ struct AdapterMaps {
   CUtensorMap rows, rows_half;  // boxes as A's and its half
   CUtensorMap w;                // boxes as B's
   const int32_t* count;
-  const int4* list;
+  const int32_t* list;
   int k_blocks;  // of 64 in the rank
 };
 

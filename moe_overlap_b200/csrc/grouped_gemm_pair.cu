@@ -355,12 +355,10 @@ __global__ void __cluster_dims__(2, 1, 1) __maxnreg__(kMaxRegs)
         }
         if (s.z < 0) break;
         int expert = s.w;
-        int4 list = make_int4(0, 0, 0, 0);
         int extra_kb = 0;
         if constexpr (ADAPTERS) {
           expert = 0;
           extra_kb = s.w * extra.k_blocks;
-          if (extra_kb > 0) list = extra.list[s.x / BM];
         }
         if (expert != ready_expert) {  // expert-ordered dispatch: this expert's rows have landed
           if (!wait_expert_rows(p, expert)) {
@@ -395,7 +393,7 @@ __global__ void __cluster_dims__(2, 1, 1) __maxnreg__(kMaxRegs)
               const int at = (kb - num_kb) / extra.k_blocks;
               k0 = (kb - num_kb - at * extra.k_blocks) * BK;
               a_row = ((s.x / BM) * Adapters::kPerTile + at) * BM + (row_a - s.x);
-              b_matrix = at == 0 ? list.x : at == 1 ? list.y : at == 2 ? list.z : list.w;
+              b_matrix = extra.list[(s.x / BM) * Adapters::kPerTile + at];
               ka = half_box ? &extra.rows_half : &extra.rows;
               kb_map = &extra.w;
             }

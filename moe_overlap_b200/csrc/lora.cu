@@ -851,8 +851,8 @@ int shared_product(const void* x, int64_t ldx, const void* w, int64_t stride_k, 
   DeviceInfo info;
   const int rc = current_device_info(&dev, &info);
   if (rc != MOE_OK) return rc;
-  const gg::Adapters extra{blocks, plan.count, reinterpret_cast<const int4*>(plan.list), second.p,
-                           second.stride_l, second.stride_row, rank, adapters};
+  const gg::Adapters extra{blocks,          plan.count,        plan.list, second.p,
+                           second.stride_l, second.stride_row, rank,      adapters};
   return gg::grouped_gemm_launch(x, ldx, w, 0, stride_k, stride_n, y, ldy, plan.base, 0, m, k, n, 1, dtype,
                                  MOE_ACT_NONE, info.sm_count, 0, nullptr, nullptr, nullptr, nullptr, 0, status,
                                  stream, nullptr, nullptr, force_single_sm_kernel() ? nullptr : &extra);
