@@ -283,6 +283,11 @@ __global__ void __cluster_dims__(2, 1, 1) __maxnreg__(kMaxRegs)
     ctrl->abort = 0;
     fence_mbar_init();
   }
+  // With adapters the launch is set up beside the kernel that prepares their rows.
+  if constexpr (ADAPTERS) {
+    let_next_kernel_start();
+    wait_for_previous_kernel();
+  }
   if (warp == 0) {
     if (lane == 0) {
       tma_prefetch_desc(&tmap_a);
@@ -564,6 +569,19 @@ int launch(const CUtensorMap& ta, const CUtensorMap& ta_half, const CUtensorMap&
                                     static_cast<int>(smem_bytes(kMaxExperts)));
   });
   if (attr_err != cudaSuccess) return MOE_ERR_CUDA;
+  if constexpr (!std::is_same<EXTRA, NoAdapters>::value) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(NUM_THREADS);
+    cfg.dynamicSmemBytes = smem_bytes(p.num_experts);
+    cfg.stream = stream;
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &early;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kern, ta, ta_half, tb, tc, p, extra) == cudaSuccess ? MOE_OK : MOE_ERR_CUDA;
+  }
   kern<<<grid, NUM_THREADS, smem_bytes(p.num_experts), stream>>>(ta, ta_half, tb, tc, p, extra);
   return cudaGetLastError() == cudaSuccess ? MOE_OK : MOE_ERR_CUDA;
 }

@@ -74,6 +74,7 @@ __device__ __forceinline__ int id_at(const void* ids, int ids64, int m, int L) {
 __global__ void __launch_bounds__(1024) plan_kernel(const void* ids, int ids64, int M, int L, int r,
                                                     PlanView plan, int per_tile, uint4* blocks,
                                                     int32_t* status) {
+  let_next_kernel_start();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tid = threadIdx.x;
   if (static_cast<int>(blockIdx.x) < L) {
     __shared__ int less[32], equal[32];
@@ -259,9 +260,17 @@ __global__ void __launch_bounds__(kThreads, 2)
                   const int32_t* place, T* blocks) {
   using C = ShrinkCfg<kT, RP>;
   extern __shared__ __align__(128) char smem[];
+  __shared__ int2 block_of[kShrinkRows];  // a row's block in the tiles' blocks and its row there
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  let_next_kernel_start();
+  wait_for_previous_kernel();
   const Tile t = find_tile(offs, L, blockIdx.x, kShrinkRows);
   if (t.i < 0) return;  // the same in every CTA of the cluster
+  const float c = scale.of(t.i);
+  if (tid < t.rows) {
+    const int row = perm[t.p0 + tid];
+    block_of[tid] = make_int2(place[row], row % kTileRows);
+  }
   const int parts = gridDim.y, part = blockIdx.y;
   const int cols = ((K + parts - 1) / parts + kShrinkCols - 1) / kShrinkCols * kShrinkCols;
   const int k0 = min(K, part * cols), k1 = min(K, k0 + cols);
@@ -382,7 +391,6 @@ __global__ void __launch_bounds__(kThreads, 2)
     cluster_sync_all();
   else
     __syncthreads();
-  const float c = scale.of(t.i);
   const int share = kShrinkRows / parts;  // rows that this CTA finishes
   for (int e = tid; e < share * (RP / 4); e += kThreads) {
     const int m = part * share + e / (RP / 4), j = e % (RP / 4) * 4;
@@ -393,10 +401,10 @@ __global__ void __launch_bounds__(kThreads, 2)
     T* out = s + int64_t(t.p0 + m) * r + j;
     *reinterpret_cast<uint2*>(out) = *reinterpret_cast<const uint2*>(hi);
     *reinterpret_cast<uint2*>(out + part_stride) = *reinterpret_cast<const uint2*>(lo);
-    const int row = perm[t.p0 + m], at = place[row];
-    if (at >= 0) {  // the shared product takes this row's
+    const int2 at = block_of[m];
+    if (at.x >= 0) {  // the shared product takes this row's
       const T o[4] = {from_f<T>(c * v.x), from_f<T>(c * v.y), from_f<T>(c * v.z), from_f<T>(c * v.w)};
-      *reinterpret_cast<uint2*>(blocks + (int64_t(at) * kTileRows + row % kTileRows) * r + j) =
+      *reinterpret_cast<uint2*>(blocks + (int64_t(at.x) * kTileRows + at.y) * r + j) =
           *reinterpret_cast<const uint2*>(o);
     }
   }
@@ -428,6 +436,8 @@ __global__ void __launch_bounds__(kThreads, 2)
   using C = ExpandCfg<kT, RP>;
   extern __shared__ __align__(128) char smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, q4 = lane & 3;
+  let_next_kernel_start();
+  wait_for_previous_kernel();
   // Usually the shared product has taken every row.
   bool any = false;
   for (int q = tid; q < tiles; q += kThreads) any |= left[q] != 0;
@@ -598,6 +608,8 @@ __global__ void __launch_bounds__(kThreads, 2)
   extern __shared__ __align__(128) char smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int parts = gridDim.x, part = blockIdx.x, n0 = blockIdx.y * C::kCols, i = blockIdx.z;
+  let_next_kernel_start();
+  wait_for_previous_kernel();
   const int o0 = offs[i], rows = offs[i + 1] - o0;
   const int share = ((rows + parts - 1) / parts + kGradRows - 1) / kGradRows * kGradRows;
   const int p0 = min(rows, part * share), p1 = min(rows, p0 + share);
@@ -726,13 +738,16 @@ int launch(dim3 grid, dim3 cluster, int smem, cudaStream_t stream, A... args) {
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = cluster.x;
-  attr.val.clusterDim.y = cluster.y;
-  attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = cluster.x * cluster.y > 1 ? 1 : 0;
+  // Set up beside the kernel before (each waits for that one's end before it reads).
+  cudaLaunchAttribute attr[2] = {};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster.x;
+  attr[1].val.clusterDim.y = cluster.y;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster.x * cluster.y > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kern, args...) == cudaSuccess ? MOE_OK : MOE_ERR_CUDA;
 }
 

@@ -78,6 +78,7 @@ struct Cfg {
 struct Ctrl {
   uint64_t full[12], empty[12];
   int id[kFewRows];
+  float scale[kFewRows];
 };
 
 template <typename T, int R, int J>
@@ -101,7 +102,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     fence_mbar_init();
   }
-  for (int m = tid; m < M; m += kThreads) ctrl->id[m] = id_at(ids, ids64, m, L);
+  for (int m = tid; m < M; m += kThreads) {
+    const int i = id_at(ids, ids64, m, L);
+    ctrl->id[m] = i;
+    ctrl->scale[m] = i >= 0 ? scale.of(i) : 0.0f;
+  }
   __syncthreads();
   const int blocks = (N + BM - 1) / BM;
   int stage = 0;
@@ -204,7 +209,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           lr[u] = low + m * r;
           add[u] = 0.0f;
         }
-#pragma unroll 1
+#pragma unroll 2
         for (int j = 0; j < r; j += 8) {
           uint4 ub[kTogether];
 #pragma unroll
@@ -228,7 +233,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int i = 0; i < C; ++i)
             v += red[(i * R + n / 16) * (NT * kRedStride) + m * kRedStride + n % 16];
-          if (br[u] != nullptr) v += scale.of(ctrl->id[m]) * add[u];
+          if (br[u] != nullptr) v += ctrl->scale[m] * add[u];
           y[m * ldy + row] = from_f<T>(v);
         }
       }

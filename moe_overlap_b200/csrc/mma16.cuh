@@ -113,13 +113,4 @@ __device__ __forceinline__ void red_release_gpu(int* p, int v) {
   asm volatile("red.release.gpu.global.add.s32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
 }
 
-// A kernel launched to start beside the one before it (programmatic stream
-// serialisation) waits here for that one's end; one that lets the next start says so.
-__device__ __forceinline__ void wait_for_previous_kernel() {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-}
-__device__ __forceinline__ void let_next_kernel_start() {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-}
-
 }  // namespace moe

@@ -358,6 +358,16 @@ __device__ __forceinline__ void fence_proxy_async_global() {
   asm volatile("fence.proxy.async.global;" ::: "memory");
 }
 
+// ------------------------------------------------- programmatic launches --
+// A kernel launched to start beside the one before it (programmatic stream
+// serialisation) waits here for that one's end; one that lets the next start says so.
+__device__ __forceinline__ void wait_for_previous_kernel() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+__device__ __forceinline__ void let_next_kernel_start() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 // ----------------------------------------------------------- status word --
 // Records the first device-side error into the caller's status word (device
 // memory or mapped pinned host memory); plain volatile store so it also works
