@@ -35,7 +35,9 @@
 // its rows, the k-blocks of the adapter's rank, A from the tile's rows of x A_i^T (zeros in
 // other adapters' rows) and B from the adapter's second matrix; boxes past the rank are
 // zero-filled, so any rank fills whole k-blocks.  The sum stays in the accumulator and is
-// rounded once.
+// rounded once.  The launch may start beside the kernel that prepares those rows: only the
+// threads that fetch and multiply them wait for its end, behind their first tile's own
+// k-blocks (everything before that kernel is complete when this one starts).
 // No load uses cluster multicast; the pair exchanges only barrier arrivals and
 // the tile ring entries through shared::cluster addresses.
 #include <algorithm>
@@ -185,13 +187,13 @@ __device__ __forceinline__ void store_swapped(uint32_t t_lane_base, int lane, in
 // each stage's data, issues its four 16-deep MMAs into the accumulator at d_tmem
 // and commits the stage back to both CTAs' producers.  SWAPPED issues the swapped
 // form (B stage as the MMA's A operand with M = 256, the A stage's first N/2 rows
-// as its B operand, N and the operand layouts in idesc_sw).  Returns false when a
-// wait gave up.
+// as its B operand, N and the operand layouts in idesc_sw).  The first MMA overwrites the
+// accumulator, or adds to it when `more`.  Returns false when a wait gave up.
 template <bool BF16, bool B_MN_MAJOR, bool SWAPPED>
 __device__ __forceinline__ bool issue_tile(Ctrl* ctrl, uint8_t* sA, uint8_t* sB, uint32_t d_tmem,
                                            int num_kb, int& stage, uint32_t& phase,
                                            const volatile int* abort_flag, bool& issued_any,
-                                           uint32_t idesc_sw) {
+                                           uint32_t idesc_sw, uint32_t more = 0u) {
   const uint32_t idesc = SWAPPED ? idesc_sw : idesc_f16(BF16, BM, BN, false, B_MN_MAJOR);
   // This thread's loop is on the critical path and shares its SM sub-partition with
   // two epilogue warps, so every per-stage quantity is formed once per tile and
@@ -217,9 +219,9 @@ __device__ __forceinline__ bool issue_tile(Ctrl* ctrl, uint8_t* sA, uint8_t* sB,
       const uint64_t adesc = adesc0 + uint64_t(kk * (UMMA_K * 2 / 16));
       const uint64_t bdesc = bdesc0 + uint64_t(B_MN_MAJOR ? kk * (UMMA_K * 128 / 16) : kk * (UMMA_K * 2 / 16));
       if constexpr (SWAPPED)
-        umma_f16_pair(d_tmem, bdesc, adesc, idesc, (kb | kk) != 0 ? 1u : 0u);
+        umma_f16_pair(d_tmem, bdesc, adesc, idesc, (kb | kk) != 0 ? 1u : more);
       else
-        umma_f16_pair(d_tmem, adesc, bdesc, idesc, (kb | kk) != 0 ? 1u : 0u);
+        umma_f16_pair(d_tmem, adesc, bdesc, idesc, (kb | kk) != 0 ? 1u : more);
     }
     issued_any = true;
     umma_commit_pair(empty_s0 + 8u * uint32_t(stage));
@@ -283,19 +285,24 @@ __global__ void __cluster_dims__(2, 1, 1) __maxnreg__(kMaxRegs)
     ctrl->abort = 0;
     fence_mbar_init();
   }
-  // With adapters the launch is set up beside the kernel that prepares their rows.
-  if constexpr (ADAPTERS) {
-    let_next_kernel_start();
-    wait_for_previous_kernel();
-  }
+  if constexpr (ADAPTERS) let_next_kernel_start();
   if (warp == 0) {
     if (lane == 0) {
       tma_prefetch_desc(&tmap_a);
       tma_prefetch_desc(&tmap_a_half);
       tma_prefetch_desc(&tmap_b);
     }
-    build_tile_prefix(p.offsets, p.offsets_int64, p.num_experts, p.m_total, BM, tiles_n,
-                      tile_prefix, seg_start, seg_rows, leader ? p.status : nullptr);
+    if constexpr (ADAPTERS) {  // one expert has every row
+      if (lane == 0) {
+        tile_prefix[0] = 0;
+        tile_prefix[1] = (p.m_total + BM - 1) / BM * tiles_n;
+        seg_start[0] = 0;
+        seg_rows[0] = p.m_total;
+      }
+    } else {
+      build_tile_prefix(p.offsets, p.offsets_int64, p.num_experts, p.m_total, BM, tiles_n,
+                        tile_prefix, seg_start, seg_rows, leader ? p.status : nullptr);
+    }
   }
   if (warp == 1) {
     __syncwarp();
@@ -323,6 +330,7 @@ __global__ void __cluster_dims__(2, 1, 1) __maxnreg__(kMaxRegs)
       uint32_t qphase = 0;
       int ready_expert = -1;
       bool failed = false;
+      [[maybe_unused]] bool waited = false;
       const int pair_id = static_cast<int>(cluster_id_x());
       const int npairs = static_cast<int>(nclusters_x());
       for (int iter = 0;; ++iter) {
@@ -339,8 +347,6 @@ __global__ void __cluster_dims__(2, 1, 1) __maxnreg__(kMaxRegs)
             const TileCoord tc = decode_tile(t, p.num_experts, tile_prefix, seg_start, seg_rows,
                                              BM, tiles_n, p.tile_order);
             s = make_int4(tc.row0, tc.rows, tc.tile_n * BN, tc.expert);
-            // the only expert is 0: its place carries the tile's adapters
-            if constexpr (ADAPTERS) s.w = extra.count[tc.row0 / BM];
           }
           ctrl->slot[q] = s;
           st_shared_cluster_v4(mapa_shared(smem_u32(&ctrl->slot[q]), 1), s);
@@ -359,18 +365,12 @@ __global__ void __cluster_dims__(2, 1, 1) __maxnreg__(kMaxRegs)
           qphase ^= 1;
         }
         if (s.z < 0) break;
-        int expert = s.w;
-        int extra_kb = 0;
-        if constexpr (ADAPTERS) {
-          expert = 0;
-          extra_kb = s.w * extra.k_blocks;
-        }
-        if (expert != ready_expert) {  // expert-ordered dispatch: this expert's rows have landed
-          if (!wait_expert_rows(p, expert)) {
+        if (s.w != ready_expert) {  // expert-ordered dispatch: this expert's rows have landed
+          if (!wait_expert_rows(p, s.w)) {
             failed = true;
             break;
           }
-          ready_expert = expert;
+          ready_expert = s.w;
         }
         // A swapped tile of N rows takes N/2 of them from each CTA (the MMA's N side),
         // CTA c from row c*N/2, through the 64-row map into the first half of the A
@@ -382,7 +382,8 @@ __global__ void __cluster_dims__(2, 1, 1) __maxnreg__(kMaxRegs)
         const CUtensorMap* map_a = half_box ? &tmap_a_half : &tmap_a;
         const uint32_t stage_tx = half_box ? PAIR_TX_BYTES_SWAPPED : PAIR_TX_BYTES;
         const int n_b = s.z + static_cast<int>(crank) * BN_CTA;
-        for (int kb = 0; kb < num_kb + extra_kb; ++kb) {
+        int tile_kb = num_kb;
+        for (int kb = 0; kb < tile_kb; ++kb) {
           if (!mbar_wait_cluster(smem_u32(&ctrl->empty[stage]), phase ^ 1, abort_flag)) {
             failed = true;
             break;
@@ -392,7 +393,7 @@ __global__ void __cluster_dims__(2, 1, 1) __maxnreg__(kMaxRegs)
           const uint32_t full_leader = mapa_shared(full_local, 0);
           const CUtensorMap* ka = map_a;
           const CUtensorMap* kb_map = &tmap_b;
-          int k0 = kb * BK, a_row = row_a, b_matrix = expert;
+          int k0 = kb * BK, a_row = row_a, b_matrix = s.w;
           if constexpr (ADAPTERS) {
             if (kb >= num_kb) {
               const int at = (kb - num_kb) / extra.k_blocks;
@@ -416,8 +417,18 @@ __global__ void __cluster_dims__(2, 1, 1) __maxnreg__(kMaxRegs)
             stage = 0;
             phase ^= 1;
           }
+          if constexpr (ADAPTERS) {
+            if (kb == num_kb - 1) {
+              if (!waited) wait_for_previous_kernel();
+              waited = true;
+              tile_kb += extra.count[s.x / BM] * extra.k_blocks;
+            }
+          }
         }
         if (failed) break;
+      }
+      if constexpr (ADAPTERS) {
+        if (!waited) wait_for_previous_kernel();  // this grid ends after the one before
       }
       if (failed) {
         record_status(p.status, MOE_ERR_TIMEOUT);
@@ -439,6 +450,7 @@ __global__ void __cluster_dims__(2, 1, 1) __maxnreg__(kMaxRegs)
       uint32_t aphase = 0;
       bool failed = false;
       bool issued_any = false;
+      [[maybe_unused]] bool waited = false;
       while (true) {
         if (!mbar_wait_cluster(smem_u32(&ctrl->qfull[q]), qphase, abort_flag)) {
           failed = true;
@@ -458,16 +470,23 @@ __global__ void __cluster_dims__(2, 1, 1) __maxnreg__(kMaxRegs)
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + uint32_t(acc * BN);
         const int n_sw = swapped_n(p, s.y);
-        int tile_kb = num_kb;
-        if constexpr (ADAPTERS) tile_kb += s.w * extra.k_blocks;
         // Two instantiations of the k-block loop, so that the usual tile's loop
         // carries no per-MMA choice between the two operand arrangements.
-        const bool ok =
-            n_sw > 0 ? issue_tile<BF16, B_MN_MAJOR, true>(ctrl, sA, sB, d_tmem, tile_kb, stage, phase,
-                                                          abort_flag, issued_any,
-                                                          idesc_f16(BF16, BM, n_sw, B_MN_MAJOR, false))
-                     : issue_tile<BF16, B_MN_MAJOR, false>(ctrl, sA, sB, d_tmem, tile_kb, stage, phase,
-                                                           abort_flag, issued_any, 0u);
+        auto issue = [&](int blocks, uint32_t more) {
+          return n_sw > 0 ? issue_tile<BF16, B_MN_MAJOR, true>(ctrl, sA, sB, d_tmem, blocks, stage, phase,
+                                                               abort_flag, issued_any,
+                                                               idesc_f16(BF16, BM, n_sw, B_MN_MAJOR, false), more)
+                          : issue_tile<BF16, B_MN_MAJOR, false>(ctrl, sA, sB, d_tmem, blocks, stage, phase,
+                                                                abort_flag, issued_any, 0u, more);
+        };
+        bool ok = issue(num_kb, 0u);
+        if constexpr (ADAPTERS) {
+          if (ok) {
+            if (!waited) wait_for_previous_kernel();
+            waited = true;
+            ok = issue(extra.count[s.x / BM] * extra.k_blocks, 1u);
+          }
+        }
         if (!ok) failed = true;
         if (failed) break;
         const uint32_t tf_local = smem_u32(&ctrl->tfull[acc]);

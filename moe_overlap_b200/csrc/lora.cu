@@ -262,8 +262,8 @@ __global__ void __launch_bounds__(kThreads, 2)
   extern __shared__ __align__(128) char smem[];
   __shared__ int2 block_of[kShrinkRows];  // a row's block in the tiles' blocks and its row there
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  let_next_kernel_start();
   wait_for_previous_kernel();
+  let_next_kernel_start();
   const Tile t = find_tile(offs, L, blockIdx.x, kShrinkRows);
   if (t.i < 0) return;  // the same in every CTA of the cluster
   const float c = scale.of(t.i);
@@ -436,8 +436,8 @@ __global__ void __launch_bounds__(kThreads, 2)
   using C = ExpandCfg<kT, RP>;
   extern __shared__ __align__(128) char smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, q4 = lane & 3;
-  let_next_kernel_start();
   wait_for_previous_kernel();
+  let_next_kernel_start();
   // Usually the shared product has taken every row.
   bool any = false;
   for (int q = tid; q < tiles; q += kThreads) any |= left[q] != 0;
@@ -608,8 +608,8 @@ __global__ void __launch_bounds__(kThreads, 2)
   extern __shared__ __align__(128) char smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int parts = gridDim.x, part = blockIdx.x, n0 = blockIdx.y * C::kCols, i = blockIdx.z;
-  let_next_kernel_start();
   wait_for_previous_kernel();
+  let_next_kernel_start();
   const int o0 = offs[i], rows = offs[i + 1] - o0;
   const int share = ((rows + parts - 1) / parts + kGradRows - 1) / kGradRows * kGradRows;
   const int p0 = min(rows, part * share), p1 = min(rows, p0 + share);
@@ -738,7 +738,9 @@ int launch(dim3 grid, dim3 cluster, int smem, cudaStream_t stream, A... args) {
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  // Set up beside the kernel before (each waits for that one's end before it reads).
+  // Set up beside the kernel before.  Each waits for that one's end and only then lets
+  // the next start, so that a kernel starts with all but its predecessor complete (the
+  // shared product relies on it).
   cudaLaunchAttribute attr[2] = {};
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
