@@ -11,7 +11,7 @@
 //   shrink  s[p] = x[perm[p]] A[i]^T           (also dy B[i], with B read along rows)
 //   expand  y[perm[p]] += scale[i] s[p] B[i]^T (also dx += scale[i] (dy B[i]) A[i]) for the
 //           rows of tiles with more adapters than the shared product takes
-//   grad    dB[i] = scale[i] sum_p dy[perm[p]]^T s[p]  (also dA[i])
+//   grads   dB[i] = scale[i] sum_p dy[perm[p]]^T s[p]  (and dA[i])
 // For the gradients and for expand s is held as two values of the inputs' type, the
 // rounded one and what the rounding left (16 bits or more in all).  The shared product
 // takes scale[i] s rounded to the type, like every operand of it; the sum with the
@@ -582,7 +582,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
 }
 
-// grad.  A CTA forms 128 MT columns of z x RP of one adapter's gradient over one part
+// grads.  A CTA forms 128 MT columns of z x RP of one adapter's gradient over one part
 // of its rows, 32 at a time: z^T by ldmatrix.trans as the 16-row side, s as the
 // 8-column side.  The CTAs of a cluster take the parts of the rows and add their sums
 // through distributed shared memory, in order.  Bound by reading z once.
@@ -599,17 +599,27 @@ struct GradCfg {
   static constexpr int kBytes = kStages * kStage > kSums ? kStages * kStage : kSums;
 };
 
+// One gradient: of rows z [m, n] and the low-rank rows s, into g of [n, rank] for each
+// adapter, or [rank, n].
+template <typename T>
+struct GradOf {
+  const T *s, *z;
+  int64_t ldz;
+  int n;
+  T* g;
+};
+
 template <typename T, bool kT, int RP>
-__global__ void __launch_bounds__(kThreads, 2)
-    grad_kernel(const T* s, int64_t part_stride, const T* z, int64_t ldz, Scale scale,
-                const int32_t* perm, const int32_t* offs, int n, int r, T* g, int64_t gl, int64_t gr) {
+__device__ __forceinline__ void grad_block(char* smem, const GradOf<T>& of, int block, int64_t part_stride,
+                                           Scale scale, const int32_t* perm, const int32_t* offs, int r) {
   using C = GradCfg<RP>;
   constexpr int MT = C::MT;
-  extern __shared__ __align__(128) char smem[];
+  const T *s = of.s, *z = of.z;
+  const int64_t ldz = of.ldz, gl = int64_t(of.n) * r, gr = kT ? of.n : r;
+  const int n = of.n;
+  T* g = of.g;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int parts = gridDim.x, part = blockIdx.x, n0 = blockIdx.y * C::kCols, i = blockIdx.z;
-  wait_for_previous_kernel();
-  let_next_kernel_start();
+  const int parts = gridDim.x, part = blockIdx.x, n0 = block * C::kCols, i = blockIdx.z;
   const int o0 = offs[i], rows = offs[i + 1] - o0;
   const int share = ((rows + parts - 1) / parts + kGradRows - 1) / kGradRows * kGradRows;
   const int p0 = min(rows, part * share), p1 = min(rows, p0 + share);
@@ -730,6 +740,21 @@ __global__ void __launch_bounds__(kThreads, 2)
   if (parts > 1) cluster_sync_all();
 }
 
+// dA and dB in one launch: the first blocks_a blocks of columns are dA's.
+template <typename T, int RP>
+__global__ void __launch_bounds__(kThreads, 2)
+    grad_kernel(GradOf<T> a, GradOf<T> b, int blocks_a, int64_t part_stride, Scale scale,
+                const int32_t* perm, const int32_t* offs, int r) {
+  extern __shared__ __align__(128) char smem[];
+  wait_for_previous_kernel();
+  let_next_kernel_start();
+  const int block = blockIdx.y;
+  if (block < blocks_a)
+    grad_block<T, true, RP>(smem, a, block, part_stride, scale, perm, offs, r);
+  else
+    grad_block<T, false, RP>(smem, b, block - blocks_a, part_stride, scale, perm, offs, r);
+}
+
 template <auto kern, typename... A>
 int launch(dim3 grid, dim3 cluster, int smem, cudaStream_t stream, A... args) {
   if (!allow_shared_memory<kern>(smem)) return MOE_ERR_CUDA;
@@ -820,21 +845,27 @@ int expand(const void* s, Weights w, bool transposed, Scale scale, const PlanVie
   });
 }
 
-// g [adapters, n, rank] (transposed: [adapters, rank, n]) = scale z^T s by adapter.
-int grad(const void* s, const void* z, int64_t ldz, bool transposed, Scale scale, const PlanView& plan,
-         int dtype, int64_t m, int64_t n, int adapters, int rank, void* g, cudaStream_t stream) {
-  return dispatch(dtype, transposed, rank, [&](auto t, auto tr, auto rp) {
-    using T = decltype(t);
-    constexpr bool kT = decltype(tr)::value;
+// da [adapters, rank, k] = scale t^T x and db [adapters, n, rank] = scale dy^T s by
+// adapter; a null one is not formed.
+int grads(const void* t, const void* x, int64_t ldx, int64_t k, void* da, const void* s, const void* dy,
+          int64_t lddy, int64_t n, void* db, Scale scale, const PlanView& plan, int dtype, int64_t m,
+          int adapters, int rank, cudaStream_t stream) {
+  return dispatch(dtype, false, rank, [&](auto tt, auto, auto rp) {
+    using T = decltype(tt);
     constexpr int RP = decltype(rp)::value;
     using C = GradCfg<RP>;
-    const unsigned blocks = static_cast<unsigned>((n + C::kCols - 1) / C::kCols);
+    const int blocks_a = da != nullptr ? static_cast<int>((k + C::kCols - 1) / C::kCols) : 0;
+    const int blocks = blocks_a + (db != nullptr ? static_cast<int>((n + C::kCols - 1) / C::kCols) : 0);
     // Adapters' rows are uneven, so several CTAs a place on the SMs: the largest's rows spread.
     const unsigned parts = cluster_parts(int64_t(blocks) * adapters, 4 * 2 * 148, m / adapters, 64);
-    return launch<&grad_kernel<T, kT, RP>>(dim3(parts, blocks, adapters), dim3(parts, 1),
-                  C::kBytes, stream, static_cast<const T*>(s), m * rank, static_cast<const T*>(z), ldz,
-                  scale, plan.perm, plan.offs, static_cast<int>(n), rank, static_cast<T*>(g), n * rank,
-                  kT ? n : int64_t(rank));
+    const GradOf<T> a{static_cast<const T*>(t), static_cast<const T*>(x), ldx, static_cast<int>(k),
+                      static_cast<T*>(da)};
+    const GradOf<T> b{static_cast<const T*>(s), static_cast<const T*>(dy), lddy, static_cast<int>(n),
+                      static_cast<T*>(db)};
+    return launch<&grad_kernel<T, RP>>(dim3(parts, static_cast<unsigned>(blocks), adapters), dim3(parts, 1),
+                                       C::kBytes, stream, a, b, blocks_a, m * rank, scale,
+                                       static_cast<const int32_t*>(plan.perm),
+                                       static_cast<const int32_t*>(plan.offs), rank);
   });
 }
 
@@ -930,7 +961,7 @@ extern "C" int32_t moe_lora_forward(const void* x, int64_t ldx, const void* weig
   if (rc == MOE_OK)
     rc = shared_product(x, ldx, weight, 1, ldw, y, ldy, plan, b, buf.blocks, m, k, n, adapters, rank, dtype, status,
                         st);
-  if (rc == MOE_OK)
+  if (rc == MOE_OK && adapters > per_tile())
     rc = lora::expand(buf.s, b, false, sc, plan, dtype, m, n, adapters, rank, y, ldy, st);
   return rc;
 }
@@ -959,12 +990,10 @@ extern "C" int32_t moe_lora_backward(const void* dy, int64_t lddy, const void* x
   if (rc == MOE_OK && m > 0 && dx != nullptr) {
     rc = shared_product(dy, lddy, weight, ldw, 1, dx, lddx, plan, a, buf.blocks, m, n, k, adapters, rank, dtype,
                         status, st);
-    if (rc == MOE_OK)
+    if (rc == MOE_OK && adapters > per_tile())
       rc = lora::expand(buf.t, a, true, sc, plan, dtype, m, k, adapters, rank, dx, lddx, st);
   }
-  if (rc == MOE_OK && da != nullptr)
-    rc = lora::grad(buf.t, x, ldx, true, sc, plan, dtype, m, k, adapters, rank, da, st);
-  if (rc == MOE_OK && db != nullptr)
-    rc = lora::grad(buf.s, dy, lddy, false, sc, plan, dtype, m, n, adapters, rank, db, st);
+  if (rc == MOE_OK && (da != nullptr || db != nullptr))
+    rc = lora::grads(buf.t, x, ldx, k, da, buf.s, dy, lddy, n, db, sc, plan, dtype, m, adapters, rank, st);
   return rc;
 }
