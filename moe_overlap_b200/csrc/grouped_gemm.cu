@@ -545,7 +545,8 @@ int moe::gg::grouped_gemm_launch(const void* a, int64_t lda, const void* b, int6
     extra.k_blocks = (adapters->rank + BK - 1) / BK;
   }
 
-  if (p.use_atomic &&
+  // With adapters the counter is 0 already: nothing comes between their kernels.
+  if (p.use_atomic && adapters == nullptr &&
       cudaMemsetAsync(work_counter, 0, sizeof(int32_t), stream) != cudaSuccess)
     return MOE_ERR_CUDA;
   const bool bf16 = dtype == MOE_DTYPE_BF16;

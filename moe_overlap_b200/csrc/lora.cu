@@ -46,9 +46,10 @@ struct PlanView {
   int32_t* perm;   // [m]
   int32_t* offs;   // [adapters + 1]
   int32_t* base;   // {0, m}
+  int32_t* queue;  // tile counters of the shared products of the forward and the backward, 0 before each
   static int64_t tiles(int64_t m) { return (m + kTileRows - 1) / kTileRows; }
   static int64_t ints(int64_t m, int adapters) {
-    return tiles(m) * (Adapters::kPerTile + 2) + 2 * m + adapters + 3;
+    return tiles(m) * (Adapters::kPerTile + 2) + 2 * m + adapters + 5;
   }
   PlanView(void* plan, int64_t m, int adapters) {
     list = static_cast<int32_t*>(plan);
@@ -58,6 +59,7 @@ struct PlanView {
     perm = place + m;
     offs = perm + m;
     base = offs + adapters + 1;
+    queue = base + 2;
   }
 };
 
@@ -116,7 +118,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(const void* ids, int ids64, 
     if (tid == 0) {
       plan.offs[i] = start;
       if (i == L - 1) plan.offs[L] = start + all;
-      if (i == 0) plan.base[0] = 0, plan.base[1] = M;
+      if (i == 0) plan.base[0] = 0, plan.base[1] = M, plan.queue[0] = plan.queue[1] = 0;
     }
     if (all == 0) return;
     at += start;
@@ -744,11 +746,13 @@ __device__ __forceinline__ void grad_block(char* smem, const GradOf<T>& of, int 
 template <typename T, int RP>
 __global__ void __launch_bounds__(kThreads, 2)
     grad_kernel(GradOf<T> a, GradOf<T> b, int blocks_a, int64_t part_stride, Scale scale,
-                const int32_t* perm, const int32_t* offs, int r) {
+                const int32_t* perm, const int32_t* offs, int r, int32_t* queue) {
   extern __shared__ __align__(128) char smem[];
   wait_for_previous_kernel();
   let_next_kernel_start();
   const int block = blockIdx.y;
+  // the shared product before is done with its counter: 0 again for another pass
+  if (block == 0 && blockIdx.x == 0 && blockIdx.z == 0 && threadIdx.x == 0) *queue = 0;
   if (block < blocks_a)
     grad_block<T, true, RP>(smem, a, block, part_stride, scale, perm, offs, r);
   else
@@ -815,7 +819,10 @@ int shrink(const void* x, int64_t ldx, Weights w, bool transposed, Scale scale, 
     constexpr bool kT = decltype(tr)::value;
     constexpr int RP = decltype(rp)::value;
     const unsigned tiles = static_cast<unsigned>(most_tiles(m, adapters, kShrinkRows));
-    const unsigned parts = cluster_parts(tiles, 2 * 148, k, 256);
+    // Few rows leave half of the SMs to the shared product, which starts at once on those
+    // (4096 rows of 2048 x 2048, a step: 104.8 us, and 111.5 with all SMs taken); many take
+    // two CTAs an SM (16384 rows: 1048 us, and 1098 with one part).
+    const unsigned parts = cluster_parts(tiles, tiles <= 74 ? 74 : 296, k, 256);
     return launch<&shrink_kernel<T, kT, RP>>(dim3(tiles, parts), dim3(1, parts),
                   ShrinkCfg<kT, RP>::kBytes, stream, static_cast<const T*>(x), ldx,
                   static_cast<const T*>(w.p), w.stride_l, w.stride_row, plan.perm, plan.offs, adapters,
@@ -865,7 +872,7 @@ int grads(const void* t, const void* x, int64_t ldx, int64_t k, void* da, const 
     return launch<&grad_kernel<T, RP>>(dim3(parts, static_cast<unsigned>(blocks), adapters), dim3(parts, 1),
                                        C::kBytes, stream, a, b, blocks_a, m * rank, scale,
                                        static_cast<const int32_t*>(plan.perm),
-                                       static_cast<const int32_t*>(plan.offs), rank);
+                                       static_cast<const int32_t*>(plan.offs), rank, plan.queue + 1);
   });
 }
 
@@ -893,8 +900,8 @@ bool weights_ok(lora::Weights w, int64_t rows, int64_t width, int32_t adapters) 
 // that have a place.
 int shared_product(const void* x, int64_t ldx, const void* w, int64_t stride_k, int64_t stride_n, void* y,
                    int64_t ldy, const lora::PlanView& plan, lora::Weights second, const void* blocks,
-                   int64_t m, int64_t k, int64_t n, int adapters, int rank, int dtype, int32_t* status,
-                   cudaStream_t stream) {
+                   int64_t m, int64_t k, int64_t n, int adapters, int rank, int dtype, int32_t* queue,
+                   int32_t* status, cudaStream_t stream) {
   int dev;
   DeviceInfo info;
   const int rc = current_device_info(&dev, &info);
@@ -902,7 +909,7 @@ int shared_product(const void* x, int64_t ldx, const void* w, int64_t stride_k, 
   const gg::Adapters extra{blocks,          plan.count,        plan.list, second.p,
                            second.stride_l, second.stride_row, rank,      adapters};
   return gg::grouped_gemm_launch(x, ldx, w, 0, stride_k, stride_n, y, ldy, plan.base, 0, m, k, n, 1, dtype,
-                                 MOE_ACT_NONE, info.sm_count, 0, nullptr, nullptr, nullptr, nullptr, 0, status,
+                                 MOE_ACT_NONE, info.sm_count, queue != nullptr, queue, nullptr, nullptr, nullptr, 0, status,
                                  stream, nullptr, nullptr, force_single_sm_kernel() ? nullptr : &extra);
 }
 // Adapters that the shared product takes in a tile of rows; none on the 1-SM kernel.
@@ -959,8 +966,8 @@ extern "C" int32_t moe_lora_forward(const void* x, int64_t ldx, const void* weig
   if (m == 0) return MOE_OK;
   int rc = lora::shrink(x, ldx, a, false, sc, plan, dtype, m, k, adapters, rank, buf.s, buf.blocks, st);
   if (rc == MOE_OK)
-    rc = shared_product(x, ldx, weight, 1, ldw, y, ldy, plan, b, buf.blocks, m, k, n, adapters, rank, dtype, status,
-                        st);
+    rc = shared_product(x, ldx, weight, 1, ldw, y, ldy, plan, b, buf.blocks, m, k, n, adapters, rank, dtype, plan.queue,
+                        status, st);
   if (rc == MOE_OK && adapters > per_tile())
     rc = lora::expand(buf.s, b, false, sc, plan, dtype, m, n, adapters, rank, y, ldy, st);
   return rc;
@@ -989,7 +996,7 @@ extern "C" int32_t moe_lora_backward(const void* dy, int64_t lddy, const void* x
     rc = lora::shrink(dy, lddy, b, true, sc, plan, dtype, m, n, adapters, rank, buf.t, buf.blocks, st);
   if (rc == MOE_OK && m > 0 && dx != nullptr) {
     rc = shared_product(dy, lddy, weight, ldw, 1, dx, lddx, plan, a, buf.blocks, m, n, k, adapters, rank, dtype,
-                        status, st);
+                        da != nullptr || db != nullptr ? plan.queue + 1 : nullptr, status, st);
     if (rc == MOE_OK && adapters > per_tile())
       rc = lora::expand(buf.t, a, true, sc, plan, dtype, m, k, adapters, rank, dx, lddx, st);
   }
