@@ -36,9 +36,9 @@ struct ArrivalWait {
 
 // Adapters' products added in the accumulator of a one-expert product: for each of the
 // first count[t] adapters of row tile t's list (256 rows), the product of `rows` (256
-// x rank for each of the tile's kPerTile places, zeros in rows of other adapters) and
-// that adapter's matrix w_i, stored in the direction of B (one matrix behind another,
-// `stride_l` apart, rows `stride_row` apart).
+// x rank for each of the tile's kPerTile places) and that adapter's matrix w_i, stored
+// in the direction of B (one matrix behind another, `stride_l` apart, rows `stride_row`
+// apart), in the adapter's own rows only.  What `rows` holds in the others is not used.
 struct Adapters {
   // Each costs ceil(rank / 64) k-blocks in every tile; left out, its rows of C are read
   // and written once more instead.  At k = 2048 and rank 64 eight add a quarter to a tile.
@@ -46,6 +46,7 @@ struct Adapters {
   const void* rows;      // [row tiles][kPerTile][256][rank], the inputs' type
   const int32_t* count;  // [row tiles]
   const int32_t* list;   // [row tiles][kPerTile]
+  const uint4* mine;     // [row tiles][kPerTile][2] a bit for each row that is the adapter's
   const void* w;
   int64_t stride_l, stride_row;
   int rank, adapters;
@@ -341,10 +342,11 @@ int launch_pair_kernel(bool bf16, bool b_mn, const CUtensorMap& ta, const CUtens
 
 // The tensor maps of Adapters and what the pair kernel reads beside them.
 struct AdapterMaps {
-  CUtensorMap rows, rows_half;  // boxes as A's and its half
-  CUtensorMap w;                // boxes as B's
+  CUtensorMap rows;  // boxes as A's
+  CUtensorMap w;     // boxes as B's
   const int32_t* count;
   const int32_t* list;
+  const uint4* mine;
   int k_blocks;  // of 64 in the rank
 };
 

@@ -508,7 +508,8 @@ int moe::gg::grouped_gemm_launch(const void* a, int64_t lda, const void* b, int6
   p.arrival = arrival != nullptr ? *arrival : ArrivalWait{nullptr, nullptr, 0};
   // Tiles of at most 224 rows (an expert's tail) run swapped on the CTA pair with
   // every epilogue but the combine push, whose rows go to their source ranks.
-  p.swap_tails = use_pair && gemm_swap_tails() && !pushing;
+  // With adapters no tile is swapped: their products go by rows of the accumulator.
+  p.swap_tails = use_pair && gemm_swap_tails() && !pushing && adapters == nullptr;
 
   // The pair kernel stores C through a {N, m_total} map in 32x32 boxes (64-byte swizzle).
   CUtensorMap tc;
@@ -531,10 +532,8 @@ int moe::gg::grouped_gemm_launch(const void* a, int64_t lda, const void* b, int6
     const uint64_t tiles = uint64_t((m_total + 255) / 256);
     const uint64_t rdims[2] = {r, tiles * Adapters::kPerTile * 256};
     const uint64_t rstrides[1] = {r * 2};
-    const uint32_t rbox[2] = {BK, BM}, rbox_half[2] = {BK, BM / 2};
+    const uint32_t rbox[2] = {BK, BM};
     if (int rc = encode_tiled(&extra.rows, dt, 2, adapters->rows, rdims, rstrides, rbox); rc != MOE_OK) return rc;
-    if (int rc = encode_tiled(&extra.rows_half, dt, 2, adapters->rows, rdims, rstrides, rbox_half); rc != MOE_OK)
-      return rc;
     const uint64_t wdims[3] = {b_mn ? uint64_t(n) : r, b_mn ? r : uint64_t(n), uint64_t(adapters->adapters)};
     const uint64_t row = uint64_t(adapters->stride_row) * 2;
     const uint64_t wstrides[2] = {row, adapters->adapters > 1 ? uint64_t(adapters->stride_l) * 2 : row * wdims[1]};
@@ -542,6 +541,7 @@ int moe::gg::grouped_gemm_launch(const void* a, int64_t lda, const void* b, int6
     if (int rc = encode_tiled(&extra.w, dt, 3, adapters->w, wdims, wstrides, wbox); rc != MOE_OK) return rc;
     extra.count = adapters->count;
     extra.list = adapters->list;
+    extra.mine = adapters->mine;
     extra.k_blocks = (adapters->rank + BK - 1) / BK;
   }
 

@@ -32,10 +32,11 @@
 // columns in its lanes and the tile's rows in N accumulator columns; the epilogue
 // stores them transposed (plain or GELU epilogues only).
 // Adapters (ADAPTERS, one expert): behind a tile's own k-blocks come, for each adapter of
-// its rows, the k-blocks of the adapter's rank, A from the tile's rows of x A_i^T (zeros in
-// other adapters' rows) and B from the adapter's second matrix; boxes past the rank are
-// zero-filled, so any rank fills whole k-blocks.  The sum stays in the accumulator and is
-// rounded once.  The launch may start beside the kernel that prepares those rows: only the
+// its rows, the k-blocks of the adapter's rank, A from the tile's rows of x A_i^T and B from
+// the adapter's second matrix, with the accumulator's other rows switched off (a product
+// with zeros there would carry one adapter's infinities into another's rows); boxes past
+// the rank are zero-filled, so any rank fills whole k-blocks.  The sum stays in the
+// accumulator and is rounded once.  The launch may start beside the kernel that prepares those rows: only the
 // threads that fetch and multiply them wait for its end, behind their first tile's own
 // k-blocks (everything before that kernel is complete when this one starts).
 // No load uses cluster multicast; the pair exchanges only barrier arrivals and
@@ -183,17 +184,20 @@ __device__ __forceinline__ void store_swapped(uint32_t t_lane_base, int lane, in
   }
 }
 
+__device__ constexpr uint32_t kNoRowsOff[8] = {};
+
 // The MMA issuer's k-block loop for one tile (leader CTA, one thread): waits for
 // each stage's data, issues its four 16-deep MMAs into the accumulator at d_tmem
 // and commits the stage back to both CTAs' producers.  SWAPPED issues the swapped
 // form (B stage as the MMA's A operand with M = 256, the A stage's first N/2 rows
 // as its B operand, N and the operand layouts in idesc_sw).  The first MMA overwrites the
-// accumulator, or adds to it when `more`.  Returns false when a wait gave up.
-template <bool BF16, bool B_MN_MAJOR, bool SWAPPED>
+// accumulator; with ROWS all add to it, but for the rows whose bits are set in `off`.
+// Returns false when a wait gave up.
+template <bool BF16, bool B_MN_MAJOR, bool SWAPPED, bool ROWS = false>
 __device__ __forceinline__ bool issue_tile(Ctrl* ctrl, uint8_t* sA, uint8_t* sB, uint32_t d_tmem,
                                            int num_kb, int& stage, uint32_t& phase,
                                            const volatile int* abort_flag, bool& issued_any,
-                                           uint32_t idesc_sw, uint32_t more = 0u) {
+                                           uint32_t idesc_sw, const uint32_t (&off)[8] = kNoRowsOff) {
   const uint32_t idesc = SWAPPED ? idesc_sw : idesc_f16(BF16, BM, BN, false, B_MN_MAJOR);
   // This thread's loop is on the critical path and shares its SM sub-partition with
   // two epilogue warps, so every per-stage quantity is formed once per tile and
@@ -218,10 +222,12 @@ __device__ __forceinline__ bool issue_tile(Ctrl* ctrl, uint8_t* sA, uint8_t* sB,
     for (int kk = 0; kk < BK / UMMA_K; ++kk) {
       const uint64_t adesc = adesc0 + uint64_t(kk * (UMMA_K * 2 / 16));
       const uint64_t bdesc = bdesc0 + uint64_t(B_MN_MAJOR ? kk * (UMMA_K * 128 / 16) : kk * (UMMA_K * 2 / 16));
-      if constexpr (SWAPPED)
-        umma_f16_pair(d_tmem, bdesc, adesc, idesc, (kb | kk) != 0 ? 1u : more);
+      if constexpr (ROWS)
+        umma_f16_pair_rows(d_tmem, adesc, bdesc, idesc, off);
+      else if constexpr (SWAPPED)
+        umma_f16_pair(d_tmem, bdesc, adesc, idesc, (kb | kk) != 0 ? 1u : 0u);
       else
-        umma_f16_pair(d_tmem, adesc, bdesc, idesc, (kb | kk) != 0 ? 1u : more);
+        umma_f16_pair(d_tmem, adesc, bdesc, idesc, (kb | kk) != 0 ? 1u : 0u);
     }
     issued_any = true;
     umma_commit_pair(empty_s0 + 8u * uint32_t(stage));
@@ -400,7 +406,7 @@ __global__ void __cluster_dims__(2, 1, 1) __maxnreg__(kMaxRegs)
               k0 = (kb - num_kb - at * extra.k_blocks) * BK;
               a_row = ((s.x / BM) * Adapters::kPerTile + at) * BM + (row_a - s.x);
               b_matrix = extra.list[(s.x / BM) * Adapters::kPerTile + at];
-              ka = half_box ? &extra.rows_half : &extra.rows;
+              ka = &extra.rows;
               kb_map = &extra.w;
             }
           }
@@ -472,19 +478,24 @@ __global__ void __cluster_dims__(2, 1, 1) __maxnreg__(kMaxRegs)
         const int n_sw = swapped_n(p, s.y);
         // Two instantiations of the k-block loop, so that the usual tile's loop
         // carries no per-MMA choice between the two operand arrangements.
-        auto issue = [&](int blocks, uint32_t more) {
-          return n_sw > 0 ? issue_tile<BF16, B_MN_MAJOR, true>(ctrl, sA, sB, d_tmem, blocks, stage, phase,
-                                                               abort_flag, issued_any,
-                                                               idesc_f16(BF16, BM, n_sw, B_MN_MAJOR, false), more)
-                          : issue_tile<BF16, B_MN_MAJOR, false>(ctrl, sA, sB, d_tmem, blocks, stage, phase,
-                                                                abort_flag, issued_any, 0u, more);
-        };
-        bool ok = issue(num_kb, 0u);
+        bool ok =
+            n_sw > 0 ? issue_tile<BF16, B_MN_MAJOR, true>(ctrl, sA, sB, d_tmem, num_kb, stage, phase,
+                                                          abort_flag, issued_any,
+                                                          idesc_f16(BF16, BM, n_sw, B_MN_MAJOR, false))
+                     : issue_tile<BF16, B_MN_MAJOR, false>(ctrl, sA, sB, d_tmem, num_kb, stage, phase,
+                                                           abort_flag, issued_any, 0u);
         if constexpr (ADAPTERS) {
           if (ok) {
             if (!waited) wait_for_previous_kernel();
             waited = true;
-            ok = issue(extra.count[s.x / BM] * extra.k_blocks, 1u);
+            const int tile = s.x / BM, adapters = extra.count[tile];
+            for (int at = 0; at < adapters && ok; ++at) {
+              const uint4* mine = extra.mine + (tile * Adapters::kPerTile + at) * 2;
+              const uint4 m0 = mine[0], m1 = mine[1];
+              const uint32_t off[8] = {~m0.x, ~m0.y, ~m0.z, ~m0.w, ~m1.x, ~m1.y, ~m1.z, ~m1.w};
+              ok = issue_tile<BF16, B_MN_MAJOR, false, true>(ctrl, sA, sB, d_tmem, extra.k_blocks, stage, phase,
+                                                             abort_flag, issued_any, 0u, off);
+            }
           }
         }
         if (!ok) failed = true;

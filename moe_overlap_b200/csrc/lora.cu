@@ -39,6 +39,7 @@ using gg::Adapters;
 
 // The caller's plan buffer (int32, 16-byte aligned): what depends on the ids alone.
 struct PlanView {
+  uint32_t* mine;  // [tiles][kPerTile][8] a bit for each row of the tile that is the adapter's
   int32_t* list;   // [tiles][kPerTile] adapters of a tile, ascending
   int32_t* count;  // [tiles] how many; 0 also for a tile with too many
   int32_t* left;   // [tiles] whether the tile's adapters are left to expand
@@ -49,10 +50,11 @@ struct PlanView {
   int32_t* queue;  // tile counters of the shared products of the forward and the backward, 0 before each
   static int64_t tiles(int64_t m) { return (m + kTileRows - 1) / kTileRows; }
   static int64_t ints(int64_t m, int adapters) {
-    return tiles(m) * (Adapters::kPerTile + 2) + 2 * m + adapters + 5;
+    return tiles(m) * (9 * Adapters::kPerTile + 2) + 2 * m + adapters + 5;
   }
   PlanView(void* plan, int64_t m, int adapters) {
-    list = static_cast<int32_t*>(plan);
+    mine = static_cast<uint32_t*>(plan);
+    list = static_cast<int32_t*>(plan) + tiles(m) * Adapters::kPerTile * 8;
     count = list + tiles(m) * Adapters::kPerTile;
     left = count + tiles(m);
     place = left + tiles(m);
@@ -71,11 +73,10 @@ __device__ __forceinline__ int id_at(const void* ids, int ids64, int m, int L) {
 
 // Blocks 0 .. L-1 each take one adapter: they count the rows of smaller adapters (the
 // segment's start) and write their own rows in order.  Blocks L .. take one row tile each:
-// the adapters in it, its rows' places, and zeros in its blocks for the rows of others.
+// the adapters in it, which rows are whose, and the rows' places.
 // No block depends on another and the order is always the same.
-__global__ void __launch_bounds__(1024) plan_kernel(const void* ids, int ids64, int M, int L, int r,
-                                                    PlanView plan, int per_tile, uint4* blocks,
-                                                    int32_t* status) {
+__global__ void __launch_bounds__(1024) plan_kernel(const void* ids, int ids64, int M, int L, PlanView plan,
+                                                    int per_tile, int32_t* status) {
   let_next_kernel_start();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tid = threadIdx.x;
   if (static_cast<int>(blockIdx.x) < L) {
@@ -162,16 +163,14 @@ __global__ void __launch_bounds__(1024) plan_kernel(const void* ids, int ids64, 
   const int n = before[32];
   const bool taken = n <= per_tile;
   if (tid == 0) plan.count[t] = taken ? n : 0, plan.left[t] = !taken;
-  if (tid < kTileRows && m < M) {
-    const int rank = id >= 0 ? before[id >> 5] + __popc(present[id >> 5] & ((1u << (id & 31)) - 1u)) : 0;
-    plan.place[m] = taken && id >= 0 ? t * Adapters::kPerTile + rank : -1;
-    // every row of the adapter writes the same word
-    if (taken && id >= 0) plan.list[t * Adapters::kPerTile + rank] = id;
-  }
-  if (taken) {
-    const int words = kTileRows * r / 8;  // of 16 bytes in one block
-    uint4* mine = blocks + int64_t(t) * Adapters::kPerTile * words;
-    for (int q = tid; q < n * words; q += 1024) mine[q] = make_uint4(0, 0, 0, 0);
+  if (tid >= kTileRows) return;
+  const int rank = id >= 0 ? before[id >> 5] + __popc(present[id >> 5] & ((1u << (id & 31)) - 1u)) : -1;
+  if (m < M) plan.place[m] = taken && id >= 0 ? t * Adapters::kPerTile + rank : -1;
+  if (!taken) return;
+  if (id >= 0) plan.list[t * Adapters::kPerTile + rank] = id;  // (every row of it writes the same word)
+  for (int q = 0; q < n; ++q) {
+    const unsigned rows = __ballot_sync(0xffffffffu, rank == q);
+    if (lane == 0) plan.mine[(t * Adapters::kPerTile + q) * 8 + warp] = rows;
   }
 }
 
@@ -906,8 +905,9 @@ int shared_product(const void* x, int64_t ldx, const void* w, int64_t stride_k, 
   DeviceInfo info;
   const int rc = current_device_info(&dev, &info);
   if (rc != MOE_OK) return rc;
-  const gg::Adapters extra{blocks,          plan.count,        plan.list, second.p,
-                           second.stride_l, second.stride_row, rank,      adapters};
+  const gg::Adapters extra{blocks,   plan.count,      plan.list,         reinterpret_cast<const uint4*>(plan.mine),
+                           second.p, second.stride_l, second.stride_row, rank,
+                           adapters};
   return gg::grouped_gemm_launch(x, ldx, w, 0, stride_k, stride_n, y, ldy, plan.base, 0, m, k, n, 1, dtype,
                                  MOE_ACT_NONE, info.sm_count, queue != nullptr, queue, nullptr, nullptr, nullptr, 0, status,
                                  stream, nullptr, nullptr, force_single_sm_kernel() ? nullptr : &extra);
@@ -960,8 +960,7 @@ extern "C" int32_t moe_lora_forward(const void* x, int64_t ldx, const void* weig
   const Buffers buf(kept, m, adapters, rank);
   const lora::PlanView plan(buf.plan, m, adapters);
   lora::plan_kernel<<<static_cast<unsigned>(adapters + lora::PlanView::tiles(m)), 1024, 0, st>>>(
-      ids, ids_int64, static_cast<int>(m), adapters, rank, plan, per_tile(),
-      reinterpret_cast<uint4*>(buf.blocks), status);
+      ids, ids_int64, static_cast<int>(m), adapters, plan, per_tile(), status);
   if (cudaGetLastError() != cudaSuccess) return MOE_ERR_CUDA;
   if (m == 0) return MOE_OK;
   int rc = lora::shrink(x, ldx, a, false, sc, plan, dtype, m, k, adapters, rank, buf.s, buf.blocks, st);
@@ -991,7 +990,6 @@ extern "C" int32_t moe_lora_backward(const void* dy, int64_t lddy, const void* x
   const lora::Scale sc{scale, scale_all};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   int rc = MOE_OK;
-  // The rows of the blocks that the forward left zero are those of this pass too.
   if (m > 0 && (dx != nullptr || da != nullptr))
     rc = lora::shrink(dy, lddy, b, true, sc, plan, dtype, m, n, adapters, rank, buf.t, buf.blocks, st);
   if (rc == MOE_OK && m > 0 && dx != nullptr) {

@@ -302,6 +302,20 @@ __device__ __forceinline__ void umma_f16_pair(uint32_t tmem_d, uint64_t adesc, u
       : "memory");
 }
 
+// The same, adding to D in the rows of the pair's 256 whose bit in `off` is clear; the
+// other rows of D stay as they are, whatever their operands hold.
+__device__ __forceinline__ void umma_f16_pair_rows(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc,
+                                                   uint32_t idesc, const uint32_t (&off)[8]) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, 1, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%4, %5, %6, %7, %8, %9, %10, %11}, p;\n\t}" ::
+          "r"(tmem_d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3]), "r"(off[4]),
+      "r"(off[5]), "r"(off[6]), "r"(off[7])
+      : "memory");
+}
+
 // Arrive on an mbarrier (own or peer CTA, shared::cluster address) once every
 // pair MMA issued so far by this thread is done.
 __device__ __forceinline__ void umma_commit_pair(uint32_t bar_cluster) {

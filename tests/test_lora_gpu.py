@@ -196,6 +196,44 @@ def test_rows_without_adapter_adapters_without_rows(cuda_device):
             assert_close(got, want)
 
 
+@pytest.mark.parametrize("M,L,dtype", [(40, 4, torch.bfloat16), (700, 4, torch.float16), (700, 12, torch.bfloat16)])
+def test_an_adapters_infinities_stay_in_its_rows(cuda_device, M, L, dtype):
+    """Requests share tiles of rows, not their adapters: infinities and NaN in two adapters
+    change no bit of the other rows, with or without an adapter, nor of the other gradients."""
+    x, w, a, b, dy, scale, ids = make(M, 192, 264, L, 16, dtype, seed=L, device=cuda_device)
+
+    def run(a, b, grad):
+        p = [t.detach().clone().requires_grad_(grad) for t in (x, a, b)]
+        y = mo.lora_linear(p[0], w, p[1], p[2], ids, scale=scale)
+        return (y.detach(), *torch.autograd.grad(y, p, dy)) if grad else (y,)
+
+    bad_a, bad_b = a.clone(), b.clone()
+    bad_a[1, 3, 5], bad_a[2] = float("inf"), float("nan")
+    bad_b[1, 7], bad_b[2, 100, 4] = float("-inf"), float("nan")
+    clean_rows = (ids != 1) & (ids != 2)
+    others = [i for i in range(L) if i not in (1, 2)]
+    for grad in (False, True):
+        good, bad = run(a, b, grad), run(bad_a, bad_b, grad)
+        assert not bool(bad[0][~clean_rows].isfinite().all())
+        for g, h in zip(good[:2], bad[:2]):
+            assert torch.equal(g[clean_rows], h[clean_rows])
+        for g, h in zip(good[2:], bad[2:]):
+            assert torch.equal(g[others], h[others])
+
+
+def test_backward_passes_may_be_repeated_but_not_differentiated(cuda_device):
+    x, w, a, b, dy, scale, ids = make(600, 128, 136, 3, 16, torch.bfloat16, device=cuda_device)
+    p = [t.requires_grad_(True) for t in (x, a, b)]
+    y = mo.lora_linear(x, w, a, b, ids, scale=scale)
+    first = torch.autograd.grad(y, p, dy, retain_graph=True)
+    (only_x,) = torch.autograd.grad(y, (x,), 2 * dy, retain_graph=True)
+    for one, two in zip(torch.autograd.grad(y, p, dy, retain_graph=True), first):
+        assert torch.equal(one, two)
+    assert torch.equal(only_x, 2 * first[0])  # powers of two change no rounding
+    with pytest.raises(RuntimeError, match="once"):
+        torch.autograd.grad(y, p, dy, create_graph=True)
+
+
 def test_no_rows(cuda_device):
     x, w, a, b, dy, scale, ids = make(0, 64, 72, 2, 8, torch.bfloat16, device=cuda_device)
     for t in (x, a, b):
