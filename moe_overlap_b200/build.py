@@ -1,10 +1,12 @@
-"""Builds the in-tree C-ABI library ``libmoe_overlap_b200.so`` for sm_100a.
+"""Builds the in-tree C-ABI library ``libmoe_overlap_b200.so`` for sm_100a, and the
+torch extension in front of it.
 
 Every ``csrc/*.cu`` file is compiled by nvcc into ``_build/`` at the repository
 root and linked into ``moe_overlap_b200/libmoe_overlap_b200.so``.  The CUDA
 runtime is linked statically and the driver API is reached through
 ``cudaGetDriverEntryPoint``, so the library loads (and its symbols can be
-inspected) on a machine without a GPU or driver.
+inspected) on a machine without a GPU or driver.  ``csrc/torch_ops.cpp`` becomes
+``moe_overlap_b200/_torch_ops.so`` (g++, against torch's headers).
 
 Usage: ``python -m moe_overlap_b200.build [--force] [--verbose]``.
 """

@@ -256,3 +256,54 @@ def test_layer_forward_few_agrees_with_the_layer(cuda_device):
         assert_close(out, ref, tol)
     finally:
         layer.close()
+
+
+def test_weights_past_32_bit_offsets(cuda_device):
+    """The last expert's weights start past 2^31 elements."""
+    E, H, F = 256, 4096, 2064
+    w1 = torch.zeros(E, F, H, dtype=torch.bfloat16, device=cuda_device)
+    w2 = torch.zeros(E, H, F, dtype=torch.bfloat16, device=cuda_device)
+    assert w1[E - 1].storage_offset() > 2 ** 31
+    x, _, a, b = make(2, 2, H, F, torch.bfloat16, seed=9, device=cuda_device)
+    w1[E - 1], w2[E - 1], w1[0], w2[0] = a[0], b[0], a[1], b[1]
+    idx = torch.tensor([[E - 1, 0], [0, E - 1]], device=cuda_device)
+    w = torch.rand(2, 2, device=cuda_device)
+    got = mo.experts_few_tokens(x, w1, w2, idx, w)
+    want, tol = experts64(x, a, b, torch.where(idx == 0, 1, 0), w)
+    assert_close(got, want, tol)
+
+
+def test_refusals(cuda_device):
+    x, rw, w1, w2 = make(4, 4, 64, 72, torch.bfloat16, device=cuda_device)
+    idx = torch.zeros(4, 2, dtype=torch.int64, device=cuda_device)
+    w = torch.zeros(4, 2, device=cuda_device)
+    few, given = mo.moe_few_tokens, mo.experts_few_tokens
+    for call, match in (
+            (lambda: few(x.float(), rw, w1, w2, 2), "bf16/fp16"),
+            (lambda: few(x, rw.half(), w1, w2, 2), "router_w must be"),
+            (lambda: few(x, rw, w1.half(), w2, 2), "w1 must be"),
+            (lambda: few(x, rw, w1, w2.cpu(), 2), "w2 must be"),
+            (lambda: few(x, rw, w1, w2.transpose(1, 2).contiguous(), 2), "Shapes"),
+            (lambda: few(x, rw, w1, w2, 0), "top_k"), (lambda: few(x, rw, w1, w2, 5), "top_k"),
+            (lambda: few(x, rw, w1, w2, 2, router_bias=torch.zeros(3, device=cuda_device)), "bias"),
+            (lambda: few(x, rw, w1, w2, 2, out=torch.empty(3, 64, dtype=x.dtype, device=cuda_device)), "out"),
+            (lambda: few(x, rw, w1, w2, 2, out=torch.empty(4, 64, device=cuda_device)), "out"),
+            (lambda: few(x, rw, w1, w2, 2, out=torch.empty(64, 4, dtype=x.dtype, device=cuda_device).t()), "out"),
+            (lambda: few(x, rw, w1[:, :, ::2], w2[:, ::2], 2), "Shapes"),
+            (lambda: given(x, w1.transpose(1, 2).contiguous().transpose(1, 2), w2, idx, w), "unit-stride"),
+            (lambda: given(x[:, :60], w1[:, :, :60], w2[:, :60], idx, w), "multiples of 8"),
+            (lambda: given(x, w1[:1].expand(4, 72, 64), w2, idx, w), "one matrix behind another"),
+            (lambda: given(x.repeat(33, 1), w1, w2, idx.repeat(33, 1), w.repeat(33, 1)), "at most 128"),
+            (lambda: given(x, w1, w2, idx.cpu(), w), "must be on"),
+            (lambda: given(x, w1, w2, idx.float(), w), "int64 or int32")):
+        with pytest.raises(ValueError, match=match):
+            call()
+    mo.check_status(cuda_device, sync=True)
+    from moe_overlap_b200.layer import MoELayer
+
+    layer = MoELayer(64, 72, 4, 2, micro_batch_size=16, expert_placement=[1, 0, 3, 2])
+    try:
+        with pytest.raises(ValueError, match="contiguous placement"):
+            layer.forward_few(x)
+    finally:
+        layer.close()

@@ -77,7 +77,7 @@ def assert_close(got, want):
 
 
 SHAPES = [
-    (1, 64, 64, 1, 8, torch.bfloat16), (1, 2048, 256, 4, 16, torch.bfloat16),
+    (1, 8, 8, 1, 8, torch.bfloat16), (70, 8, 16, 2, 8, torch.float16), (1, 64, 64, 1, 8, torch.bfloat16), (1, 2048, 256, 4, 16, torch.bfloat16),
     (3, 72, 136, 2, 8, torch.float16), (7, 512, 1000, 5, 24, torch.bfloat16),
     (16, 264, 520, 16, 32, torch.bfloat16), (33, 1000, 72, 3, 64, torch.float16),
     (64, 256, 256, 64, 16, torch.bfloat16), (65, 128, 384, 2, 128, torch.bfloat16),
@@ -407,3 +407,49 @@ def test_a_decode_step_with_adapters_then_the_experts(cuda_device):
 
     want, tol = experts64(y, w1, w2, idx, wt.double())
     assert bool(((padded.double() - want).abs() <= tol).all())
+
+
+def test_rows_past_32_bit_offsets(cuda_device):
+    """The last rows of x start past 2^31 elements."""
+    M, K, N, L, r = 262152 + 300, 8192, 8, 2, 8
+    _, w, a, b, _, scale, _ = make(1, K, N, L, r, torch.bfloat16, seed=3, device=cuda_device)
+    x = torch.zeros(M, K, dtype=torch.bfloat16, device=cuda_device)
+    at = [0, 5, M // 2, M - 300, M - 1]
+    x[at] = make(len(at), K, N, L, r, torch.bfloat16, seed=4, device=cuda_device)[0]
+    ids = torch.full((M,), -1, device=cuda_device)
+    ids[at] = torch.tensor([0, 1, -1, 1, 0], device=cuda_device)
+    dy = torch.zeros(M, N, dtype=torch.bfloat16, device=cuda_device)
+    dy[at] = make(len(at), K, N, L, r, torch.bfloat16, seed=4, device=cuda_device)[4]
+    for t in (x, a, b):
+        t.requires_grad_(True)
+    y = mo.lora_linear(x, w, a, b, ids, scale=scale)
+    dx, da, db = torch.autograd.grad(y, (x, a, b), dy)
+    mo.check_status(cuda_device, sync=True)
+    want = reference(x[at], w, a, b, dy[at], scale, ids[at])
+    for got, ref in zip((y[at], dx[at], da, db), want):
+        assert_close(got, ref)
+    rest = torch.ones(M, dtype=torch.bool, device=cuda_device)
+    rest[at] = False
+    assert not bool(y[rest].any()) and not bool((dx[M - 299:M - 1] != 0).any())
+
+
+def test_refusals(cuda_device):
+    x, w, a, b, _, scale, ids = make(6, 64, 72, 3, 8, torch.bfloat16, device=cuda_device)
+    f = mo.lora_linear
+    for call, match in (
+            (lambda: f(x.float(), w, a, b, ids), "bf16/fp16"), (lambda: f(x, w.half(), a, b, ids), "weight must be"),
+            (lambda: f(x, w, a.cpu(), b, ids), "lora_a must be"), (lambda: f(x, w, a, b.float(), ids), "lora_b must be"),
+            (lambda: f(x[0], w, a, b, ids), "Shapes"), (lambda: f(x, w, a, b[:2], ids), "Shapes"),
+            (lambda: f(x, w, a[:, :, :56], b, ids), "Shapes"), (lambda: f(x, w.t(), a, b, ids), "Shapes"),
+            (lambda: f(x, w, a, b, ids[:5]), "adapter_ids"), (lambda: f(x, w, a, b, ids.float()), "adapter_ids"),
+            (lambda: f(x, w, a, b, ids.cpu()), "adapter_ids"),
+            (lambda: f(x, w, a, b, ids, scale=scale[:2]), "scale"), (lambda: f(x, w, a, b, ids, scale=ids[:3]), "scale"),
+            (lambda: f(x, w, a.new_zeros(3, 136, 64), b.new_zeros(3, 72, 136), ids), "ranks"),
+            (lambda: f(x, w, a[:0], b[:0], ids), "adapters"),
+            (lambda: f(x, w.clone().requires_grad_(True), a, b, ids), "frozen"),
+            (lambda: f(x, w, a, b, ids, scale=scale.clone().requires_grad_(True)), "no gradient")):
+        with pytest.raises(ValueError, match=match):
+            call()
+    with torch.no_grad():  # nothing asks for those gradients here
+        assert f(x, w.clone().requires_grad_(True), a, b, ids).shape == (6, 72)
+    mo.check_status(cuda_device, sync=True)
