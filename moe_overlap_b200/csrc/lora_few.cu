@@ -63,7 +63,7 @@ __global__ void __launch_bounds__(32 * kLowWarps)
 // side.  The order of k inside a slice is free: lane (g, q) takes the 16 contiguous
 // columns 16q.. of its rows, so both operands come by 16-byte conflict-free loads.
 constexpr int kConsumers = 8;
-constexpr int kThreads = 32 * (2 + kConsumers);
+constexpr int kThreads = 32 * (1 + kConsumers);
 constexpr int kStageBytes = 16 * 1024;
 constexpr int kRedStride = 20;
 
@@ -134,17 +134,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (++stage == kStages) stage = 0, phase ^= 1;
         }
     }
-    return;
-  }
-  if (warp == 1 + kConsumers) {  // the epilogues' rows of B, on their way to L2 by then
-    for (int blk = blockIdx.x; blk < blocks; blk += gridDim.x)
-      for (int m = 0; m < M; ++m) {
-        const int i = ctrl->id[m];
-        if (i < 0) continue;
-        for (int row = blk * BM + lane; row < min(N, (blk + 1) * BM); row += 32)
-          for (int j = 0; j < r; j += 64)
-            asm volatile("prefetch.global.L2 [%0];" ::"l"(b + i * sl + row * sr + j));
-      }
     return;
   }
   const int cw = warp - 1, rt = cw % R, cs = cw / R, g8 = lane >> 2, q4 = lane & 3;
