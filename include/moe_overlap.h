@@ -576,14 +576,14 @@ MOE_API int32_t moe_few_tokens(const void* x, int64_t ldx, const void* router_w,
  *   ids [m]         int32, or int64 if ids_int64; an id outside [-1, adapters) counts
  *                   as -1 and records MOE_ERR_INVALID_ARG in `status`
  *   scale           float[adapters], or NULL: scale_all for every adapter
- *   for_backward    nonzero: `kept` is for moe_lora_backward; 0: it is workspace, and at
- *                   most 64 rows take kernels of their own
+ *   for_backward    nonzero: `kept` is for moe_lora_backward; 0: it is workspace, and few
+ *                   rows take kernels of their own
  *   kept            moe_lora_kept_bytes(...) bytes (-1: sizes out of bounds), of this call
  *                   and its backward passes alone; its contents need no set-up
  * dtype is MOE_DTYPE_BF16 or MOE_DTYPE_F16.  Rows and kept start on 16 bytes; k, n and
  * rank are multiples of 8; rank <= 128; adapters <= 1024.  Sums are fp32.
  */
-MOE_API int64_t moe_lora_kept_bytes(int64_t m, int32_t adapters, int32_t rank, int32_t for_backward);
+MOE_API int64_t moe_lora_kept_bytes(int64_t m, int32_t adapters, int32_t rank);
 MOE_API int32_t moe_lora_forward(const void* x, int64_t ldx, const void* weight, int64_t ldw,
                                  const void* lora_a, int64_t a_stride_l, int64_t a_stride_row,
                                  const void* lora_b, int64_t b_stride_l, int64_t b_stride_row,

@@ -196,7 +196,7 @@ SIGNATURES: dict[str, tuple] = {
          _c_void_p, _c_void_p, _c_void_p, _i64,  # topk_idx, topk_weights, out, ldo
          _c_void_p, _i64, _c_void_p, _c_void_p],  # workspace, bytes, status, stream
     ),
-    "moe_lora_kept_bytes": (_i64, [_i64, _i32, _i32, _i32]),
+    "moe_lora_kept_bytes": (_i64, [_i64, _i32, _i32]),
     "moe_lora_forward": (
         _i32,
         [_c_void_p, _i64, _c_void_p, _i64,  # x, ldx, weight, ldw

@@ -938,9 +938,8 @@ struct Buffers {
 };
 }  // namespace
 
-extern "C" int64_t moe_lora_kept_bytes(int64_t m, int32_t adapters, int32_t rank, int32_t for_backward) {
+extern "C" int64_t moe_lora_kept_bytes(int64_t m, int32_t adapters, int32_t rank) {
   if (!dims_ok(MOE_DTYPE_BF16, m, 8, 8, adapters, rank)) return -1;
-  if (!for_backward && m <= lora::kFewRows) return low_bytes(m, rank);
   return Buffers(nullptr, m, adapters, rank).bytes;
 }
 
@@ -958,7 +957,7 @@ extern "C" int32_t moe_lora_forward(const void* x, int64_t ldx, const void* weig
     return MOE_ERR_INVALID_ARG;
   const lora::Scale sc{scale, scale_all};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (!for_backward && m > 0 && m <= lora::kFewRows)
+  if (!for_backward && m > 0 && lora::takes_few_rows(m, k, n, rank))
     return lora::forward_few_rows(x, ldx, weight, ldw, a, b, ids, ids_int64, sc, dtype,
                                   static_cast<int>(m), static_cast<int>(k), static_cast<int>(n), adapters,
                                   rank, y, ldy, static_cast<float*>(kept), status, st);

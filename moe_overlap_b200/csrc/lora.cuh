@@ -20,11 +20,10 @@ struct Weights {  // of all adapters
   int64_t stride_l, stride_row;
 };
 
-// Batches of at most this many rows, of which no gradient is wanted, take the kernels
-// of lora_few.cu.
-constexpr int kFewRows = 64;
+// Whether a batch of which no gradient is wanted takes the kernels of lora_few.cu.
+bool takes_few_rows(int64_t m, int64_t k, int64_t n, int rank);
 
-// y = x weight^T + scale (x a^T) b^T by row for m <= kFewRows; low: float [m][rank].
+// y = x weight^T + scale (x a^T) b^T by row for such a batch; low: float [m][rank].
 int forward_few_rows(const void* x, int64_t ldx, const void* weight, int64_t ldw, Weights a, Weights b,
                      const void* ids, int ids64, Scale scale, int dtype, int m, int k, int n, int adapters,
                      int rank, void* y, int64_t ldy, float* low, int32_t* status, cudaStream_t stream);

@@ -1,12 +1,12 @@
-// The adapters' projection for a decode batch (at most 64 rows) on sm_100a, in two
-// kernels:  low[m] = x[m] A[i]^T  and  y[m] = x[m] W^T + scale[i] low[m] B[i]^T.
+// The adapters' projection for few rows (decode batches) on sm_100a, in two kernels:
+// low[m] = x[m] A[i]^T  and  y[m] = x[m] W^T + scale[i] low[m] B[i]^T.
 //
-// The shared weight is the traffic: it is read once, and the second kernel starts
-// beside the first and has its first weights under way while `low` is formed; only its
-// epilogue waits for it.  The adapters' products are a few thousand products an output
+// The shared weight is the traffic: it is read once for 64 rows, and the second kernel
+// starts beside the first and has its first weights under way while `low` is formed; only
+// its epilogue waits for it.  The adapters' products are a few thousand products an output
 // block and run on the CUDA cores in fp32, so y is rounded once.  Both kernels, measured:
-// 1 row of 2048 x 2048 8.3 us (launch latency), 48 rows of 2048 x 8192 with 32 adapters of
-// rank 16 22.6 us, 1 row of the same 12.3 us (2.7 TB/s; a cuBLAS product alone 10.3).
+// 1 row of 2048 x 2048 at rank 16 8.2 us (launch latency), 1 row of 2048 x 8192 11.9 us
+// (2.8 TB/s; a cuBLAS product alone 10.3), 64 rows of it with 32 adapters 22 us.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -67,6 +67,13 @@ constexpr int kThreads = 32 * (1 + kConsumers);
 constexpr int kStageBytes = 16 * 1024;
 constexpr int kRedStride = 20;
 
+template <typename T>
+__device__ __forceinline__ float dot8(const uint4& u, const float4& l0, const float4& l1) {
+  const T* p = reinterpret_cast<const T*>(&u);
+  return to_f(p[0]) * l0.x + to_f(p[1]) * l0.y + to_f(p[2]) * l0.z + to_f(p[3]) * l0.w + to_f(p[4]) * l1.x +
+         to_f(p[5]) * l1.y + to_f(p[6]) * l1.z + to_f(p[7]) * l1.w;
+}
+
 template <int R, int J>
 struct Cfg {
   static constexpr int BM = 16 * R, C = kConsumers / R, BKS = 64 * C, NT = 8 * J;
@@ -79,8 +86,8 @@ struct Cfg {
 
 struct Ctrl {
   uint64_t full[12], empty[12];
-  int id[kFewRows];
-  float scale[kFewRows];
+  int id[64];
+  float scale[64];
 };
 
 template <typename T, int R, int J>
@@ -104,8 +111,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     fence_mbar_init();
   }
-  for (int m = tid; m < M; m += kThreads) {
-    const int i = id_at(ids, ids64, m, L);
+  const int mb = blockIdx.y * NT, Mt = min(NT, M - mb);  // this CTA's rows of x
+  for (int m = tid; m < Mt; m += kThreads) {
+    const int i = id_at(ids, ids64, mb + m, L);
     ctrl->id[m] = i;
     ctrl->scale[m] = i >= 0 ? scale.of(i) : 0.0f;
   }
@@ -129,7 +137,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int i = 0; i < C; ++i) {
             tma_load_2d(dst + i * kSliceBytes, &wmap, full, c + 64 * i, blk * BM);
-            tma_load_2d(xdst + i * NT * 128, &xmap, full, c + 64 * i, 0);
+            tma_load_2d(xdst + i * NT * 128, &xmap, full, c + 64 * i, mb);
           }
           if (++stage == kStages) stage = 0, phase ^= 1;
         }
@@ -184,48 +192,86 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("bar.sync 1, 256;" ::: "memory");
     if (!waited) wait_for_previous_kernel();  // for `low`
     waited = true;
-    // One column of W a thread (row n of the block) and every 256 / BM-th row of x, eight at
-    // a time so that their adapters' rows are under way together.
-    constexpr int kStep = 32 * kConsumers / BM, kTogether = 8;
-    const int n = (cw * 32 + lane) % BM, row = blk * BM + n;
-    if (row < N)
-      for (int m0 = (cw * 32 + lane) / BM; m0 < M; m0 += kTogether * kStep) {
-        const T* br[kTogether];
-        const float* lr[kTogether];
+    const int tid_c = cw * 32 + lane;
+    // At most 8 requests of low rank, or fewer of a high one, by rows of B (their latency
+    // counts); more by columns of W (their loads do: 8 rows of 2048 x 8192 at rank 64 19 us
+    // so and 22 by rows of B; 1 row at rank 128, 18.7 and 13.2).
+    const bool by_rows = J == 1 && Mt * r <= 256;
+    if (by_rows) {
+      // The adapters' part is added to the first slice's sums, 512 bytes of neighbouring rows of
+      // one request's B a warp, 16 bytes a lane, 2^lg lanes a row, four of those under way.
+      constexpr int kTogether = 4;
+      const int lg = r <= 8 ? 0 : 32 - __clz((r / 8) - 1), lanes = 1 << lg, rows = 32 >> lg;
+      const int chunks = rows < BM ? BM / rows : 1, piece = lane & (lanes - 1);
+      for (int u0 = cw; u0 < Mt * chunks; u0 += kTogether * kConsumers) {
         float add[kTogether];
+        int at[kTogether];
+        float c[kTogether];
 #pragma unroll
-        for (int u = 0; u < kTogether; ++u) {
-          const int m = m0 + u * kStep, i = m < M ? ctrl->id[m] : -1;
-          br[u] = i >= 0 ? b + i * sl + row * sr : nullptr;
-          lr[u] = low + m * r;
-          add[u] = 0.0f;
+        for (int q = 0; q < kTogether; ++q) {
+          const int u = u0 + q * kConsumers, m = u / chunks, n = u % chunks * rows + (lane >> lg);
+          const int i = m < Mt ? ctrl->id[m] : -1, row = blk * BM + n;
+          const bool there = i >= 0 && n < BM && row < N;
+          uint4 ub = make_uint4(0, 0, 0, 0);
+          float4 l0 = make_float4(0.0f, 0.0f, 0.0f, 0.0f), l1 = l0;
+          if (there && piece * 8 < r) {
+            ub = *reinterpret_cast<const uint4*>(b + i * sl + row * sr + piece * 8);
+            const float* lr = low + (mb + m) * r + piece * 8;
+            l0 = *reinterpret_cast<const float4*>(lr);
+            l1 = *reinterpret_cast<const float4*>(lr + 4);
+          }
+          add[q] = dot8<T>(ub, l0, l1);
+          at[q] = there && piece == 0 ? n / 16 * (NT * kRedStride) + m * kRedStride + n % 16 : -1;
+          c[q] = there ? ctrl->scale[m] : 0.0f;
         }
-#pragma unroll 2
-        for (int j = 0; j < r; j += 8) {
-          uint4 ub[kTogether];
 #pragma unroll
-          for (int u = 0; u < kTogether; ++u)
-            ub[u] = br[u] != nullptr ? *reinterpret_cast<const uint4*>(br[u] + j) : make_uint4(0, 0, 0, 0);
+        for (int q = 0; q < kTogether; ++q) {
+          for (int o = 1; o < lanes; o <<= 1) add[q] += __shfl_xor_sync(0xffffffffu, add[q], o);
+          if (at[q] >= 0) red[at[q]] += c[q] * add[q];
+        }
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+    }
+    // One column of W a thread (row n of the block) and every 256 / BM-th row of x, eight of
+    // them at a time, so that their adapters' rows are under way together.
+    constexpr int kStep = 32 * kConsumers / BM, kTogether = 8;
+    const int n = tid_c % BM, row = blk * BM + n;
+    if (row < N)
+      for (int m0 = tid_c / BM; m0 < Mt; m0 += kTogether * kStep) {
+        float add[kTogether];
+        if (!by_rows) {
+          const T* br[kTogether];
+          const float* lr[kTogether];
 #pragma unroll
           for (int u = 0; u < kTogether; ++u) {
-            if (br[u] == nullptr) continue;
-            const float4 l0 = *reinterpret_cast<const float4*>(lr[u] + j);
-            const float4 l1 = *reinterpret_cast<const float4*>(lr[u] + j + 4);
-            const T* pb = reinterpret_cast<const T*>(&ub[u]);
-            add[u] += to_f(pb[0]) * l0.x + to_f(pb[1]) * l0.y + to_f(pb[2]) * l0.z + to_f(pb[3]) * l0.w +
-                      to_f(pb[4]) * l1.x + to_f(pb[5]) * l1.y + to_f(pb[6]) * l1.z + to_f(pb[7]) * l1.w;
+            const int m = m0 + u * kStep, i = m < Mt ? ctrl->id[m] : -1;
+            br[u] = i >= 0 ? b + i * sl + row * sr : nullptr;
+            lr[u] = low + (mb + m) * r;
+            add[u] = 0.0f;
+          }
+#pragma unroll 2
+          for (int j = 0; j < r; j += 8) {
+            uint4 ub[kTogether];
+#pragma unroll
+            for (int u = 0; u < kTogether; ++u)
+              ub[u] = br[u] != nullptr ? *reinterpret_cast<const uint4*>(br[u] + j) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int u = 0; u < kTogether; ++u)
+              if (br[u] != nullptr)
+                add[u] += dot8<T>(ub[u], *reinterpret_cast<const float4*>(lr[u] + j),
+                                  *reinterpret_cast<const float4*>(lr[u] + j + 4));
           }
         }
 #pragma unroll
         for (int u = 0; u < kTogether; ++u) {
           const int m = m0 + u * kStep;
-          if (m >= M) continue;
+          if (m >= Mt) continue;
           float v = 0.0f;
 #pragma unroll
           for (int i = 0; i < C; ++i)
             v += red[(i * R + n / 16) * (NT * kRedStride) + m * kRedStride + n % 16];
-          if (br[u] != nullptr) v += ctrl->scale[m] * add[u];
-          y[m * ldy + row] = from_f<T>(v);
+          if (!by_rows && ctrl->id[m] >= 0) v += ctrl->scale[m] * add[u];
+          y[(mb + m) * ldy + row] = from_f<T>(v);
         }
       }
     asm volatile("bar.sync 1, 256;" ::: "memory");  // the buffer is free again
@@ -252,7 +298,7 @@ int project(const T* x, int64_t ldx, const void* weight, int64_t ldw, Weights b,
   if (!allow_shared_memory<kern>(kSmem)) return MOE_ERR_CUDA;
   const int blocks = (n + Q::BM - 1) / Q::BM;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(blocks < sms ? blocks : sms);
+  cfg.gridDim = dim3(blocks < sms ? blocks : sms, (m + Q::NT - 1) / Q::NT);
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = kSmem;
   cfg.stream = stream;
@@ -266,6 +312,9 @@ int project(const T* x, int64_t ldx, const void* weight, int64_t ldw, Weights b,
              ? MOE_OK
              : MOE_ERR_CUDA;
 }
+
+// Weights with at least so many rows are taken 64 at a time.
+constexpr int64_t kWide = 64 * 100;
 
 template <typename T>
 int forward(const void* x, int64_t ldx, const void* weight, int64_t ldw, Weights a, Weights b, const void* ids,
@@ -289,15 +338,30 @@ int forward(const void* x, int64_t ldx, const void* weight, int64_t ldw, Weights
     if (m <= 48) return go(wide, integral_constant<int, 6>());
     return go(wide, integral_constant<int, 8>());
   };
-  // The widest row blocks that still give most SMs one; with more rows of x the narrow
-  // ones would leave too few stages of shared memory.
+  // row_block(): the widest row blocks that still give most SMs one; with more rows of x the
+  // narrow ones would leave too few stages of shared memory.
   using std::integral_constant;
-  if (n >= 64 * 100) return by_width(integral_constant<int, 4>(), integral_constant<int, 4>());
-  if (n >= 32 * 100) return by_width(integral_constant<int, 2>(), integral_constant<int, 2>());
+  if (n >= kWide) return by_width(integral_constant<int, 4>(), integral_constant<int, 4>());
+  if (n >= kWide / 2) return by_width(integral_constant<int, 2>(), integral_constant<int, 2>());
   return by_width(integral_constant<int, 1>(), integral_constant<int, 2>());
 }
 
 }  // namespace few
+
+bool takes_few_rows(int64_t m, int64_t k, int64_t n, int rank) {
+  // What the adapters' rows cost each block of W: with many of high rank the tensor-core
+  // path is faster (64 rows of 2048 x 8192 at rank 64: 52 us here and 45 there; at rank 16,
+  // 22 and 40).
+  const bool wide = n >= few::kWide;
+  const int64_t rows = m < 64 ? m : 64;
+  if (rows * rank > (wide ? 2048 : 4096)) return false;
+  if (m <= 64) return true;
+  // Further tiles of 64 rows read the weight again, from L2: worth it for up to two blocks an
+  // SM, one at rank 64 (128 rows of 2048 x 2048 at rank 16: 14 us, 33 there; 192 rows at
+  // rank 64, 45 and 36), while x A^T, by the CUDA cores, stays small.
+  const int64_t blocks = (m + 63) / 64 * ((n + (wide ? 63 : 31)) / (wide ? 64 : 32));
+  return blocks <= 2 * 148 && blocks * rank <= 2 * 148 * 32 && m * rank * k <= (int64_t(1) << 25);
+}
 
 int forward_few_rows(const void* x, int64_t ldx, const void* weight, int64_t ldw, Weights a, Weights b,
                      const void* ids, int ids64, Scale scale, int dtype, int m, int k, int n, int adapters,

@@ -196,7 +196,7 @@ std::pair<Tensor, Tensor> lora_forward(const Tensor& x, const Tensor& weight, co
   int32_t* status = checked_status(dev);
   const c10::cuda::OptionalCUDAGuard guard(dev);
   Tensor y = at::empty({z.m, z.n}, x.options());
-  Tensor kept = at::empty({abi.lora_kept_bytes(z.m, z.adapters, z.rank, for_backward)},
+  Tensor kept = at::empty({abi.lora_kept_bytes(z.m, z.adapters, z.rank)},
                           x.options().dtype(at::kByte));
   const int32_t rc = abi.lora_forward(
       data(x), x.stride(0), data(weight), weight.stride(0), data(a), a.stride(0), a.stride(1), data(b),

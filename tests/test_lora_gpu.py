@@ -355,7 +355,9 @@ def test_streams_and_graph(cuda_device, M):
 
 @pytest.mark.parametrize("M,N,dtype", [(1, 2048, torch.bfloat16), (5, 6408, torch.float16),
                                        (13, 3208, torch.bfloat16), (29, 8200, torch.bfloat16),
-                                       (40, 72, torch.float16), (64, 4000, torch.bfloat16)])
+                                       (40, 72, torch.float16), (64, 4000, torch.bfloat16),
+                                       (65, 136, torch.bfloat16), (200, 520, torch.float16),
+                                       (128, 6400, torch.bfloat16)])
 def test_decode_batches_on_streams_and_in_a_graph(cuda_device, M, N, dtype):
     """Few rows without gradients: against 64 bits over the widths of the weight, two
     calls at once, a replayed capture, and in inference mode."""
