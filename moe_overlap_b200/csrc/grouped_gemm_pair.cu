@@ -39,6 +39,9 @@
 // accumulator and is rounded once.  The launch may start beside the kernel that prepares those rows: only the
 // threads that fetch and multiply them wait for its end, behind their first tile's own
 // k-blocks (everything before that kernel is complete when this one starts).
+// Parts (with adapters, few tiles): a cluster of 2 or 4 pairs takes one tile, each pair a
+// share of the k-blocks and every 2nd or 4th adapter.  The pairs leave their sums in their
+// shared memory, and each CTA adds one share of the columns over the parts, in their order.
 // No load uses cluster multicast; the pair exchanges only barrier arrivals and
 // the tile ring entries through shared::cluster addresses.
 #include <algorithm>
@@ -193,7 +196,7 @@ __device__ constexpr uint32_t kNoRowsOff[8] = {};
 // as its B operand, N and the operand layouts in idesc_sw).  The first MMA overwrites the
 // accumulator; with ROWS all add to it, but for the rows whose bits are set in `off`.
 // Returns false when a wait gave up.
-template <bool BF16, bool B_MN_MAJOR, bool SWAPPED, bool ROWS = false>
+template <bool BF16, bool B_MN_MAJOR, bool SWAPPED, bool ROWS = false, int PARTS = 1>
 __device__ __forceinline__ bool issue_tile(Ctrl* ctrl, uint8_t* sA, uint8_t* sB, uint32_t d_tmem,
                                            int num_kb, int& stage, uint32_t& phase,
                                            const volatile int* abort_flag, bool& issued_any,
@@ -212,7 +215,7 @@ __device__ __forceinline__ bool issue_tile(Ctrl* ctrl, uint8_t* sA, uint8_t* sB,
                                        : smem_desc_sw128(smem_u32(sB), 16, 1024);
   const uint32_t full_s0 = smem_u32(&ctrl->full[0]);
   const uint32_t empty_s0 = smem_u32(&ctrl->empty[0]);
-  const uint32_t empty_peer_s0 = mapa_shared(empty_s0, 1);
+  const uint32_t empty_peer_s0 = mapa_shared(empty_s0, PARTS == 1 ? 1u : cluster_ctarank() + 1u);
   for (int kb = 0; kb < num_kb; ++kb) {
     if (!mbar_wait_cluster(full_s0 + 8u * uint32_t(stage), phase, abort_flag)) return false;
     tc_fence_after();
@@ -240,26 +243,88 @@ __device__ __forceinline__ bool issue_tile(Ctrl* ctrl, uint8_t* sA, uint8_t* sB,
   return true;
 }
 
+// With the contraction split over PARTS pairs each CTA leaves its 128 x 256 sums in its
+// shared memory, column by column (128 rows together, so that a warp's 32 rows meet every
+// bank once); row `row` of columns c0 .. c0 + 127, those behind the matrix's n left out.
+constexpr int kSumsPitch = BM_CTA;
+static_assert(kSumsPitch * BN * 4 <= STAGES * (A_STAGE_BYTES + B_STAGE_BYTES), "the sums lie in the stages");
+__device__ __forceinline__ void leave_sums(uint32_t t_lane_base, float* sums, int row, int c0, int n) {
+#pragma unroll 1
+  for (int c = c0; c < c0 + 128 && c < n; c += 32) {
+    uint32_t r[32];
+    tmem_ld_32x32b_x32(t_lane_base + uint32_t(c), r);
+    tmem_wait_ld();
+#pragma unroll
+    for (int j = 0; j < 32; ++j) sums[(c + j) * kSumsPitch + row] = __uint_as_float(r[j]);
+  }
+}
+
+// The sums of one row over the parts, in their order, for half `half` of the columns that
+// part `part`'s CTA finishes; rounded and stored.
+template <bool BF16, int PARTS>
+__device__ __forceinline__ void add_parts(const float* sums, uint32_t crank, int row, int part, int half,
+                                          const int4& tile, const Params& p) {
+  constexpr int kCols = BN / PARTS / 2;
+  const int m = static_cast<int>(crank) * BM_CTA + row;  // of the tile's rows
+  if (m >= tile.y) return;
+  const int c0 = part * (BN / PARTS) + half * kCols;
+  uint32_t from[PARTS];
+#pragma unroll
+  for (int q = 0; q < PARTS; ++q)
+    from[q] = mapa_shared(smem_u32(sums + c0 * kSumsPitch + row), 2u * uint32_t(q) + crank);
+  uint16_t* out = static_cast<uint16_t*>(p.c) + (int64_t(tile.x) + m) * p.ldc + tile.z + c0;
+#pragma unroll
+  for (int c = 0; c < kCols; c += 8) {
+    if (tile.z + c0 + c >= p.n) break;  // n is a multiple of 8
+    float v[PARTS][8];
+#pragma unroll
+    for (int q = 0; q < PARTS; ++q)
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        asm volatile("ld.shared::cluster.f32 %0, [%1];"
+                     : "=f"(v[q][j])
+                     : "r"(from[q] + uint32_t((c + j) * kSumsPitch * 4))
+                     : "memory");
+#pragma unroll
+    for (int q = 1; q < PARTS; ++q)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[0][j] += v[q][j];
+    *reinterpret_cast<uint4*>(out + c) = make_uint4(pack2<BF16>(v[0][0], v[0][1]), pack2<BF16>(v[0][2], v[0][3]),
+                                                    pack2<BF16>(v[0][4], v[0][5]), pack2<BF16>(v[0][6], v[0][7]));
+  }
+}
+
 // 144 registers: with 10 warps, SM sub-partitions 0 and 1 hold three of them
 // (3 x 32 x 144 = 13,824 of their 16,384 registers), which leaves room for one
 // warp per sub-partition of a 4-warp exchange block at <= 80 registers, so the
 // dispatch/combine kernels run beside this persistent kernel.  PUSH compiles the
 // expert-parallel combine push into the epilogue (rows go to their source ranks).
-struct NoAdapters {};
+struct NoAdapters {
+  static constexpr int kParts = 1;
+};
+// Adapters with the contraction split over `P` pairs of a cluster.
+template <int P>
+struct SplitAdapters : AdapterMaps {
+  static constexpr int kParts = P;
+  static_assert(P == 1 || P == 2 || P == 4, "clusters of up to 8 CTAs");
+};
 
 template <bool BF16, bool B_MN_MAJOR, bool PUSH, class EXTRA>
-__global__ void __cluster_dims__(2, 1, 1) __maxnreg__(kMaxRegs)
+__global__ void __cluster_dims__(2 * EXTRA::kParts, 1, 1) __maxnreg__(kMaxRegs)
     grouped_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a,
                              const __grid_constant__ CUtensorMap tmap_a_half,
                              const __grid_constant__ CUtensorMap tmap_b,
                              const __grid_constant__ CUtensorMap tmap_c, const Params p,
                              const __grid_constant__ EXTRA extra) {
   constexpr bool ADAPTERS = !std::is_same<EXTRA, NoAdapters>::value;
+  constexpr int PARTS = EXTRA::kParts;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
   uint8_t* sA = smem;
   uint8_t* sB = smem + STAGES * A_STAGE_BYTES;
+  // With PARTS: the accumulator, in the stages that its products are done with.
+  [[maybe_unused]] float* sums = reinterpret_cast<float*>(smem);
   uint8_t* sEpi = sB + STAGES * B_STAGE_BYTES;  // 1024-aligned, EPI_STAGE_BYTES per epilogue warp
   Ctrl* ctrl = reinterpret_cast<Ctrl*>(sEpi + NUM_EPI_WARPS * EPI_STAGE_BYTES);
   int* tile_prefix = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(ctrl) +
@@ -269,7 +334,9 @@ __global__ void __cluster_dims__(2, 1, 1) __maxnreg__(kMaxRegs)
 
   const int warp = threadIdx.x >> 5;
   const int lane = lane_id();
-  const uint32_t crank = cluster_ctarank();
+  // Rank in the pair; the cluster's ranks of the pair's CTAs are first and first + 1.
+  const uint32_t crank = PARTS == 1 ? cluster_ctarank() : cluster_ctarank() & 1u;
+  const uint32_t first = PARTS == 1 ? 0u : cluster_ctarank() & ~1u;
   const bool leader = crank == 0;
   const int tiles_n = (p.n + BN - 1) / BN;
 
@@ -322,7 +389,12 @@ __global__ void __cluster_dims__(2, 1, 1) __maxnreg__(kMaxRegs)
 
   const uint32_t tmem_base = ctrl->tmem_base;
   const int total_tiles = tile_prefix[p.num_experts];
-  const int num_kb = (p.k + BK - 1) / BK;
+  // This pair's k-blocks: all of them, or with PARTS its share.  The pairs take the adapters
+  // in turn.
+  const int all_kb = (p.k + BK - 1) / BK, part = PARTS == 1 ? 0 : static_cast<int>(first >> 1);
+  const int kb_first = PARTS == 1 ? 0 : part * all_kb / PARTS;
+  const int num_kb = PARTS == 1 ? all_kb : (part + 1) * all_kb / PARTS - kb_first;
+  [[maybe_unused]] int4 done = make_int4(0, 0, -1, 0);  // the tile whose sums this warp has left (PARTS > 1)
   volatile int* abort_flag = &ctrl->abort;
 
   if (total_tiles == 0) {
@@ -355,16 +427,16 @@ __global__ void __cluster_dims__(2, 1, 1) __maxnreg__(kMaxRegs)
             s = make_int4(tc.row0, tc.rows, tc.tile_n * BN, tc.expert);
           }
           ctrl->slot[q] = s;
-          st_shared_cluster_v4(mapa_shared(smem_u32(&ctrl->slot[q]), 1), s);
+          st_shared_cluster_v4(mapa_shared(smem_u32(&ctrl->slot[q]), first + 1), s);
           mbar_arrive(smem_u32(&ctrl->qfull[q]));
-          mbar_arrive_cluster(mapa_shared(smem_u32(&ctrl->qfull[q]), 1));
+          mbar_arrive_cluster(mapa_shared(smem_u32(&ctrl->qfull[q]), first + 1));
         } else {
           if (!mbar_wait_cluster(smem_u32(&ctrl->qfull[q]), qphase, abort_flag)) {
             failed = true;
             break;
           }
           s = ctrl->slot[q];
-          mbar_arrive_cluster(mapa_shared(smem_u32(&ctrl->qempty[q]), 0));
+          mbar_arrive_cluster(mapa_shared(smem_u32(&ctrl->qempty[q]), first));
         }
         if (++q == QDEPTH) {
           q = 0;
@@ -396,14 +468,14 @@ __global__ void __cluster_dims__(2, 1, 1) __maxnreg__(kMaxRegs)
           }
           const uint32_t full_local = smem_u32(&ctrl->full[stage]);
           if (leader) mbar_arrive_expect_tx(full_local, stage_tx);
-          const uint32_t full_leader = mapa_shared(full_local, 0);
+          const uint32_t full_leader = mapa_shared(full_local, first);
           const CUtensorMap* ka = map_a;
           const CUtensorMap* kb_map = &tmap_b;
-          int k0 = kb * BK, a_row = row_a, b_matrix = s.w;
+          int k0 = (kb_first + kb) * BK, a_row = row_a, b_matrix = s.w;
           if constexpr (ADAPTERS) {
             if (kb >= num_kb) {
-              const int at = (kb - num_kb) / extra.k_blocks;
-              k0 = (kb - num_kb - at * extra.k_blocks) * BK;
+              const int nth = (kb - num_kb) / extra.k_blocks, at = part + nth * PARTS;
+              k0 = (kb - num_kb - nth * extra.k_blocks) * BK;
               a_row = ((s.x / BM) * Adapters::kPerTile + at) * BM + (row_a - s.x);
               b_matrix = extra.list[(s.x / BM) * Adapters::kPerTile + at];
               ka = &extra.rows;
@@ -427,7 +499,7 @@ __global__ void __cluster_dims__(2, 1, 1) __maxnreg__(kMaxRegs)
             if (kb == num_kb - 1) {
               if (!waited) wait_for_previous_kernel();
               waited = true;
-              tile_kb += extra.count[s.x / BM] * extra.k_blocks;
+              tile_kb += (extra.count[s.x / BM] - part + PARTS - 1) / PARTS * extra.k_blocks;
             }
           }
         }
@@ -479,21 +551,21 @@ __global__ void __cluster_dims__(2, 1, 1) __maxnreg__(kMaxRegs)
         // Two instantiations of the k-block loop, so that the usual tile's loop
         // carries no per-MMA choice between the two operand arrangements.
         bool ok =
-            n_sw > 0 ? issue_tile<BF16, B_MN_MAJOR, true>(ctrl, sA, sB, d_tmem, num_kb, stage, phase,
+            n_sw > 0 ? issue_tile<BF16, B_MN_MAJOR, true, false, PARTS>(ctrl, sA, sB, d_tmem, num_kb, stage, phase,
                                                           abort_flag, issued_any,
                                                           idesc_f16(BF16, BM, n_sw, B_MN_MAJOR, false))
-                     : issue_tile<BF16, B_MN_MAJOR, false>(ctrl, sA, sB, d_tmem, num_kb, stage, phase,
+                     : issue_tile<BF16, B_MN_MAJOR, false, false, PARTS>(ctrl, sA, sB, d_tmem, num_kb, stage, phase,
                                                            abort_flag, issued_any, 0u);
         if constexpr (ADAPTERS) {
           if (ok) {
             if (!waited) wait_for_previous_kernel();
             waited = true;
             const int tile = s.x / BM, adapters = extra.count[tile];
-            for (int at = 0; at < adapters && ok; ++at) {
+            for (int at = part; at < adapters && ok; at += PARTS) {
               const uint4* mine = extra.mine + (tile * Adapters::kPerTile + at) * 2;
               const uint4 m0 = mine[0], m1 = mine[1];
               const uint32_t off[8] = {~m0.x, ~m0.y, ~m0.z, ~m0.w, ~m1.x, ~m1.y, ~m1.z, ~m1.w};
-              ok = issue_tile<BF16, B_MN_MAJOR, false, true>(ctrl, sA, sB, d_tmem, extra.k_blocks, stage, phase,
+              ok = issue_tile<BF16, B_MN_MAJOR, false, true, PARTS>(ctrl, sA, sB, d_tmem, extra.k_blocks, stage, phase,
                                                              abort_flag, issued_any, 0u, off);
             }
           }
@@ -502,7 +574,7 @@ __global__ void __cluster_dims__(2, 1, 1) __maxnreg__(kMaxRegs)
         if (failed) break;
         const uint32_t tf_local = smem_u32(&ctrl->tfull[acc]);
         umma_commit_pair(tf_local);
-        umma_commit_pair(mapa_shared(tf_local, 1));
+        umma_commit_pair(mapa_shared(tf_local, first + 1));
         if (++acc == 2) {
           acc = 0;
           aphase ^= 1;
@@ -534,7 +606,7 @@ __global__ void __cluster_dims__(2, 1, 1) __maxnreg__(kMaxRegs)
       }
       const int4 s = ctrl->slot[q];
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&ctrl->qempty[q]), 0));
+      if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&ctrl->qempty[q]), first));
       if (++q == QDEPTH) {
         q = 0;
         qphase ^= 1;
@@ -547,7 +619,11 @@ __global__ void __cluster_dims__(2, 1, 1) __maxnreg__(kMaxRegs)
       }
       tc_fence_after();
       const int n_sw = PUSH ? 0 : swapped_n(p, s.y);
-      if (n_sw > 0) {
+      if constexpr (PARTS > 1) {
+        leave_sums(tmem_base + (uint32_t(quad * 32) << 16) + uint32_t(acc * BN), sums, quad * 32 + lane,
+                   col_half * 128, p.n - s.z);
+        done = s;
+      } else if (n_sw > 0) {
         // The two warps of a lane quadrant split the tile's rows in 32-row chunks.
         const int half = ((n_sw / 2) + 31) & ~31;
         store_swapped<BF16>(tmem_base + (uint32_t(quad * 32) << 16) + uint32_t(acc * BN), lane, quad,
@@ -562,7 +638,7 @@ __global__ void __cluster_dims__(2, 1, 1) __maxnreg__(kMaxRegs)
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&ctrl->tempty[acc]), 0));
+      if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&ctrl->tempty[acc]), first));
       if (++acc == 2) {
         acc = 0;
         aphase ^= 1;
@@ -579,6 +655,12 @@ __global__ void __cluster_dims__(2, 1, 1) __maxnreg__(kMaxRegs)
   __syncthreads();
   cluster_sync_all();  // neither CTA leaves while the pair still uses its memory
   tc_fence_after();
+  if constexpr (PARTS > 1) {
+    if (done.z >= 0)
+      add_parts<BF16, PARTS>(sums, crank, (warp & 3) * 32 + lane, part, (warp - 2) >> 2, done, p);
+    __syncthreads();
+    cluster_sync_all();  // no CTA leaves while another reads its sums
+  }
   if (warp == 1) {
     __syncwarp();
     tmem_dealloc_pair(tmem_base, TMEM_COLS);
@@ -623,12 +705,27 @@ int launch_pair_kernel(bool bf16, bool b_mn, const CUtensorMap& ta, const CUtens
                        cudaStream_t stream, const AdapterMaps* adapters) {
   if (grid < 2 || grid % 2 != 0) return MOE_ERR_INVALID_ARG;
   if (adapters != nullptr) {
-    using X = AdapterMaps;
     if (p.push.src != nullptr) return MOE_ERR_INVALID_ARG;
-    if (bf16 && b_mn) return pair::launch<true, true, false, X>(ta, ta_half, tb, tc, p, grid, stream, *adapters);
-    if (bf16) return pair::launch<true, false, false, X>(ta, ta_half, tb, tc, p, grid, stream, *adapters);
-    if (b_mn) return pair::launch<false, true, false, X>(ta, ta_half, tb, tc, p, grid, stream, *adapters);
-    return pair::launch<false, false, false, X>(ta, ta_half, tb, tc, p, grid, stream, *adapters);
+    auto go = [&](auto parts, const Params& q, int ctas) {
+      using X = pair::SplitAdapters<decltype(parts)::value>;
+      const X x{*adapters};
+      if (bf16 && b_mn) return pair::launch<true, true, false, X>(ta, ta_half, tb, tc, q, ctas, stream, x);
+      if (bf16) return pair::launch<true, false, false, X>(ta, ta_half, tb, tc, q, ctas, stream, x);
+      if (b_mn) return pair::launch<false, true, false, X>(ta, ta_half, tb, tc, q, ctas, stream, x);
+      return pair::launch<false, false, false, X>(ta, ta_half, tb, tc, q, ctas, stream, x);
+    };
+    const int64_t tiles = (int64_t(p.m_total) + pair::BM - 1) / pair::BM * ((p.n + pair::BN - 1) / pair::BN);
+    const int k_blocks = (p.k + pair::BK - 1) / pair::BK;
+    Params q = p;
+    q.use_atomic = 0;  // one tile a cluster
+    // Few tiles: the contraction over 2 or 4 pairs each, as far as SMs are left for the
+    // kernel that this one starts beside.  Projection of 300 x 8192 x 1024 (8 tiles, 8
+    // adapters of rank 64), all kernels: 59.5 us with one pair a tile, 37.9 with two, 36.9 with
+    // four; 700 x 8192 x 2048 (24 tiles) 57.5, 39.0 and, with clusters that wait for SMs,
+    // 58.2; 1000 x 512 x 1024 (8 k-blocks) 22.6, 22.5 and 30.8.
+    if (k_blocks >= 16 && tiles * 8 <= grid / 2) return go(std::integral_constant<int, 4>(), q, int(tiles) * 8);
+    if (k_blocks >= 16 && tiles * 4 <= grid * 7 / 8) return go(std::integral_constant<int, 2>(), q, int(tiles) * 4);
+    return go(std::integral_constant<int, 1>(), p, grid);
   }
   if (p.push.src != nullptr) {  // combine push (bf16 only)
     if (!bf16) return MOE_ERR_INVALID_ARG;

@@ -455,3 +455,73 @@ def test_refusals(cuda_device):
     with torch.no_grad():  # nothing asks for those gradients here
         assert f(x, w.clone().requires_grad_(True), a, b, ids).shape == (6, 72)
     mo.check_status(cuda_device, sync=True)
+
+
+@pytest.mark.parametrize("M,K,N,L,r,dtype", [
+    (66, 1032, 264, 3, 8, torch.bfloat16), (200, 264, 1048, 8, 40, torch.float16),
+    (300, 1040, 1104, 1, 128, torch.bfloat16), (700, 2056, 1000, 8, 64, torch.float16),
+    (515, 1096, 1160, 20, 16, torch.bfloat16), (1500, 1024, 1100, 9, 24, torch.bfloat16)])
+@pytest.mark.parametrize("runs", [False, True])
+def test_few_tiles_of_long_contractions(cuda_device, M, K, N, L, r, dtype, runs):
+    """Few tiles of the output: their contraction over K (backward: over N) is split, and
+    the adapters of a tile with it; rows of an adapter together or in any order."""
+    x, w, a, b, dy, scale, ids = make(M, K, N, L, r, dtype, seed=M + K, device=cuda_device)
+    if runs:
+        ids = torch.sort(ids).values
+    for t in (x, a, b):
+        t.requires_grad_(True)
+    y = mo.lora_linear(x, w, a, b, ids, scale=scale)
+    grads = torch.autograd.grad(y, (x, a, b), dy)
+    mo.check_status(cuda_device, sync=True)
+    for got, want in zip((y, *grads), reference(x, w, a, b, dy, scale, ids)):
+        assert_close(got, want)
+    y2 = mo.lora_linear(x, w, a, b, ids, scale=scale)
+    for one, two in zip((y2, *torch.autograd.grad(y2, (x, a, b), dy)), (y, *grads)):
+        assert torch.equal(one, two)  # sums in a fixed order
+
+
+@pytest.mark.parametrize("M,K,N", [(300, 1040, 264), (300, 264, 1040), (900, 1032, 1032)])
+def test_infinities_with_split_contractions(cuda_device, M, K, N):
+    x, w, a, b, dy, scale, ids = make(M, K, N, 5, 16, torch.bfloat16, seed=M, device=cuda_device)
+
+    def run(a, b):
+        p = [t.detach().clone().requires_grad_() for t in (x, a, b)]
+        y = mo.lora_linear(p[0], w, p[1], p[2], ids, scale=scale)
+        return (y.detach(), *torch.autograd.grad(y, p, dy))
+
+    bad_a, bad_b = a.clone(), b.clone()
+    bad_a[1, 3, 5], bad_b[2, 7] = float("inf"), float("nan")
+    clean_rows = (ids != 1) & (ids != 2)
+    good, bad = run(a, b), run(bad_a, bad_b)
+    assert not bool(bad[0][~clean_rows].isfinite().all())
+    for g, h in zip(good[:2], bad[:2]):
+        assert torch.equal(g[clean_rows], h[clean_rows])
+    for g, h in zip(good[2:], bad[2:]):
+        assert torch.equal(g[[0, 3, 4]], h[[0, 3, 4]])
+
+
+@pytest.mark.parametrize("M", [1, 40, 300])
+def test_broadcast_inputs_and_shared_adapters(cuda_device, M):
+    """An output summed (a gradient of stride 0), one adapter expanded over all requests, and
+    adapters that stand twice in one graph."""
+    x, w, a, b, _, scale, ids = make(M, 264, 264, 4, 16, torch.bfloat16, seed=M, device=cuda_device)
+    one = a[:1].clone().requires_grad_()
+    x.requires_grad_()
+    y = mo.lora_linear(x, w, one.expand_as(a), b, ids, scale=scale)
+    dx, da = torch.autograd.grad(y.sum(), (x, one))
+    want = reference(x, w, one.expand_as(a), b, torch.ones_like(y), scale, ids)
+    assert_close(dx, want[1])
+    per_adapter, tol = want[2]
+    # each adapter's gradient is rounded, then their sum (three additions and a rounding of it)
+    u = torch.finfo(a.dtype).eps / 2
+    assert_close(da[0], (per_adapter.sum(0), tol.sum(0) + 4 * u * per_adapter.abs().sum(0)))
+
+    a.requires_grad_(), b.requires_grad_()
+    h = mo.lora_linear(x.detach(), w, a, b, ids, scale=scale)
+    y = mo.lora_linear(h, w, a, b, ids, scale=scale)
+    both = torch.autograd.grad(y, (a, b), torch.ones_like(y))
+    h2 = h.detach().requires_grad_()
+    second = torch.autograd.grad(mo.lora_linear(h2, w, a, b, ids, scale=scale), (h2, a, b), torch.ones_like(y))
+    first = torch.autograd.grad(mo.lora_linear(x.detach(), w, a, b, ids, scale=scale), (a, b), second[0])
+    for got, p, q in zip(both, first, second[1:]):
+        assert torch.equal(got, p + q)
