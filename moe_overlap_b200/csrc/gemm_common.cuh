@@ -5,6 +5,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <cstddef>
 #include <cstdint>
 
 #include "../../include/moe_overlap.h"
@@ -34,19 +35,28 @@ struct ArrivalWait {
   uint64_t wait_ns;         // bound on each wait
 };
 
+// The adapters of a tile of 256 rows.
+struct alignas(16) TileAdapters {
+  static constexpr int kMost = 16;
+  int32_t list[kMost];      // the first `count`
+  int32_t count, left;      // left: there are more, or too many, and the product takes none
+  int32_t unused[2];
+  uint32_t mine[kMost][8];  // a bit for each row of the tile that is the adapter's
+};
+static_assert(sizeof(TileAdapters) % 16 == 0 && offsetof(TileAdapters, count) % 16 == 0, "copied by parts");
+
 // Adapters' products added in the accumulator of a one-expert product: for each of the
-// first count[t] adapters of row tile t's list (256 rows), the product of `rows` (256
-// x rank for each of the tile's kPerTile places) and that adapter's matrix w_i, stored
-// in the direction of B (one matrix behind another, `stride_l` apart, rows `stride_row`
-// apart), in the adapter's own rows only.  What `rows` holds in the others is not used.
+// first `count` adapters of a row tile's list, the product of the tile's
+// `rows` and that adapter's matrix w_i, stored in the direction of B (one matrix behind
+// another, `stride_l` apart, rows `stride_row` apart), in the adapter's own rows only.
+// `rows` of no listed adapter may hold anything.
 struct Adapters {
-  // Each costs ceil(rank / 64) k-blocks in every tile; left out, its rows of C are read
-  // and written once more instead.  At k = 2048 and rank 64 eight add a quarter to a tile.
-  static constexpr int kPerTile = 8;
-  const void* rows;      // [row tiles][kPerTile][256][rank], the inputs' type
-  const int32_t* count;  // [row tiles]
-  const int32_t* list;   // [row tiles][kPerTile]
-  const uint4* mine;     // [row tiles][kPerTile][2] a bit for each row that is the adapter's
+  // Columns of the rank that one box takes; adapters of 16 or 32 share a stage.
+  static constexpr int width(int rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : 64; }
+  // Adapters of a tile that the product takes.
+  static constexpr int most(int rank) { return rank <= 32 ? TileAdapters::kMost : 8; }
+  const void* rows;      // [m][rank], the inputs' type
+  const TileAdapters* tiles;
   const void* w;
   int64_t stride_l, stride_row;
   int rank, adapters;
@@ -342,12 +352,12 @@ int launch_pair_kernel(bool bf16, bool b_mn, const CUtensorMap& ta, const CUtens
 
 // The tensor maps of Adapters and what the pair kernel reads beside them.
 struct AdapterMaps {
-  CUtensorMap rows;  // boxes as A's
-  CUtensorMap w;     // boxes as B's
-  const int32_t* count;
-  const int32_t* list;
-  const uint4* mine;
-  int k_blocks;  // of 64 in the rank
+  CUtensorMap rows;  // boxes of `width` columns x 128 rows
+  CUtensorMap w;     // of `width` columns x 128 rows, or 64 columns x `width` rows of the rank
+  const TileAdapters* tiles;
+  int width;  // of a box in the rank: 16, 32 or 64
+  int boxes;  // of an adapter: 1, of ranks above 64 2
+  int steps;  // of 16 in the rank
 };
 
 }  // namespace gg

@@ -529,20 +529,27 @@ int moe::gg::grouped_gemm_launch(const void* a, int64_t lda, const void* b, int6
     // The pair kernel's row tiles, with one expert, are the adapters' tiles.
     if (!use_pair || num_experts != 1) return MOE_ERR_UNSUPPORTED;
     const uint64_t r = uint64_t(adapters->rank);
-    const uint64_t tiles = uint64_t((m_total + 255) / 256);
-    const uint64_t rdims[2] = {r, tiles * Adapters::kPerTile * 256};
+    const uint64_t rdims[2] = {r, uint64_t(m_total)};
     const uint64_t rstrides[1] = {r * 2};
-    const uint32_t rbox[2] = {BK, BM};
-    if (int rc = encode_tiled(&extra.rows, dt, 2, adapters->rows, rdims, rstrides, rbox); rc != MOE_OK) return rc;
+    extra.width = Adapters::width(adapters->rank);
+    const uint32_t width = uint32_t(extra.width);
+    const CUtensorMapSwizzle by_width = width == 16   ? CU_TENSOR_MAP_SWIZZLE_32B
+                                        : width == 32 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                                      : CU_TENSOR_MAP_SWIZZLE_128B;
+    const uint32_t rbox[2] = {width, 128};
+    if (int rc = encode_tiled(&extra.rows, dt, 2, adapters->rows, rdims, rstrides, rbox, by_width); rc != MOE_OK)
+      return rc;
     const uint64_t wdims[3] = {b_mn ? uint64_t(n) : r, b_mn ? r : uint64_t(n), uint64_t(adapters->adapters)};
     const uint64_t row = uint64_t(adapters->stride_row) * 2;
     const uint64_t wstrides[2] = {row, adapters->adapters > 1 ? uint64_t(adapters->stride_l) * 2 : row * wdims[1]};
-    const uint32_t wbox[3] = {64, b_mn ? uint32_t(BK) : uint32_t(BN / 2), 1};
-    if (int rc = encode_tiled(&extra.w, dt, 3, adapters->w, wdims, wstrides, wbox); rc != MOE_OK) return rc;
-    extra.count = adapters->count;
-    extra.list = adapters->list;
-    extra.mine = adapters->mine;
-    extra.k_blocks = (adapters->rank + BK - 1) / BK;
+    const uint32_t wbox[3] = {b_mn ? 64u : width, b_mn ? width : 128u, 1};
+    if (int rc = encode_tiled(&extra.w, dt, 3, adapters->w, wdims, wstrides, wbox,
+                              b_mn ? CU_TENSOR_MAP_SWIZZLE_128B : by_width);
+        rc != MOE_OK)
+      return rc;
+    extra.tiles = adapters->tiles;
+    extra.boxes = (adapters->rank + extra.width - 1) / extra.width;
+    extra.steps = (adapters->rank + 15) / 16;
   }
 
   // With adapters the counter is 0 already: nothing comes between their kernels.

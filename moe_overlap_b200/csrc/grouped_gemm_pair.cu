@@ -32,13 +32,15 @@
 // columns in its lanes and the tile's rows in N accumulator columns; the epilogue
 // stores them transposed (plain or GELU epilogues only).
 // Adapters (ADAPTERS, one expert): behind a tile's own k-blocks come, for each adapter of
-// its rows, the k-blocks of the adapter's rank, A from the tile's rows of x A_i^T and B from
-// the adapter's second matrix, with the accumulator's other rows switched off (a product
-// with zeros there would carry one adapter's infinities into another's rows); boxes past
-// the rank are zero-filled, so any rank fills whole k-blocks.  The sum stays in the
-// accumulator and is rounded once.  The launch may start beside the kernel that prepares those rows: only the
-// threads that fetch and multiply them wait for its end, behind their first tile's own
-// k-blocks (everything before that kernel is complete when this one starts).
+// its rows, the steps of the adapter's rank: A from the tile's rows of x A_i^T and B from the
+// adapter's second matrix, with the accumulator's other rows switched off (a product with
+// zeros there would carry one adapter's infinities into another's rows).  A stage takes two
+// adapters of rank up to 32, four of up to 16, in rows and swizzles of 64 or 32 bytes: boxes
+// cost by their rows, and one of A serves all of a stage.  Boxes past the rank are
+// zero-filled.  The sum stays in the accumulator and is rounded once.  The launch may start beside the kernel
+// that prepares those rows: only the threads that fetch them wait for its end, behind their
+// first tile's own k-blocks (everything before that kernel, the tiles' adapters among it, is
+// complete when this one starts).
 // Parts (with adapters, few tiles): a cluster of 2 or 4 pairs takes one tile, each pair a
 // share of the k-blocks and every 2nd or 4th adapter.  The pairs leave their sums in their
 // shared memory, and each CTA adds one share of the columns over the parts, in their order.
@@ -92,6 +94,19 @@ struct Ctrl {
   uint32_t tmem_base;
   int abort;
 };
+
+// A tile's adapters, brought in beside the tile's own k-blocks: list and count for the
+// thread that fetches, count and rows for the one that multiplies.
+struct AdapterCtrl {
+  TileAdapters fetch, multiply;
+  uint64_t fetch_in, multiply_in;
+};
+constexpr uint32_t FETCH_BYTES = offsetof(TileAdapters, mine);
+constexpr uint32_t MULTIPLY_FROM = offsetof(TileAdapters, count);
+constexpr uint32_t MULTIPLY_BYTES = sizeof(TileAdapters) - MULTIPLY_FROM;
+// Bytes of a box of the rank for one column of it: 128 rows of A or B, or of an N-major B
+// twice 64 columns.
+constexpr int BOX_COLUMN_BYTES = 128 * 2;
 
 __host__ __device__ constexpr size_t smem_bytes(int num_experts) {
   return 1024 + size_t(STAGES) * (A_STAGE_BYTES + B_STAGE_BYTES) + size_t(NUM_EPI_WARPS) * EPI_STAGE_BYTES +
@@ -187,20 +202,17 @@ __device__ __forceinline__ void store_swapped(uint32_t t_lane_base, int lane, in
   }
 }
 
-__device__ constexpr uint32_t kNoRowsOff[8] = {};
-
 // The MMA issuer's k-block loop for one tile (leader CTA, one thread): waits for
 // each stage's data, issues its four 16-deep MMAs into the accumulator at d_tmem
 // and commits the stage back to both CTAs' producers.  SWAPPED issues the swapped
 // form (B stage as the MMA's A operand with M = 256, the A stage's first N/2 rows
 // as its B operand, N and the operand layouts in idesc_sw).  The first MMA overwrites the
-// accumulator; with ROWS all add to it, but for the rows whose bits are set in `off`.
-// Returns false when a wait gave up.
-template <bool BF16, bool B_MN_MAJOR, bool SWAPPED, bool ROWS = false, int PARTS = 1>
+// accumulator.  Returns false when a wait gave up.
+template <bool BF16, bool B_MN_MAJOR, bool SWAPPED, int PARTS = 1>
 __device__ __forceinline__ bool issue_tile(Ctrl* ctrl, uint8_t* sA, uint8_t* sB, uint32_t d_tmem,
                                            int num_kb, int& stage, uint32_t& phase,
                                            const volatile int* abort_flag, bool& issued_any,
-                                           uint32_t idesc_sw, const uint32_t (&off)[8] = kNoRowsOff) {
+                                           uint32_t idesc_sw) {
   const uint32_t idesc = SWAPPED ? idesc_sw : idesc_f16(BF16, BM, BN, false, B_MN_MAJOR);
   // This thread's loop is on the critical path and shares its SM sub-partition with
   // two epilogue warps, so every per-stage quantity is formed once per tile and
@@ -225,9 +237,7 @@ __device__ __forceinline__ bool issue_tile(Ctrl* ctrl, uint8_t* sA, uint8_t* sB,
     for (int kk = 0; kk < BK / UMMA_K; ++kk) {
       const uint64_t adesc = adesc0 + uint64_t(kk * (UMMA_K * 2 / 16));
       const uint64_t bdesc = bdesc0 + uint64_t(B_MN_MAJOR ? kk * (UMMA_K * 128 / 16) : kk * (UMMA_K * 2 / 16));
-      if constexpr (ROWS)
-        umma_f16_pair_rows(d_tmem, adesc, bdesc, idesc, off);
-      else if constexpr (SWAPPED)
+      if constexpr (SWAPPED)
         umma_f16_pair(d_tmem, bdesc, adesc, idesc, (kb | kk) != 0 ? 1u : 0u);
       else
         umma_f16_pair(d_tmem, adesc, bdesc, idesc, (kb | kk) != 0 ? 1u : 0u);
@@ -239,6 +249,44 @@ __device__ __forceinline__ bool issue_tile(Ctrl* ctrl, uint8_t* sA, uint8_t* sB,
       stage = 0;
       phase ^= 1;
     }
+  }
+  return true;
+}
+
+// The same for the adapters `at`, `at` + PARTS, ... of a tile's `count`: each step of 16 of
+// an adapter's rank adds to the accumulator's rows that are the adapter's.
+template <bool BF16, bool B_MN_MAJOR, int PARTS, int WIDTH>
+__device__ __forceinline__ bool issue_adapters(Ctrl* ctrl, const TileAdapters& of, uint8_t* sA, uint8_t* sB,
+                                               uint32_t d_tmem, int at, const AdapterMaps& extra, int& stage,
+                                               uint32_t& phase, const volatile int* abort_flag) {
+  const uint32_t idesc = idesc_f16(BF16, BM, BN, false, B_MN_MAJOR);
+  const uint32_t peer = PARTS == 1 ? 1u : cluster_ctarank() + 1u;
+  const int count = min(of.count, TileAdapters::kMost);
+  int box = 0;
+  while (at < count) {
+    if (!mbar_wait_cluster(smem_u32(&ctrl->full[stage]), phase, abort_flag)) return false;
+    tc_fence_after();
+    const uint64_t adesc = smem_desc_rows(smem_u32(sA + stage * A_STAGE_BYTES), WIDTH * 2);
+    const uint32_t b0 = smem_u32(sB + stage * B_STAGE_BYTES);
+    const uint64_t bdesc = B_MN_MAJOR ? smem_desc_sw128(b0, B_SLAB_BYTES, 1024) : smem_desc_rows(b0, WIDTH * 2);
+#pragma unroll
+    for (int u = 0; u < BK; u += WIDTH) {
+      if (at >= count) break;
+      const uint4 m0 = *reinterpret_cast<const uint4*>(&of.mine[at][0]);
+      const uint4 m1 = *reinterpret_cast<const uint4*>(&of.mine[at][4]);
+      const uint32_t off[8] = {~m0.x, ~m0.y, ~m0.z, ~m0.w, ~m1.x, ~m1.y, ~m1.z, ~m1.w};
+#pragma unroll
+      for (int k = 0; k < WIDTH; k += UMMA_K) {
+        if (box * BK + k >= extra.steps * UMMA_K) break;
+        umma_f16_pair_rows(d_tmem, adesc + k * 2 / 16,
+                           bdesc + (B_MN_MAJOR ? (u + k) * 128 : u * BOX_COLUMN_BYTES + k * 2) / 16, idesc, off);
+      }
+      if (++box == extra.boxes) box = 0, at += PARTS;
+    }
+    const uint32_t empty = smem_u32(&ctrl->empty[stage]);
+    umma_commit_pair(empty);
+    umma_commit_pair(mapa_shared(empty, peer));
+    if (++stage == STAGES) stage = 0, phase ^= 1;
   }
   return true;
 }
@@ -331,6 +379,8 @@ __global__ void __cluster_dims__(2 * EXTRA::kParts, 1, 1) __maxnreg__(kMaxRegs)
                                             ((sizeof(Ctrl) + 15) / 16) * 16);
   int* seg_start = tile_prefix + (p.num_experts + 1);
   int* seg_rows = seg_start + (p.num_experts + 1);
+  [[maybe_unused]] AdapterCtrl* names =  // (of one expert: 2 ints in each of the three arrays)
+      reinterpret_cast<AdapterCtrl*>(reinterpret_cast<uint8_t*>(tile_prefix) + 32);
 
   const int warp = threadIdx.x >> 5;
   const int lane = lane_id();
@@ -355,6 +405,10 @@ __global__ void __cluster_dims__(2 * EXTRA::kParts, 1, 1) __maxnreg__(kMaxRegs)
       mbar_init(smem_u32(&ctrl->qempty[q]), 2 + 2 * NUM_EPI_WARPS);
     }
     mbar_init(smem_u32(&ctrl->drain), 1);
+    if constexpr (ADAPTERS) {
+      mbar_init(smem_u32(&names->fetch_in), 1);
+      mbar_init(smem_u32(&names->multiply_in), 1);
+    }
     ctrl->abort = 0;
     fence_mbar_init();
   }
@@ -409,6 +463,7 @@ __global__ void __cluster_dims__(2 * EXTRA::kParts, 1, 1) __maxnreg__(kMaxRegs)
       int ready_expert = -1;
       bool failed = false;
       [[maybe_unused]] bool waited = false;
+      [[maybe_unused]] uint32_t tile_phase = 0;
       const int pair_id = static_cast<int>(cluster_id_x());
       const int npairs = static_cast<int>(nclusters_x());
       for (int iter = 0;; ++iter) {
@@ -460,8 +515,12 @@ __global__ void __cluster_dims__(2 * EXTRA::kParts, 1, 1) __maxnreg__(kMaxRegs)
         const CUtensorMap* map_a = half_box ? &tmap_a_half : &tmap_a;
         const uint32_t stage_tx = half_box ? PAIR_TX_BYTES_SWAPPED : PAIR_TX_BYTES;
         const int n_b = s.z + static_cast<int>(crank) * BN_CTA;
-        int tile_kb = num_kb;
-        for (int kb = 0; kb < tile_kb; ++kb) {
+        if constexpr (ADAPTERS) {
+          const uint32_t bar = smem_u32(&names->fetch_in);
+          mbar_arrive_expect_tx(bar, FETCH_BYTES);
+          bulk_load(smem_u32(&names->fetch), extra.tiles + s.x / BM, FETCH_BYTES, bar);
+        }
+        for (int kb = 0; kb < num_kb; ++kb) {
           if (!mbar_wait_cluster(smem_u32(&ctrl->empty[stage]), phase ^ 1, abort_flag)) {
             failed = true;
             break;
@@ -469,41 +528,64 @@ __global__ void __cluster_dims__(2 * EXTRA::kParts, 1, 1) __maxnreg__(kMaxRegs)
           const uint32_t full_local = smem_u32(&ctrl->full[stage]);
           if (leader) mbar_arrive_expect_tx(full_local, stage_tx);
           const uint32_t full_leader = mapa_shared(full_local, first);
-          const CUtensorMap* ka = map_a;
-          const CUtensorMap* kb_map = &tmap_b;
-          int k0 = (kb_first + kb) * BK, a_row = row_a, b_matrix = s.w;
-          if constexpr (ADAPTERS) {
-            if (kb >= num_kb) {
-              const int nth = (kb - num_kb) / extra.k_blocks, at = part + nth * PARTS;
-              k0 = (kb - num_kb - nth * extra.k_blocks) * BK;
-              a_row = ((s.x / BM) * Adapters::kPerTile + at) * BM + (row_a - s.x);
-              b_matrix = extra.list[(s.x / BM) * Adapters::kPerTile + at];
-              ka = &extra.rows;
-              kb_map = &extra.w;
-            }
-          }
-          tma_load_2d_pair(smem_u32(sA + stage * A_STAGE_BYTES), ka, full_leader, k0, a_row);
+          const int k0 = (kb_first + kb) * BK;
+          tma_load_2d_pair(smem_u32(sA + stage * A_STAGE_BYTES), map_a, full_leader, k0, row_a);
           const uint32_t b_dst = smem_u32(sB + stage * B_STAGE_BYTES);
           if constexpr (B_MN_MAJOR) {
 #pragma unroll
             for (int j = 0; j < BN_CTA / 64; ++j)
-              tma_load_3d_pair(b_dst + j * B_SLAB_BYTES, kb_map, full_leader, n_b + 64 * j, k0, b_matrix);
+              tma_load_3d_pair(b_dst + j * B_SLAB_BYTES, &tmap_b, full_leader, n_b + 64 * j, k0, s.w);
           } else {
-            tma_load_3d_pair(b_dst, kb_map, full_leader, k0, n_b, b_matrix);
+            tma_load_3d_pair(b_dst, &tmap_b, full_leader, k0, n_b, s.w);
           }
           if (++stage == STAGES) {
             stage = 0;
             phase ^= 1;
           }
-          if constexpr (ADAPTERS) {
-            if (kb == num_kb - 1) {
-              if (!waited) wait_for_previous_kernel();
-              waited = true;
-              tile_kb += (extra.count[s.x / BM] - part + PARTS - 1) / PARTS * extra.k_blocks;
-            }
-          }
         }
         if (failed) break;
+        if constexpr (ADAPTERS) {
+          if (!mbar_wait(smem_u32(&names->fetch_in), tile_phase, abort_flag)) {
+            failed = true;
+            break;
+          }
+          tile_phase ^= 1;
+          if (!waited) wait_for_previous_kernel();
+          waited = true;
+          // Boxes of the adapters' matrices, as many as fill a stage; one of the rows for all.
+          const int count = min(names->fetch.count, TileAdapters::kMost);
+          const int boxes = (count - part + PARTS - 1) / PARTS * extra.boxes, width = extra.width;
+          int at = part, box = 0;
+          for (int t = 0; t < boxes; t += BK / width) {
+            if (!mbar_wait_cluster(smem_u32(&ctrl->empty[stage]), phase ^ 1, abort_flag)) {
+              failed = true;
+              break;
+            }
+            const uint32_t full_local = smem_u32(&ctrl->full[stage]);
+            const uint32_t full_leader = mapa_shared(full_local, first);
+            const int here = min(BK / width, boxes - t);
+            if (leader) mbar_arrive_expect_tx(full_local, 2 * (1 + here) * width * BOX_COLUMN_BYTES);
+            const uint32_t b_dst = smem_u32(sB + stage * B_STAGE_BYTES);
+            tma_load_2d_pair(smem_u32(sA + stage * A_STAGE_BYTES), &extra.rows, full_leader, box * BK, row_a);
+            for (int u = 0; u < here; ++u) {
+              const int k0 = box * BK, matrix = names->fetch.list[at];
+              if constexpr (B_MN_MAJOR) {
+#pragma unroll
+                for (int j = 0; j < BN_CTA / 64; ++j)
+                  tma_load_3d_pair(b_dst + j * B_SLAB_BYTES + u * width * 128, &extra.w, full_leader, n_b + 64 * j,
+                                   k0, matrix);
+              } else {
+                tma_load_3d_pair(b_dst + u * width * BOX_COLUMN_BYTES, &extra.w, full_leader, k0, n_b, matrix);
+              }
+              if (++box == extra.boxes) box = 0, at += PARTS;
+            }
+            if (++stage == STAGES) {
+              stage = 0;
+              phase ^= 1;
+            }
+          }
+          if (failed) break;
+        }
       }
       if constexpr (ADAPTERS) {
         if (!waited) wait_for_previous_kernel();  // this grid ends after the one before
@@ -528,7 +610,7 @@ __global__ void __cluster_dims__(2 * EXTRA::kParts, 1, 1) __maxnreg__(kMaxRegs)
       uint32_t aphase = 0;
       bool failed = false;
       bool issued_any = false;
-      [[maybe_unused]] bool waited = false;
+      [[maybe_unused]] uint32_t tile_phase = 0;
       while (true) {
         if (!mbar_wait_cluster(smem_u32(&ctrl->qfull[q]), qphase, abort_flag)) {
           failed = true;
@@ -547,28 +629,31 @@ __global__ void __cluster_dims__(2 * EXTRA::kParts, 1, 1) __maxnreg__(kMaxRegs)
         }
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + uint32_t(acc * BN);
+        if constexpr (ADAPTERS) {
+          const uint32_t bar = smem_u32(&names->multiply_in);
+          mbar_arrive_expect_tx(bar, MULTIPLY_BYTES);
+          bulk_load(smem_u32(&names->multiply.count), &extra.tiles[s.x / BM].count, MULTIPLY_BYTES, bar);
+        }
         const int n_sw = swapped_n(p, s.y);
         // Two instantiations of the k-block loop, so that the usual tile's loop
         // carries no per-MMA choice between the two operand arrangements.
         bool ok =
-            n_sw > 0 ? issue_tile<BF16, B_MN_MAJOR, true, false, PARTS>(ctrl, sA, sB, d_tmem, num_kb, stage, phase,
+            n_sw > 0 ? issue_tile<BF16, B_MN_MAJOR, true, PARTS>(ctrl, sA, sB, d_tmem, num_kb, stage, phase,
                                                           abort_flag, issued_any,
                                                           idesc_f16(BF16, BM, n_sw, B_MN_MAJOR, false))
-                     : issue_tile<BF16, B_MN_MAJOR, false, false, PARTS>(ctrl, sA, sB, d_tmem, num_kb, stage, phase,
+                     : issue_tile<BF16, B_MN_MAJOR, false, PARTS>(ctrl, sA, sB, d_tmem, num_kb, stage, phase,
                                                            abort_flag, issued_any, 0u);
         if constexpr (ADAPTERS) {
-          if (ok) {
-            if (!waited) wait_for_previous_kernel();
-            waited = true;
-            const int tile = s.x / BM, adapters = extra.count[tile];
-            for (int at = part; at < adapters && ok; at += PARTS) {
-              const uint4* mine = extra.mine + (tile * Adapters::kPerTile + at) * 2;
-              const uint4 m0 = mine[0], m1 = mine[1];
-              const uint32_t off[8] = {~m0.x, ~m0.y, ~m0.z, ~m0.w, ~m1.x, ~m1.y, ~m1.z, ~m1.w};
-              ok = issue_tile<BF16, B_MN_MAJOR, false, true, PARTS>(ctrl, sA, sB, d_tmem, extra.k_blocks, stage, phase,
-                                                             abort_flag, issued_any, 0u, off);
-            }
-          }
+          ok = ok && mbar_wait(smem_u32(&names->multiply_in), tile_phase, abort_flag);
+          auto issue = [&](auto width) {
+            return issue_adapters<BF16, B_MN_MAJOR, PARTS, decltype(width)::value>(
+                ctrl, names->multiply, sA, sB, d_tmem, part, extra, stage, phase, abort_flag);
+          };
+          if (ok)
+            ok = extra.width == 64   ? issue(std::integral_constant<int, 64>())
+                 : extra.width == 32 ? issue(std::integral_constant<int, 32>())
+                                     : issue(std::integral_constant<int, 16>());
+          tile_phase ^= 1;
         }
         if (!ok) failed = true;
         if (failed) break;
@@ -682,10 +767,12 @@ int launch(const CUtensorMap& ta, const CUtensorMap& ta_half, const CUtensorMap&
   });
   if (attr_err != cudaSuccess) return MOE_ERR_CUDA;
   if constexpr (!std::is_same<EXTRA, NoAdapters>::value) {
+    constexpr size_t kAdaptersSmem = smem_bytes(1) + 16 + sizeof(AdapterCtrl);
+    static_assert(kAdaptersSmem <= smem_bytes(kMaxExperts), "what the attribute allows");
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(NUM_THREADS);
-    cfg.dynamicSmemBytes = smem_bytes(p.num_experts);
+    cfg.dynamicSmemBytes = kAdaptersSmem;
     cfg.stream = stream;
     cudaLaunchAttribute early{};
     early.id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -7,7 +7,7 @@
 // gradients.  Rows are taken in adapter order through a permutation, so each adapter is
 // read once per block of its rows:
 //   plan    perm (the rows with an adapter, by adapter, in row order), offs, and for each
-//           tile of 256 rows the adapters in it
+//           tile of 256 rows the adapters in it and which rows are whose
 //   shrink  s[p] = x[perm[p]] A[i]^T           (also dy B[i], with B read along rows)
 //   expand  y[perm[p]] += scale[i] s[p] B[i]^T (also dx += scale[i] (dy B[i]) A[i]) for the
 //           rows of tiles with more adapters than the shared product takes
@@ -35,30 +35,24 @@ constexpr int kMaxAdapters = 1024;
 constexpr int kMaxRank = 128;
 
 constexpr int kTileRows = 256;  // of the shared product
-using gg::Adapters;
+using gg::TileAdapters;
 
 // The caller's plan buffer (int32, 16-byte aligned): what depends on the ids alone.
 struct PlanView {
-  uint32_t* mine;  // [tiles][kPerTile][8] a bit for each row of the tile that is the adapter's
-  int32_t* list;   // [tiles][kPerTile] adapters of a tile, ascending
-  int32_t* count;  // [tiles] how many; 0 also for a tile with too many
-  int32_t* left;   // [tiles] whether the tile's adapters are left to expand
-  int32_t* place;  // [m] block of the row in the tiles' blocks, -1: left to expand
+  TileAdapters* tile;  // [tiles]
+  int32_t* taken;  // [m] whether the shared product takes the row's adapter
   int32_t* perm;   // [m]
   int32_t* offs;   // [adapters + 1]
   int32_t* base;   // {0, m}
   int32_t* queue;  // tile counters of the shared products of the forward and the backward, 0 before each
   static int64_t tiles(int64_t m) { return (m + kTileRows - 1) / kTileRows; }
   static int64_t ints(int64_t m, int adapters) {
-    return tiles(m) * (9 * Adapters::kPerTile + 2) + 2 * m + adapters + 5;
+    return tiles(m) * int64_t(sizeof(TileAdapters) / 4) + 2 * m + adapters + 5;
   }
   PlanView(void* plan, int64_t m, int adapters) {
-    mine = static_cast<uint32_t*>(plan);
-    list = static_cast<int32_t*>(plan) + tiles(m) * Adapters::kPerTile * 8;
-    count = list + tiles(m) * Adapters::kPerTile;
-    left = count + tiles(m);
-    place = left + tiles(m);
-    perm = place + m;
+    tile = static_cast<TileAdapters*>(plan);
+    taken = reinterpret_cast<int32_t*>(tile + tiles(m));
+    perm = taken + m;
     offs = perm + m;
     base = offs + adapters + 1;
     queue = base + 2;
@@ -73,7 +67,7 @@ __device__ __forceinline__ int id_at(const void* ids, int ids64, int m, int L) {
 
 // Blocks 0 .. L-1 each take one adapter: they count the rows of smaller adapters (the
 // segment's start) and write their own rows in order.  Blocks L .. take one row tile each:
-// the adapters in it, which rows are whose, and the rows' places.
+// the adapters in it, which rows are whose, and whether the shared product takes them.
 // No block depends on another and the order is always the same.
 __global__ void __launch_bounds__(1024) plan_kernel(const void* ids, int ids64, int M, int L, PlanView plan,
                                                     int per_tile, int32_t* status) {
@@ -161,16 +155,17 @@ __global__ void __launch_bounds__(1024) plan_kernel(const void* ids, int ids64, 
   }
   __syncthreads();
   const int n = before[32];
-  const bool taken = n <= per_tile;
-  if (tid == 0) plan.count[t] = taken ? n : 0, plan.left[t] = !taken;
+  const bool take = n <= per_tile;
+  TileAdapters& of = plan.tile[t];
+  if (tid == 0) of.count = take ? n : 0, of.left = !take;
   if (tid >= kTileRows) return;
   const int rank = id >= 0 ? before[id >> 5] + __popc(present[id >> 5] & ((1u << (id & 31)) - 1u)) : -1;
-  if (m < M) plan.place[m] = taken && id >= 0 ? t * Adapters::kPerTile + rank : -1;
-  if (!taken) return;
-  if (id >= 0) plan.list[t * Adapters::kPerTile + rank] = id;  // (every row of it writes the same word)
+  if (m < M) plan.taken[m] = take && id >= 0;
+  if (!take) return;
+  if (id >= 0) of.list[rank] = id;  // (every row of it writes the same word)
   for (int q = 0; q < n; ++q) {
     const unsigned rows = __ballot_sync(0xffffffffu, rank == q);
-    if (lane == 0) plan.mine[(t * Adapters::kPerTile + q) * 8 + warp] = rows;
+    if (lane == 0) of.mine[q][warp] = rows;
   }
 }
 
@@ -260,10 +255,10 @@ template <typename T, bool kT, int RP>
 __global__ void __launch_bounds__(kThreads, 2)
     shrink_kernel(const T* x, int64_t ldx, const T* w, int64_t sl, int64_t sr, const int32_t* perm,
                   const int32_t* offs, int L, int K, int r, int64_t part_stride, T* s, Scale scale,
-                  const int32_t* place, T* blocks) {
+                  const int32_t* taken, T* rows) {
   using C = ShrinkCfg<kT, RP>;
   extern __shared__ __align__(128) char smem[];
-  __shared__ int2 block_of[kShrinkRows];  // a row's block in the tiles' blocks and its row there
+  __shared__ int row_of[kShrinkRows];  // -1: not the shared product's
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   wait_for_previous_kernel();
   let_next_kernel_start();
@@ -272,7 +267,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   const float c = scale.of(t.i);
   if (tid < t.rows) {
     const int row = perm[t.p0 + tid];
-    block_of[tid] = make_int2(place[row], row % kTileRows);
+    row_of[tid] = taken[row] ? row : -1;
   }
   const int parts = gridDim.y, part = blockIdx.y;
   const int cols = ((K + parts - 1) / parts + kShrinkCols - 1) / kShrinkCols * kShrinkCols;
@@ -404,11 +399,10 @@ __global__ void __launch_bounds__(kThreads, 2)
     T* out = s + int64_t(t.p0 + m) * r + j;
     *reinterpret_cast<uint2*>(out) = *reinterpret_cast<const uint2*>(hi);
     *reinterpret_cast<uint2*>(out + part_stride) = *reinterpret_cast<const uint2*>(lo);
-    const int2 at = block_of[m];
-    if (at.x >= 0) {  // the shared product takes this row's
+    const int row = row_of[m];
+    if (row >= 0) {
       const T o[4] = {from_f<T>(c * v.x), from_f<T>(c * v.y), from_f<T>(c * v.z), from_f<T>(c * v.w)};
-      *reinterpret_cast<uint2*>(blocks + (int64_t(at.x) * kTileRows + at.y) * r + j) =
-          *reinterpret_cast<const uint2*>(o);
+      *reinterpret_cast<uint2*>(rows + int64_t(row) * r + j) = *reinterpret_cast<const uint2*>(o);
     }
   }
   if (parts > 1) cluster_sync_all();  // no CTA leaves while another reads its sums
@@ -435,8 +429,8 @@ struct ExpandCfg {
 template <typename T, bool kT, int RP>
 __global__ void __launch_bounds__(kThreads, 2)
     expand_kernel(const T* s, int64_t part_stride, const T* w, int64_t sl, int64_t sr,
-                  Scale scale, const int32_t* perm, const int32_t* offs, const int32_t* place,
-                  const int32_t* left, int tiles, int splits, int L, int N, int r, T* y, int64_t ldy) {
+                  Scale scale, const int32_t* perm, const int32_t* offs, const int32_t* taken,
+                  const TileAdapters* tile, int tiles, int splits, int L, int N, int r, T* y, int64_t ldy) {
   using C = ExpandCfg<kT, RP>;
   extern __shared__ __align__(128) char smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, q4 = lane & 3;
@@ -444,7 +438,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   let_next_kernel_start();
   // Usually the shared product has taken every row.
   bool any = false;
-  for (int q = tid; q < tiles; q += kThreads) any |= left[q] != 0;
+  for (int q = tid; q < tiles; q += kThreads) any |= tile[q].left != 0;
   if (!__syncthreads_or(any)) return;
   const int mg = warp & 3, half = warp >> 2;
   for (int unit = blockIdx.x;; unit += gridDim.x) {
@@ -455,7 +449,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     const int m = mg * 16 + g8 + 8 * u, row = m < t.rows ? perm[t.p0 + m] : -1;
-    yrow[u] = row >= 0 && place[row] < 0 ? y + row * ldy + half * 64 + q4 * 8 : nullptr;
+    yrow[u] = row >= 0 && !taken[row] ? y + row * ldy + half * 64 + q4 * 8 : nullptr;
   }
   if (!__syncthreads_or(yrow[0] != nullptr || yrow[1] != nullptr)) continue;
   const T* wi = w + t.i * sl;
@@ -815,9 +809,9 @@ inline int cluster_parts(int64_t blocks, int64_t most, int64_t length, int64_t l
 }
 
 // s = x w^T by adapter, w in rows of k (transposed: in rows of the rank); scale s also
-// into the blocks of the shared product's row tiles.
+// by row, for the shared product.
 int shrink(const void* x, int64_t ldx, Weights w, bool transposed, Scale scale, const PlanView& plan, int dtype,
-           int64_t m, int64_t k, int adapters, int rank, void* s, void* blocks, cudaStream_t stream) {
+           int64_t m, int64_t k, int adapters, int rank, void* s, void* rows, cudaStream_t stream) {
   return dispatch(dtype, transposed, rank, [&](auto t, auto tr, auto rp) {
     using T = decltype(t);
     constexpr bool kT = decltype(tr)::value;
@@ -830,8 +824,8 @@ int shrink(const void* x, int64_t ldx, Weights w, bool transposed, Scale scale, 
     return launch<&shrink_kernel<T, kT, RP>>(dim3(tiles, parts), dim3(1, parts),
                   ShrinkCfg<kT, RP>::kBytes, stream, static_cast<const T*>(x), ldx,
                   static_cast<const T*>(w.p), w.stride_l, w.stride_row, plan.perm, plan.offs, adapters,
-                  static_cast<int>(k), rank, m * rank, static_cast<T*>(s), scale, plan.place,
-                  static_cast<T*>(blocks));
+                  static_cast<int>(k), rank, m * rank, static_cast<T*>(s), scale, plan.taken,
+                  static_cast<T*>(rows));
   });
 }
 
@@ -851,7 +845,7 @@ int expand(const void* s, Weights w, bool transposed, Scale scale, const PlanVie
     return launch<&expand_kernel<T, kT, RP>>(dim3(static_cast<unsigned>(units < places ? units : places)),
                   dim3(1, 1), ExpandCfg<kT, RP>::kBytes, stream, static_cast<const T*>(s),
                   m * rank, static_cast<const T*>(w.p), w.stride_l, w.stride_row, scale, plan.perm,
-                  plan.offs, plan.place, plan.left, static_cast<int>(PlanView::tiles(m)), splits, adapters,
+                  plan.offs, plan.taken, plan.tile, static_cast<int>(PlanView::tiles(m)), splits, adapters,
                   static_cast<int>(n), rank, static_cast<T*>(y), ldy);
   });
 }
@@ -901,39 +895,35 @@ bool weights_ok(lora::Weights w, int64_t rows, int64_t width, int32_t adapters) 
          (adapters == 1 || (w.stride_l % 8 == 0 && w.stride_l >= (rows - 1) * w.stride_row + width));
 }
 // y = x w^T, w(k, n) at the given strides, with the adapters' second product of the rows
-// that have a place.
+// that it takes.
 int shared_product(const void* x, int64_t ldx, const void* w, int64_t stride_k, int64_t stride_n, void* y,
-                   int64_t ldy, const lora::PlanView& plan, lora::Weights second, const void* blocks,
+                   int64_t ldy, const lora::PlanView& plan, lora::Weights second, const void* rows,
                    int64_t m, int64_t k, int64_t n, int adapters, int rank, int dtype, int32_t* queue,
                    int32_t* status, cudaStream_t stream) {
   int dev;
   DeviceInfo info;
   const int rc = current_device_info(&dev, &info);
   if (rc != MOE_OK) return rc;
-  const gg::Adapters extra{blocks,   plan.count,      plan.list,         reinterpret_cast<const uint4*>(plan.mine),
-                           second.p, second.stride_l, second.stride_row, rank,
-                           adapters};
+  const gg::Adapters extra{rows, plan.tile, second.p, second.stride_l, second.stride_row, rank, adapters};
   return gg::grouped_gemm_launch(x, ldx, w, 0, stride_k, stride_n, y, ldy, plan.base, 0, m, k, n, 1, dtype,
                                  MOE_ACT_NONE, info.sm_count, queue != nullptr, queue, nullptr, nullptr, nullptr, 0, status,
                                  stream, nullptr, nullptr, force_single_sm_kernel() ? nullptr : &extra);
 }
 // Adapters that the shared product takes in a tile of rows; none on the 1-SM kernel.
-int per_tile() { return force_single_sm_kernel() ? 0 : gg::Adapters::kPerTile; }
+int per_tile(int rank) { return force_single_sm_kernel() ? 0 : gg::Adapters::most(rank); }
 int64_t low_bytes(int64_t m, int32_t rank) { return 4 * m * rank; }
-// The caller's buffer: x A^T by adapter and dy B by adapter (two parts each), the row
-// tiles' blocks, the plan.
+// The caller's buffer: x A^T by adapter and dy B by adapter (two parts each), the shared
+// product's operand by row, the plan.
 struct Buffers {
-  char *s, *t, *blocks, *plan;
+  char *s, *t, *rows, *plan;
   int64_t bytes;
   Buffers(void* kept, int64_t m, int32_t adapters, int32_t rank) {
     const int64_t low = low_bytes(m, rank);
-    const int64_t in_blocks =
-        lora::PlanView::tiles(m) * gg::Adapters::kPerTile * lora::kTileRows * int64_t(rank) * 2;
     s = static_cast<char*>(kept);
     t = s + low;
-    blocks = t + low;
-    plan = blocks + in_blocks;
-    bytes = 2 * low + in_blocks + 4 * lora::PlanView::ints(m, adapters);
+    rows = t + low;
+    plan = rows + low / 2;
+    bytes = 2 * low + low / 2 + 4 * lora::PlanView::ints(m, adapters);
   }
 };
 }  // namespace
@@ -964,14 +954,14 @@ extern "C" int32_t moe_lora_forward(const void* x, int64_t ldx, const void* weig
   const Buffers buf(kept, m, adapters, rank);
   const lora::PlanView plan(buf.plan, m, adapters);
   lora::plan_kernel<<<static_cast<unsigned>(adapters + lora::PlanView::tiles(m)), 1024, 0, st>>>(
-      ids, ids_int64, static_cast<int>(m), adapters, plan, per_tile(), status);
+      ids, ids_int64, static_cast<int>(m), adapters, plan, per_tile(rank), status);
   if (cudaGetLastError() != cudaSuccess) return MOE_ERR_CUDA;
   if (m == 0) return MOE_OK;
-  int rc = lora::shrink(x, ldx, a, false, sc, plan, dtype, m, k, adapters, rank, buf.s, buf.blocks, st);
+  int rc = lora::shrink(x, ldx, a, false, sc, plan, dtype, m, k, adapters, rank, buf.s, buf.rows, st);
   if (rc == MOE_OK)
-    rc = shared_product(x, ldx, weight, 1, ldw, y, ldy, plan, b, buf.blocks, m, k, n, adapters, rank, dtype, plan.queue,
+    rc = shared_product(x, ldx, weight, 1, ldw, y, ldy, plan, b, buf.rows, m, k, n, adapters, rank, dtype, plan.queue,
                         status, st);
-  if (rc == MOE_OK && adapters > per_tile())
+  if (rc == MOE_OK && adapters > per_tile(rank))
     rc = lora::expand(buf.s, b, false, sc, plan, dtype, m, n, adapters, rank, y, ldy, st);
   return rc;
 }
@@ -995,11 +985,11 @@ extern "C" int32_t moe_lora_backward(const void* dy, int64_t lddy, const void* x
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   int rc = MOE_OK;
   if (m > 0 && (dx != nullptr || da != nullptr))
-    rc = lora::shrink(dy, lddy, b, true, sc, plan, dtype, m, n, adapters, rank, buf.t, buf.blocks, st);
+    rc = lora::shrink(dy, lddy, b, true, sc, plan, dtype, m, n, adapters, rank, buf.t, buf.rows, st);
   if (rc == MOE_OK && m > 0 && dx != nullptr) {
-    rc = shared_product(dy, lddy, weight, ldw, 1, dx, lddx, plan, a, buf.blocks, m, n, k, adapters, rank, dtype,
+    rc = shared_product(dy, lddy, weight, ldw, 1, dx, lddx, plan, a, buf.rows, m, n, k, adapters, rank, dtype,
                         da != nullptr || db != nullptr ? plan.queue + 1 : nullptr, status, st);
-    if (rc == MOE_OK && adapters > per_tile())
+    if (rc == MOE_OK && adapters > per_tile(rank))
       rc = lora::expand(buf.t, a, true, sc, plan, dtype, m, k, adapters, rank, dx, lddx, st);
   }
   if (rc == MOE_OK && (da != nullptr || db != nullptr))

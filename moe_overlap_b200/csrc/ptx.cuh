@@ -246,6 +246,14 @@ __device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const void* tmap,
       : "memory");
 }
 
+// `bytes` (a multiple of 16) from global memory into this CTA's shared memory, both on 16
+// bytes, counted on an mbarrier of this CTA.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(bar)
+               : "memory");
+}
+
 // ---- TMA stores (shared::cta -> global, bulk async-group completion) -------
 __device__ __forceinline__ void tma_store_2d(const void* tmap, uint32_t src, int c0, int c1) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
@@ -338,6 +346,13 @@ __device__ __forceinline__ uint64_t smem_desc_sw128(uint32_t saddr, uint32_t lbo
   d |= 1ull << 46;
   d |= 2ull << 61;
   return d;
+}
+
+// A K-major operand in rows of 32, 64 or 128 bytes with the swizzle of that width (modes 6, 4
+// and 2), 8 rows an atom.
+__device__ __forceinline__ uint64_t smem_desc_rows(uint32_t saddr, uint32_t row_bytes) {
+  const uint64_t mode = row_bytes == 32 ? 6 : row_bytes == 64 ? 4 : 2;
+  return (smem_desc_sw128(saddr, 16, 8 * row_bytes) & ~(7ull << 61)) | (mode << 61);
 }
 
 // Instruction descriptor for kind::f16 with an fp32 accumulator.
