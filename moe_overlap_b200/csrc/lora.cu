@@ -233,7 +233,8 @@ __device__ __forceinline__ Tile find_tile(const int32_t* offs, int L, int tile, 
 }
 
 // shrink.  A CTA forms 128 rows x RP of s over one part of k: 4 warps of 32 rows (each
-// reads all of w's tile from shared memory) for each half of a stage's columns; the CTAs of a cluster
+// reads all of w's tile from shared memory) for each half of a stage's columns (of the rank,
+// if it is 128: all of it would be 128 sums a lane); the CTAs of a cluster
 // share the rows and add their parts through distributed shared memory, in order.
 // Bound by reading x once (and w once a block of 128 rows); measured 28 us for 16384 rows
 // of 2048 (67 MB, rank 64) and 80 us for 16384 of 8192 (268 MB, 3.4 TB/s): the gathers'
@@ -322,16 +323,18 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
     copies_commit();
   };
-  float acc[2][RP / 8][4];
+  constexpr bool kByRank = RP == 128;
+  constexpr int kRanks = kByRank ? RP / 2 : RP, kDeep = kByRank ? kShrinkCols : kShrinkCols / 2;
+  float acc[2][kRanks / 8][4];
 #pragma unroll
   for (int m = 0; m < 2; ++m)
 #pragma unroll
-    for (int n = 0; n < RP / 8; ++n)
+    for (int n = 0; n < kRanks / 8; ++n)
 #pragma unroll
       for (int q = 0; q < 4; ++q) acc[m][n][q] = 0.0f;
 #pragma unroll
   for (int q = 0; q < C::kStages - 1; ++q) fetch();
-  const int mg = warp & 3, kg = warp >> 2;
+  const int mg = warp & 3, kg = warp >> 2, n_first = kByRank ? kg * kRanks : 0;
   const bool busy = mg * 32 < t.rows;  // a warp without rows only copies
   for (int step = 0, stage = 0; step < steps; ++step, stage = stage + 1 == C::kStages ? 0 : stage + 1) {
     copies_wait<C::kStages - 2>();
@@ -341,20 +344,20 @@ __global__ void __launch_bounds__(kThreads, 2)
     const uint32_t ws = xs + kShrinkRows * kShrinkPitch;
     if (!busy) continue;
 #pragma unroll
-    for (int q = 0; q < kShrinkCols / 2; q += 16) {
-      const int kk = kg * (kShrinkCols / 2) + q;
+    for (int q = 0; q < kDeep; q += 16) {
+      const int kk = kByRank ? q : kg * kDeep + q;
       uint32_t a[2][4];
 #pragma unroll
       for (int m = 0; m < 2; ++m)
         ldmatrix_x4<false>(a[m], xs + (mg * 32 + m * 16 + (lane & 15)) * kShrinkPitch +
                                      (kk + (lane >> 4) * 8) * 2);
 #pragma unroll
-      for (int n = 0; n < RP / 8; n += 2) {
+      for (int n = 0; n < kRanks / 8; n += 2) {
         uint32_t b[4];
         if constexpr (kT)
-          ldmatrix_x4<true>(b, ws + (kk + (lane & 15)) * (RP * 2 + 16) + (n + (lane >> 4)) * 16);
+          ldmatrix_x4<true>(b, ws + (kk + (lane & 15)) * (RP * 2 + 16) + (n_first / 8 + n + (lane >> 4)) * 16);
         else
-          ldmatrix_x4<false>(b, ws + (n * 8 + (lane >> 4) * 8 + (lane & 7)) * kShrinkPitch +
+          ldmatrix_x4<false>(b, ws + (n_first + n * 8 + (lane >> 4) * 8 + (lane & 7)) * kShrinkPitch +
                                     (kk + ((lane >> 3) & 1) * 8) * 2);
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
@@ -369,21 +372,21 @@ __global__ void __launch_bounds__(kThreads, 2)
   constexpr int kPitch = RP + 4;
   float* sums = reinterpret_cast<float*>(smem);
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {  // the second half's warps add to the first's
-    if (kg == half)
+  for (int half = 0; half < (kByRank ? 1 : 2); ++half) {  // the second half's warps add to the first's
+    if (kByRank || kg == half)
 #pragma unroll
       for (int m = 0; m < 2; ++m)
 #pragma unroll
-        for (int n = 0; n < RP / 8; ++n)
+        for (int n = 0; n < kRanks / 8; ++n)
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
             float2* at = reinterpret_cast<float2*>(sums + (mg * 32 + m * 16 + (lane >> 2) + 8 * q) * kPitch +
-                                                   n * 8 + (lane & 3) * 2);
+                                                   n_first + n * 8 + (lane & 3) * 2);
             float2 v = make_float2(acc[m][n][2 * q], acc[m][n][2 * q + 1]);
             if (half == 1) v.x += at->x, v.y += at->y;
             *at = v;
           }
-    if (half == 0) __syncthreads();
+    if (!kByRank && half == 0) __syncthreads();
   }
   if (parts > 1)
     cluster_sync_all();
