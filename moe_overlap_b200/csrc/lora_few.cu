@@ -349,18 +349,21 @@ int forward(const void* x, int64_t ldx, const void* weight, int64_t ldw, Weights
 }  // namespace few
 
 bool takes_few_rows(int64_t m, int64_t k, int64_t n, int rank) {
-  // What the adapters' rows cost each block of W: with many of high rank the tensor-core
-  // path is faster (64 rows of 2048 x 8192 at rank 64: 52 us here and 45 there; at rank 16,
-  // 22 and 40).
+  // The rows of x and the adapters' products cost each block of W; the tensor-core path is
+  // faster from about here on.  Measured, here and there, 8 adapters: 2048 x 2048, 48 rows of
+  // rank 64 18.5 and 22.6 us, 64 rows 22.6 and 22.6; 512 x 1024, 32 rows of rank 128 16.5
+  // and 26.4; 8192 x 1024, 48 rows of rank 16 22.6 and 24.7, 64 rows 27.0 and 24.7.
   const bool wide = n >= few::kWide;
   const int64_t rows = m < 64 ? m : 64;
-  if (rows * rank > (wide ? 2048 : 4096)) return false;
+  if (rows * (k + 96 * rank) >= (int64_t(1) << 19)) return false;
+  // Wide weights have that epilogue on every SM.
+  if (wide && rows * rank > 2048) return false;
   if (m <= 64) return true;
-  // Further tiles of 64 rows read the weight again, from L2: worth it for up to two blocks an
-  // SM, one at rank 64 (128 rows of 2048 x 2048 at rank 16: 14 us, 33 there; 192 rows at
-  // rank 64, 45 and 36), while x A^T, by the CUDA cores, stays small.
+  // Further tiles of 64 rows read the weight again, from L2: worth it for one block an SM
+  // (2048 x 2048 at rank 16, 128 rows: 12.7 and 22.0 us, 192 rows: 20.6 and 19.3), while
+  // x A^T, by the CUDA cores, stays small.
   const int64_t blocks = (m + 63) / 64 * ((n + (wide ? 63 : 31)) / (wide ? 64 : 32));
-  return blocks <= 2 * 148 && blocks * rank <= 2 * 148 * 32 && m * rank * k <= (int64_t(1) << 25);
+  return blocks <= 148 && m * rank * k <= (int64_t(1) << 25);
 }
 
 int forward_few_rows(const void* x, int64_t ldx, const void* weight, int64_t ldw, Weights a, Weights b,
