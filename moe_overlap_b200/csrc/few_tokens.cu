@@ -177,7 +177,7 @@ __global__ void __cluster_dims__(kGateCluster, 1, 1) __launch_bounds__(32 * kWar
 //
 // Bound by reading the weights of the experts taken.  Gate and experts together, measured:
 // 16 tokens, 16 experts of 2048 x 8192, top-2: 141 us, 6.7 TB/s; 64 tokens of the same
-// 173 us, 6.2 TB/s; one token of 2048 x 4096: 28.6 us, of which some 15 read weights and
+// 173-185 us, 5.8-6.2 TB/s; one token of 2048 x 4096: 28.6 us, of which some 15 read weights and
 // the rest is the chain from the gate to the last sum.
 constexpr int kConsumers = 8;
 constexpr int kSets = 2;         // of consumers, on items in turn
@@ -501,17 +501,18 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     const int pos0 = grp[it.g] & 0xffff;
     const int rows = (it.g + 1 < G ? (grp[it.g + 1] & 0xffff) : S) - pos0;
-    float acc[J][4];
+    // Two sums of every output, so that no product waits for the one before it (a stage's
+    // products are a chain of latencies otherwise); added at the end.
+    float acc[J][4], acc2[J][4];
 #pragma unroll
     for (int j = 0; j < J; ++j)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[j][i] = 0.0f;
+      for (int i = 0; i < 4; ++i) acc[j][i] = acc2[j][i] = 0.0f;
 
-    for (int c = it.c0; c < it.c1; c += BKS) {
-      if (!mbar_wait(smem_u32(&ctrl->full[stage]), phase, nullptr)) {
-        record_status(p.status, MOE_ERR_TIMEOUT);
-        return;
-      }
+    // A stage with NJ tiles of 8 slots (what is in slots behind the group's stays in their
+    // sums, which nobody reads), of x or of both parts of h.
+    auto multiply = [&](auto nj, auto parts) {
+      constexpr int NJ = decltype(nj)::value, P = decltype(parts)::value;
       uint32_t a[2][8];  // rows g8 and g8 + 8, 16 columns each
       const uint32_t sa = a_base + stage * kStageBytes;
       ld_shared_v4(sa + off0, &a[0][0]);
@@ -519,25 +520,34 @@ __global__ void __launch_bounds__(kThreads, 1)
       ld_shared_v4(sa + 1024 + off0, &a[1][0]);
       ld_shared_v4(sa + 1024 + off1, &a[1][4]);
 #pragma unroll
-      for (int j = 0; j < J; ++j) {
-        if (j * 8 < rows) {
-          const uint32_t sb = b_base + stage * 2 * K::kSlotBytes + j * 1024;
-          uint32_t b[8];
-          ld_shared_v4(sb + off0, &b[0]);
-          ld_shared_v4(sb + off1, &b[4]);
+      for (int part = 0; part < P; ++part) {
+        uint32_t v[NJ][8];
 #pragma unroll
-          for (int s = 0; s < 4; ++s)
-            mma<T>(acc[j], a[0][2 * s], a[1][2 * s], a[0][2 * s + 1], a[1][2 * s + 1], b[2 * s],
-                   b[2 * s + 1]);
-          if (it.down) {
-            ld_shared_v4(sb + K::kSlotBytes + off0, &b[0]);
-            ld_shared_v4(sb + K::kSlotBytes + off1, &b[4]);
-#pragma unroll
-            for (int s = 0; s < 4; ++s)
-              mma<T>(acc[j], a[0][2 * s], a[1][2 * s], a[0][2 * s + 1], a[1][2 * s + 1], b[2 * s],
-                     b[2 * s + 1]);
-          }
+        for (int j = 0; j < NJ; ++j) {
+          const uint32_t sb = b_base + stage * 2 * K::kSlotBytes + part * K::kSlotBytes + j * 1024;
+          ld_shared_v4(sb + off0, &v[j][0]);
+          ld_shared_v4(sb + off1, &v[j][4]);
         }
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+          for (int j = 0; j < NJ; ++j)
+            mma<T>(s & 1 ? acc2[j] : acc[j], a[0][2 * s], a[1][2 * s], a[0][2 * s + 1], a[1][2 * s + 1],
+                   v[j][2 * s], v[j][2 * s + 1]);
+      }
+    };
+    for (int c = it.c0; c < it.c1; c += BKS) {
+      if (!mbar_wait(smem_u32(&ctrl->full[stage]), phase, nullptr)) {
+        record_status(p.status, MOE_ERR_TIMEOUT);
+        return;
+      }
+      using std::integral_constant;
+      if (J > 1 && rows > 8) {
+        it.down ? multiply(integral_constant<int, J>(), integral_constant<int, 2>())
+                : multiply(integral_constant<int, J>(), integral_constant<int, 1>());
+      } else {
+        it.down ? multiply(integral_constant<int, 1>(), integral_constant<int, 2>())
+                : multiply(integral_constant<int, 1>(), integral_constant<int, 1>());
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&ctrl->empty[stage]));
@@ -545,6 +555,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 
     if (lane == 0) mbar_arrive(smem_u32(&ctrl->turn[set ^ 1]));
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[j][i] += acc2[j][i];
 
     if (!it.down) {
       auto put_h = [&](int nn, int row, float v) {
@@ -724,16 +738,16 @@ int launch(Params p, const void* rw, int64_t ldr, const float* bias, const void*
   };
   using std::integral_constant;
   // Blocks of 128 rows need no sums across warps and fetch each slot's columns once for
-  // all 8 warps; a few tokens' few experts make too few of them for every SM and get
-  // blocks of 32 rows (one token of 16 experts of 2048 x 4096: 28.6 us with 32 rows,
-  // 33.5 with 128; 37 tokens of 64 experts of 2048 x 1024, 174 and 98 us).
+  // all 8 warps; a few slots' few experts make too few of them for every SM and get blocks
+  // of 32 rows.  Measured with 32 and 128 rows, experts x hidden x ffn: one token's 2 slots
+  // of 16 x 2048 x 4096 28.6 and 32.8 us; 8 tokens' 16 of 8 x 512 x 1024 18.7 and 20.5; 16
+  // tokens' 32 of 8 x 4096 x 1024 49.6 and 44.0; 128 tokens' 256 of it 168 and 76.
   const int64_t S = int64_t(p.T) * p.k, groups = S < p.E ? S : p.E;
-  const bool narrow = groups * ((p.F + 127) / 128) < sms;
-  if (p.T <= 8)  // no expert has more than 8 slots, unless it is repeated
-    return narrow ? go(integral_constant<int, 2>(), integral_constant<int, 1>())
-                  : go(integral_constant<int, 8>(), integral_constant<int, 1>());
-  return narrow ? go(integral_constant<int, 2>(), integral_constant<int, 2>())
-                : go(integral_constant<int, 8>(), integral_constant<int, 2>());
+  const bool narrow = S <= 16 && groups * ((p.F + 127) / 128) < sms;
+  if (p.T > 8) return go(integral_constant<int, 8>(), integral_constant<int, 2>());
+  // No expert has more than 8 slots, unless it is repeated.
+  return narrow ? go(integral_constant<int, 2>(), integral_constant<int, 1>())
+                : go(integral_constant<int, 8>(), integral_constant<int, 1>());
 }
 
 }  // namespace few
