@@ -53,7 +53,8 @@ static_assert(sizeof(TileAdapters) % 16 == 0 && offsetof(TileAdapters, count) % 
 struct Adapters {
   // Columns of the rank that one box takes; adapters of 16 or 32 share a stage.
   static constexpr int width(int rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : 64; }
-  // Adapters of a tile that the product takes.
+  // Adapters of a tile that the product takes: with more, adding their products to C
+  // afterwards is about as fast (8192 x 2048 x 8192, 16 of rank 32: 297 us here, 316 there).
   static constexpr int most(int rank) { return rank <= 32 ? TileAdapters::kMost : 8; }
   const void* rows;      // [m][rank], the inputs' type
   const TileAdapters* tiles;

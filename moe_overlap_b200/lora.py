@@ -33,7 +33,7 @@ def lora_linear(x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor, lor
     that type, with its scale, as the shared product's operand, and held in two parts
     of it for the gradients.  The shared weight is frozen.  Sizes that are not multiples
     of 8, and rows that do not start on 16 bytes, are copied with padding on every call.
-    The graph keeps about 24 r bytes a row beside its inputs.
+    The graph keeps about 10 r bytes a row beside its inputs.
 
     A training step can be captured into a CUDA graph (forward and backward together);
     as for every autograd graph, no graph of the same leaves from before the capture

@@ -480,6 +480,24 @@ def test_few_tiles_of_long_contractions(cuda_device, M, K, N, L, r, dtype, runs)
         assert torch.equal(one, two)  # sums in a fixed order
 
 
+@pytest.mark.parametrize("M,K,N,L,r,dtype", [
+    (600, 264, 520, 14, 32, torch.bfloat16), (600, 136, 264, 16, 8, torch.float16),
+    (513, 200, 72, 12, 16, torch.bfloat16), (700, 320, 264, 8, 24, torch.float16),
+    (300, 1040, 1032, 16, 32, torch.bfloat16), (260, 72, 1000, 17, 32, torch.float16),
+    (400, 72, 264, 8, 72, torch.bfloat16), (400, 72, 264, 9, 40, torch.bfloat16)])
+def test_stages_shared_by_adapters(cuda_device, M, K, N, L, r, dtype):
+    """Every adapter in every tile of rows: as many as the shared product takes, and one more."""
+    x, w, a, b, dy, scale, _ = make(M, K, N, L, r, dtype, seed=L * r, device=cuda_device)
+    ids = (torch.arange(M) % (L + 1) - 1).to(cuda_device)
+    for t in (x, a, b):
+        t.requires_grad_(True)
+    y = mo.lora_linear(x, w, a, b, ids, scale=scale)
+    grads = torch.autograd.grad(y, (x, a, b), dy)
+    mo.check_status(cuda_device, sync=True)
+    for got, want in zip((y, *grads), reference(x, w, a, b, dy, scale, ids)):
+        assert_close(got, want)
+
+
 @pytest.mark.parametrize("M,K,N", [(300, 1040, 264), (300, 264, 1040), (900, 1032, 1032)])
 def test_infinities_with_split_contractions(cuda_device, M, K, N):
     x, w, a, b, dy, scale, ids = make(M, K, N, 5, 16, torch.bfloat16, seed=M, device=cuda_device)
