@@ -165,11 +165,13 @@ __global__ void __cluster_dims__(kGateCluster, 1, 1) __launch_bounds__(32 * kWar
 //
 // Warp 0 fetches weights: TMA boxes of BM rows x 64 columns into a ring of stages of
 // 16 KB.  The weights do not depend on h, so the ring runs ahead into W2 while h is
-// still being finished.  Warp 1 copies the slots' columns of the same stage beside
-// them (rows of x picked by token, or rows of h).  Two sets of 8 warps multiply, on
-// items in turn, so that one set's sums, stores and fences (several microseconds'
-// worth of latency an item) pass under the other's products: a stage is R tiles of 16 rows x C = 8/R slices of 64 columns, one (tile, slice) per warp,
-// m16n8k16 with the weights as the 16-row side and the slots as the 8-column side.
+// still being finished.  Up to four warps copy the slots' columns of the same stage beside
+// them (rows of x picked by token, or rows of h; one warp's instructions bound
+// many slots: 215 us of 46 tokens' top-8 of 9 x 1712 x 6320, 200 by four).  Two sets of 8 warps
+// multiply, on items in turn, so that one set's sums, stores and fences (several
+// microseconds' worth of latency an item) pass under the other's products, or (SHARE) on
+// half of an item's slots each: a stage is R tiles of 16 rows x C = 8/R slices of 64
+// columns, one (tile, slice) per warp of a set, m16n8k16 with the weights as the 16-row side and the slots as the 8-column side.
 // (tcgen05's 128-row tiles would leave too few items for 148 SMs at one token, and
 // the tensor work here is a few percent of the time either way.)  The order of k
 // inside a slice is free, so lane (g, q) takes the 16 contiguous columns 16q.. of its
@@ -180,8 +182,11 @@ __global__ void __cluster_dims__(kGateCluster, 1, 1) __launch_bounds__(32 * kWar
 // 173-185 us, 5.8-6.2 TB/s; one token of 2048 x 4096: 28.6 us, of which some 15 read weights and
 // the rest is the chain from the gate to the last sum.
 constexpr int kConsumers = 8;
-constexpr int kSets = 2;         // of consumers, on items in turn
-constexpr int kThreads = 32 * (2 + kSets * kConsumers);
+constexpr int kSets = 2;         // of consumers
+// Warps that copy slots: more than their rows need only add arrivals to every stage (16
+// tokens, top-2 of 16 x 1024 x 2048: 43 us with one, 46 with four).
+constexpr int copy_warps(int J, bool share) { return share ? 4 : J == 1 ? 1 : 2; }
+constexpr int threads(int J, bool share) { return 32 * (1 + copy_warps(J, share) + kSets * kConsumers); }
 constexpr int kStageBytes = 16 * 1024;
 constexpr int kRedStride = 20;  // floats between slots in the reduction buffer: no bank conflicts
 constexpr int kMaxSlots = kMaxTokens * kMaxK;
@@ -234,15 +239,15 @@ __device__ __forceinline__ void set_sync(int set) {
 
 // The slots by expert and the groups of at most NT of them: grp holds
 // expert << 16 | place of the group's first slot.
-__device__ __forceinline__ void build_plan(const Params& p, int NT, Plan* pl, int* grp, int* cnt,
+__device__ __forceinline__ void build_plan(const Params& p, int NT, int block, Plan* pl, int* grp, int* cnt,
                                            int* grp_first) {
   const int tid = threadIdx.x, S = p.T * p.k;
-  for (int i = tid; i < S; i += kThreads) {
+  for (int i = tid; i < S; i += block) {
     const int64_t e = p.idx[i];
     if (e < -1 || e >= p.E) record_status(p.status, MOE_ERR_INVALID_ARG);
     pl->expert_of_slot[i] = (e >= 0 && e < p.E) ? static_cast<int16_t>(e) : int16_t(-1);
   }
-  for (int e = tid; e < p.E; e += kThreads) cnt[e] = 0;
+  for (int e = tid; e < p.E; e += block) cnt[e] = 0;
   __syncthreads();
   if (tid < 32) {
     // Each slot's rank among its expert's, 32 slots at a time in slot order.
@@ -281,7 +286,7 @@ __device__ __forceinline__ void build_plan(const Params& p, int NT, Plan* pl, in
     }
   }
   __syncthreads();
-  for (int i = tid; i < S; i += kThreads) {
+  for (int i = tid; i < S; i += block) {
     const int e = pl->expert_of_slot[i], rank = pl->pos_of[i];
     if (e < 0) {
       pl->pos_of[i] = 0xffff;
@@ -301,13 +306,18 @@ struct Item {
   int g, blk, ks, c0, c1;  // group, row block, part of ffn, its columns [c0, c1)
 };
 
-template <typename T, int R, int J>
-__global__ void __launch_bounds__(kThreads, 1)
+template <typename T, int R, int J, bool SHARE>
+__global__ void __launch_bounds__(threads(J, SHARE), 1)
     experts_kernel(const __grid_constant__ CUtensorMap map1, const __grid_constant__ CUtensorMap map2,
                    const __grid_constant__ Params p) {
   using K = Cfg<R, J>;
   constexpr int BM = K::BM, C = K::C, BKS = K::BKS, NT = K::NT, kStages = K::kStages;
   constexpr int kSliceBytes = BM * 128;
+  static_assert(!SHARE || (C == 1 && J % kSets == 0), "whole tiles of 8 slots a set");
+  constexpr int kCopyWarps = copy_warps(J, SHARE), kFirstConsumer = 1 + kCopyWarps;
+  constexpr int kThreads = threads(J, SHARE);
+  constexpr int JS = SHARE ? J / kSets : J;                         // tiles of 8 slots of a warp
+  constexpr int kWarpsOn = SHARE ? kSets * kConsumers : kConsumers;  // on an item
   extern __shared__ char smem_raw[];
   char* base = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   // Stages' weights, then their slots, then two reduction buffers.
@@ -321,13 +331,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     for (int s = 0; s < kStages; ++s) {
-      mbar_init(smem_u32(&ctrl->full[s]), 1 + 32);
-      mbar_init(smem_u32(&ctrl->empty[s]), kConsumers);
+      mbar_init(smem_u32(&ctrl->full[s]), 1 + 32 * kCopyWarps);
+      mbar_init(smem_u32(&ctrl->empty[s]), kWarpsOn);
     }
     for (int s = 0; s < kSets; ++s) mbar_init(smem_u32(&ctrl->turn[s]), kConsumers);
     for (int s = 0; s < kQueue; ++s) {
       mbar_init(smem_u32(&ctrl->qfull[s]), 1);
-      mbar_init(smem_u32(&ctrl->qempty[s]), 1 + kSets * kConsumers);
+      mbar_init(smem_u32(&ctrl->qempty[s]), kCopyWarps + kSets * kConsumers);
     }
     fence_mbar_init();
     tma_prefetch_desc(&map1);
@@ -336,7 +346,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   wait_for_previous_kernel();  // the gate's idx, w and counters
   int ticket = 0;  // the fetching thread's first, on its way while the plan is made
   if (tid == 0) ticket = atomicAdd(p.count, 1);
-  build_plan(p, NT, plan, grp, cnt, grp_first);
+  build_plan(p, NT, kThreads, plan, grp, cnt, grp_first);
   const int G = plan->n_groups, S = plan->n_slots;
   const int FB = (p.F + BM - 1) / BM, HB = (p.H + BM - 1) / BM;
   if (G == 0) {  // no slot is routed: zeros
@@ -416,15 +426,17 @@ __global__ void __launch_bounds__(kThreads, 1)
   const T* x = static_cast<const T*>(p.x);
   T* h = static_cast<T*>(p.h);
   T* h_lo = h + int64_t(p.T) * p.k * p.F;
-  if (warp == 1) {
+  if (warp < kFirstConsumer) {
     // A stage's slots: row nn of slice s at (s NT + nn) * 128, its 16-byte pieces
     // XOR-ed with nn & 7 like the weights' TMA swizzle.
     constexpr int kPieces = BKS / 8;              // of 16 bytes in a row
-    constexpr int kPasses = NT * kPieces / 32;
+    constexpr int kPasses = (NT * kPieces / 32 + kCopyWarps - 1) / kCopyWarps;
+    const int first = (warp - 1) * 32 + lane;     // its pieces: this one and every 32 kCopyWarps-th
+    constexpr int kNext = 32 * kCopyWarps;
     uint32_t off[kPasses];
 #pragma unroll
     for (int i = 0; i < kPasses; ++i) {
-      const int nn = (lane + 32 * i) / kPieces, piece = (lane + 32 * i) % kPieces;
+      const int nn = (first + kNext * i) / kPieces, piece = (first + kNext * i) % kPieces;
       off[i] = ((piece >> 3) * NT + nn) * 128 + (((piece & 7) ^ (nn & 7)) << 4);
     }
     const int piece8 = lane % kPieces * 8;  // (32 is a multiple of kPieces: the same in every pass)
@@ -438,7 +450,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int rows = (it.g + 1 < G ? (grp[it.g + 1] & 0xffff) : S) - pos0;
       if (it.down) {  // this group's h, complete and visible to this thread
         const long long t0 = clock64();
-        while (ld_acquire_gpu(ready + it.g) < FB * kConsumers)
+        while (ld_acquire_gpu(ready + it.g) < FB * kWarpsOn)
           if (clock64() - t0 > kWaitBudgetCycles) {
             record_status(p.status, MOE_ERR_TIMEOUT);
             break;  // carry on with what is there: the pipeline still ends
@@ -447,7 +459,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const T* src[kPasses];
 #pragma unroll
       for (int i = 0; i < kPasses; ++i) {
-        const int nn = (lane + 32 * i) / kPieces;
+        const int nn = (first + kNext * i) / kPieces;
         src[i] = nullptr;
         if (nn < rows)
           src[i] = (it.down ? h + int64_t(pos0 + nn) * p.F
@@ -465,7 +477,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int from = in ? c : it.c0;
 #pragma unroll
         for (int i = 0; i < kPasses; ++i) {
-          if (i * 32 / kPieces >= rows) break;
+          if (i * kNext / kPieces >= rows) break;
           if (src[i] != nullptr) {
             copy_async_16(dst + off[i], src[i] + from, in);
             if (it.down) copy_async_16(dst + off[i] + K::kSlotBytes, src[i] + from + (h_lo - h), in);
@@ -477,10 +489,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   }
 
-  const int set = (warp - 2) / kConsumers, cw = (warp - 2) % kConsumers;
+  const int set = (warp - kFirstConsumer) / kConsumers, cw = (warp - kFirstConsumer) % kConsumers;
   const int rt = cw % R, cs = cw / R, g8 = lane >> 2, q4 = lane & 3;
   const uint32_t a_base = smem_u32(base) + cs * kSliceBytes + (rt * 16 + g8) * 128;
-  const uint32_t b_base = smem_u32(slots) + (cs * NT + g8) * 128;
+  const int s0 = SHARE ? set * 8 * JS : 0;  // this set's first slot of a group
+  const uint32_t b_base = smem_u32(slots) + (cs * NT + s0 + g8) * 128;
   const uint32_t off0 = ((2 * q4) ^ g8) * 16, off1 = ((2 * q4 + 1) ^ g8) * 16;
   int stage = 0;
   uint32_t phase = 0;
@@ -488,14 +501,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int item = pop(n);
     if (item < 0) break;
     const Item it = decode(item);
-    if (n % kSets != set) {  // the other set's item: past its stages
+    if (!SHARE && n % kSets != set) {  // the other set's item: past its stages
       stage += (it.c1 - it.c0 + BKS - 1) / BKS;
       while (stage >= kStages) stage -= kStages, phase ^= 1;
       continue;
     }
     // The other set has used every stage before this item's: a parity wait on a stage
     // is only sound within one turn of the ring.
-    if (!mbar_wait(smem_u32(&ctrl->turn[set]), ((n / kSets) & 1) ^ (set == 0), nullptr)) {
+    if (!SHARE && !mbar_wait(smem_u32(&ctrl->turn[set]), ((n / kSets) & 1) ^ (set == 0), nullptr)) {
       record_status(p.status, MOE_ERR_TIMEOUT);
       return;
     }
@@ -503,9 +516,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int rows = (it.g + 1 < G ? (grp[it.g + 1] & 0xffff) : S) - pos0;
     // Two sums of every output, so that no product waits for the one before it (a stage's
     // products are a chain of latencies otherwise); added at the end.
-    float acc[J][4], acc2[J][4];
+    float acc[JS][4], acc2[JS][4];
 #pragma unroll
-    for (int j = 0; j < J; ++j)
+    for (int j = 0; j < JS; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[j][i] = acc2[j][i] = 0.0f;
 
@@ -542,10 +555,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         return;
       }
       using std::integral_constant;
-      if (J > 1 && rows > 8) {
-        it.down ? multiply(integral_constant<int, J>(), integral_constant<int, 2>())
-                : multiply(integral_constant<int, J>(), integral_constant<int, 1>());
-      } else {
+      if (JS > 1 && rows > s0 + 8) {
+        it.down ? multiply(integral_constant<int, JS>(), integral_constant<int, 2>())
+                : multiply(integral_constant<int, JS>(), integral_constant<int, 1>());
+      } else if (rows > s0) {
         it.down ? multiply(integral_constant<int, 1>(), integral_constant<int, 2>())
                 : multiply(integral_constant<int, 1>(), integral_constant<int, 1>());
       }
@@ -554,9 +567,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (++stage == kStages) stage = 0, phase ^= 1;
     }
 
-    if (lane == 0) mbar_arrive(smem_u32(&ctrl->turn[set ^ 1]));
+    if (!SHARE && lane == 0) mbar_arrive(smem_u32(&ctrl->turn[set ^ 1]));
 #pragma unroll
-    for (int j = 0; j < J; ++j)
+    for (int j = 0; j < JS; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[j][i] += acc2[j][i];
 
@@ -568,16 +581,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       if constexpr (C == 1) {
 #pragma unroll
-        for (int j = 0; j < J; ++j)
+        for (int j = 0; j < JS; ++j)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int nn = j * 8 + 2 * q4 + (i & 1), row = it.blk * BM + rt * 16 + g8 + 8 * (i >> 1);
+            const int nn = s0 + j * 8 + 2 * q4 + (i & 1), row = it.blk * BM + rt * 16 + g8 + 8 * (i >> 1);
             if (nn < rows && row < p.F) put_h(nn, row, acc[j][i]);
           }
       } else {  // the C column slices' sums, through shared memory
         float* rb = red + (set * kConsumers + cw) * (NT * kRedStride);
 #pragma unroll
-        for (int j = 0; j < J; ++j)
+        for (int j = 0; j < JS; ++j)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             rb[(j * 8 + 2 * q4 + (i & 1)) * kRedStride + g8 + 8 * (i >> 1)] = acc[j][i];
@@ -603,10 +616,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (row16 >= p.H) continue;
     float* part = p.part + (int64_t(it.ks * C + cs) * p.T * p.k + pos0) * p.H + row16;
 #pragma unroll
-    for (int j = 0; j < J; ++j)
+    for (int j = 0; j < JS; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int nn = j * 8 + 2 * q4 + (i & 1), m = g8 + 8 * (i >> 1);
+        const int nn = s0 + j * 8 + 2 * q4 + (i & 1), m = g8 + 8 * (i >> 1);
         if (nn < rows && row16 + m < p.H) part[int64_t(nn) * p.H + m] = acc[j][i];
       }
     __syncwarp();
@@ -619,11 +632,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int t_groups = (p.T + 7) / 8, units = (p.H + 15) / 16 * t_groups;
   const int parts = p.KS * C, terms = p.k * parts;
   const int64_t part_stride = int64_t(p.T) * p.k * p.H;
-  for (int u = (warp - 2) * gridDim.x + blockIdx.x; u < units; u += kSets * kConsumers * gridDim.x) {
+  for (int u = (warp - kFirstConsumer) * gridDim.x + blockIdx.x; u < units; u += kSets * kConsumers * gridDim.x) {
     const int blk16 = u / t_groups, t = u % t_groups * 8 + (lane >> 2);
     const int col = blk16 * 16 + (lane & 3) * 4;  // 4 columns of one token a lane (H: a multiple of 8)
     const long long t0 = clock64();
-    while (ld_acquire_gpu(done + blk16) < G * parts)
+    while (ld_acquire_gpu(done + blk16) < G * parts * (kWarpsOn / kConsumers))
       if (clock64() - t0 > kWaitBudgetCycles) {
         record_status(p.status, MOE_ERR_TIMEOUT);
         break;
@@ -675,7 +688,7 @@ struct Workspace {
   int64_t count_bytes() const { return total - count; }
 };
 
-template <typename T, int R, int J>
+template <typename T, int R, int J, bool SHARE>
 int launch_experts(const Params& p, const void* w1, int64_t w1_se, int64_t w1_sr, const void* w2,
                    int64_t w2_se, int64_t w2_sr, bool after_gate, int sms, cudaStream_t s) {
   using K = Cfg<R, J>;
@@ -695,14 +708,14 @@ int launch_experts(const Params& p, const void* w1, int64_t w1_se, int64_t w1_sr
   const int smem = kFixed + 4 * (max_groups(J, p.E) + 2 * p.E);
   constexpr int kMost = kFixed + 4 * (max_groups(J, kMaxE) + 2 * kMaxE);
   static_assert(K::kStages <= 12 && kMost <= 227 * 1024, "shared memory");
-  constexpr auto kern = &experts_kernel<T, R, J>;
+  constexpr auto kern = &experts_kernel<T, R, J, SHARE>;
   if (!allow_shared_memory<kern>(kMost)) return MOE_ERR_CUDA;
   // No more CTAs than there can be items: every slot in a group of its own.
   const int64_t most = int64_t(p.T) * p.k * ((p.F + K::BM - 1) / K::BM + (p.H + K::BM - 1) / K::BM * p.KS);
   const int grid = static_cast<int>(most < sms ? most : sms);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(threads(J, SHARE));
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute early{};  // set up beside the gate's kernel
@@ -732,8 +745,8 @@ int launch(Params p, const void* rw, int64_t ldr, const float* bias, const void*
   } else if (cudaMemsetAsync(p.count, 0, lay.count_bytes(), s) != cudaSuccess) {
     return MOE_ERR_CUDA;
   }
-  auto go = [&](auto r, auto j) {
-    return launch_experts<T, decltype(r)::value, decltype(j)::value>(p, w1, w1_se, w1_sr, w2, w2_se, w2_sr,
+  auto go = [&](auto r, auto j, auto share) {
+    return launch_experts<T, decltype(r)::value, decltype(j)::value, decltype(share)::value>(p, w1, w1_se, w1_sr, w2, w2_se, w2_sr,
                                                                      rw != nullptr, sms, s);
   };
   using std::integral_constant;
@@ -744,10 +757,17 @@ int launch(Params p, const void* rw, int64_t ldr, const float* bias, const void*
   // tokens' 32 of 8 x 4096 x 1024 49.6 and 44.0; 128 tokens' 256 of it 168 and 76.
   const int64_t S = int64_t(p.T) * p.k, groups = S < p.E ? S : p.E;
   const bool narrow = S <= 16 && groups * ((p.F + 127) / 128) < sms;
-  if (p.T > 8) return go(integral_constant<int, 8>(), integral_constant<int, 2>());
+  // With 16 slots or more an expert both sets of consumers take an item, 16 of its 32 slots
+  // each, so that the weights go by half as often; but no set's sums pass under the other's
+  // products then, which wants long items and enough of them.  128 tokens, top-2 of 8 x 2048 x
+  // 8192: 168 us, 199 with 16 slots an item; 62 tokens, top-6 of 12 x 600 x 7888 126 and 111;
+  // 32 tokens, top-2 of 2 x 2048 x 2048 45 and 37.
+  if (p.T > 8 && S >= 16 * int64_t(p.E) && p.H >= 1024 && groups * ((p.F + 127) / 128) >= sms / 2)
+    return go(integral_constant<int, 8>(), integral_constant<int, 4>(), std::true_type());
+  if (p.T > 8) return go(integral_constant<int, 8>(), integral_constant<int, 2>(), std::false_type());
   // No expert has more than 8 slots, unless it is repeated.
-  return narrow ? go(integral_constant<int, 2>(), integral_constant<int, 1>())
-                : go(integral_constant<int, 8>(), integral_constant<int, 1>());
+  return narrow ? go(integral_constant<int, 2>(), integral_constant<int, 1>(), std::false_type())
+                : go(integral_constant<int, 8>(), integral_constant<int, 1>(), std::false_type());
 }
 
 }  // namespace few

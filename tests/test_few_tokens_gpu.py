@@ -312,7 +312,9 @@ def test_refusals(cuda_device):
 @pytest.mark.parametrize("T,E,H,F,k,dtype", [
     (100, 3, 264, 520, 3, torch.bfloat16), (128, 5, 136, 328, 4, torch.float16),
     (17, 2, 1032, 72, 2, torch.bfloat16), (8, 4, 264, 136, 2, torch.float16),
-    (8, 4, 264, 136, 3, torch.bfloat16), (9, 40, 520, 264, 2, torch.bfloat16)])
+    (8, 4, 264, 136, 3, torch.bfloat16), (9, 40, 520, 264, 2, torch.bfloat16),
+    (100, 3, 1032, 3208, 3, torch.bfloat16), (128, 40, 1024, 264, 5, torch.float16),
+    (49, 9, 1080, 1096, 8, torch.bfloat16)])
 def test_many_slots_an_expert(cuda_device, T, E, H, F, k, dtype):
     """Several groups of slots an expert, the last one short, and both row blocks' limits."""
     test_moe_few_tokens_matches_64_bit_reference(cuda_device, T, E, H, F, k, True, True, dtype)
