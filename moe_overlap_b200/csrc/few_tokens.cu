@@ -179,7 +179,7 @@ __global__ void __cluster_dims__(kGateCluster, 1, 1) __launch_bounds__(32 * kWar
 //
 // Bound by reading the weights of the experts taken.  Gate and experts together, measured:
 // 16 tokens, 16 experts of 2048 x 8192, top-2: 141 us, 6.7 TB/s; 64 tokens of the same
-// 173-185 us, 5.8-6.2 TB/s; one token of 2048 x 4096: 28.6 us, of which some 15 read weights and
+// 173-178 us, 6.0-6.2 TB/s; one token of 2048 x 4096: 28.6 us, of which some 15 read weights and
 // the rest is the chain from the gate to the last sum.
 constexpr int kConsumers = 8;
 constexpr int kSets = 2;         // of consumers
