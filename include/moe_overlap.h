@@ -557,6 +557,14 @@ MOE_API int32_t moe_router_topk_backward(const float* probs, const int64_t* topk
  */
 MOE_API int64_t moe_few_tokens_workspace(int32_t num_tokens, int32_t hidden, int32_t ffn,
                                          int32_t num_experts, int32_t topk);
+/*
+ * How moe_few_tokens divides the down-projection's sum over ffn: the number of parts (-1:
+ * sizes out of bounds), each but the last of *part_cols columns.  narrow != 0: with row
+ * blocks of 32 (a few slots on few experts), else of 128.  The workspace holds the parts'
+ * sums.
+ */
+MOE_API int32_t moe_few_tokens_parts(int32_t num_tokens, int32_t ffn, int32_t num_experts, int32_t topk,
+                                     int32_t narrow, int32_t* part_cols);
 MOE_API int32_t moe_few_tokens(const void* x, int64_t ldx, const void* router_w, int64_t ldr,
                                const float* router_bias, const void* w1, int64_t w1_stride_e,
                                int64_t w1_stride_row, const void* w2, int64_t w2_stride_e,

@@ -188,6 +188,7 @@ SIGNATURES: dict[str, tuple] = {
          _c_void_p, _c_void_p],  # grad_logits, stream
     ),
     "moe_few_tokens_workspace": (_i64, [_i32, _i32, _i32, _i32, _i32]),
+    "moe_few_tokens_parts": (_i32, [_i32, _i32, _i32, _i32, _i32, ctypes.POINTER(_i32)]),  # T, F, E, k, narrow
     "moe_few_tokens": (
         _i32,
         [_c_void_p, _i64, _c_void_p, _i64, _c_void_p,  # x, ldx, router_w, ldr, router_bias

@@ -217,7 +217,7 @@ struct Params {
   float* part;     // [KS * C][slots][H]
   int32_t* count;  // ticket, then per group its finished W1 items, then per 16 rows of H its finished parts
   int32_t* status;
-  int T, H, F, E, k, KS;
+  int T, H, F, E, k, KS, part_cols;  // W2's items: KS parts of F, of part_cols columns (see parts_of)
 };
 
 struct Plan {  // in shared memory; every CTA derives the same one from idx
@@ -358,8 +358,6 @@ __global__ void __launch_bounds__(threads(J, SHARE), 1)
   const int up_items = G * FB, items = up_items + G * HB * p.KS;
   int* ready = p.count + 1;
   int* done = ready + G;
-  // columns of F that one part of a W2 item covers (a multiple of a stage's)
-  const int part_cols = ((p.F + p.KS - 1) / p.KS + BKS - 1) / BKS * BKS;
   auto decode = [&](int item) {
     Item it;
     it.down = item >= up_items;
@@ -368,8 +366,8 @@ __global__ void __launch_bounds__(threads(J, SHARE), 1)
     const int r = q - it.g * per;
     it.blk = it.down ? r / p.KS : r;
     it.ks = it.down ? r - it.blk * p.KS : 0;
-    it.c0 = it.ks * part_cols;
-    it.c1 = it.down ? min(it.c0 + part_cols, p.F) : p.H;
+    it.c0 = it.ks * p.part_cols;
+    it.c1 = it.down ? min(it.c0 + p.part_cols, p.F) : p.H;
     return it;
   };
   // Takes the queue's next item; -1 at the end (or when the wait ran out).
@@ -669,29 +667,45 @@ __global__ void __launch_bounds__(threads(J, SHARE), 1)
   }
 }
 
-// Parts of F in W2's items, of about 2048 columns, fewer when there are many slots (then
-// there are many groups, and the parts' sums cost more than their balance gains).
-inline int k_splits(int F, int64_t S) {
+// The parts of F in W2's items: about 2048 columns each, more when there are many slots (then
+// there are many groups, and the parts' sums cost more than their balance gains), in whole
+// stages of `stage` columns.  No part is empty: the consumers that skip an item count its
+// stages from its columns, so the number of parts follows from their rounded width.
+struct Parts {
+  int n, cols;
+};
+inline Parts parts_of(int F, int64_t S, int stage) {
   const int64_t fine = (F + 2047) / 2048, most = S < 1 || S >= 1024 ? 1 : 1024 / S;
-  return static_cast<int>(fine < most ? fine : most);
+  const int64_t n = fine < most ? fine : most;
+  const int64_t cols = ((F + n - 1) / n + stage - 1) / stage * stage;
+  return {static_cast<int>((F + cols - 1) / cols), static_cast<int>(cols)};
 }
+// Column slices of a stage, and its columns, with row blocks of 16 R.
+constexpr int slices(int R) { return kConsumers / R; }
+constexpr int stage_cols(int R) { return 64 * slices(R); }
+constexpr int kWideR = 8, kNarrowR = 2;  // what launch() chooses between
 
 struct Workspace {
   int64_t part, count, total;
   Workspace(int T, int H, int F, int E, int k) {
     const int64_t S = int64_t(T) * k;
     part = (S * F * 4 + 15) / 16 * 16;
-    // a variant with column slices splits each part into up to 4
-    count = part + (S * H * 4 * k_splits(F, S) * 4 + 15) / 16 * 16;
+    // Each part's slices have sums of their own.
+    const int wide = parts_of(F, S, stage_cols(kWideR)).n * slices(kWideR);
+    const int narrow = parts_of(F, S, stage_cols(kNarrowR)).n * slices(kNarrowR);
+    count = part + (S * H * 4 * (wide > narrow ? wide : narrow) + 15) / 16 * 16;
     total = count + 4 * (int64_t(1) + max_groups(1, E) + (H + 15) / 16);
   }
   int64_t count_bytes() const { return total - count; }
 };
 
 template <typename T, int R, int J, bool SHARE>
-int launch_experts(const Params& p, const void* w1, int64_t w1_se, int64_t w1_sr, const void* w2,
+int launch_experts(Params p, const void* w1, int64_t w1_se, int64_t w1_sr, const void* w2,
                    int64_t w2_se, int64_t w2_sr, bool after_gate, int sms, cudaStream_t s) {
   using K = Cfg<R, J>;
+  static_assert(K::BKS == stage_cols(R) && K::C == slices(R) && (R == kWideR || R == kNarrowR), "the workspace's");
+  const Parts parts = parts_of(p.F, int64_t(p.T) * p.k, K::BKS);
+  p.KS = parts.n, p.part_cols = parts.cols;
   CUtensorMap m1, m2;
   const CUtensorMapDataType dt = std::is_same<T, __nv_bfloat16>::value
                                      ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
@@ -736,7 +750,6 @@ int launch(Params p, const void* rw, int64_t ldr, const float* bias, const void*
   p.h = ws;
   p.part = reinterpret_cast<float*>(static_cast<char*>(ws) + lay.part);
   p.count = reinterpret_cast<int32_t*>(static_cast<char*>(ws) + lay.count);
-  p.KS = k_splits(p.F, int64_t(p.T) * p.k);
   if (rw != nullptr) {
     gate_kernel<T><<<p.T * kGateCluster, 32 * kWarps, 0, s>>>(
         static_cast<const T*>(p.x), p.ldx, static_cast<const T*>(rw), ldr, bias, p.H, p.E, p.k, renorm,
@@ -763,11 +776,11 @@ int launch(Params p, const void* rw, int64_t ldr, const float* bias, const void*
   // 8192: 168 us, 199 with 16 slots an item; 62 tokens, top-6 of 12 x 600 x 7888 126 and 111;
   // 32 tokens, top-2 of 2 x 2048 x 2048 45 and 37.
   if (p.T > 8 && S >= 16 * int64_t(p.E) && p.H >= 1024 && groups * ((p.F + 127) / 128) >= sms / 2)
-    return go(integral_constant<int, 8>(), integral_constant<int, 4>(), std::true_type());
-  if (p.T > 8) return go(integral_constant<int, 8>(), integral_constant<int, 2>(), std::false_type());
+    return go(integral_constant<int, kWideR>(), integral_constant<int, 4>(), std::true_type());
+  if (p.T > 8) return go(integral_constant<int, kWideR>(), integral_constant<int, 2>(), std::false_type());
   // No expert has more than 8 slots, unless it is repeated.
-  return narrow ? go(integral_constant<int, 2>(), integral_constant<int, 1>(), std::false_type())
-                : go(integral_constant<int, 8>(), integral_constant<int, 1>(), std::false_type());
+  return narrow ? go(integral_constant<int, kNarrowR>(), integral_constant<int, 1>(), std::false_type())
+                : go(integral_constant<int, kWideR>(), integral_constant<int, 1>(), std::false_type());
 }
 
 }  // namespace few
@@ -789,6 +802,15 @@ extern "C" int64_t moe_few_tokens_workspace(int32_t num_tokens, int32_t hidden, 
                                             int32_t num_experts, int32_t topk) {
   if (!sizes_ok(num_tokens, hidden, ffn, num_experts, topk)) return -1;
   return moe::few::Workspace(num_tokens, hidden, ffn, num_experts, topk).total;
+}
+
+extern "C" int32_t moe_few_tokens_parts(int32_t num_tokens, int32_t ffn, int32_t num_experts, int32_t topk,
+                                        int32_t narrow, int32_t* part_cols) {
+  using namespace moe::few;
+  if (!sizes_ok(num_tokens, 8, ffn, num_experts, topk) || part_cols == nullptr) return -1;
+  const Parts parts = parts_of(ffn, int64_t(num_tokens) * topk, stage_cols(narrow != 0 ? kNarrowR : kWideR));
+  *part_cols = parts.cols;
+  return parts.n;
 }
 
 extern "C" int32_t moe_few_tokens(const void* x, int64_t ldx, const void* router_w, int64_t ldr,
