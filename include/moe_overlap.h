@@ -552,7 +552,7 @@ MOE_API int32_t moe_router_topk_backward(const float* probs, const int64_t* topk
  *   workspace     moe_few_tokens_workspace(...) bytes of device memory, 16-byte
  *                 aligned, used by this call only; its contents need no set-up
  * dtype (MOE_DTYPE_BF16 or MOE_DTYPE_F16) is that of x, router_w, w1, w2 and out.
- * Rows start on 16 bytes; hidden and ffn are multiples of 8; num_experts <= 256;
+ * Rows start on 16 bytes; hidden and ffn are multiples of 8 up to 2^30; num_experts <= 256;
  * topk <= 16.
  */
 MOE_API int64_t moe_few_tokens_workspace(int32_t num_tokens, int32_t hidden, int32_t ffn,

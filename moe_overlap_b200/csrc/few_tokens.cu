@@ -24,6 +24,7 @@ namespace moe {
 namespace few {
 
 constexpr int kMaxTokens = 128;
+constexpr int kMaxWidth = 1 << 30;  // of hidden and ffn: a column and a stage behind it fit in an int
 constexpr int kMaxE = 256;
 constexpr int kMaxK = 16;
 constexpr int kWarps = 8;
@@ -351,7 +352,7 @@ __global__ void __launch_bounds__(threads(J, SHARE), 1)
   const int FB = (p.F + BM - 1) / BM, HB = (p.H + BM - 1) / BM;
   if (G == 0) {  // no slot is routed: zeros
     T* out = static_cast<T*>(p.out);
-    for (int i = blockIdx.x * kThreads + tid; i < p.T * p.H; i += gridDim.x * kThreads)
+    for (int64_t i = blockIdx.x * kThreads + tid; i < int64_t(p.T) * p.H; i += gridDim.x * kThreads)
       out[(i / p.H) * p.ldo + i % p.H] = from_f<T>(0.0f);
     return;
   }
@@ -789,8 +790,8 @@ int launch(Params p, const void* rw, int64_t ldr, const float* bias, const void*
 namespace {
 bool sizes_ok(int32_t num_tokens, int32_t hidden, int32_t ffn, int32_t num_experts, int32_t topk) {
   using namespace moe::few;
-  return num_tokens >= 0 && num_tokens <= kMaxTokens && hidden >= 8 && hidden % 8 == 0 && ffn >= 8 &&
-         ffn % 8 == 0 && num_experts >= 1 && num_experts <= kMaxE && topk >= 1 && topk <= kMaxK &&
+  return num_tokens >= 0 && num_tokens <= kMaxTokens && hidden >= 8 && hidden % 8 == 0 && hidden <= kMaxWidth &&
+         ffn >= 8 && ffn % 8 == 0 && ffn <= kMaxWidth && num_experts >= 1 && num_experts <= kMaxE && topk >= 1 && topk <= kMaxK &&
          topk <= num_experts;
 }
 bool rows_ok(const void* p, int64_t ld, int64_t width) {

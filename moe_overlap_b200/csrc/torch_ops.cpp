@@ -89,7 +89,7 @@ Tensor with_rows(const Tensor& t) { return rows_ok(t) ? t : t.clone(at::MemoryFo
 void* data(const Tensor& t) { return const_cast<void*>(t.const_data_ptr()); }
 
 // ------------------------------------------------------------ few tokens --
-constexpr int64_t kMaxFewTokens = 128;
+constexpr int64_t kMaxFewTokens = 128, kMaxWidth = int64_t(1) << 30;
 
 void check_weights(const char* name, const Tensor& t, const Tensor& x) {
   if (t.device() != x.device() || t.scalar_type() != x.scalar_type())
@@ -137,6 +137,7 @@ void check_few(const Tensor& x, const Tensor& w1, const Tensor& w2, int64_t top_
   if (w1.size(2) != hidden || w2.size(0) != experts || w2.size(1) != hidden || w2.size(2) != ffn) refuse(shapes);
   if (hidden % 8 != 0 || ffn % 8 != 0 || hidden == 0 || ffn == 0)
     refuse("hidden and ffn sizes must be multiples of 8");
+  if (hidden > kMaxWidth || ffn > kMaxWidth) refuse("hidden and ffn sizes go up to 2^30");
   if (x.size(0) > kMaxFewTokens)
     refuse("at most ", kMaxFewTokens, " tokens: use MoELayer.forward for larger batches");
   if (top_k < 1 || top_k > 16 || top_k > experts || experts > 256)

@@ -28,3 +28,11 @@ def test_many_parts_of_ffn(cuda_device, T, E, H, F, k, dtype):
     """Long sums of the down-projection: several parts an item, of widths that leave a
     short last one (and, were the parts not counted by their width, an empty one)."""
     check(cuda_device, T, E, H, F, k, dtype, seed=T)
+
+
+def test_widths_past_what_an_int_holds_are_refused(cuda_device):
+    z = torch.zeros(1, dtype=torch.bfloat16, device=cuda_device)
+    idx, w = torch.zeros(1, 1, dtype=torch.int64, device=cuda_device), torch.zeros(1, 1, device=cuda_device)
+    for H, F in ((2 ** 30 + 8, 8), (8, 2 ** 30 + 8), (2 ** 32 + 8, 8)):  # (views of one element)
+        with pytest.raises(ValueError, match="up to 2\\^30"):
+            mo.experts_few_tokens(z.expand(1, H), z.expand(1, F, H), z.expand(1, H, F), idx, w)

@@ -24,3 +24,16 @@ def test_no_part_of_ffn_is_empty():
     for bad in ((129, 64, 4, 2, 0), (4, 60, 4, 2, 0), (4, 64, 4, 5, 0)):
         assert lib.moe_few_tokens_parts(*bad, ctypes.byref(cols)) == -1
     assert lib.moe_few_tokens_parts(4, 64, 4, 2, 0, None) == -1
+
+
+def test_widths_past_what_an_int_holds_are_refused():
+    """A column, and the stage behind the last one, have to fit in 32 bits."""
+    lib, cols, wide = _lib.load(), ctypes.c_int32(), 2 ** 30 + 8
+    assert lib.moe_few_tokens_parts(1, 2 ** 30, 4, 1, 0, ctypes.byref(cols)) > 0
+    assert lib.moe_few_tokens_workspace(1, 2 ** 30, 64, 4, 1) > 0
+    assert lib.moe_few_tokens_parts(1, wide, 4, 1, 0, ctypes.byref(cols)) == -1
+    assert lib.moe_few_tokens_workspace(1, wide, 64, 4, 1) == -1
+    assert lib.moe_few_tokens_workspace(1, 64, wide, 4, 1) == -1
+    for H, F in ((wide, 64), (64, wide)):
+        assert lib.moe_few_tokens(16, H, 16, H, None, 16, F * H, H, 16, F * H, F, 0, 1, H, F, 4, 1, 0, 16, 16, 16, H,
+                                  16, 1 << 62, None, None) == _lib.MOE_ERR_INVALID_ARG
