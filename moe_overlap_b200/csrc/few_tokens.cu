@@ -128,6 +128,7 @@ __global__ void __cluster_dims__(kGateCluster, 1, 1) __launch_bounds__(32 * kWar
   __shared__ double z[kMaxE];
   __shared__ double partial[kMaxE / kGateCluster][kWarps];
   let_next_kernel_start();
+  cluster_arrive();  // this CTA is there; the first one's memory is written only when it is
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int rank = static_cast<int>(cluster_ctarank()), t = blockIdx.x / kGateCluster;
   if (blockIdx.x == 0)
@@ -142,6 +143,7 @@ __global__ void __cluster_dims__(kGateCluster, 1, 1) __launch_bounds__(32 * kWar
     if (lane == 0) partial[i][u % parts] = d;
   }
   __syncthreads();
+  cluster_wait();
   if (threadIdx.x < mine) {
     const int e = rank + static_cast<int>(threadIdx.x) * kGateCluster;
     double d = 0;

@@ -36,3 +36,11 @@ def test_widths_past_what_an_int_holds_are_refused(cuda_device):
     for H, F in ((2 ** 30 + 8, 8), (8, 2 ** 30 + 8), (2 ** 32 + 8, 8)):  # (views of one element)
         with pytest.raises(ValueError, match="up to 2\\^30"):
             mo.experts_few_tokens(z.expand(1, H), z.expand(1, F, H), z.expand(1, H, F), idx, w)
+
+
+@pytest.mark.parametrize("T,E,H", [(128, 256, 8), (128, 3, 8), (1, 256, 16), (77, 9, 24)])
+def test_gate_of_few_columns(cuda_device, T, E, H):
+    """Logits of a column block or two: the gate's CTAs are done with their products before
+    the one that gathers them need have started."""
+    for seed in range(3):
+        check(cuda_device, T, E, H, 16, min(E, 2), torch.bfloat16, seed=seed)
