@@ -231,14 +231,10 @@ struct Plan {  // in shared memory; every CTA derives the same one from idx
 };
 
 struct Ctrl {
-  uint64_t full[12], empty[12], qfull[kQueue], qempty[kQueue], turn[kSets];
+  uint64_t full[12], empty[12], qfull[kQueue], qempty[kQueue], turn[kSets], sums[kSets];
   int item[kQueue];
+  int abort;  // a wait ran out: every role leaves
 };
-
-// The 8 warps of one set.
-__device__ __forceinline__ void set_sync(int set) {
-  asm volatile("bar.sync %0, 256;" ::"r"(1 + set) : "memory");
-}
 
 // The slots by expert and the groups of at most NT of them: grp holds
 // expert << 16 | place of the group's first slot.
@@ -337,11 +333,15 @@ __global__ void __launch_bounds__(threads(J, SHARE), 1)
       mbar_init(smem_u32(&ctrl->full[s]), 1 + 32 * kCopyWarps);
       mbar_init(smem_u32(&ctrl->empty[s]), kWarpsOn);
     }
-    for (int s = 0; s < kSets; ++s) mbar_init(smem_u32(&ctrl->turn[s]), kConsumers);
+    for (int s = 0; s < kSets; ++s) {
+      mbar_init(smem_u32(&ctrl->turn[s]), kConsumers);
+      mbar_init(smem_u32(&ctrl->sums[s]), kConsumers);
+    }
     for (int s = 0; s < kQueue; ++s) {
       mbar_init(smem_u32(&ctrl->qfull[s]), 1);
       mbar_init(smem_u32(&ctrl->qempty[s]), kCopyWarps + kSets * kConsumers);
     }
+    ctrl->abort = 0;
     fence_mbar_init();
     tma_prefetch_desc(&map1);
     tma_prefetch_desc(&map2);
@@ -373,14 +373,28 @@ __global__ void __launch_bounds__(threads(J, SHARE), 1)
     it.c1 = it.down ? min(it.c0 + p.part_cols, p.F) : p.H;
     return it;
   };
-  // Takes the queue's next item; -1 at the end (or when the wait ran out).
+  // A warp whose wait has run out (or another's has) leaves; no one waits for it unbounded.
+  volatile int* abort_flag = &ctrl->abort;
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    if (mbar_wait(smem_u32(bar), parity, abort_flag)) return true;
+    give_up(abort_flag, p.status, MOE_ERR_TIMEOUT);
+    return false;
+  };
+  // Until a counter that other CTAs raise has come to `n`.
+  auto wait_count = [&](const int* count, int n) {
+    const long long t0 = clock64();
+    while (ld_acquire_gpu(count) < n)
+      if (*abort_flag || clock64() - t0 > kWaitBudgetCycles) {
+        give_up(abort_flag, p.status, MOE_ERR_TIMEOUT);
+        return false;
+      }
+    return true;
+  };
+  // Takes the queue's next item; -1 at the end, -2 when the wait ran out.
   auto pop = [&](int n) {
     const int slot = n % kQueue;
-    int item = -1;
-    if (mbar_wait(smem_u32(&ctrl->qfull[slot]), (n / kQueue) & 1, nullptr))
-      item = ctrl->item[slot];
-    else
-      record_status(p.status, MOE_ERR_TIMEOUT);
+    if (!__all_sync(0xffffffffu, wait(&ctrl->qfull[slot], (n / kQueue) & 1))) return -2;
+    const int item = ctrl->item[slot];
     __syncwarp();
     if (lane == 0) mbar_arrive(smem_u32(&ctrl->qempty[slot]));
     return item;
@@ -396,10 +410,7 @@ __global__ void __launch_bounds__(threads(J, SHARE), 1)
         const bool end = item >= items;
         if (!end) next = atomicAdd(p.count, 1);
         const int slot = n % kQueue;
-        if (!mbar_wait(smem_u32(&ctrl->qempty[slot]), ((n / kQueue) & 1) ^ 1, nullptr)) {
-          record_status(p.status, MOE_ERR_TIMEOUT);
-          return;
-        }
+        if (!wait(&ctrl->qempty[slot], ((n / kQueue) & 1) ^ 1)) return;
         ctrl->item[slot] = end ? -1 : item;
         mbar_arrive(smem_u32(&ctrl->qfull[slot]));
         if (end) return;
@@ -408,10 +419,7 @@ __global__ void __launch_bounds__(threads(J, SHARE), 1)
         const CUtensorMap* map = it.down ? &map2 : &map1;
         for (int c = it.c0; c < it.c1; c += BKS) {
           const uint32_t full = smem_u32(&ctrl->full[stage]);
-          if (!mbar_wait(smem_u32(&ctrl->empty[stage]), phase ^ 1, nullptr)) {
-            record_status(p.status, MOE_ERR_TIMEOUT);
-            return;
-          }
+          if (!wait(&ctrl->empty[stage], phase ^ 1)) return;
           mbar_arrive_expect_tx(full, kStageBytes);
           const uint32_t dst = smem_u32(base + stage * kStageBytes);
 #pragma unroll
@@ -445,18 +453,12 @@ __global__ void __launch_bounds__(threads(J, SHARE), 1)
     uint32_t phase = 0;
     for (int n = 0;; ++n) {
       const int item = pop(n);
-      if (item < 0) return;
+      if (item < 0) return copies_wait_all();
       const Item it = decode(item);
       const int pos0 = grp[it.g] & 0xffff;
       const int rows = (it.g + 1 < G ? (grp[it.g + 1] & 0xffff) : S) - pos0;
-      if (it.down) {  // this group's h, complete and visible to this thread
-        const long long t0 = clock64();
-        while (ld_acquire_gpu(ready + it.g) < FB * kWarpsOn)
-          if (clock64() - t0 > kWaitBudgetCycles) {
-            record_status(p.status, MOE_ERR_TIMEOUT);
-            break;  // carry on with what is there: the pipeline still ends
-          }
-      }
+      // (in a down item) this group's h, complete and visible to this thread
+      if (it.down && !__all_sync(0xffffffffu, wait_count(ready + it.g, FB * kWarpsOn))) return copies_wait_all();
       const T* src[kPasses];
 #pragma unroll
       for (int i = 0; i < kPasses; ++i) {
@@ -469,10 +471,7 @@ __global__ void __launch_bounds__(threads(J, SHARE), 1)
       }
       for (int c = it.c0; c < it.c1; c += BKS) {
         const uint32_t full = smem_u32(&ctrl->full[stage]);
-        if (!mbar_wait(smem_u32(&ctrl->empty[stage]), phase ^ 1, nullptr)) {
-          record_status(p.status, MOE_ERR_TIMEOUT);
-          return;
-        }
+        if (!__all_sync(0xffffffffu, wait(&ctrl->empty[stage], phase ^ 1))) return copies_wait_all();
         const uint32_t dst = smem_u32(slots + stage * 2 * K::kSlotBytes);
         const bool in = c + piece8 < it.c1;
         const int from = in ? c : it.c0;
@@ -498,9 +497,11 @@ __global__ void __launch_bounds__(threads(J, SHARE), 1)
   const uint32_t off0 = ((2 * q4) ^ g8) * 16, off1 = ((2 * q4 + 1) ^ g8) * 16;
   int stage = 0;
   uint32_t phase = 0;
+  [[maybe_unused]] uint32_t sums_parity = 0;
   for (int n = 0;; ++n) {
     const int item = pop(n);
-    if (item < 0) break;
+    if (item == -1) break;
+    if (item < 0) return;
     const Item it = decode(item);
     if (!SHARE && n % kSets != set) {  // the other set's item: past its stages
       stage += (it.c1 - it.c0 + BKS - 1) / BKS;
@@ -509,10 +510,7 @@ __global__ void __launch_bounds__(threads(J, SHARE), 1)
     }
     // The other set has used every stage before this item's: a parity wait on a stage
     // is only sound within one turn of the ring.
-    if (!SHARE && !mbar_wait(smem_u32(&ctrl->turn[set]), ((n / kSets) & 1) ^ (set == 0), nullptr)) {
-      record_status(p.status, MOE_ERR_TIMEOUT);
-      return;
-    }
+    if (!SHARE && !__all_sync(0xffffffffu, wait(&ctrl->turn[set], ((n / kSets) & 1) ^ (set == 0)))) return;
     const int pos0 = grp[it.g] & 0xffff;
     const int rows = (it.g + 1 < G ? (grp[it.g + 1] & 0xffff) : S) - pos0;
     // Two sums of every output, so that no product waits for the one before it (a stage's
@@ -551,10 +549,7 @@ __global__ void __launch_bounds__(threads(J, SHARE), 1)
       }
     };
     for (int c = it.c0; c < it.c1; c += BKS) {
-      if (!mbar_wait(smem_u32(&ctrl->full[stage]), phase, nullptr)) {
-        record_status(p.status, MOE_ERR_TIMEOUT);
-        return;
-      }
+      if (!__all_sync(0xffffffffu, wait(&ctrl->full[stage], phase))) return;
       using std::integral_constant;
       if (JS > 1 && rows > s0 + 8) {
         it.down ? multiply(integral_constant<int, JS>(), integral_constant<int, 2>())
@@ -595,7 +590,9 @@ __global__ void __launch_bounds__(threads(J, SHARE), 1)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             rb[(j * 8 + 2 * q4 + (i & 1)) * kRedStride + g8 + 8 * (i >> 1)] = acc[j][i];
-        set_sync(set);
+        const uint32_t bar = smem_u32(&ctrl->sums[set]);
+        if (!__all_sync(0xffffffffu, warps_sync(bar, sums_parity, abort_flag)))
+          return give_up(abort_flag, p.status, MOE_ERR_TIMEOUT);
         const float* rs = red + set * kConsumers * (NT * kRedStride);
         for (int o = cw * 32 + lane; o < BM * rows; o += 32 * kConsumers) {
           const int m = o % BM, nn = o / BM, row = it.blk * BM + m;
@@ -605,7 +602,8 @@ __global__ void __launch_bounds__(threads(J, SHARE), 1)
             v += rs[(i * R + m / 16) * (NT * kRedStride) + nn * kRedStride + m % 16];
           if (row < p.F) put_h(nn, row, v);
         }
-        set_sync(set);  // the buffer is free again
+        if (!__all_sync(0xffffffffu, warps_sync(bar, sums_parity, abort_flag)))  // the buffer is free again
+          return give_up(abort_flag, p.status, MOE_ERR_TIMEOUT);
       }
       __syncwarp();
       if (lane == 0) red_release_gpu(ready + it.g, 1);
@@ -636,12 +634,7 @@ __global__ void __launch_bounds__(threads(J, SHARE), 1)
   for (int u = (warp - kFirstConsumer) * gridDim.x + blockIdx.x; u < units; u += kSets * kConsumers * gridDim.x) {
     const int blk16 = u / t_groups, t = u % t_groups * 8 + (lane >> 2);
     const int col = blk16 * 16 + (lane & 3) * 4;  // 4 columns of one token a lane (H: a multiple of 8)
-    const long long t0 = clock64();
-    while (ld_acquire_gpu(done + blk16) < G * parts * (kWarpsOn / kConsumers))
-      if (clock64() - t0 > kWaitBudgetCycles) {
-        record_status(p.status, MOE_ERR_TIMEOUT);
-        break;
-      }
+    if (!wait_count(done + blk16, G * parts * (kWarpsOn / kConsumers))) return;
     if (t >= p.T || col >= p.H) continue;
     float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     int j = 0, i = 0;

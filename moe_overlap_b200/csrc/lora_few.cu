@@ -85,7 +85,8 @@ struct Cfg {
 };
 
 struct Ctrl {
-  uint64_t full[12], empty[12];
+  uint64_t full[12], empty[12], sums;
+  int abort;  // a wait ran out: every role leaves
   int id[64];
   float scale[64];
 };
@@ -109,6 +110,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(smem_u32(&ctrl->full[s]), 1);
       mbar_init(smem_u32(&ctrl->empty[s]), kConsumers);
     }
+    mbar_init(smem_u32(&ctrl->sums), kConsumers);
+    ctrl->abort = 0;
     fence_mbar_init();
   }
   const int mb = blockIdx.y * NT, Mt = min(NT, M - mb);  // this CTA's rows of x
@@ -121,16 +124,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int blocks = (N + BM - 1) / BM;
   int stage = 0;
   uint32_t phase = 0;
+  volatile int* abort_flag = &ctrl->abort;
 
   if (warp == 0) {
     if (lane == 0) {
       for (int blk = blockIdx.x; blk < blocks; blk += gridDim.x)
         for (int c = 0; c < K; c += BKS) {
           const uint32_t full = smem_u32(&ctrl->full[stage]);
-          if (!mbar_wait(smem_u32(&ctrl->empty[stage]), phase ^ 1, nullptr)) {
-            record_status(status, MOE_ERR_TIMEOUT);
-            return;
-          }
+          if (!mbar_wait(smem_u32(&ctrl->empty[stage]), phase ^ 1, abort_flag))
+            return give_up(abort_flag, status, MOE_ERR_TIMEOUT);
           mbar_arrive_expect_tx(full, kStageBytes + Q::kSlotBytes);
           const uint32_t dst = smem_u32(base + stage * kStageBytes);
           const uint32_t xdst = smem_u32(slots + stage * Q::kSlotBytes);
@@ -149,6 +151,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t b_base = smem_u32(slots) + (cs * NT + g8) * 128;
   const uint32_t off0 = ((2 * q4) ^ g8) * 16, off1 = ((2 * q4 + 1) ^ g8) * 16;
   bool waited = false;
+  // A warp whose wait has run out leaves, but this grid still ends after the one before.
+  auto leave = [&] {
+    give_up(abort_flag, status, MOE_ERR_TIMEOUT);
+    if (!waited) wait_for_previous_kernel();
+  };
+  uint32_t sums_parity = 0;
+  auto sync = [&] { return __all_sync(0xffffffffu, warps_sync(smem_u32(&ctrl->sums), sums_parity, abort_flag)); };
   for (int blk = blockIdx.x; blk < blocks; blk += gridDim.x) {
     float acc[J][4];
 #pragma unroll
@@ -156,10 +165,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[j][i] = 0.0f;
     for (int c = 0; c < K; c += BKS) {
-      if (!mbar_wait(smem_u32(&ctrl->full[stage]), phase, nullptr)) {
-        record_status(status, MOE_ERR_TIMEOUT);
-        return;
-      }
+      if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&ctrl->full[stage]), phase, abort_flag))) return leave();
       uint32_t a[2][8];  // rows g8 and g8 + 8, 16 columns each
       const uint32_t sa = a_base + stage * kStageBytes;
       ld_shared_v4(sa + off0, &a[0][0]);
@@ -189,7 +195,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         rb[(j * 8 + 2 * q4 + (i & 1)) * kRedStride + g8 + 8 * (i >> 1)] = acc[j][i];
-    asm volatile("bar.sync 1, 256;" ::: "memory");
+    if (!sync()) return leave();
     if (!waited) wait_for_previous_kernel();  // for `low`
     waited = true;
     const int tid_c = cw * 32 + lane;
@@ -230,7 +236,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (at[q] >= 0) red[at[q]] += c[q] * add[q];
         }
       }
-      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (!sync()) return leave();
     }
     // One column of W a thread (row n of the block) and every 256 / BM-th row of x, eight of
     // them at a time, so that their adapters' rows are under way together.
@@ -274,7 +280,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           y[(mb + m) * ldy + row] = from_f<T>(v);
         }
       }
-    asm volatile("bar.sync 1, 256;" ::: "memory");  // the buffer is free again
+    if (!sync()) return leave();  // the buffer is free again
   }
 }
 

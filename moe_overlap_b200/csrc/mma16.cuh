@@ -99,6 +99,7 @@ template <int kLeft>
 __device__ __forceinline__ void copies_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory");
 }
+__device__ __forceinline__ void copies_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 // Arrives on `bar` when this thread's earlier copies have landed.
 __device__ __forceinline__ void copies_arrive(uint32_t bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");

@@ -67,6 +67,16 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity,
   }
 }
 
+// A barrier over the warps that `bar` counts, bounded: false when it was given up.  Each
+// warp keeps its own `parity`, 0 at first.
+__device__ __forceinline__ bool warps_sync(uint32_t bar, uint32_t& parity, const volatile int* abort_flag) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+  const bool ok = mbar_wait(bar, parity, abort_flag);
+  parity ^= 1;
+  return ok;
+}
+
 // Same as mbar_wait with acquire at cluster scope, for barriers that other
 // CTAs of the cluster arrive on.
 __device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar, uint32_t parity) {
@@ -221,7 +231,7 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
                : "memory");
 }
 
-// Its two halves: between them a CTA may work on its own memory; behind the second every
+// A cluster barrier in two halves: between them a CTA may work on its own memory; behind the second every
 // CTA of the cluster has started and its memory may be reached.
 __device__ __forceinline__ void cluster_arrive() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
@@ -411,6 +421,17 @@ __device__ __forceinline__ void record_status(int32_t* status, int32_t code) {
   if (status != nullptr) {
     volatile int32_t* s = status;
     if (*s == 0) *s = code;
+  }
+}
+
+// What a thread does whose wait ran out, in a kernel whose roles share `abort_flag`: the
+// others' waits end with it, and copies already issued get time to land before this
+// thread, and with it the CTA, leaves.
+__device__ __forceinline__ void give_up(volatile int* abort_flag, int32_t* status, int32_t code) {
+  record_status(status, code);
+  *abort_flag = 1;
+  const long long t0 = clock64();
+  while (clock64() - t0 < (1ll << 22)) {
   }
 }
 
