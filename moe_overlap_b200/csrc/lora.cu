@@ -13,9 +13,15 @@
 //           rows of tiles with more adapters than the shared product takes
 //   grads   dB[i] = scale[i] sum_p dy[perm[p]]^T s[p]  (and dA[i])
 // For the gradients and for expand s is held as two values of the inputs' type, the
-// rounded one and what the rounding left (16 bits or more in all).  The shared product
-// takes scale[i] s rounded to the type, like every operand of it; the sum with the
-// shared part is then rounded once, where expand rounds it a second time.
+// rounded one and what the rounding left: 16 bits of bf16.  fp16 has 22 bits but little
+// range (dy B of gradients of 1e-5 lies below its normal numbers, where the second part is
+// nothing), so s is scaled before it is split: by a power of two common to 16 rows of an
+// adapter, the grads' step, which puts their largest between 2^6 and 2^14; what is lost is
+// 2^-31 of that one at most.  expand undoes it by row, the grads step by step.
+// The shared product takes scale[i] s rounded to the type, like every operand of it; the sum
+// with the shared part is then rounded once, where expand rounds it a second time.  A row of
+// fp16 whose largest |scale[i] s| is beyond 65504 or below the normal numbers (2^-14) has no
+// such operand: it is left to expand, with zeros in the product.
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -45,9 +51,18 @@ struct PlanView {
   int32_t* offs;   // [adapters + 1]
   int32_t* base;   // {0, m}
   int32_t* queue;  // tile counters of the shared products of the forward and the backward, 0 before each
+  // With fp16, per pass: whether shrink has left a row to expand (once set it stays: expand
+  // then looks at `put`), the rows by place that the shared product takes, and the powers of
+  // two of s and of t by blocks of 16 rows (see Range).
+  int32_t* left;
+  int32_t* put;  // [m]
+  int32_t* exps[2];
   static int64_t tiles(int64_t m) { return (m + kTileRows - 1) / kTileRows; }
+  // Entries of exps: block o / 16 of adapter i, whose rows start at place offs[i], is
+  // number offs[i] / 16 + i + o / 16 (n rows make at most n / 16 + 1 blocks).
+  static int64_t blocks16(int64_t m, int adapters) { return m / 16 + adapters + 1; }
   static int64_t ints(int64_t m, int adapters) {
-    return tiles(m) * int64_t(sizeof(TileAdapters) / 4) + 2 * m + adapters + 5;
+    return tiles(m) * int64_t(sizeof(TileAdapters) / 4) + 3 * m + adapters + 6 + 2 * blocks16(m, adapters);
   }
   PlanView(void* plan, int64_t m, int adapters) {
     tile = static_cast<TileAdapters*>(plan);
@@ -56,6 +71,10 @@ struct PlanView {
     offs = perm + m;
     base = offs + adapters + 1;
     queue = base + 2;
+    left = queue + 2;
+    put = left + 1;
+    exps[0] = put + m;
+    exps[1] = exps[0] + blocks16(m, adapters);
   }
 };
 
@@ -113,7 +132,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(const void* ids, int ids64, 
     if (tid == 0) {
       plan.offs[i] = start;
       if (i == L - 1) plan.offs[L] = start + all;
-      if (i == 0) plan.base[0] = 0, plan.base[1] = M, plan.queue[0] = plan.queue[1] = 0;
+      if (i == 0) plan.base[0] = 0, plan.base[1] = M, plan.queue[0] = plan.queue[1] = 0, *plan.left = 0;
     }
     if (all == 0) return;
     at += start;
@@ -232,6 +251,31 @@ __device__ __forceinline__ Tile find_tile(const int32_t* offs, int L, int tile, 
   return t;
 }
 
+// What fp16 needs beside the two parts of s (bf16 has fp32's range and needs nothing).
+struct Range {
+  int32_t* exps;  // of s: the powers of two that it was divided by, kNoExp where there is nothing to scale
+  int32_t* put;   // [m] by place
+  int32_t* left;
+};
+constexpr int kNoExp = -1000;
+__device__ __forceinline__ float exp2i(int e) { return __int_as_float((e + 127) << 23); }  // -126 .. 127
+// |v| if it is finite, else 0, as the bits of the float (which order as integers do).
+__device__ __forceinline__ uint32_t finite_abs(float v) {
+  const uint32_t b = __float_as_uint(v) & 0x7fffffffu;
+  return b < 0x7f800000u ? b : 0u;
+}
+__device__ __forceinline__ uint32_t finite_abs(const float4& v) {
+  return max(max(finite_abs(v.x), finite_abs(v.y)), max(finite_abs(v.z), finite_abs(v.w)));
+}
+// The power of two for a block whose largest value has these bits: multiples of 8, so that
+// neighbouring blocks mostly share it, leave that value between 2^6 and 2^14.  The bounds
+// keep sums of such blocks within fp32; products of fp16 values reach neither of them.
+__device__ __forceinline__ int exp_of(uint32_t largest) {
+  if (largest == 0) return kNoExp;
+  const int e = (static_cast<int>(largest >> 23) - 127 - 6) & ~7;  // (a two's complement floor)
+  return min(max(e, -56), 64);
+}
+
 // shrink.  A CTA forms 128 rows x RP of s over one part of k: 4 warps of 32 rows (each
 // reads all of w's tile from shared memory) for each half of a stage's columns (of the rank,
 // if it is 128: all of it would be 128 sums a lane); the CTAs of a cluster
@@ -256,10 +300,12 @@ template <typename T, bool kT, int RP>
 __global__ void __launch_bounds__(kThreads, 2)
     shrink_kernel(const T* x, int64_t ldx, const T* w, int64_t sl, int64_t sr, const int32_t* perm,
                   const int32_t* offs, int L, int K, int r, int64_t part_stride, T* s, Scale scale,
-                  const int32_t* taken, T* rows) {
+                  const int32_t* taken, T* rows, Range range) {
   using C = ShrinkCfg<kT, RP>;
   extern __shared__ __align__(128) char smem[];
+  constexpr bool kScaled = std::is_same<T, __half>::value;
   __shared__ int row_of[kShrinkRows];  // -1: not the shared product's
+  [[maybe_unused]] __shared__ uint32_t largest[kShrinkRows / 16];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   wait_for_previous_kernel();
   let_next_kernel_start();
@@ -270,6 +316,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     const int row = perm[t.p0 + tid];
     row_of[tid] = taken[row] ? row : -1;
   }
+  if (kScaled && tid < kShrinkRows / 16) largest[tid] = 0;
   const int parts = gridDim.y, part = blockIdx.y;
   const int cols = ((K + parts - 1) / parts + kShrinkCols - 1) / kShrinkCols * kShrinkCols;
   const int k0 = min(K, part * cols), k1 = min(K, k0 + cols);
@@ -393,19 +440,69 @@ __global__ void __launch_bounds__(kThreads, 2)
   else
     __syncthreads();
   const int share = kShrinkRows / parts;  // rows that this CTA finishes
-  for (int e = tid; e < share * (RP / 4); e += kThreads) {
-    const int m = part * share + e / (RP / 4), j = e % (RP / 4) * 4;
-    if (m >= t.rows || j >= r) continue;
-    const float4 v = cluster_sum4(sums + m * kPitch + j, parts);
-    T hi[4], lo[4];
-    split(v.x, hi, lo), split(v.y, hi + 1, lo + 1), split(v.z, hi + 2, lo + 2), split(v.w, hi + 3, lo + 3);
-    T* out = s + int64_t(t.p0 + m) * r + j;
-    *reinterpret_cast<uint2*>(out) = *reinterpret_cast<const uint2*>(hi);
-    *reinterpret_cast<uint2*>(out + part_stride) = *reinterpret_cast<const uint2*>(lo);
-    const int row = row_of[m];
-    if (row >= 0) {
-      const T o[4] = {from_f<T>(c * v.x), from_f<T>(c * v.y), from_f<T>(c * v.z), from_f<T>(c * v.w)};
-      *reinterpret_cast<uint2*>(rows + int64_t(row) * r + j) = *reinterpret_cast<const uint2*>(o);
+  if constexpr (kScaled) {
+    // The totals replace this CTA's sums in the rows that it alone finishes (a warp's 32
+    // quads lie in one block of 16 rows), then they are scaled and split.
+    constexpr int kLanes = RP / 4;  // of a row
+    for (int e = tid; e < share * kLanes; e += kThreads) {
+      const int m = part * share + e / kLanes, j = e % kLanes * 4;
+      uint32_t top = 0;
+      if (m < t.rows && j < r) {
+        const float4 v = cluster_sum4(sums + m * kPitch + j, parts);
+        *reinterpret_cast<float4*>(sums + m * kPitch + j) = v;
+        top = finite_abs(v);
+      }
+      top = __reduce_max_sync(0xffffffffu, top);
+      if (lane == 0) atomicMax(&largest[m / 16], top);
+    }
+    __syncthreads();
+    const int first = offs[t.i], block0 = first / 16 + t.i + (t.p0 - first) / 16;
+    for (int e = tid; e < share * kLanes; e += kThreads) {
+      const int m = part * share + e / kLanes, j = e % kLanes * 4;
+      const bool there = m < t.rows && j < r;
+      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (there) v = *reinterpret_cast<const float4*>(sums + m * kPitch + j);
+      const float4 op = make_float4(c * v.x, c * v.y, c * v.z, c * v.w);
+      uint32_t top = there ? finite_abs(op) : 0u;  // the row's largest
+#pragma unroll
+      for (int o = 1; o < kLanes; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const bool fits = top == 0 || (top >= __float_as_uint(0x1p-14f) && top <= __float_as_uint(65504.0f));
+      if (!there) continue;
+      const int x2 = exp_of(largest[m / 16]);
+      const float f = x2 == kNoExp ? 1.0f : exp2i(-x2);
+      T hi[4], lo[4];
+      split(v.x * f, hi, lo), split(v.y * f, hi + 1, lo + 1), split(v.z * f, hi + 2, lo + 2);
+      split(v.w * f, hi + 3, lo + 3);
+      T* out = s + int64_t(t.p0 + m) * r + j;
+      *reinterpret_cast<uint2*>(out) = *reinterpret_cast<const uint2*>(hi);
+      *reinterpret_cast<uint2*>(out + part_stride) = *reinterpret_cast<const uint2*>(lo);
+      const int row = row_of[m];
+      if (row >= 0) {
+        T o[4] = {from_f<T>(op.x), from_f<T>(op.y), from_f<T>(op.z), from_f<T>(op.w)};
+        if (!fits) o[0] = o[1] = o[2] = o[3] = from_f<T>(0.0f);
+        *reinterpret_cast<uint2*>(rows + int64_t(row) * r + j) = *reinterpret_cast<const uint2*>(o);
+      }
+      if (j == 0) {
+        range.put[t.p0 + m] = row >= 0 && fits;
+        if (row >= 0 && !fits) *range.left = 1;  // (every writer the same)
+        if (m % 16 == 0) range.exps[block0 + m / 16] = x2;
+      }
+    }
+  } else {
+    for (int e = tid; e < share * (RP / 4); e += kThreads) {
+      const int m = part * share + e / (RP / 4), j = e % (RP / 4) * 4;
+      if (m >= t.rows || j >= r) continue;
+      const float4 v = cluster_sum4(sums + m * kPitch + j, parts);
+      T hi[4], lo[4];
+      split(v.x, hi, lo), split(v.y, hi + 1, lo + 1), split(v.z, hi + 2, lo + 2), split(v.w, hi + 3, lo + 3);
+      T* out = s + int64_t(t.p0 + m) * r + j;
+      *reinterpret_cast<uint2*>(out) = *reinterpret_cast<const uint2*>(hi);
+      *reinterpret_cast<uint2*>(out + part_stride) = *reinterpret_cast<const uint2*>(lo);
+      const int row = row_of[m];
+      if (row >= 0) {
+        const T o[4] = {from_f<T>(c * v.x), from_f<T>(c * v.y), from_f<T>(c * v.z), from_f<T>(c * v.w)};
+        *reinterpret_cast<uint2*>(rows + int64_t(row) * r + j) = *reinterpret_cast<const uint2*>(o);
+      }
     }
   }
   if (parts > 1) cluster_sync_all();  // no CTA leaves while another reads its sums
@@ -432,7 +529,7 @@ struct ExpandCfg {
 template <typename T, bool kT, int RP>
 __global__ void __launch_bounds__(kThreads, 2)
     expand_kernel(const T* s, int64_t part_stride, const T* w, int64_t sl, int64_t sr,
-                  Scale scale, const int32_t* perm, const int32_t* offs, const int32_t* taken,
+                  Scale scale, const int32_t* perm, const int32_t* offs, const int32_t* taken, Range range,
                   const TileAdapters* tile, int tiles, int splits, int L, int N, int r, T* y, int64_t ldy) {
   using C = ExpandCfg<kT, RP>;
   extern __shared__ __align__(128) char smem[];
@@ -440,7 +537,8 @@ __global__ void __launch_bounds__(kThreads, 2)
   wait_for_previous_kernel();
   let_next_kernel_start();
   // Usually the shared product has taken every row.
-  bool any = false;
+  constexpr bool kScaled = std::is_same<T, __half>::value;
+  bool any = kScaled && *range.left != 0;
   for (int q = tid; q < tiles; q += kThreads) any |= tile[q].left != 0;
   if (!__syncthreads_or(any)) return;
   const int mg = warp & 3, half = warp >> 2;
@@ -448,11 +546,19 @@ __global__ void __launch_bounds__(kThreads, 2)
   const Tile t = find_tile(offs, L, unit / splits, kExpandRows);
   if (t.i < 0) return;
   const int first = unit % splits * kExpandCols;
+  const float c = scale.of(t.i);
+  float cu[2] = {c, c};
+  if constexpr (kScaled) {  // these 16 rows' power of two
+    const int o0 = offs[t.i], o = t.p0 - o0 + mg * 16;
+    const int x2 = mg * 16 < t.rows ? range.exps[o0 / 16 + t.i + o / 16] : kNoExp;
+    if (x2 != kNoExp) cu[0] = cu[1] = c * exp2i(x2);
+  }
   T* yrow[2];  // rows mg*16 + g8 and + 8; null for those that the shared product has taken
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     const int m = mg * 16 + g8 + 8 * u, row = m < t.rows ? perm[t.p0 + m] : -1;
-    yrow[u] = row >= 0 && !taken[row] ? y + row * ldy + half * 64 + q4 * 8 : nullptr;
+    const bool done = row >= 0 && (kScaled ? range.put[t.p0 + m] : taken[row]) != 0;
+    yrow[u] = row >= 0 && !done ? y + row * ldy + half * 64 + q4 * 8 : nullptr;
   }
   if (!__syncthreads_or(yrow[0] != nullptr || yrow[1] != nullptr)) continue;
   const T* wi = w + t.i * sl;
@@ -480,7 +586,6 @@ __global__ void __launch_bounds__(kThreads, 2)
     copies_commit();
   };
   fetch_w(first, 0);
-  const float c = scale.of(t.i);
   const int ncol = half * 64 + q4 * 8;  // this lane's first column of a block; + 32 for the second
   auto fetch_y = [&](int n0, uint4(&v)[2][2]) {
 #pragma unroll
@@ -568,7 +673,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         if (yrow[u] == nullptr || n0 + ncol + g * 32 >= N) continue;
         T* v = reinterpret_cast<T*>(&yv[g][u]);
 #pragma unroll
-        for (int q = 0; q < 8; ++q) v[q] = from_f<T>(to_f(v[q]) + c * add[u][q]);
+        for (int q = 0; q < 8; ++q) v[q] = from_f<T>(to_f(v[q]) + cu[u] * add[u][q]);
         *reinterpret_cast<uint4*>(yrow[u] + n0 + g * 32) = yv[g][u];
       }
     }
@@ -610,6 +715,7 @@ struct GradOf {
   int64_t ldz;
   int n;
   T* g;
+  const int32_t* exps;  // fp16: s's powers of two
 };
 
 template <typename T, bool kT, int RP>
@@ -648,6 +754,20 @@ __device__ __forceinline__ void grad_block(char* smem, const GradOf<T>& of, int 
     const int j = f % kSPieces * 8;
     sp[q] = s + (j < r && half < 2 ? half * part_stride + int64_t(o0 + p0 + f / kSPieces) * r + j : 0);
   }
+  // fp16: the powers of two of a step's two blocks of 16 rows, known a step ahead.  The sums
+  // are held divided by the last block's, `unit`: a block with another one changes it in all
+  // of them first, which is exact and seldom (multiples of 8), and loses nothing of small
+  // rows behind large ones.
+  constexpr bool kScaled = std::is_same<T, __half>::value;
+  [[maybe_unused]] int unit = kNoExp, next_exp[2] = {kNoExp, kNoExp};
+  auto look_up_exps = [&](int step) {
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const int o = p0 + step * kGradRows + 16 * q;
+      next_exp[q] = o < p1 ? of.exps[o0 / 16 + i + o / 16] : kNoExp;
+    }
+  };
+  if constexpr (kScaled) look_up_exps(0);
   int step_f = 0, at = 0;  // the step and the stage of the next fetch
   auto fetch = [&]() {
     if (step_f < steps) {
@@ -689,8 +809,25 @@ __device__ __forceinline__ void grad_block(char* smem, const GradOf<T>& of, int 
     fetch();
     const uint32_t zs = smem_u32(smem) + stage * C::kStage;
     const uint32_t ss = zs + kGradRows * C::kZPitch;
+    [[maybe_unused]] const int exps[2] = {next_exp[0], next_exp[1]};
+    if constexpr (kScaled) look_up_exps(step + 1);
 #pragma unroll
     for (int kk = 0; kk < kGradRows; kk += 16) {
+      if constexpr (kScaled) {
+        const int x2 = exps[kk / 16];
+        if (x2 != unit && x2 != kNoExp) {
+          if (unit != kNoExp) {
+            const float f = exp2i(unit - x2);
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+              for (int k = 0; k < RP / 8; ++k)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) acc[m][k][q] *= f;
+          }
+          unit = x2;
+        }
+      }
       uint32_t a[MT][4];
 #pragma unroll
       for (int m = 0; m < MT; ++m)
@@ -716,6 +853,7 @@ __device__ __forceinline__ void grad_block(char* smem, const GradOf<T>& of, int 
   // The sums lie as the gradient does: [column][rank], or [rank][column] with kT.
   constexpr int kPitch = kT ? C::kCols + 4 : RP + 4;
   float* sums = reinterpret_cast<float*>(smem);
+  const float f = kScaled && unit != kNoExp ? exp2i(unit) : 1.0f;
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -723,7 +861,7 @@ __device__ __forceinline__ void grad_block(char* smem, const GradOf<T>& of, int 
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int col = (warp * MT + m) * 16 + (lane >> 2) + 8 * (q >> 1), j = k * 8 + (lane & 3) * 2 + (q & 1);
-        sums[kT ? j * kPitch + col : col * kPitch + j] = acc[m][k][q];
+        sums[kT ? j * kPitch + col : col * kPitch + j] = f * acc[m][k][q];
       }
   if (parts > 1)
     cluster_sync_all();
@@ -814,7 +952,8 @@ inline int cluster_parts(int64_t blocks, int64_t most, int64_t length, int64_t l
 // s = x w^T by adapter, w in rows of k (transposed: in rows of the rank); scale s also
 // by row, for the shared product.
 int shrink(const void* x, int64_t ldx, Weights w, bool transposed, Scale scale, const PlanView& plan, int dtype,
-           int64_t m, int64_t k, int adapters, int rank, void* s, void* rows, cudaStream_t stream) {
+           int64_t m, int64_t k, int adapters, int rank, void* s, void* rows, int32_t* exps,
+           cudaStream_t stream) {
   return dispatch(dtype, transposed, rank, [&](auto t, auto tr, auto rp) {
     using T = decltype(t);
     constexpr bool kT = decltype(tr)::value;
@@ -828,14 +967,15 @@ int shrink(const void* x, int64_t ldx, Weights w, bool transposed, Scale scale, 
                   ShrinkCfg<kT, RP>::kBytes, stream, static_cast<const T*>(x), ldx,
                   static_cast<const T*>(w.p), w.stride_l, w.stride_row, plan.perm, plan.offs, adapters,
                   static_cast<int>(k), rank, m * rank, static_cast<T*>(s), scale, plan.taken,
-                  static_cast<T*>(rows));
+                  static_cast<T*>(rows), Range{exps, plan.put, plan.left});
   });
 }
 
 // y += scale s w^T for the rows that the shared product has left, w in rows of the rank
 // (transposed: in rows of n).
 int expand(const void* s, Weights w, bool transposed, Scale scale, const PlanView& plan, int dtype,
-           int64_t m, int64_t n, int adapters, int rank, void* y, int64_t ldy, cudaStream_t stream) {
+           int64_t m, int64_t n, int adapters, int rank, int32_t* exps, void* y, int64_t ldy,
+           cudaStream_t stream) {
   return dispatch(dtype, transposed, rank, [&](auto t, auto tr, auto rp) {
     using T = decltype(t);
     constexpr bool kT = decltype(tr)::value;
@@ -848,7 +988,7 @@ int expand(const void* s, Weights w, bool transposed, Scale scale, const PlanVie
     return launch<&expand_kernel<T, kT, RP>>(dim3(static_cast<unsigned>(units < places ? units : places)),
                   dim3(1, 1), ExpandCfg<kT, RP>::kBytes, stream, static_cast<const T*>(s),
                   m * rank, static_cast<const T*>(w.p), w.stride_l, w.stride_row, scale, plan.perm,
-                  plan.offs, plan.taken, plan.tile, static_cast<int>(PlanView::tiles(m)), splits, adapters,
+                  plan.offs, plan.taken, Range{exps, plan.put, plan.left}, plan.tile, static_cast<int>(PlanView::tiles(m)), splits, adapters,
                   static_cast<int>(n), rank, static_cast<T*>(y), ldy);
   });
 }
@@ -867,9 +1007,9 @@ int grads(const void* t, const void* x, int64_t ldx, int64_t k, void* da, const 
     // Adapters' rows are uneven, so several CTAs a place on the SMs: the largest's rows spread.
     const unsigned parts = cluster_parts(int64_t(blocks) * adapters, 4 * 2 * 148, m / adapters, 64);
     const GradOf<T> a{static_cast<const T*>(t), static_cast<const T*>(x), ldx, static_cast<int>(k),
-                      static_cast<T*>(da)};
+                      static_cast<T*>(da), plan.exps[1]};
     const GradOf<T> b{static_cast<const T*>(s), static_cast<const T*>(dy), lddy, static_cast<int>(n),
-                      static_cast<T*>(db)};
+                      static_cast<T*>(db), plan.exps[0]};
     return launch<&grad_kernel<T, RP>>(dim3(parts, static_cast<unsigned>(blocks), adapters), dim3(parts, 1),
                                        C::kBytes, stream, a, b, blocks_a, m * rank, scale,
                                        static_cast<const int32_t*>(plan.perm),
@@ -914,6 +1054,11 @@ int shared_product(const void* x, int64_t ldx, const void* w, int64_t stride_k, 
 }
 // Adapters that the shared product takes in a tile of rows; none on the 1-SM kernel.
 int per_tile(int rank) { return force_single_sm_kernel() ? 0 : gg::Adapters::most(rank); }
+// Whether expand may have rows to do: of tiles with more adapters than that, or, with fp16,
+// out of the type's range.
+bool may_leave_rows(int adapters, int rank, int dtype) {
+  return adapters > per_tile(rank) || dtype == MOE_DTYPE_F16;
+}
 int64_t low_bytes(int64_t m, int32_t rank) { return 4 * m * rank; }
 // The caller's buffer: x A^T by adapter and dy B by adapter (two parts each), the shared
 // product's operand by row, the plan.
@@ -960,12 +1105,12 @@ extern "C" int32_t moe_lora_forward(const void* x, int64_t ldx, const void* weig
       ids, ids_int64, static_cast<int>(m), adapters, plan, per_tile(rank), status);
   if (cudaGetLastError() != cudaSuccess) return MOE_ERR_CUDA;
   if (m == 0) return MOE_OK;
-  int rc = lora::shrink(x, ldx, a, false, sc, plan, dtype, m, k, adapters, rank, buf.s, buf.rows, st);
+  int rc = lora::shrink(x, ldx, a, false, sc, plan, dtype, m, k, adapters, rank, buf.s, buf.rows, plan.exps[0], st);
   if (rc == MOE_OK)
     rc = shared_product(x, ldx, weight, 1, ldw, y, ldy, plan, b, buf.rows, m, k, n, adapters, rank, dtype, plan.queue,
                         status, st);
-  if (rc == MOE_OK && adapters > per_tile(rank))
-    rc = lora::expand(buf.s, b, false, sc, plan, dtype, m, n, adapters, rank, y, ldy, st);
+  if (rc == MOE_OK && may_leave_rows(adapters, rank, dtype))
+    rc = lora::expand(buf.s, b, false, sc, plan, dtype, m, n, adapters, rank, plan.exps[0], y, ldy, st);
   return rc;
 }
 
@@ -988,12 +1133,12 @@ extern "C" int32_t moe_lora_backward(const void* dy, int64_t lddy, const void* x
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   int rc = MOE_OK;
   if (m > 0 && (dx != nullptr || da != nullptr))
-    rc = lora::shrink(dy, lddy, b, true, sc, plan, dtype, m, n, adapters, rank, buf.t, buf.rows, st);
+    rc = lora::shrink(dy, lddy, b, true, sc, plan, dtype, m, n, adapters, rank, buf.t, buf.rows, plan.exps[1], st);
   if (rc == MOE_OK && m > 0 && dx != nullptr) {
     rc = shared_product(dy, lddy, weight, ldw, 1, dx, lddx, plan, a, buf.rows, m, n, k, adapters, rank, dtype,
                         da != nullptr || db != nullptr ? plan.queue + 1 : nullptr, status, st);
-    if (rc == MOE_OK && adapters > per_tile(rank))
-      rc = lora::expand(buf.t, a, true, sc, plan, dtype, m, k, adapters, rank, dx, lddx, st);
+    if (rc == MOE_OK && may_leave_rows(adapters, rank, dtype))
+      rc = lora::expand(buf.t, a, true, sc, plan, dtype, m, k, adapters, rank, plan.exps[1], dx, lddx, st);
   }
   if (rc == MOE_OK && (da != nullptr || db != nullptr))
     rc = lora::grads(buf.t, x, ldx, k, da, buf.s, dy, lddy, n, db, sc, plan, dtype, m, adapters, rank, st);

@@ -31,7 +31,9 @@ def lora_linear(x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor, lor
     Differentiable (once) in ``x``, ``lora_a`` and ``lora_b``: sums in fp32, the
     gradients in the inputs' type; the product of rank r between the two is rounded to
     that type, with its scale, as the shared product's operand, and held in two parts
-    of it for the gradients.  The shared weight is frozen.  Sizes that are not multiples
+    of it for the gradients.  fp16 keeps fp32's range there: the two parts carry a power
+    of two, and rows that the type cannot hold as that operand are added to the rounded
+    shared product instead.  The shared weight is frozen.  Sizes that are not multiples
     of 8, and rows that do not start on 16 bytes, are copied with padding on every call.
     The graph keeps about 10 r bytes a row beside its inputs.
 
