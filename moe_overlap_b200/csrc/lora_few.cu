@@ -85,8 +85,8 @@ struct Cfg {
 };
 
 struct Ctrl {
-  uint64_t full[12], empty[12], sums;
-  int abort;  // a wait ran out: every role leaves
+  uint64_t full[12], empty[12];
+  int abort;  // a wait ran out: no other waits any more
   int id[64];
   float scale[64];
 };
@@ -110,7 +110,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(smem_u32(&ctrl->full[s]), 1);
       mbar_init(smem_u32(&ctrl->empty[s]), kConsumers);
     }
-    mbar_init(smem_u32(&ctrl->sums), kConsumers);
     ctrl->abort = 0;
     fence_mbar_init();
   }
@@ -151,13 +150,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t b_base = smem_u32(slots) + (cs * NT + g8) * 128;
   const uint32_t off0 = ((2 * q4) ^ g8) * 16, off1 = ((2 * q4 + 1) ^ g8) * 16;
   bool waited = false;
-  // A warp whose wait has run out leaves, but this grid still ends after the one before.
-  auto leave = [&] {
-    give_up(abort_flag, status, MOE_ERR_TIMEOUT);
-    if (!waited) wait_for_previous_kernel();
-  };
-  uint32_t sums_parity = 0;
-  auto sync = [&] { return __all_sync(0xffffffffu, warps_sync(smem_u32(&ctrl->sums), sums_parity, abort_flag)); };
+  // A thread whose wait has run out carries on with what is there, without further waits, so
+  // that every warp still comes to the barriers below.
+  bool failed = false;
   for (int blk = blockIdx.x; blk < blocks; blk += gridDim.x) {
     float acc[J][4];
 #pragma unroll
@@ -165,7 +160,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[j][i] = 0.0f;
     for (int c = 0; c < K; c += BKS) {
-      if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&ctrl->full[stage]), phase, abort_flag))) return leave();
+      if (!failed && !mbar_wait(smem_u32(&ctrl->full[stage]), phase, abort_flag)) {
+        failed = true;
+        give_up(abort_flag, status, MOE_ERR_TIMEOUT);
+      }
+      __syncwarp();
       uint32_t a[2][8];  // rows g8 and g8 + 8, 16 columns each
       const uint32_t sa = a_base + stage * kStageBytes;
       ld_shared_v4(sa + off0, &a[0][0]);
@@ -195,7 +194,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         rb[(j * 8 + 2 * q4 + (i & 1)) * kRedStride + g8 + 8 * (i >> 1)] = acc[j][i];
-    if (!sync()) return leave();
+    asm volatile("bar.sync 1, 256;" ::: "memory");
     if (!waited) wait_for_previous_kernel();  // for `low`
     waited = true;
     const int tid_c = cw * 32 + lane;
@@ -236,7 +235,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (at[q] >= 0) red[at[q]] += c[q] * add[q];
         }
       }
-      if (!sync()) return leave();
+      asm volatile("bar.sync 1, 256;" ::: "memory");
     }
     // One column of W a thread (row n of the block) and every 256 / BM-th row of x, eight of
     // them at a time, so that their adapters' rows are under way together.
@@ -280,7 +279,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           y[(mb + m) * ldy + row] = from_f<T>(v);
         }
       }
-    if (!sync()) return leave();  // the buffer is free again
+    asm volatile("bar.sync 1, 256;" ::: "memory");  // the buffer is free again
   }
 }
 
