@@ -86,6 +86,22 @@ bool rows_ok(const Tensor& t) {
 }
 Tensor with_rows(const Tensor& t) { return rows_ok(t) ? t : t.clone(at::MemoryFormat::Contiguous); }
 
+// For calls, or inputs of them, that pass no gradient on: refused rather than lost without
+// a word.
+bool wants_gradient(const Tensor& t) {
+  return t.defined() && ((at::GradMode::is_enabled() && t.requires_grad()) || t._fw_grad(0).defined());
+}
+void forward_only(const char* op, std::initializer_list<Tensor> inputs) {
+  for (const Tensor& t : inputs)
+    if (wants_gradient(t))
+      refuse(op, " is forward only: detach the inputs that require a gradient, or call it under no_grad");
+}
+// Neither does a forward-mode tangent pass lora_linear.
+void no_tangent(std::initializer_list<Tensor> inputs) {
+  for (const Tensor& t : inputs)
+    if (t.defined() && t._fw_grad(0).defined()) refuse("lora_linear has no forward-mode derivative");
+}
+
 void* data(const Tensor& t) { return const_cast<void*>(t.const_data_ptr()); }
 
 // ------------------------------------------------------------ few tokens --
@@ -148,6 +164,7 @@ std::tuple<Tensor, Tensor, Tensor> moe_few_tokens_op(const Tensor& x, const Tens
                                                      const Tensor& w2, int64_t top_k,
                                                      const std::optional<Tensor>& router_bias, bool renormalize,
                                                      const std::optional<Tensor>& out) {
+  forward_only("moe_few_tokens", {x, router_w, w1, w2, router_bias.value_or(Tensor()), out.value_or(Tensor())});
   if (router_w.dim() != 2 || w1.dim() != 3 || x.dim() < 1 || router_w.size(0) != w1.size(0) ||
       router_w.size(1) != x.size(-1))
     refuse("router_w must be [E, H]");
@@ -166,6 +183,7 @@ std::tuple<Tensor, Tensor, Tensor> moe_few_tokens_op(const Tensor& x, const Tens
 
 Tensor experts_few_tokens_op(const Tensor& x, const Tensor& w1, const Tensor& w2, const Tensor& topk_idx,
                              const Tensor& topk_w, const std::optional<Tensor>& out) {
+  forward_only("experts_few_tokens", {x, w1, w2, topk_w, out.value_or(Tensor())});
   if (topk_idx.dim() != 2 || x.dim() < 1 || topk_idx.size(0) != x.size(0) || topk_w.sizes() != topk_idx.sizes())
     refuse("topk_idx and topk_w must be [T, k]");
   if (topk_idx.device() != x.device() || topk_w.device() != x.device())
@@ -267,6 +285,7 @@ Tensor pad(const Tensor& t, int64_t last, int64_t before_last) {
 
 Tensor lora_linear_op(const Tensor& x, const Tensor& weight, const Tensor& lora_a, const Tensor& lora_b,
                       const Tensor& adapter_ids, const std::optional<Tensor>& scale_in, double scale_all) {
+  no_tangent({x, weight, lora_a, lora_b, scale_in.value_or(Tensor())});
   if (!x.is_cuda()) refuse("lora_linear requires CUDA tensors.");
   const char* shapes = "Shapes must be x [M, K], weight [N, K], lora_a [L, r, K], lora_b [L, N, r].";
   if (x.dim() != 2 || weight.dim() != 2 || lora_a.dim() != 3 || lora_b.dim() != 3) refuse(shapes);

@@ -8,8 +8,9 @@ weights once (src/train_moe_baseline.py:315-441 without the exchange):
 * ``moe_few_tokens``: gate, top-k, experts and weighted sum;
 * ``experts_few_tokens``: the same from a routing that the caller has.
 
-Forward only.  Both can be captured into a CUDA graph and allocate only torch
-tensors on the current stream.
+Forward only: inputs that require a gradient are refused while gradients are recorded.
+Both can be captured into a CUDA graph and allocate only torch tensors on the current
+stream.
 """
 from __future__ import annotations
 

@@ -389,7 +389,8 @@ class MoELayer:
         no exchange (few_tokens.moe_few_tokens), so one rank must hold every expert.
         ``routing`` = (topk_idx, topk_w) to reuse; slots of -1 (padding) add nothing.
         Unlike ``route``, which rounds the gate's logits to bf16, the logits keep
-        64 bits here.  Forward only.
+        64 bits here.  Forward only: the layer's weights are taken detached, and ``x`` or
+        routing weights that require a gradient are refused (call it under ``no_grad``).
         """
         if self.world != 1 or self._slot_of_expert is not None:
             raise ValueError("forward_few needs every expert on this rank, in contiguous placement")
@@ -398,8 +399,9 @@ class MoELayer:
         if routing is not None:
             idx, w = routing
             return experts_few_tokens(x, w1, w2, idx, w, out=out), idx, w
+        bias = self.router_b.detach() if self.router_b is not None else None
         return moe_few_tokens(x, self.router_w.detach(), w1, w2, self.top_k,
-                              router_bias=self.router_b, renormalize=self.renormalize, out=out)
+                              router_bias=bias, renormalize=self.renormalize, out=out)
 
     def forward_serialized(self, x: torch.Tensor, routing,
                            host_cover_cycles: int = 2_000_000) -> tuple[torch.Tensor, dict]:

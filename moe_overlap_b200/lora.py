@@ -28,7 +28,7 @@ def lora_linear(x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor, lor
     row without adapter, and an id outside [-1, L) counts as -1 and raises ``MoeError``
     at a later call.  ``scale`` is a number or a float tensor [L].
 
-    Differentiable (once) in ``x``, ``lora_a`` and ``lora_b``: sums in fp32, the
+    Differentiable (once, in reverse mode) in ``x``, ``lora_a`` and ``lora_b``: sums in fp32, the
     gradients in the inputs' type; the product of rank r between the two is rounded to
     that type, with its scale, as the shared product's operand, and held in two parts
     of it for the gradients.  fp16 keeps fp32's range there: the two parts carry a power
