@@ -125,6 +125,8 @@ Tensor few(const Tensor& x_in, const Tensor* router_w, const Tensor* router_bias
     out = *out_in;
     if (out.dim() != 2 || out.size(0) != tokens || out.size(1) != hidden) refuse("out must be [T, H]");
     check_weights("out", out, x);
+    // what autograd has saved of it is not what it was
+    if (!out.is_inference()) out.unsafeGetTensorImpl()->bump_version();
   } else {
     out = at::empty({tokens, hidden}, x.options());
   }

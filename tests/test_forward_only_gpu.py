@@ -1,4 +1,4 @@
-"""The forward-only calls and autograd."""
+"""What the forward-only calls do to autograd: refuse gradients, and mark `out` as written."""
 import pytest
 import torch
 
@@ -25,3 +25,18 @@ def test_layer_refuses_a_gradient_and_runs_without_one(cuda_device):
             assert torch.equal(layer.forward_few(x)[0], want)
     finally:
         layer.close()
+
+
+def test_out_is_marked_as_written(cuda_device):
+    """A product saved from `out` before the call may not be differentiated after it."""
+    x, rw, w1, w2 = make(3, 4, 64, 72, torch.bfloat16, device=cuda_device)
+    out = torch.ones(3, 64, dtype=x.dtype, device=cuda_device)
+    p = torch.ones_like(out, requires_grad=True)
+    y = (p * out).sum()
+    mo.moe_few_tokens(x, rw, w1, w2, 2, out=out)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.backward()
+    with torch.inference_mode():
+        again = torch.empty_like(x)
+        mo.moe_few_tokens(x, rw, w1, w2, 2, out=again)
+    assert torch.equal(again, out)
