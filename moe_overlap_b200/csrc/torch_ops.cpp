@@ -53,20 +53,32 @@ template <typename... A>
 
 py::object lib() { return py::module_::import("moe_overlap_b200._lib"); }
 
-// The device's status word; raises what an earlier kernel has recorded there.
+// The device's status word; raises what an earlier kernel has recorded there.  (Both
+// functions take the GIL where they need it: a backward pass runs without.)
 int32_t* checked_status(c10::Device device) {
   int32_t*& word = status_words[device.index()];
-  if (word == nullptr) lib().attr("status_word")(py::cast(device));
-  if (*static_cast<volatile int32_t*>(word) != MOE_OK) lib().attr("check_status")(py::cast(device));
+  if (word == nullptr) {
+    const py::gil_scoped_acquire gil;
+    lib().attr("status_word")(py::cast(device));
+  }
+  if (*static_cast<volatile int32_t*>(word) != MOE_OK) {
+    const py::gil_scoped_acquire gil;
+    lib().attr("check_status")(py::cast(device));
+  }
   return word;
 }
 
 void check_call(int32_t code, const char* where, c10::Device device) {
-  if (code != MOE_OK) lib().attr("check_call")(code, where);
+  if (code != MOE_OK) {
+    const py::gil_scoped_acquire gil;
+    lib().attr("check_call")(code, where);
+  }
   // MOE_B200_SYNC_CHECK=1: wait for the kernels and raise what they have recorded
   const char* env = std::getenv("MOE_B200_SYNC_CHECK");
-  if (env != nullptr && *env != 0 && std::strcmp(env, "0") != 0)
+  if (env != nullptr && *env != 0 && std::strcmp(env, "0") != 0) {
+    const py::gil_scoped_acquire gil;
     lib().attr("check_status")(py::cast(device), true);
+  }
 }
 
 void* stream_of(c10::Device device) { return c10::cuda::getCurrentCUDAStream(device.index()).stream(); }
@@ -251,6 +263,7 @@ struct LoraLinear : torch::autograd::Function<LoraLinear> {
     const Sizes z(x, weight, a);
     const Tensor dy = with_rows(grads[0]);
     const c10::Device dev = x.device();
+    int32_t* status = checked_status(dev);
     const c10::cuda::OptionalCUDAGuard guard(dev);
     Tensor dx, da, db;
     if (ctx->needs_input_grad(0)) dx = at::empty({z.m, z.k}, x.options());
@@ -261,8 +274,8 @@ struct LoraLinear : torch::autograd::Function<LoraLinear> {
         a.stride(1), data(b), b.stride(0), b.stride(1), scale_data(scale),
         static_cast<float>(ctx->saved_data["scale"].toDouble()), dtype_code(x), z.m, z.k, z.n, z.adapters,
         z.rank, data(kept), dx.defined() ? data(dx) : nullptr, z.k, da.defined() ? data(da) : nullptr,
-        db.defined() ? data(db) : nullptr, status_words[dev.index()], stream_of(dev));
-    TORCH_CHECK(rc == MOE_OK, "moe_lora_backward: status ", rc);
+        db.defined() ? data(db) : nullptr, status, stream_of(dev));
+    check_call(rc, "moe_lora_backward", dev);
     return {dx, Tensor(), da, db, Tensor(), Tensor(), Tensor()};
   }
 };
