@@ -6,12 +6,17 @@
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/autograd/variable.h>
 #include <torch/extension.h>
 
 #include <cstdlib>
 #include <cstring>
+#include <memory>
 #include <sstream>
+#include <unordered_set>
+#include <vector>
 
 #include "../../include/moe_overlap.h"
 
@@ -240,6 +245,53 @@ std::pair<Tensor, Tensor> lora_forward(const Tensor& x, const Tensor& weight, co
   return {y, kept};
 }
 
+// A leaf's gradient accumulator belongs to the stream that it was made on and lives as
+// long as any graph of the leaf.  Under capture, one from another stream would pull that
+// stream into the captured backward and break the capture in the autograd engine.
+bool capturing() {
+  return c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None;
+}
+void refuse_foreign(torch::autograd::Node& accumulator) {
+  const auto stream = accumulator.stream();
+  if (!stream.has_value() || *stream == c10::cuda::getCurrentCUDAStream(stream->device_index()).unwrap()) return;
+  // (the legacy stream is never captured, and may not be asked)
+  const cudaStream_t raw = c10::cuda::CUDAStream(*stream).stream();
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  if (raw != nullptr && cudaStreamIsCapturing(raw, &status) == cudaSuccess && status == cudaStreamCaptureStatusActive)
+    return;
+  throw std::runtime_error(
+      "lora_linear: a gradient accumulator of the captured step's inputs belongs to a stream outside the capture: "
+      "a graph of the same leaves from before is alive, or something else (a hook, a data-parallel wrapper) holds "
+      "the accumulator; drop it before capturing a training step");
+}
+// In the forward the inputs that are leaves, whatever the pass will ask for.
+void refuse_foreign_graphs(const Tensor& leaf) {
+  if (!leaf.requires_grad() || !leaf.is_leaf()) return;
+  const auto node = torch::autograd::impl::try_get_grad_accumulator(leaf);
+  if (node != nullptr) refuse_foreign(*node);
+}
+// In the backward those that this pass will come to behind its inputs (adapters cast from
+// the leaves that are trained).
+void refuse_foreign_graphs_behind(const std::shared_ptr<torch::autograd::Node>& node) {
+  const auto* run = torch::autograd::get_current_graph_task_exec_info();
+  std::vector<torch::autograd::Node*> next{node.get()};
+  std::unordered_set<torch::autograd::Node*> seen{node.get()};
+  while (!next.empty()) {
+    torch::autograd::Node* at = next.back();
+    next.pop_back();
+    if (dynamic_cast<torch::autograd::AccumulateGrad*>(at) != nullptr) refuse_foreign(*at);
+    for (const auto& edge : at->next_edges()) {
+      torch::autograd::Node* to = edge.function.get();
+      if (to == nullptr || !seen.insert(to).second) continue;
+      if (run != nullptr && !run->empty()) {
+        const auto it = run->find(to);
+        if (it == run->end() || !it->second.should_execute()) continue;
+      }
+      next.push_back(to);
+    }
+  }
+}
+
 // x [M, K], a [L, r, K], b [L, N, r] -> y [M, N]; the weight, the ids and the scale get no
 // gradient.
 struct LoraLinear : torch::autograd::Function<LoraLinear> {
@@ -257,6 +309,7 @@ struct LoraLinear : torch::autograd::Function<LoraLinear> {
                                                  torch::autograd::variable_list grads) {
     TORCH_CHECK(!at::GradMode::is_enabled(),
                 "lora_linear can be differentiated once: its backward takes no create_graph");
+    if (capturing()) refuse_foreign_graphs_behind(torch::autograd::get_current_node());
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &weight = saved[1], &a = saved[2], &b = saved[3], &kept = saved[4],
                  &scale = saved[5];
@@ -279,20 +332,6 @@ struct LoraLinear : torch::autograd::Function<LoraLinear> {
     return {dx, Tensor(), da, db, Tensor(), Tensor(), Tensor()};
   }
 };
-
-// A leaf's gradient accumulator belongs to the stream that it was made on and lives as
-// long as any graph of the leaf.  Under capture, one from another stream would pull that
-// stream into the captured backward and break the capture in the autograd engine.
-void refuse_foreign_graphs(const Tensor& leaf) {
-  if (!leaf.requires_grad() || !leaf.is_leaf()) return;
-  const auto node = torch::autograd::impl::try_get_grad_accumulator(leaf);
-  if (node == nullptr) return;
-  const auto stream = node->stream();
-  if (stream.has_value() && *stream != c10::cuda::getCurrentCUDAStream(leaf.device().index()).unwrap())
-    throw std::runtime_error(
-        "lora_linear: a graph of the same inputs from outside the capture is alive; drop its outputs before "
-        "capturing a training step");
-}
 
 Tensor pad(const Tensor& t, int64_t last, int64_t before_last) {
   return last == 0 && before_last == 0 ? t : at::constant_pad_nd(t, {0, last, 0, before_last}, 0);
@@ -337,7 +376,7 @@ Tensor lora_linear_op(const Tensor& x, const Tensor& weight, const Tensor& lora_
                ids = adapter_ids.contiguous();
   Tensor y;
   if (grad_mode && (x.requires_grad() || lora_a.requires_grad() || lora_b.requires_grad())) {
-    if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) {
+    if (capturing()) {
       refuse_foreign_graphs(x);
       refuse_foreign_graphs(lora_a);
       refuse_foreign_graphs(lora_b);

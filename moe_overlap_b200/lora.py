@@ -39,7 +39,9 @@ def lora_linear(x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor, lor
 
     A training step can be captured into a CUDA graph (forward and backward together);
     as for every autograd graph, no graph of the same leaves from before the capture
-    may be alive then, which is refused.
+    may be alive then, nor anything else that holds their gradient accumulators, which
+    is refused: in the forward for inputs that are leaves, in the backward for leaves
+    that the inputs were computed from.
     """
     if isinstance(scale, torch.Tensor):
         return _lib.torch_ops().lora_linear(x, weight, lora_a, lora_b, adapter_ids, scale, 0.0)
