@@ -387,7 +387,8 @@ class MoELayer:
 
         One pass over the weights of the experts taken, on the caller's stream, with
         no exchange (few_tokens.moe_few_tokens), so one rank must hold every expert.
-        ``routing`` = (topk_idx, topk_w) to reuse; slots of -1 (padding) add nothing.
+        ``routing`` = what ``route`` gives, (probs, topk_idx, topk_w), or (topk_idx, topk_w),
+        to reuse; slots of -1 (padding) add nothing.
         Unlike ``route``, which rounds the gate's logits to bf16, the logits keep
         64 bits here.  Forward only: the layer's weights are taken detached, and ``x`` or
         routing weights that require a gradient are refused (call it under ``no_grad``).
@@ -397,7 +398,9 @@ class MoELayer:
         x = x.to(torch.bfloat16)
         w1, w2 = self.w1.detach(), self.w2.detach()
         if routing is not None:
-            idx, w = routing
+            if len(routing) not in (2, 3):
+                raise ValueError("routing must be (probs, topk_idx, topk_w) or (topk_idx, topk_w)")
+            idx, w = routing[-2:]
             return experts_few_tokens(x, w1, w2, idx, w, out=out), idx, w
         bias = self.router_b.detach() if self.router_b is not None else None
         return moe_few_tokens(x, self.router_w.detach(), w1, w2, self.top_k,
