@@ -949,11 +949,22 @@ inline int cluster_parts(int64_t blocks, int64_t most, int64_t length, int64_t l
   return parts;
 }
 
+// The current device's SMs, for the rules below.
+inline int device_sms(int* sms) {
+  int dev;
+  DeviceInfo info;
+  const int rc = current_device_info(&dev, &info);
+  if (rc == MOE_OK) *sms = info.sm_count;
+  return rc;
+}
+
 // s = x w^T by adapter, w in rows of k (transposed: in rows of the rank); scale s also
 // by row, for the shared product.
 int shrink(const void* x, int64_t ldx, Weights w, bool transposed, Scale scale, const PlanView& plan, int dtype,
            int64_t m, int64_t k, int adapters, int rank, void* s, void* rows, int32_t* exps,
            cudaStream_t stream) {
+  int sms;
+  if (const int rc = device_sms(&sms); rc != MOE_OK) return rc;
   return dispatch(dtype, transposed, rank, [&](auto t, auto tr, auto rp) {
     using T = decltype(t);
     constexpr bool kT = decltype(tr)::value;
@@ -962,7 +973,7 @@ int shrink(const void* x, int64_t ldx, Weights w, bool transposed, Scale scale, 
     // Few rows leave half of the SMs to the shared product, which starts at once on those
     // (4096 rows of 2048 x 2048, a step: 104.8 us, and 111.5 with all SMs taken); many take
     // two CTAs an SM (16384 rows: 1048 us, and 1098 with one part).
-    const unsigned parts = cluster_parts(tiles, tiles <= 74 ? 74 : 296, k, 256);
+    const unsigned parts = cluster_parts(tiles, int(tiles) <= sms / 2 ? sms / 2 : 2 * sms, k, 256);
     return launch<&shrink_kernel<T, kT, RP>>(dim3(tiles, parts), dim3(1, parts),
                   ShrinkCfg<kT, RP>::kBytes, stream, static_cast<const T*>(x), ldx,
                   static_cast<const T*>(w.p), w.stride_l, w.stride_row, plan.perm, plan.offs, adapters,
@@ -976,15 +987,18 @@ int shrink(const void* x, int64_t ldx, Weights w, bool transposed, Scale scale, 
 int expand(const void* s, Weights w, bool transposed, Scale scale, const PlanView& plan, int dtype,
            int64_t m, int64_t n, int adapters, int rank, int32_t* exps, void* y, int64_t ldy,
            cudaStream_t stream) {
+  int sms;
+  if (const int rc = device_sms(&sms); rc != MOE_OK) return rc;
   return dispatch(dtype, transposed, rank, [&](auto t, auto tr, auto rp) {
     using T = decltype(t);
     constexpr bool kT = decltype(tr)::value;
     constexpr int RP = decltype(rp)::value;
     const int64_t blocks = (n + kExpandCols - 1) / kExpandCols;
-    // Work for about four CTAs a place on the SMs, if every row were left.
-    const int64_t tiles = most_tiles(m, adapters, kExpandRows), want = (1200 + tiles - 1) / tiles;
+    // Two CTAs an SM; work for about four times as many, if every row were left.
+    const int64_t places = 2 * sms, tiles = most_tiles(m, adapters, kExpandRows);
+    const int64_t want = (4 * places + tiles - 1) / tiles;
     const int splits = static_cast<int>(want < blocks ? want : blocks);
-    const int64_t units = tiles * splits, places = 2 * 148;
+    const int64_t units = tiles * splits;
     return launch<&expand_kernel<T, kT, RP>>(dim3(static_cast<unsigned>(units < places ? units : places)),
                   dim3(1, 1), ExpandCfg<kT, RP>::kBytes, stream, static_cast<const T*>(s),
                   m * rank, static_cast<const T*>(w.p), w.stride_l, w.stride_row, scale, plan.perm,
@@ -998,14 +1012,19 @@ int expand(const void* s, Weights w, bool transposed, Scale scale, const PlanVie
 int grads(const void* t, const void* x, int64_t ldx, int64_t k, void* da, const void* s, const void* dy,
           int64_t lddy, int64_t n, void* db, Scale scale, const PlanView& plan, int dtype, int64_t m,
           int adapters, int rank, cudaStream_t stream) {
+  int sms;
+  if (const int rc = device_sms(&sms); rc != MOE_OK) return rc;
   return dispatch(dtype, false, rank, [&](auto tt, auto, auto rp) {
     using T = decltype(tt);
     constexpr int RP = decltype(rp)::value;
     using C = GradCfg<RP>;
     const int blocks_a = da != nullptr ? static_cast<int>((k + C::kCols - 1) / C::kCols) : 0;
     const int blocks = blocks_a + (db != nullptr ? static_cast<int>((n + C::kCols - 1) / C::kCols) : 0);
-    // Adapters' rows are uneven, so several CTAs a place on the SMs: the largest's rows spread.
-    const unsigned parts = cluster_parts(int64_t(blocks) * adapters, 4 * 2 * 148, m / adapters, 64);
+    // Parts of an adapter's rows, as many as leave about four CTAs for each of the two places on
+    // an SM, since adapters' rows are uneven.  The rule knows the adapters' average only: where
+    // many columns and adapters leave one part, a single adapter with most of the rows is
+    // summed by its column blocks alone.
+    const unsigned parts = cluster_parts(int64_t(blocks) * adapters, 4 * 2 * sms, m / adapters, 64);
     const GradOf<T> a{static_cast<const T*>(t), static_cast<const T*>(x), ldx, static_cast<int>(k),
                       static_cast<T*>(da), plan.exps[1]};
     const GradOf<T> b{static_cast<const T*>(s), static_cast<const T*>(dy), lddy, static_cast<int>(n),
@@ -1095,7 +1114,10 @@ extern "C" int32_t moe_lora_forward(const void* x, int64_t ldx, const void* weig
     return MOE_ERR_INVALID_ARG;
   const lora::Scale sc{scale, scale_all};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (!for_backward && m > 0 && lora::takes_few_rows(m, k, n, rank))
+  int sms = 0;
+  if (m > 0)
+    if (const int rc = lora::device_sms(&sms); rc != MOE_OK) return rc;
+  if (!for_backward && m > 0 && lora::takes_few_rows(m, k, n, rank, sms))
     return lora::forward_few_rows(x, ldx, weight, ldw, a, b, ids, ids_int64, sc, dtype,
                                   static_cast<int>(m), static_cast<int>(k), static_cast<int>(n), adapters,
                                   rank, y, ldy, static_cast<float*>(kept), status, st);

@@ -20,8 +20,9 @@ struct Weights {  // of all adapters
   int64_t stride_l, stride_row;
 };
 
-// Whether a batch of which no gradient is wanted takes the kernels of lora_few.cu.
-bool takes_few_rows(int64_t m, int64_t k, int64_t n, int rank);
+// Whether a batch of which no gradient is wanted takes the kernels of lora_few.cu on a
+// device of `sms` SMs.
+bool takes_few_rows(int64_t m, int64_t k, int64_t n, int rank, int sms);
 
 // y = x weight^T + scale (x a^T) b^T by row for such a batch; low: float [m][rank].
 int forward_few_rows(const void* x, int64_t ldx, const void* weight, int64_t ldw, Weights a, Weights b,

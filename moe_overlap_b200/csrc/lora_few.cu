@@ -353,7 +353,7 @@ int forward(const void* x, int64_t ldx, const void* weight, int64_t ldw, Weights
 
 }  // namespace few
 
-bool takes_few_rows(int64_t m, int64_t k, int64_t n, int rank) {
+bool takes_few_rows(int64_t m, int64_t k, int64_t n, int rank, int sms) {
   // The rows of x and the adapters' products cost each block of W; the tensor-core path is
   // faster from about here on.  Measured, here and there, 8 adapters: 2048 x 2048, 48 rows of
   // rank 64 18.5 and 22.6 us, 64 rows 22.6 and 22.6; 512 x 1024, 32 rows of rank 128 16.5
@@ -368,7 +368,7 @@ bool takes_few_rows(int64_t m, int64_t k, int64_t n, int rank) {
   // (2048 x 2048 at rank 16, 128 rows: 12.7 and 22.0 us, 192 rows: 20.6 and 19.3), while
   // x A^T, by the CUDA cores, stays small.
   const int64_t blocks = (m + 63) / 64 * ((n + (wide ? 63 : 31)) / (wide ? 64 : 32));
-  return blocks <= 148 && m * rank * k <= (int64_t(1) << 25);
+  return blocks <= sms && m * rank * k <= (int64_t(1) << 25);
 }
 
 int forward_few_rows(const void* x, int64_t ldx, const void* weight, int64_t ldw, Weights a, Weights b,
