@@ -719,7 +719,7 @@ struct GradOf {
 };
 
 template <typename T, bool kT, int RP>
-__device__ __forceinline__ void grad_block(char* smem, const GradOf<T>& of, int block, int64_t part_stride,
+__device__ __forceinline__ void grad_block(char* smem, const GradOf<T>& of, int block, int parts, int64_t part_stride,
                                            Scale scale, const int32_t* perm, const int32_t* offs, int r) {
   using C = GradCfg<RP>;
   constexpr int MT = C::MT;
@@ -728,7 +728,7 @@ __device__ __forceinline__ void grad_block(char* smem, const GradOf<T>& of, int 
   const int n = of.n;
   T* g = of.g;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int parts = gridDim.x, part = blockIdx.x, n0 = block * C::kCols, i = blockIdx.z;
+  const int part = blockIdx.x % parts, n0 = block * C::kCols, i = blockIdx.y;
   const int o0 = offs[i], rows = offs[i + 1] - o0;
   const int share = ((rows + parts - 1) / parts + kGradRows - 1) / kGradRows * kGradRows;
   const int p0 = min(rows, part * share), p1 = min(rows, p0 + share);
@@ -881,21 +881,22 @@ __device__ __forceinline__ void grad_block(char* smem, const GradOf<T>& of, int 
   if (parts > 1) cluster_sync_all();
 }
 
-// dA and dB in one launch: the first blocks_a blocks of columns are dA's.
+// dA and dB in one launch: the first blocks_a blocks of columns are dA's.  Blocks and their
+// parts share the grid's x, the one direction that takes any number of them.
 template <typename T, int RP>
 __global__ void __launch_bounds__(kThreads, 2)
-    grad_kernel(GradOf<T> a, GradOf<T> b, int blocks_a, int64_t part_stride, Scale scale,
+    grad_kernel(GradOf<T> a, GradOf<T> b, int blocks_a, int parts, int64_t part_stride, Scale scale,
                 const int32_t* perm, const int32_t* offs, int r, int32_t* queue) {
   extern __shared__ __align__(128) char smem[];
   wait_for_previous_kernel();
   let_next_kernel_start();
-  const int block = blockIdx.y;
+  const int block = blockIdx.x / parts;
   // the shared product before is done with its counter: 0 again for another pass
-  if (block == 0 && blockIdx.x == 0 && blockIdx.z == 0 && threadIdx.x == 0) *queue = 0;
+  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *queue = 0;
   if (block < blocks_a)
-    grad_block<T, true, RP>(smem, a, block, part_stride, scale, perm, offs, r);
+    grad_block<T, true, RP>(smem, a, block, parts, part_stride, scale, perm, offs, r);
   else
-    grad_block<T, false, RP>(smem, b, block - blocks_a, part_stride, scale, perm, offs, r);
+    grad_block<T, false, RP>(smem, b, block - blocks_a, parts, part_stride, scale, perm, offs, r);
 }
 
 template <auto kern, typename... A>
@@ -1029,8 +1030,8 @@ int grads(const void* t, const void* x, int64_t ldx, int64_t k, void* da, const 
                       static_cast<T*>(da), plan.exps[1]};
     const GradOf<T> b{static_cast<const T*>(s), static_cast<const T*>(dy), lddy, static_cast<int>(n),
                       static_cast<T*>(db), plan.exps[0]};
-    return launch<&grad_kernel<T, RP>>(dim3(parts, static_cast<unsigned>(blocks), adapters), dim3(parts, 1),
-                                       C::kBytes, stream, a, b, blocks_a, m * rank, scale,
+    return launch<&grad_kernel<T, RP>>(dim3(parts * static_cast<unsigned>(blocks), adapters), dim3(parts, 1),
+                                       C::kBytes, stream, a, b, blocks_a, static_cast<int>(parts), m * rank, scale,
                                        static_cast<const int32_t*>(plan.perm),
                                        static_cast<const int32_t*>(plan.offs), rank, plan.queue + 1);
   });
