@@ -8,8 +8,9 @@
 // (the routed path of src/train_moe_baseline.py:315-441 at decode batch sizes).
 // A slot with expert -1 adds nothing; a token without any expert gets zeros.
 // Sums are fp32 (the gate's fp64); h is held as two values of the input type, the rounded
-// one and what the rounding left, since it is the operand of a second tensor-core product
-// and the weights' bytes, not the products, bound the time; the output is rounded once.
+// one and what the rounding left, since it is the operand of a second tensor-core product:
+// 16 bits of bf16; of fp16 22 bits, but not below 2^-25, and up to 131008 (an fp16 h of its
+// own ends at 65504).  The output is rounded once.
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -30,7 +31,8 @@ constexpr int kMaxK = 16;
 constexpr int kWarps = 8;
 
 // Dot product of two rows of `n` elements (a multiple of 8, 16-byte aligned) over one
-// warp.  A product of two bf16 or fp16 values is exact in fp32; the sum is fp64.
+// warp.  A product of two bf16 or fp16 values is exact in fp32 (of bf16 within fp32's
+// range); the sum is fp64.
 template <typename T>
 __device__ __forceinline__ double warp_dot(const T* a, const T* b, int n, int lane) {
   double s = 0;
@@ -158,7 +160,8 @@ __global__ void __cluster_dims__(kGateCluster, 1, 1) __launch_bounds__(32 * kWar
 }
 
 // ------------------------------------------------------------ the experts --
-// One persistent kernel streams the weights of the experts taken exactly once.
+// One persistent kernel streams the weights of the experts taken, once for each group of at
+// most 8 J of an expert's slots; an expert's later groups find them in L2 for the most part.
 // A work item is BM rows of W1[e] (all of hidden) for one group of at most 8 J slots
 // of expert e, or BM rows of W2[e] (one of KS parts of ffn) for such a group.  Items
 // are taken from a ticket counter, all of W1's before any of W2's; the items of W2
@@ -176,14 +179,17 @@ __global__ void __cluster_dims__(kGateCluster, 1, 1) __launch_bounds__(32 * kWar
 // half of an item's slots each: a stage is R tiles of 16 rows x C = 8/R slices of 64
 // columns, one (tile, slice) per warp of a set, m16n8k16 with the weights as the 16-row side and the slots as the 8-column side.
 // (tcgen05's 128-row tiles would leave too few items for 148 SMs at one token, and
-// the tensor work here is a few percent of the time either way.)  The order of k
+// at a few slots an expert the tensor work is a few percent of the time.)  The order of k
 // inside a slice is free, so lane (g, q) takes the 16 contiguous columns 16q.. of its
 // rows and of its slot: both come by conflict-free 16-byte shared loads.
 //
-// Bound by reading the weights of the experts taken.  Gate and experts together, measured:
-// 16 tokens, 16 experts of 2048 x 8192, top-2: 141 us, 6.7 TB/s; 64 tokens of the same
-// 173-178 us, 6.0-6.2 TB/s; one token of 2048 x 4096: 28.6 us, of which some 15 read weights and
-// the rest is the chain from the gate to the last sum.
+// Bound at a few slots an expert by reading the weights of the experts taken.  Gate and
+// experts together, measured: 16 tokens, 16 experts of 2048 x 8192, top-2: 140-146 us,
+// 6.5-6.7 TB/s; 64 tokens of the same 173-178 us, 6.0-6.2 TB/s; one token of 2048 x 4096: 28.3 us,
+// of which some 15 read weights and the rest is the chain from the gate to the last sum.
+// At many slots an expert (41: 46 tokens, top-8 of 9 x 1712 x 6320, 179 us) by the slots'
+// way through shared memory and registers once a row block: DRAM is at 28 % then, the
+// shared-memory pipe at 53 %, the tensor pipe at 28 %.
 constexpr int kConsumers = 8;
 constexpr int kSets = 2;         // of consumers
 // Warps that copy slots: more than their rows need only add arrivals to every stage (16

@@ -342,11 +342,6 @@ __device__ __forceinline__ void add_parts(const float* sums, uint32_t crank, int
   }
 }
 
-// 144 registers: with 10 warps, SM sub-partitions 0 and 1 hold three of them
-// (3 x 32 x 144 = 13,824 of their 16,384 registers), which leaves room for one
-// warp per sub-partition of a 4-warp exchange block at <= 80 registers, so the
-// dispatch/combine kernels run beside this persistent kernel.  PUSH compiles the
-// expert-parallel combine push into the epilogue (rows go to their source ranks).
 struct NoAdapters {
   static constexpr int kParts = 1;
 };
@@ -357,6 +352,11 @@ struct SplitAdapters : AdapterMaps {
   static_assert(P == 1 || P == 2 || P == 4, "clusters of up to 8 CTAs");
 };
 
+// 144 registers: with 10 warps, SM sub-partitions 0 and 1 hold three of them
+// (3 x 32 x 144 = 13,824 of their 16,384 registers), which leaves room for one
+// warp per sub-partition of a 4-warp exchange block at <= 80 registers, so the
+// dispatch/combine kernels run beside this persistent kernel.  PUSH compiles the
+// expert-parallel combine push into the epilogue (rows go to their source ranks).
 template <bool BF16, bool B_MN_MAJOR, bool PUSH, class EXTRA>
 __global__ void __cluster_dims__(2 * EXTRA::kParts, 1, 1) __maxnreg__(kMaxRegs)
     grouped_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a,

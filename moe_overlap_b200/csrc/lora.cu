@@ -87,7 +87,10 @@ __device__ __forceinline__ int id_at(const void* ids, int ids64, int m, int L) {
 // Blocks 0 .. L-1 each take one adapter: they count the rows of smaller adapters (the
 // segment's start) and write their own rows in order.  Blocks L .. take one row tile each:
 // the adapters in it, which rows are whose, and whether the shared product takes them.
-// No block depends on another and the order is always the same.
+// No block depends on another and the order is always the same.  Every adapter's block reads
+// all ids (from L2): nothing beside the products at tens of adapters, but 1024 of them take
+// 0.05 ms more at 16384 rows and 0.6 ms at a million (64 x 64 products, with what expand
+// then costs).
 __global__ void __launch_bounds__(1024) plan_kernel(const void* ids, int ids64, int M, int L, PlanView plan,
                                                     int per_tile, int32_t* status) {
   let_next_kernel_start();

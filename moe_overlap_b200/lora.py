@@ -28,14 +28,19 @@ def lora_linear(x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor, lor
     row without adapter, and an id outside [-1, L) counts as -1 and raises ``MoeError``
     at a later call.  ``scale`` is a number or a float tensor [L].
 
-    Differentiable (once, in reverse mode) in ``x``, ``lora_a`` and ``lora_b``: sums in fp32, the
-    gradients in the inputs' type; the product of rank r between the two is rounded to
-    that type, with its scale, as the shared product's operand, and held in two parts
-    of it for the gradients.  fp16 keeps fp32's range there: the two parts carry a power
-    of two, and rows that the type cannot hold as that operand are added to the rounded
-    shared product instead.  The shared weight is frozen.  Sizes that are not multiples
-    of 8, and rows that do not start on 16 bytes, are copied with padding on every call.
-    The graph keeps about 10 r bytes a row beside its inputs.
+    Sums are fp32.  The product of rank r is rounded to the inputs' type, with its scale, as
+    an operand of the shared product, whose sum is rounded once.  Decode batches hold it in
+    fp32 instead; rows of tiles with too many adapters, and rows of fp16 whose operand the
+    type does not hold (largest value beyond 65504 or below 2^-14), hold it in two parts of
+    the type and are added to the rounded shared product.  So a row's last bit depends on
+    the batch that it is in.
+
+    Differentiable (once, in reverse mode) in ``x``, ``lora_a`` and ``lora_b``, with the
+    gradients in the inputs' type.  For them the product of rank r is held in two parts of
+    the type, in fp16 with a power of two, so that small gradients lose nothing.  The shared
+    weight is frozen.  Sizes that are not multiples of 8, and rows that do not start on 16
+    bytes, are copied with padding on every call.  The graph keeps about 10 r bytes a row
+    beside its inputs.
 
     A training step can be captured into a CUDA graph (forward and backward together);
     as for every autograd graph, no graph of the same leaves from before the capture
