@@ -17,7 +17,9 @@
 // range (dy B of gradients of 1e-5 lies below its normal numbers, where the second part is
 // nothing), so s is scaled before it is split: by a power of two common to 16 rows of an
 // adapter, the grads' step, which puts their largest between 2^6 and 2^14; what is lost is
-// 2^-31 of that one at most.  expand undoes it by row, the grads step by step.
+// 2^-31 of that one at most.  expand undoes it by row, the grads step by step.  (x and dy
+// themselves are taken as they are: the tensor cores add the products of a subnormal number
+// at the place of 2^-14, so those of dy near 2^-24 keep some 14 bits, as in any product.)
 // The shared product takes scale[i] s rounded to the type, like every operand of it; the sum
 // with the shared part is then rounded once, where expand rounds it a second time.  A row of
 // fp16 whose largest |scale[i] s| is beyond 65504 or below the normal numbers (2^-14) has no
