@@ -669,7 +669,7 @@ __global__ void __launch_bounds__(threads(J, SHARE), 1)
   }
 }
 
-// The parts of F in W2's items: about 2048 columns each, more when there are many slots (then
+// The parts of F in W2's items: about 2048 columns each, wider ones when there are many slots (then
 // there are many groups, and the parts' sums cost more than their balance gains), in whole
 // stages of `stage` columns.  No part is empty: the consumers that skip an item count its
 // stages from its columns, so the number of parts follows from their rounded width.
@@ -792,8 +792,8 @@ namespace {
 bool sizes_ok(int32_t num_tokens, int32_t hidden, int32_t ffn, int32_t num_experts, int32_t topk) {
   using namespace moe::few;
   return num_tokens >= 0 && num_tokens <= kMaxTokens && hidden >= 8 && hidden % 8 == 0 && hidden <= kMaxWidth &&
-         ffn >= 8 && ffn % 8 == 0 && ffn <= kMaxWidth && num_experts >= 1 && num_experts <= kMaxE && topk >= 1 && topk <= kMaxK &&
-         topk <= num_experts;
+         ffn >= 8 && ffn % 8 == 0 && ffn <= kMaxWidth && num_experts >= 1 && num_experts <= kMaxE &&
+         topk >= 1 && topk <= kMaxK && topk <= num_experts;
 }
 bool rows_ok(const void* p, int64_t ld, int64_t width) {
   return p != nullptr && moe::aligned16(p) && ld >= width && ld % 8 == 0;

@@ -40,7 +40,8 @@ def lora_linear(x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor, lor
     the type, in fp16 with a power of two, so that small gradients lose nothing.  The shared
     weight is frozen.  Sizes that are not multiples of 8, and rows that do not start on 16
     bytes, are copied with padding on every call.  The graph keeps about 10 r bytes a row
-    beside its inputs.
+    beside its inputs, the workspace of its backward among them: passes over one graph may
+    be repeated, but not from two threads at once.
 
     A training step can be captured into a CUDA graph (forward and backward together);
     as for every autograd graph, no graph of the same leaves from before the capture
